@@ -306,6 +306,36 @@ int tt_gemm_dd(const double* A_hi, const double* A_lo, int a_kmajor, long long s
                double* C_hi, double* C_lo, long long strideC, int M, int N, int K, int batch,
                void* stream);
 
+/*
+ * Matrices held in 4 bits: W^[n,k] = s[n, k / group] c[n,k], c in -8..7,
+ * group 32, 64 or 128. Stored in 16 x 128 blocks of 1 KB (zero padded, order
+ * in csrc/q4.cuh) with scales [row tile][k block][128 / group][16 rows].
+ * Types: 0 fp32, 1 bf16, 2 fp16; scales are fp32 or bf16. Sizes of the two
+ * buffers (the packed one 16-byte aligned):
+ */
+size_t tt_q4_packed_bytes(int N, int K);
+size_t tt_q4_scale_count(int N, int K, int group);
+/* From codes (N, K), of which the low four bits are kept, and scales
+ * (N, ceil(K / group)), both contiguous. */
+int tt_q4_pack(const signed char* codes, const void* scales, int scale_type, int N, int K,
+               int group, void* packed, void* packed_scales, void* stream);
+/* From W (N, K; row stride ldw): s = amax / 7 rounded to the scale's type (NaN
+ * for a group with an infinity or NaN), c = rint(w / s) clamped to -8..7. */
+int tt_q4_quantize(const void* W, int type, long long ldw, int scale_type, int N, int K, int group,
+                   void* packed, void* packed_scales, void* stream);
+/* out (N, K) contiguous = s c, rounded once. */
+int tt_q4_dequantize(const void* packed, const void* packed_scales, int scale_type, int N, int K,
+                     int group, void* out, int type, void* stream);
+/* y (M, N; row stride ldy) = x (M, K; row stride ldx) W^T: fp32 sums, rounded
+ * once to x's type. */
+int tt_q4_matmul(const void* x, int type, long long ldx, const void* packed,
+                 const void* packed_scales, int scale_type, int M, int N, int K, int group, void* y,
+                 long long ldy, void* stream);
+/* dx (M, K; row stride lddx) = dy (M, N; row stride lddy) W. */
+int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed,
+                   const void* packed_scales, int scale_type, int M, int N, int K, int group,
+                   void* dx, long long lddx, void* stream);
+
 /* Failure-detection check (no counterpart in the reference): one thread waits,
  * through the same bounded mbarrier wait every kernel here uses, on a phase
  * that nothing completes. After budget_cycles (at most the kernels' own

@@ -5,7 +5,8 @@ Drop-in for the trnsci/trntensor 0.4.0 public namespace
 ``mp2_energy`` and ``ao_to_mo_transform`` run hand-written sm_100a kernels
 (int8 Ozaki-split ``tcgen05.mma`` with exact int32 accumulation, for fp32
 and for fp64) through the C ABI in ``include/trntensor_b200.h``;
-``einsum``/``multi_einsum``/planning stay host Python. The tensor
+``einsum``/``multi_einsum``/planning stay host Python. ``einsum`` also takes
+a matrix held in 4 bits (``quantize_q4``). The tensor
 decompositions are outside this build and raise ``NotImplementedError``.
 """
 
@@ -35,6 +36,7 @@ from .quantum import (
     mp2_energy_dd,
     mp2_pair_energies,
 )
+from .quantized import Q4Matrix, pack_q4, q4_matmul, quantize_q4
 
 __all__ = [
     "einsum",
@@ -60,4 +62,8 @@ __all__ = [
     "mp2_pair_energies",
     "mp2_energy_dd",
     "df_mp2_energy",
+    "Q4Matrix",
+    "quantize_q4",
+    "pack_q4",
+    "q4_matmul",
 ]

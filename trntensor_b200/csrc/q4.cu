@@ -1,0 +1,706 @@
+// 4-bit matrices with group scales: packing, quantisation, decoding, and the
+// products with few rows (csrc/q4.cuh describes the storage).
+//
+//   y[m,n]  = sum_k x[m,k] s[n,g(k)] c[n,k]
+//   dx[m,k] = sum_n dy[m,n] s[n,g(k)] c[n,k]
+//
+// Both products with few rows read the matrix once (4.1 bits a weight) and
+// are bound by that. The codes are exact in bf16 and fp16, so the products
+// run on mma.sync tensor-core fragments decoded in registers and accumulate
+// in fp32; tcgen05 would want the decoded matrix in shared memory first,
+// which costs more than it saves while the rows fit one fragment.
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+#include "q4.cuh"
+
+namespace tt {
+namespace q4 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 8;
+constexpr int kMaxCluster = 8;
+
+// ------------------------------------------------------- packing and decoding
+
+// One warp a block of 16 x 128. kFrom: the codes are given (pack) or made from
+// W (quantise: s = amax / 7 rounded to the scale's type, c = rint(w / s)).
+template <typename WT, typename ST>
+__global__ void quantize_kernel(const WT* __restrict__ W, long long ldw, int N, int K, int group,
+                                uint4* __restrict__ packed, ST* __restrict__ scales,
+                                long long blocks, int kblocks) {
+  const long long blk = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (blk >= blocks) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long rt = blk / kblocks;
+  const int kb = (int)(blk % kblocks);
+  const int words = group / 32, gpb = 4 / words;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const long long row = rt * kRows + g + 8 * h;
+    float v[4][8];
+    uint32_t top[4];  // largest |w| by its bits, whose order puts infinities and NaN on top
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      top[w] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long k = (long long)kb * kCols + 32 * w + 8 * t + i;
+        v[w][i] = row < N && k < K ? to_f(W[row * ldw + k]) : 0.f;
+        top[w] = max(top[w], __float_as_uint(fabsf(v[w][i])));
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) top[w] = max(top[w], __shfl_xor_sync(0xffffffffu, top[w], o));
+    uint32_t out[4];
+#pragma unroll
+    for (int gi = 0; gi < 4; ++gi) {
+      if (gi >= gpb) break;
+      uint32_t bits = 0;
+      for (int w = gi * words; w < (gi + 1) * words; ++w) bits = max(bits, top[w]);
+      const float m = bits >= 0x7f800000u ? __int_as_float(0x7fffffff) : __uint_as_float(bits);
+      const ST st = from_f<ST>(__fdiv_rn(m, 7.f));
+      const float s = to_f(st);
+      if (t == 0) scales[(blk * gpb + gi) * kRows + g + 8 * h] = st;
+      for (int w = gi * words; w < (gi + 1) * words; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float c = s > 0.f ? rintf(__fdiv_rn(v[w][i], s)) : 0.f;
+          c = fminf(fmaxf(c, -8.f), 7.f);
+          word |= (uint32_t)((int)c + 8) << (4 * (i / 2 + 4 * (i & 1)));
+        }
+        out[w] = word;
+      }
+    }
+    packed[blk * 64 + h * 32 + lane] = make_uint4(out[0], out[1], out[2], out[3]);
+  }
+}
+
+template <typename ST>
+__global__ void pack_kernel(const signed char* __restrict__ codes, const ST* __restrict__ in_scales,
+                            int N, int K, int group, uint4* __restrict__ packed,
+                            ST* __restrict__ scales, long long blocks, int kblocks) {
+  const long long blk = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (blk >= blocks) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long rt = blk / kblocks;
+  const int kb = (int)(blk % kblocks);
+  const int gpb = kCols / group;
+  const long long groups = ((long long)K + group - 1) / group;
+  const bool wide = K % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7u) == 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const long long row = rt * kRows + g + 8 * h;
+    uint32_t out[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const long long k0 = (long long)kb * kCols + 32 * w + 8 * t;
+      signed char c[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (row < N && wide && k0 < K) {
+        *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(codes + row * K + k0);
+      } else if (row < N) {
+        for (int i = 0; i < 8; ++i)
+          if (k0 + i < K) c[i] = codes[row * K + k0 + i];
+      }
+      uint32_t word = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        word |= (uint32_t)((c[i] + 8) & 15) << (4 * (i / 2 + 4 * (i & 1)));
+      out[w] = word;
+    }
+    packed[blk * 64 + h * 32 + lane] = make_uint4(out[0], out[1], out[2], out[3]);
+    if (t < gpb) {
+      const long long gi = (long long)kb * gpb + t;
+      scales[(blk * gpb + t) * kRows + g + 8 * h] =
+          row < N && gi < groups ? in_scales[row * groups + gi] : from_f<ST>(0.f);
+    }
+  }
+}
+
+template <typename OT, typename ST>
+__global__ void dequantize_kernel(const uint4* __restrict__ packed, const ST* __restrict__ scales,
+                                  int N, int K, int group, OT* __restrict__ out, long long blocks,
+                                  int kblocks) {
+  const long long blk = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  if (blk >= blocks) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const long long rt = blk / kblocks;
+  const int kb = (int)(blk % kblocks);
+  const int gpb = kCols / group;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const long long row = rt * kRows + g + 8 * h;
+    if (row >= N) continue;
+    const uint4 q = packed[blk * 64 + h * 32 + lane];
+    const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float s = to_f(scales[(blk * gpb + w * gpb / 4) * kRows + g + 8 * h]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long k = (long long)kb * kCols + 32 * w + 8 * t + i;
+        const int c = (int)((word[w] >> (4 * (i / 2 + 4 * (i & 1)))) & 15u) - 8;
+        if (k < K) out[row * K + k] = from_f<OT>(s * (float)c);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ operands
+
+// Eight neighbouring k of a row as pairs for kTerms fragments; what lies
+// behind the row's end is zero. `wide`: rows start on 16 bytes and hold a
+// multiple of 8 values, so that eight values are all there or none is.
+template <typename XT, int kTerms>
+__device__ __forceinline__ void load_eight(const XT* __restrict__ row, long long k0, int K, bool wide,
+                                           uint32_t (&out)[kTerms][4]) {
+  if constexpr (sizeof(XT) == 2) {
+    if (wide) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (k0 < K) v = __ldg(reinterpret_cast<const uint4*>(row + k0));
+      out[0][0] = v.x; out[0][1] = v.y; out[0][2] = v.z; out[0][3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t lo = 0, hi = 0;
+        if (k0 + 2 * j < K) lo = __ldg(reinterpret_cast<const unsigned short*>(row) + k0 + 2 * j);
+        if (k0 + 2 * j + 1 < K) hi = __ldg(reinterpret_cast<const unsigned short*>(row) + k0 + 2 * j + 1);
+        out[0][j] = lo | hi << 16;
+      }
+    }
+  } else {
+    float f[8];
+    if (wide) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+      if (k0 < K) {
+        a = __ldg(reinterpret_cast<const float4*>(row + k0));
+        b = __ldg(reinterpret_cast<const float4*>(row + k0) + 1);
+      }
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = k0 + i < K ? __ldg(row + k0 + i) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t p[kTerms];
+      split_bf16<kTerms>(f[2 * j], f[2 * j + 1], p);
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) out[i][j] = p[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------ y = x W^T, few rows
+
+// A CTA owns 16 rows of W and 8 kTiles tokens; its warps take the row tile's
+// blocks in turn, and the CTAs of a cluster (blockIdx.x is the rank) share
+// them, so that a short matrix still fills the GPU. Each group of k gets a
+// fragment of its own, which is scaled in fp32 when the group ends. The parts
+// are added in a fixed order: warps through shared memory, CTAs through the
+// cluster's.
+template <typename XT, typename ST, int kTiles, int kGroups>
+__global__ void __launch_bounds__(kWarps * 32)
+matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ packed,
+              const ST* __restrict__ scales, int M, int N, int K, int kblocks, int wide,
+              XT* __restrict__ y, long long ldy) {
+  constexpr bool kHalf = sizeof(XT) == 2 && !std::is_same<XT, __nv_bfloat16>::value;
+  constexpr int kTerms = sizeof(XT) == 2 ? 1 : 3;
+  constexpr int kOut = kRows * 8 * kTiles;
+  __shared__ float part[kWarps * kOut];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int warp = threadIdx.x / 32, warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x;
+  const long long rt = blockIdx.y + (long long)blockIdx.z * gridDim.y;
+  const long long rtiles = ((long long)N + kRows - 1) / kRows;
+  const long long mtiles = ((long long)M + 8 * kTiles - 1) / (8 * kTiles);
+  const long long tile = rt;  // row tile fastest: neighbours share x in L2
+  const bool active = tile < rtiles * mtiles;
+  const long long row_tile = active ? tile % rtiles : 0;
+  const long long m0 = active ? tile / rtiles * (8 * kTiles) : 0;
+
+  float acc[kTiles][4];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+
+  if (active) {
+    const XT* xr[kTiles];
+    bool has[kTiles];
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) {
+      has[j] = m0 + 8 * j + g < M;
+      xr[j] = x + (has[j] ? (m0 + 8 * j + g) * ldx : 0);
+    }
+#pragma unroll 2
+    for (int kb = blockIdx.x * warps + warp; kb < kblocks; kb += splits * warps) {
+      const long long blk = row_tile * kblocks + kb;
+      const uint4 qa = ldg_stream(packed + blk * 64 + lane);
+      const uint4 qb = ldg_stream(packed + blk * 64 + 32 + lane);
+      const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
+      uint32_t xp[kTiles][4][kTerms][4];
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          load_eight<XT, kTerms>(xr[j], (long long)kb * kCols + 32 * w + 8 * t, has[j] ? K : 0,
+                                 wide != 0, xp[j][w]);
+#pragma unroll
+      for (int gi = 0; gi < kGroups; ++gi) {
+        float c[kTiles][4];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+#pragma unroll
+        for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a0 = decode_pair<kHalf>(wa[w] >> (8 * half));
+            const uint32_t a1 = decode_pair<kHalf>(wb[w] >> (8 * half));
+            const uint32_t a2 = decode_pair<kHalf>(wa[w] >> (8 * half + 4));
+            const uint32_t a3 = decode_pair<kHalf>(wb[w] >> (8 * half + 4));
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+              for (int i = 0; i < kTerms; ++i)
+                mma16816<kHalf>(c[j], a0, a1, a2, a3, xp[j][w][i][2 * half], xp[j][w][i][2 * half + 1]);
+          }
+        const ST* sp = scales + (blk * kGroups + gi) * kRows + g;
+        const float s0 = to_f(sp[0]), s1 = to_f(sp[8]);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          acc[j][0] += s0 * c[j][0];
+          acc[j][1] += s0 * c[j][1];
+          acc[j][2] += s1 * c[j][2];
+          acc[j][3] += s1 * c[j][3];
+        }
+      }
+    }
+  }
+  // part[warp][token][row]
+  float* mine = part + warp * kOut;
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) {
+    mine[(8 * j + 2 * t) * kRows + g] = acc[j][0];
+    mine[(8 * j + 2 * t + 1) * kRows + g] = acc[j][1];
+    mine[(8 * j + 2 * t) * kRows + g + 8] = acc[j][2];
+    mine[(8 * j + 2 * t + 1) * kRows + g + 8] = acc[j][3];
+  }
+  __syncthreads();
+  for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
+    float v = part[o];
+    for (int w = 1; w < warps; ++w) v += part[w * kOut + o];
+    part[o] = v;
+  }
+  if (splits > 1) {
+    cluster.sync();
+    if (blockIdx.x == 0) {
+      for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
+        float v = part[o];
+        for (int r = 1; r < splits; ++r) v += cluster.map_shared_rank(part, r)[o];
+        part[o] = v;
+      }
+    }
+    cluster.sync();
+  } else {
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && active) {
+    for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
+      const long long m = m0 + o / kRows, n = row_tile * kRows + o % kRows;
+      if (m < M && n < N) y[m * ldy + n] = from_f<XT>(part[o]);
+    }
+  }
+}
+
+// ------------------------------------------------------------ dx = dy W, few rows
+
+// A CTA owns 128 columns of W and 16 tokens; the rows of W are shared among
+// its warps and the CTAs of its cluster. Here the scale varies along the sum,
+// so it goes into the other operand: dy s is split into bf16 terms (two for
+// 16-bit types: 2^-16 of each product, against 2^-9 or 2^-12 for the result's
+// own rounding; three for fp32). Tile (w, j) of a block takes the columns
+// k = 32 w + 8 (c / 2) + 2 j + c % 2, so that all its columns share a group.
+template <typename XT, typename ST, int kGroups>
+__global__ void __launch_bounds__(kWarps * 32)
+matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restrict__ packed,
+                const ST* __restrict__ scales, int M, int N, int K, int kblocks,
+                XT* __restrict__ dx, long long lddx) {
+  constexpr int kTerms = sizeof(XT) == 2 ? 2 : 3;
+  extern __shared__ float tpart[];  // [warp][16 tokens][128]
+  cg::cluster_group cluster = cg::this_cluster();
+  const int warp = threadIdx.x / 32, warps = blockDim.x / 32, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x;
+  const long long tile = blockIdx.y + (long long)blockIdx.z * gridDim.y;
+  const long long mtiles = ((long long)M + 15) / 16;
+  const bool active = tile < (long long)kblocks * mtiles;
+  const int kb = active ? (int)(tile % kblocks) : 0;
+  const long long m0 = active ? tile / kblocks * 16 : 0;
+  const long long rtiles = ((long long)N + kRows - 1) / kRows;
+
+  float acc[16][4];
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+
+  if (active) {
+    for (long long rt = blockIdx.x * warps + warp; rt < rtiles; rt += splits * warps) {
+      const long long blk = rt * kblocks + kb;
+      const long long n0 = rt * kRows;
+      // rows 2t, 2t+1 (half 0) and 8+2t, 9+2t (half 1); the words of t' = g / 2
+      uint4 q[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        q[r] = __ldg(packed + blk * 64 + (r >> 1) * 32 + (2 * t + (r & 1)) * 4 + (g >> 1));
+      float d[2][4];  // token g / g + 8, rows as in q
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long m = m0 + g + 8 * h;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const long long n = n0 + (r >> 1) * 8 + 2 * t + (r & 1);
+          d[h][r] = m < M && n < N ? to_f(dy[m * lddy + n]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int gi = 0; gi < kGroups; ++gi) {
+        const ST* sp = scales + (blk * kGroups + gi) * kRows + 2 * t;
+        const float s[4] = {to_f(sp[0]), to_f(sp[1]), to_f(sp[8]), to_f(sp[9])};
+        uint32_t a[4][kTerms];  // a0: token g rows 0,1; a1: token g+8; a2, a3: rows 2,3
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          split_bf16<kTerms>(d[h][0] * s[0], d[h][1] * s[1], a[h]);
+          split_bf16<kTerms>(d[h][2] * s[2], d[h][3] * s[3], a[2 + h]);
+        }
+#pragma unroll
+        for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w) {
+          const uint32_t sel = g & 1 ? 0x7632 : 0x5410;
+          const uint32_t w0 = w == 0 ? q[0].x : w == 1 ? q[0].y : w == 2 ? q[0].z : q[0].w;
+          const uint32_t w1 = w == 0 ? q[1].x : w == 1 ? q[1].y : w == 2 ? q[1].z : q[1].w;
+          const uint32_t w2 = w == 0 ? q[2].x : w == 1 ? q[2].y : w == 2 ? q[2].z : q[2].w;
+          const uint32_t w3 = w == 0 ? q[3].x : w == 1 ? q[3].y : w == 2 ? q[3].z : q[3].w;
+          const uint32_t lo = __byte_perm(w0, w1, sel), hi = __byte_perm(w2, w3, sel);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t b0 = decode_pair<false>(lo >> (4 * j));
+            const uint32_t b1 = decode_pair<false>(hi >> (4 * j));
+#pragma unroll
+            for (int i = 0; i < kTerms; ++i)
+              mma16816<false>(acc[4 * w + j], a[0][i], a[1][i], a[2][i], a[3][i], b0, b1);
+          }
+        }
+      }
+    }
+  }
+  // columns of this lane: 32 w + 8 t + 2 j + {0, 1}
+  float* mine = tpart + warp * 16 * kCols;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = 32 * w + 8 * t + 2 * j;
+      *reinterpret_cast<float2*>(mine + g * kCols + col) = make_float2(acc[4 * w + j][0], acc[4 * w + j][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * kCols + col) = make_float2(acc[4 * w + j][2], acc[4 * w + j][3]);
+    }
+  __syncthreads();
+  constexpr int kOut = 16 * kCols;
+  for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
+    float v = tpart[o];
+    for (int w = 1; w < warps; ++w) v += tpart[w * kOut + o];
+    tpart[o] = v;
+  }
+  if (splits > 1) {
+    cluster.sync();
+    // every rank adds a share of the outputs, in rank order, and keeps it to itself
+    if (active) {
+      for (int o = threadIdx.x + blockIdx.x * blockDim.x; o < kOut; o += splits * blockDim.x) {
+        float v = cluster.map_shared_rank(tpart, 0)[o];
+        for (int r = 1; r < splits; ++r) v += cluster.map_shared_rank(tpart, r)[o];
+        const long long m = m0 + o / kCols, k = (long long)kb * kCols + o % kCols;
+        if (m < M && k < K) dx[m * lddx + k] = from_f<XT>(v);
+      }
+    }
+    cluster.sync();
+  } else {
+    __syncthreads();
+    if (active) {
+      for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
+        const long long m = m0 + o / kCols, k = (long long)kb * kCols + o % kCols;
+        if (m < M && k < K) dx[m * lddx + k] = from_f<XT>(tpart[o]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- host
+
+bool good_group(int g) { return g == 32 || g == 64 || g == 128; }
+
+std::once_flag g_flags[kMaxDevices];
+int g_ok[kMaxDevices];
+int g_sms[kMaxDevices];
+
+template <typename F>
+int launch_cluster(F kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t s,
+                   void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), args));
+}
+
+// tiles as (y, z) with y <= 65535; false when there are too many.
+bool grid_of(long long tiles, int splits, dim3* grid) {
+  const long long y = tiles < 65535 ? tiles : 65535, z = (tiles + y - 1) / y;
+  if (z > 65535) return false;
+  *grid = dim3((unsigned)splits, (unsigned)y, (unsigned)z);
+  return true;
+}
+
+// CTAs of a cluster: as many (a power of two) as leave each warp a block and
+// the GPU no more than about two CTAs an SM.
+int pick_splits(long long tiles, long long steps, int sms) {
+  int s = 1;
+  while (s < kMaxCluster && tiles * s * 2 <= 2LL * sms + sms / 2 && steps >= (long long)s * 2 * kWarps) s *= 2;
+  return s;
+}
+
+template <typename XT, typename ST, int kTiles, int kGroups>
+int run_matvec(const void* x, long long ldx, const void* packed, const void* scales, int M, int N,
+               int K, void* y, long long ldy, int sms, cudaStream_t s) {
+  const int kblocks = (int)(((long long)K + kCols - 1) / kCols);
+  const long long rtiles = ((long long)N + kRows - 1) / kRows;
+  const long long mtiles = ((long long)M + 8 * kTiles - 1) / (8 * kTiles);
+  const int splits = pick_splits(rtiles * mtiles, kblocks, sms);
+  dim3 grid;
+  if (!grid_of(rtiles * mtiles, splits, &grid)) return TT_ERR_SHAPE;
+  int wide = K % 8 == 0 && ldx % (16 / (int)sizeof(XT)) == 0 && aligned16(x);
+  int kb = kblocks;
+  void* args[] = {&x, &ldx, &packed, &scales, &M, &N, &K, &kb, &wide, &y, &ldy};
+  return launch_cluster(matvec_kernel<XT, ST, kTiles, kGroups>, grid, kWarps * 32, 0, splits, s, args);
+}
+
+template <typename XT, typename ST, int kGroups>
+int run_matvec_t(const void* dy, long long lddy, const void* packed, const void* scales, int M,
+                 int N, int K, void* dx, long long lddx, int sms, cudaStream_t s) {
+  int kblocks = (int)(((long long)K + kCols - 1) / kCols);
+  const long long rtiles = ((long long)N + kRows - 1) / kRows;
+  const long long tiles = (long long)kblocks * (((long long)M + 15) / 16);
+  const int splits = pick_splits(tiles, rtiles, sms);
+  dim3 grid;
+  if (!grid_of(tiles, splits, &grid)) return TT_ERR_SHAPE;
+  void* args[] = {&dy, &lddy, &packed, &scales, &M, &N, &K, &kblocks, &dx, &lddx};
+  return launch_cluster(matvec_t_kernel<XT, ST, kGroups>, grid, kWarps * 32,
+                        kWarps * 16 * kCols * 4, splits, s, args);
+}
+
+template <typename XT, typename ST>
+int set_attrs() {
+  const int bytes = kWarps * 16 * kCols * 4;
+  if (cudaFuncSetAttribute(matvec_t_kernel<XT, ST, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(matvec_t_kernel<XT, ST, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaFuncSetAttribute(matvec_t_kernel<XT, ST, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return TT_ERR_CUDA;
+  return TT_OK;
+}
+
+int setup(int dev) {
+  return once_per_device(g_flags, g_ok, dev, [dev]() -> int {
+    if (cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return TT_ERR_CUDA;
+    int st = set_attrs<float, float>();
+    if (st == TT_OK) st = set_attrs<float, __nv_bfloat16>();
+    if (st == TT_OK) st = set_attrs<__nv_bfloat16, float>();
+    if (st == TT_OK) st = set_attrs<__nv_bfloat16, __nv_bfloat16>();
+    if (st == TT_OK) st = set_attrs<__half, float>();
+    if (st == TT_OK) st = set_attrs<__half, __nv_bfloat16>();
+    return st;
+  });
+}
+
+template <typename XT, typename ST>
+int matmul_typed(bool transposed, const void* x, long long ldx, const void* packed,
+                 const void* scales, int M, int N, int K, int group, void* y, long long ldy,
+                 int sms, cudaStream_t s) {
+  const int gpb = kCols / group;
+  if (transposed) {
+    if (gpb == 1) return run_matvec_t<XT, ST, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (gpb == 2) return run_matvec_t<XT, ST, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    return run_matvec_t<XT, ST, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  }
+  if (M <= 8) {
+    if (gpb == 1) return run_matvec<XT, ST, 1, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (gpb == 2) return run_matvec<XT, ST, 1, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    return run_matvec<XT, ST, 1, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  }
+  if (gpb == 1) return run_matvec<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  if (gpb == 2) return run_matvec<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  return run_matvec<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+}
+
+template <typename XT>
+int matmul_scaled(bool transposed, const void* x, long long ldx, const void* packed,
+                  const void* scales, int scale_type, int M, int N, int K, int group, void* y,
+                  long long ldy, int sms, cudaStream_t s) {
+  return scale_type == kF32
+             ? matmul_typed<XT, float>(transposed, x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s)
+             : matmul_typed<XT, __nv_bfloat16>(transposed, x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
+}
+
+int matmul(bool transposed, const void* x, int type, long long ldx, const void* packed,
+           const void* scales, int scale_type, int M, int N, int K, int group, void* y,
+           long long ldy, void* stream) {
+  if (!x || !packed || !scales || !y) return TT_ERR_NULL;
+  if (M <= 0 || N <= 0 || K <= 0 || !good_group(group)) return TT_ERR_SHAPE;
+  if (type < 0 || type > 2 || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
+  if (ldx < (transposed ? N : K) || ldy < (transposed ? K : N)) return TT_ERR_SHAPE;
+  if (!aligned16(packed) || !aligned16(scales)) return TT_ERR_ALIGN;
+  int dev = 0;
+  int st = check_device(&dev);
+  if (st != TT_OK) return st;
+  if ((st = setup(dev)) != TT_OK) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  const int sms = g_sms[dev];
+  if (type == kF32)
+    return matmul_scaled<float>(transposed, x, ldx, packed, scales, scale_type, M, N, K, group, y, ldy, sms, s);
+  if (type == kBF16)
+    return matmul_scaled<__nv_bfloat16>(transposed, x, ldx, packed, scales, scale_type, M, N, K, group, y, ldy, sms, s);
+  return matmul_scaled<__half>(transposed, x, ldx, packed, scales, scale_type, M, N, K, group, y, ldy, sms, s);
+}
+
+template <typename WT, typename ST>
+int run_quantize(const void* W, long long ldw, int N, int K, int group, void* packed, void* scales,
+                 cudaStream_t s) {
+  const int kblocks = (int)(((long long)K + kCols - 1) / kCols);
+  const long long blocks = ((long long)N + kRows - 1) / kRows * kblocks;
+  const long long ctas = (blocks + 7) / 8;
+  if (ctas > 0x7fffffffLL) return TT_ERR_SHAPE;
+  quantize_kernel<WT, ST><<<(unsigned)ctas, 256, 0, s>>>((const WT*)W, ldw, N, K, group,
+                                                         (uint4*)packed, (ST*)scales, blocks, kblocks);
+  return cuda_status(cudaGetLastError());
+}
+
+template <typename OT, typename ST>
+int run_dequantize(const void* packed, const void* scales, int N, int K, int group, void* out,
+                   cudaStream_t s) {
+  const int kblocks = (int)(((long long)K + kCols - 1) / kCols);
+  const long long blocks = ((long long)N + kRows - 1) / kRows * kblocks;
+  const long long ctas = (blocks + 7) / 8;
+  if (ctas > 0x7fffffffLL) return TT_ERR_SHAPE;
+  dequantize_kernel<OT, ST><<<(unsigned)ctas, 256, 0, s>>>((const uint4*)packed, (const ST*)scales, N, K,
+                                                           group, (OT*)out, blocks, kblocks);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+}  // namespace q4
+}  // namespace tt
+
+extern "C" {
+
+size_t tt_q4_packed_bytes(int N, int K) {
+  if (N <= 0 || K <= 0) return 0;
+  return ((size_t)N + 15) / 16 * (((size_t)K + 127) / 128) * tt::q4::kBlockBytes;
+}
+
+size_t tt_q4_scale_count(int N, int K, int group) {
+  if (N <= 0 || K <= 0 || !tt::q4::good_group(group)) return 0;
+  return ((size_t)N + 15) / 16 * (((size_t)K + 127) / 128) * (128 / group) * 16;
+}
+
+int tt_q4_pack(const signed char* codes, const void* scales, int scale_type, int N, int K, int group,
+               void* packed, void* packed_scales, void* stream) {
+  using namespace tt;
+  if (!codes || !scales || !packed || !packed_scales) return TT_ERR_NULL;
+  if (N <= 0 || K <= 0 || !q4::good_group(group) || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
+  if (!aligned16(packed)) return TT_ERR_ALIGN;
+  int st = check_device(nullptr);
+  if (st != TT_OK) return st;
+  const int kblocks = (int)(((long long)K + q4::kCols - 1) / q4::kCols);
+  const long long blocks = ((long long)N + q4::kRows - 1) / q4::kRows * kblocks;
+  const long long ctas = (blocks + 7) / 8;
+  if (ctas > 0x7fffffffLL) return TT_ERR_SHAPE;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (scale_type == q4::kF32)
+    q4::pack_kernel<float><<<(unsigned)ctas, 256, 0, s>>>(codes, (const float*)scales, N, K, group,
+                                                          (uint4*)packed, (float*)packed_scales, blocks, kblocks);
+  else
+    q4::pack_kernel<__nv_bfloat16><<<(unsigned)ctas, 256, 0, s>>>(
+        codes, (const __nv_bfloat16*)scales, N, K, group, (uint4*)packed, (__nv_bfloat16*)packed_scales,
+        blocks, kblocks);
+  return cuda_status(cudaGetLastError());
+}
+
+int tt_q4_quantize(const void* W, int type, long long ldw, int scale_type, int N, int K, int group,
+                   void* packed, void* packed_scales, void* stream) {
+  using namespace tt;
+  if (!W || !packed || !packed_scales) return TT_ERR_NULL;
+  if (N <= 0 || K <= 0 || !q4::good_group(group) || ldw < K) return TT_ERR_SHAPE;
+  if (type < 0 || type > 2 || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
+  if (!aligned16(packed)) return TT_ERR_ALIGN;
+  int st = check_device(nullptr);
+  if (st != TT_OK) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  using BF = __nv_bfloat16;
+  if (type == q4::kF32)
+    return scale_type == q4::kF32 ? q4::run_quantize<float, float>(W, ldw, N, K, group, packed, packed_scales, s)
+                                  : q4::run_quantize<float, BF>(W, ldw, N, K, group, packed, packed_scales, s);
+  if (type == q4::kBF16)
+    return scale_type == q4::kF32 ? q4::run_quantize<BF, float>(W, ldw, N, K, group, packed, packed_scales, s)
+                                  : q4::run_quantize<BF, BF>(W, ldw, N, K, group, packed, packed_scales, s);
+  return scale_type == q4::kF32 ? q4::run_quantize<__half, float>(W, ldw, N, K, group, packed, packed_scales, s)
+                                : q4::run_quantize<__half, BF>(W, ldw, N, K, group, packed, packed_scales, s);
+}
+
+int tt_q4_dequantize(const void* packed, const void* packed_scales, int scale_type, int N, int K,
+                     int group, void* out, int type, void* stream) {
+  using namespace tt;
+  if (!packed || !packed_scales || !out) return TT_ERR_NULL;
+  if (N <= 0 || K <= 0 || !q4::good_group(group)) return TT_ERR_SHAPE;
+  if (type < 0 || type > 2 || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
+  if (!aligned16(packed)) return TT_ERR_ALIGN;
+  int st = check_device(nullptr);
+  if (st != TT_OK) return st;
+  cudaStream_t s = (cudaStream_t)stream;
+  using BF = __nv_bfloat16;
+  if (type == q4::kF32)
+    return scale_type == q4::kF32 ? q4::run_dequantize<float, float>(packed, packed_scales, N, K, group, out, s)
+                                  : q4::run_dequantize<float, BF>(packed, packed_scales, N, K, group, out, s);
+  if (type == q4::kBF16)
+    return scale_type == q4::kF32 ? q4::run_dequantize<BF, float>(packed, packed_scales, N, K, group, out, s)
+                                  : q4::run_dequantize<BF, BF>(packed, packed_scales, N, K, group, out, s);
+  return scale_type == q4::kF32 ? q4::run_dequantize<__half, float>(packed, packed_scales, N, K, group, out, s)
+                                : q4::run_dequantize<__half, BF>(packed, packed_scales, N, K, group, out, s);
+}
+
+int tt_q4_matmul(const void* x, int type, long long ldx, const void* packed, const void* packed_scales,
+                 int scale_type, int M, int N, int K, int group, void* y, long long ldy, void* stream) {
+  return tt::q4::matmul(false, x, type, ldx, packed, packed_scales, scale_type, M, N, K, group, y, ldy, stream);
+}
+
+int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed, const void* packed_scales,
+                   int scale_type, int M, int N, int K, int group, void* dx, long long lddx, void* stream) {
+  return tt::q4::matmul(true, dy, type, lddy, packed, packed_scales, scale_type, M, N, K, group, dx, lddx, stream);
+}
+
+}  // extern "C"

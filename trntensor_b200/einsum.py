@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from .plan import ContractionPlan, _parse_subscripts, plan_contraction
+from .quantized import Q4Matrix, einsum_q4
 
 _DTYPES: dict[str, torch.dtype] = {
     "bf16": torch.bfloat16,
@@ -48,12 +49,17 @@ def einsum(
     """Einstein summation with contraction planning.
 
     Returns ``alpha * contract(operands) + beta * out`` (``out`` optional).
+    One of two operands may be a 4-bit matrix (``Q4Matrix``), contracted over
+    either of its indices; ``dtype`` casts the dense operand.
     """
     target = _resolve_dtype(dtype)
     if target is not None:
-        operands = tuple(op.to(target) for op in operands)
-    plan = plan_contraction(subscripts, *operands, precision=precision)
-    result = _execute(subscripts, operands, plan)
+        operands = tuple(op if isinstance(op, Q4Matrix) else op.to(target) for op in operands)
+    if any(isinstance(op, Q4Matrix) for op in operands):
+        result = einsum_q4(subscripts, operands, precision)
+    else:
+        plan = plan_contraction(subscripts, *operands, precision=precision)
+        result = _execute(subscripts, operands, plan)
     if alpha != 1.0:
         result = result.mul(alpha)
     if out is not None:

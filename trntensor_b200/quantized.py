@@ -1,0 +1,257 @@
+"""Contractions with a matrix that is held in 4 bits.
+
+``W^[n, k] = s[n, k // group] * c[n, k]`` with integer codes ``c`` in -8..7 and
+one scale for each group of 32, 64 or 128 neighbouring k of a row. A
+:class:`Q4Matrix` is laid out once (``quantize_q4`` from a float matrix,
+``pack_q4`` from codes and scales) and stands as an operand of
+:func:`trntensor_b200.einsum`, or of :func:`q4_matmul`, for any number of rows.
+Both contractions exist: over k (``"mk,nk->mn"``) and over n (``"mn,nk->mk"``),
+each the gradient of the other for the dense operand; the matrix itself gets no
+gradient. Nothing here has a counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .dispatch import _device, _ptr
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_GROUPS = (32, 64, 128)
+
+
+def _stream_of(dev: torch.device) -> ctypes.c_void_p:
+    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+
+
+class Q4Matrix:
+    """An (N, K) matrix of 4-bit codes with group scales, in kernel order.
+
+    Made by :func:`quantize_q4` or :func:`pack_q4`; ``packed`` and ``scales``
+    are the stored bytes and scales (bf16 or fp32), padded to 16 x 128 blocks.
+    """
+
+    ndim = 2
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int],
+                 group: int):
+        self.packed, self.scales, self.group = packed, scales, group
+        self.shape = torch.Size(shape)
+
+    @property
+    def device(self) -> torch.device:
+        return self.packed.device
+
+    def dim(self) -> int:
+        return 2
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The (N, K) matrix as floats (each product rounded once to ``dtype``)."""
+        kind = torch.float32 if dtype == torch.float64 else dtype
+        if kind not in _TYPES:
+            raise ValueError(f"dequantize: dtype must be a float type, got {dtype}")
+        if dtype == torch.float64 and self.scales.dtype == torch.float32:
+            # an fp32 scale times a code needs up to 27 bits
+            codes = self.codes().double()
+            wide = self.group_scales().double().repeat_interleave(self.group, dim=1)
+            return codes * wide[:, : self.shape[1]]
+        n, k = self.shape
+        out = torch.empty((n, k), dtype=kind, device=self.device)
+        if out.numel():
+            lib = _lib.load()
+            with torch.cuda.device(self.device):
+                _lib.check(lib.tt_q4_dequantize(
+                    _ptr(self.packed), _ptr(self.scales), _TYPES[self.scales.dtype], n, k,
+                    self.group, _ptr(out), _TYPES[kind], _stream_of(self.device)),
+                    "tt_q4_dequantize")
+        return out.to(dtype)
+
+    def codes(self) -> torch.Tensor:
+        """The (N, K) int8 codes."""
+        n, k = self.shape
+        if n == 0 or k == 0:
+            return torch.empty((n, k), dtype=torch.int8, device=self.device)
+        # [row tile][k block][row half][g][t][word][byte], two codes a byte
+        b = self.packed.view(-(-n // 16), -(-k // 128), 2, 8, 4, 4, 4)
+        nib = torch.stack((b & 15, b >> 4), dim=-1).flatten(-2)  # nibble p of the word
+        nib = nib.unflatten(-1, (2, 4)).transpose(-1, -2).flatten(-2)  # code i = 2 j + e
+        full = nib.permute(0, 2, 3, 1, 5, 4, 6).reshape(16 * b.shape[0], 128 * b.shape[1])
+        return (full[:n, :k].to(torch.int16) - 8).to(torch.int8)
+
+    def group_scales(self) -> torch.Tensor:
+        """The (N, ceil(K / group)) scales."""
+        n, k = self.shape
+        s = self.scales.view(-(-n // 16), -(-k // 128), 128 // self.group, 16)
+        s = s.permute(0, 3, 1, 2).reshape(16 * s.shape[0], -1)
+        return s[:n, : -(-k // self.group)].contiguous()
+
+    def __repr__(self) -> str:
+        return f"Q4Matrix(shape={tuple(self.shape)}, group={self.group}, device={self.device})"
+
+
+def _check_group(group: int) -> None:
+    if group not in _GROUPS:
+        raise ValueError(f"group must be one of {_GROUPS}, got {group!r}")
+
+
+def _on_device(t: torch.Tensor) -> torch.Tensor:
+    return t if t.device.type == "cuda" else t.to(_device())
+
+
+def _empty_q4(n: int, k: int, group: int, scale_dtype: torch.dtype, dev: torch.device):
+    lib = _lib.load()
+    packed = torch.empty(int(lib.tt_q4_packed_bytes(n, k)), dtype=torch.uint8, device=dev)
+    scales = torch.empty(int(lib.tt_q4_scale_count(n, k, group)), dtype=scale_dtype, device=dev)
+    return packed, scales
+
+
+def quantize_q4(weight: torch.Tensor, *, group: int = 128,
+                scale_dtype: torch.dtype = torch.bfloat16) -> Q4Matrix:
+    """Quantise an (N, K) float matrix: ``s = amax / 7`` of each group, rounded to
+    ``scale_dtype``, and ``c = round(w / s)`` clamped to -8..7.
+
+    A group that holds an infinity or NaN gets the scale NaN. Host matrices are
+    copied to the current CUDA device, where the result lives.
+    """
+    if weight.dim() != 2:
+        raise ValueError(f"quantize_q4: weight must be 2D (N, K), got {tuple(weight.shape)}")
+    if weight.dtype not in _TYPES:
+        raise ValueError(f"quantize_q4: weight must be fp32, bf16 or fp16, got {weight.dtype}")
+    _check_group(group)
+    if scale_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"quantize_q4: scale_dtype must be bf16 or fp32, got {scale_dtype}")
+    w = _on_device(weight.detach())
+    if w.stride(1) != 1 or w.stride(0) < max(1, w.shape[1]):
+        w = w.contiguous()
+    n, k = (int(s) for s in w.shape)
+    packed, scales = _empty_q4(n, k, group, scale_dtype, w.device)
+    if n and k:
+        with torch.cuda.device(w.device):
+            _lib.check(_lib.load().tt_q4_quantize(
+                _ptr(w), _TYPES[w.dtype], int(w.stride(0)) if n > 1 else k, _TYPES[scale_dtype],
+                n, k, group, _ptr(packed), _ptr(scales), _stream_of(w.device)), "tt_q4_quantize")
+    return Q4Matrix(packed, scales, (n, k), group)
+
+
+def pack_q4(codes: torch.Tensor, scales: torch.Tensor, *, group: int = 128) -> Q4Matrix:
+    """Lay out given codes (N, K; int8 in -8..7, of which the low four bits are
+    kept) and scales (N, ceil(K / group); bf16, or fp32, or fp16, which is kept
+    as fp32)."""
+    _check_group(group)
+    if codes.dim() != 2 or codes.dtype != torch.int8:
+        raise ValueError(f"pack_q4: codes must be 2D int8, got {tuple(codes.shape)} {codes.dtype}")
+    n, k = (int(s) for s in codes.shape)
+    if scales.dtype not in _TYPES or tuple(scales.shape) != (n, -(-k // group)):
+        raise ValueError(
+            f"pack_q4: scales must be bf16, fp16 or fp32 of shape {(n, -(-k // group))}, "
+            f"got {tuple(scales.shape)} {scales.dtype}")
+    c = _on_device(codes).contiguous()
+    s = scales.detach().to(c.device)
+    s = (s.float() if s.dtype == torch.float16 else s).contiguous()
+    packed, out = _empty_q4(n, k, group, s.dtype, c.device)
+    if n and k:
+        with torch.cuda.device(c.device):
+            _lib.check(_lib.load().tt_q4_pack(
+                _ptr(c), _ptr(s), _TYPES[s.dtype], n, k, group, _ptr(packed), _ptr(out),
+                _stream_of(c.device)), "tt_q4_pack")
+    return Q4Matrix(packed, out, (n, k), group)
+
+
+def _product(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
+    """(M, K) -> (M, N) or, over_n, (M, N) -> (M, K) on the matrix's device."""
+    n, k = w.shape
+    m, cols = int(x.shape[0]), (k if over_n else n)
+    out = torch.empty((m, cols), dtype=x.dtype, device=x.device)
+    if out.numel() == 0:
+        return out
+    if n == 0 or k == 0:
+        return out.zero_()
+    if x.stride(1) != 1 or (m > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    lib = _lib.load()
+    fn = lib.tt_q4_matmul_t if over_n else lib.tt_q4_matmul
+    with torch.cuda.device(x.device):
+        _lib.check(fn(_ptr(x), _TYPES[x.dtype], int(x.stride(0)) if m > 1 else int(x.shape[1]),
+                      _ptr(w.packed), _ptr(w.scales), _TYPES[w.scales.dtype], m, n, k, w.group,
+                      _ptr(out), cols, _stream_of(x.device)),
+                   "tt_q4_matmul_t" if over_n else "tt_q4_matmul")
+    return out
+
+
+class _Q4Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, over_n):
+        ctx.w, ctx.over_n = w, over_n
+        return _product(x, w, over_n)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _Q4Product.apply(dy, ctx.w, not ctx.over_n), None, None
+
+
+def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> torch.Tensor:
+    """``x @ W^T``: (..., K) -> (..., N); with ``over_n`` ``x @ W``: (..., N) -> (..., K).
+
+    x is fp32, bf16 or fp16; products are exact, sums are fp32, and the result
+    is rounded once to x's type (over n the scaled operand is split into bf16
+    terms, which keeps 2^-16 of each product for 16-bit types and fp32's own
+    bits for fp32). Differentiable in x, any number of times. A host x is
+    copied to the matrix's device and the result comes back.
+    """
+    if not isinstance(weight, Q4Matrix):
+        raise ValueError(f"q4_matmul: weight must be a Q4Matrix, got {type(weight).__name__}")
+    if x.dtype not in _TYPES:
+        raise ValueError(f"q4_matmul: x must be fp32, bf16 or fp16, got {x.dtype}")
+    want = weight.shape[0] if over_n else weight.shape[1]
+    if x.dim() < 1 or x.shape[-1] != want:
+        raise ValueError(f"q4_matmul: x must end in {want} for {weight!r}, got {tuple(x.shape)}")
+    if x.device.type == "cuda" and x.device != weight.device:
+        raise ValueError(f"q4_matmul: x is on {x.device}, the matrix on {weight.device}")
+    lead = x.shape[:-1]
+    rows = 1
+    for s in lead:
+        rows *= int(s)
+    flat = x.to(weight.device).reshape(rows, want)
+    y = _Q4Product.apply(flat, weight, over_n)
+    return y.reshape(*lead, y.shape[-1]).to(x.device)
+
+
+def einsum_q4(subscripts: str, operands: tuple, precision: str) -> torch.Tensor:
+    """Two-operand einsum with one :class:`Q4Matrix`: a product over k or over n
+    with the dense operand's other indices kept."""
+    from .plan import _check_precision, _parse_subscripts, _validate_subscripts
+
+    _validate_subscripts(subscripts, operands)
+    _check_precision(precision)
+    lhs, out = _parse_subscripts(subscripts)
+    terms = lhs.split(",")
+    held = [i for i, op in enumerate(operands) if isinstance(op, Q4Matrix)]
+    if len(operands) != 2 or len(held) != 1:
+        raise ValueError(
+            f"einsum {subscripts!r}: a Q4Matrix contracts with one dense operand; "
+            "use dequantize() for other forms")
+    w, x = operands[held[0]], operands[1 - held[0]]
+    tw, tx = terms[held[0]], terms[1 - held[0]]
+    shared = [c for c in tw if c in tx]
+    if (len(set(tw)) != 2 or len(set(tx)) != len(tx) or len(set(out)) != len(out)
+            or len(shared) != 1 or shared[0] in out):
+        raise ValueError(
+            f"einsum {subscripts!r}: a Q4Matrix is contracted over exactly one of its indices, "
+            "which the output drops; use dequantize() for other forms")
+    c = shared[0]
+    free = tw[1] if c == tw[0] else tw[0]
+    rest = [ch for ch in tx if ch != c]
+    if set(out) != set(rest) | {free}:
+        raise ValueError(f"einsum {subscripts!r}: every uncontracted index must be in the output")
+    if precision != "fast":
+        from .einsum import einsum
+
+        ops = [w.dequantize(torch.float64), x]
+        return einsum(f"{tw},{tx}->{out}", ops[0].to(x.device), x.double(),
+                      precision=precision).to(x.dtype)
+    y = q4_matmul(x.permute([tx.index(ch) for ch in rest + [c]]), w, over_n=c == tw[0])
+    order = [(rest + [free]).index(ch) for ch in out]
+    return y if order == list(range(len(order))) else y.permute(order).contiguous()
