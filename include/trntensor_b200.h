@@ -336,6 +336,62 @@ int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed,
                    const void* packed_scales, int scale_type, int M, int N, int K, int group,
                    void* dx, long long lddx, void* stream);
 
+/*
+ * Paged key-value cache held in 8 bits: x^ = s c, c in -127..127 stored biased
+ * by 128, one fp32 scale for each page and head. A page holds `page` tokens
+ * (16, 32, 64 or 128) of all `heads` heads of `dim` values (a multiple of 16,
+ * at most 256):
+ *   k_codes [pages][heads][page][dim]
+ *   v_codes [pages][heads][page / 16][dim][16]
+ *   k_scales, v_scales [pages][heads]
+ * (16-byte aligned). block_table (batch rows of `columns` page ids, row stride
+ * table_stride) gives the page of each sequence's tokens page by page.
+ * Lengths, counts, tables and the status word live on the device; the kernels
+ * leave out what points outside the cache and OR a bit into *status: 1 a page
+ * id outside the cache, 2 a length or count out of range, 4 one append that
+ * writes a page for two places, 8 a copy that never arrived. Activations are
+ * fp32, bf16 or fp16 (types as above) with strides in elements over (batch,
+ * token, head) and neighbouring values in a head.
+ */
+/* Append k, v (batch, S, heads, dim): token i of sequence b at position
+ * lengths[b] + i for i < n_new[b] (n_new NULL: S). Keys are turned first by the
+ * angles position * inv_freq[j] for `pairs` pairs (0: not at all), (j, j +
+ * pairs) or, interleaved, (2 j, 2 j + 1). A page's scale grows to its largest
+ * value / 127, its earlier tokens' codes are rounded onto it; a call that
+ * writes slot 0 starts the page anew. An infinity or NaN makes the scale NaN.
+ * Pages that a call writes belong to one sequence. */
+int tt_kv8_append(const void* k, const void* v, int type, long long k_stride_b, long long k_stride_s,
+                  long long k_stride_h, long long v_stride_b, long long v_stride_s,
+                  long long v_stride_h, const int* block_table, long long table_stride, int columns,
+                  const int* lengths, const int* n_new, const float* inv_freq, int pairs,
+                  int interleaved, void* k_codes, void* v_codes, float* k_scales, float* v_scales,
+                  int* status, int batch, int S, int heads, int dim, int page, int pages,
+                  void* stream);
+/* out (batch, S, heads, dim; contiguous): x turned as the keys are. */
+int tt_kv8_rotate(const void* x, int type, long long stride_b, long long stride_s, long long stride_h,
+                  const int* lengths, const float* inv_freq, int pairs, int interleaved, void* out,
+                  int batch, int S, int heads, int dim, void* stream);
+/* k, v (count, heads, page, dim; contiguous) = the pages page_ids (NULL: the
+ * first `count`) as values. */
+int tt_kv8_read(const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
+                const int* page_ids, int count, void* k, void* v, int type, int* status, int pages,
+                int heads, int page, int dim, void* stream);
+/* out (batch, S, heads_q, dim; contiguous) = softmax(scale q K^T) V over the
+ * first lengths[b] tokens of each sequence; head h of q reads kv head
+ * h / (heads_q / heads). Causal: query i < n_query[b] (NULL: S) stands at
+ * position lengths[b] - n_query[b] + i and sees what is not behind it. Rows
+ * that see nothing, and those from n_query[b] on, are zero. q and its strides
+ * are 16-byte aligned; scale is one host float, read during the call. Workspace
+ * for the current device: */
+size_t tt_kv8_attention_workspace_bytes(int dim);
+int tt_kv8_attention(const void* q, int type, long long q_stride_b, long long q_stride_s,
+                     long long q_stride_h, const void* k_codes, const void* v_codes,
+                     const float* k_scales, const float* v_scales, const int* block_table,
+                     long long table_stride, int columns, const int* lengths, const int* n_query,
+                     const float* scale, int causal, void* out, void* workspace, size_t workspace_bytes,
+                     int* status, int batch, int S, int heads_q, int heads, int dim, int page,
+                     int pages, void* stream);
+
 /* Failure-detection check (no counterpart in the reference): one thread waits,
  * through the same bounded mbarrier wait every kernel here uses, on a phase
  * that nothing completes. After budget_cycles (at most the kernels' own

@@ -6,7 +6,8 @@ Drop-in for the trnsci/trntensor 0.4.0 public namespace
 (int8 Ozaki-split ``tcgen05.mma`` with exact int32 accumulation, for fp32
 and for fp64) through the C ABI in ``include/trntensor_b200.h``;
 ``einsum``/``multi_einsum``/planning stay host Python. ``einsum`` also takes
-a matrix held in 4 bits (``quantize_q4``). The tensor
+a matrix held in 4 bits (``quantize_q4``), and ``kv_attention`` contracts
+queries with a paged cache held in 8 bits (``KVCache8``). The tensor
 decompositions are outside this build and raise ``NotImplementedError``.
 """
 
@@ -22,6 +23,7 @@ from .decompose import (
 )
 from .dispatch import HAS_NKI, from_xla, get_backend, set_backend, to_xla
 from .einsum import einsum, multi_einsum
+from .kv_cache import KVCache8, kv_append, kv_attention, kv_rotate
 from .plan import (
     ContractionPlan,
     clear_plan_cache,
@@ -66,4 +68,8 @@ __all__ = [
     "quantize_q4",
     "pack_q4",
     "q4_matmul",
+    "KVCache8",
+    "kv_append",
+    "kv_attention",
+    "kv_rotate",
 ]

@@ -63,6 +63,13 @@ SIGNATURES: dict[str, tuple] = {
     "tt_debug_wait_timeout": (_I, [_P, _LL, _P, _P]),
     "tt_gemm_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "tt_gemm_f32": (_I, [_P, _I, _LL, _P, _I, _LL, _P, _LL, _I, _I, _I, _I, _P, _SZ, _P, _P]),
+    "tt_kv8_append": (_I, [_P, _P, _I, _LL, _LL, _LL, _LL, _LL, _LL, _P, _LL, _I, _P, _P, _P, _I, _I,
+                           _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
+    "tt_kv8_rotate": (_I, [_P, _I, _LL, _LL, _LL, _P, _P, _I, _I, _P, _I, _I, _I, _I, _P]),
+    "tt_kv8_read": (_I, [_P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I, _I, _P]),
+    "tt_kv8_attention_workspace_bytes": (_SZ, [_I]),
+    "tt_kv8_attention": (_I, [_P, _I, _LL, _LL, _LL, _P, _P, _P, _P, _P, _LL, _I, _P, _P, _P, _I, _P, _P,
+                              _SZ, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
     "tt_q4_packed_bytes": (_SZ, [_I, _I]),
     "tt_q4_scale_count": (_SZ, [_I, _I, _I]),
     "tt_q4_pack": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),

@@ -1,0 +1,127 @@
+// Attention over a paged 8-bit cache: launches (csrc/kv8_attn.cuh).
+#include "common.cuh"
+#include "kv8_attn.cuh"
+
+namespace tt {
+namespace kv8 {
+namespace {
+
+std::once_flag g_flags[kMaxDevices];
+int g_ok[kMaxDevices];
+int g_sms[kMaxDevices];
+
+template <typename T, int DP>
+int set_attr() {
+  constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+  return cudaFuncSetAttribute(attend_kernel<T, DP, kTerms>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Shape<DP, kTerms>::kSmem) == cudaSuccess
+             ? TT_OK
+             : TT_ERR_CUDA;
+}
+template <typename T>
+int set_attrs() {
+  int st = set_attr<T, 64>();
+  if (st == TT_OK) st = set_attr<T, 128>();
+  if (st == TT_OK) st = set_attr<T, 192>();
+  if (st == TT_OK) st = set_attr<T, 256>();
+  return st;
+}
+
+int setup(int dev) {
+  return once_per_device(g_flags, g_ok, dev, [dev]() -> int {
+    if (cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return TT_ERR_CUDA;
+    int st = set_attrs<float>();
+    if (st == TT_OK) st = set_attrs<__nv_bfloat16>();
+    if (st == TT_OK) st = set_attrs<__half>();
+    return st;
+  });
+}
+
+// Warps of the grid: one CTA an SM.
+int warps_of(int dim, int sms) { return sms * (dim <= 128 ? 8 : 4); }
+
+size_t workspace_bytes(int dim, int sms) {
+  const size_t warps = warps_of(dim, sms);
+  return warps * 16 + warps * 2 * 16 * (dim + 2) * 4;
+}
+
+template <typename T, int DP>
+int launch(const Attend& p, int sms, cudaStream_t s) {
+  constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+  using S = Shape<DP, kTerms>;
+  attend_kernel<T, DP, kTerms><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+  int st = cuda_status(cudaGetLastError());
+  if (st != TT_OK) return st;
+  join_kernel<T><<<p.warps, 256, 0, s>>>(p);
+  return cuda_status(cudaGetLastError());
+}
+template <typename T>
+int launch_dim(const Attend& p, int sms, cudaStream_t s) {
+  if (p.dim <= 64) return launch<T, 64>(p, sms, s);
+  if (p.dim <= 128) return launch<T, 128>(p, sms, s);
+  if (p.dim <= 192) return launch<T, 192>(p, sms, s);
+  return launch<T, 256>(p, sms, s);
+}
+
+}  // namespace
+}  // namespace kv8
+}  // namespace tt
+
+extern "C" {
+
+size_t tt_kv8_attention_workspace_bytes(int dim) {
+  using namespace tt;
+  int dev = 0;
+  if (dim < 16 || dim > 256 || dim % 16 || check_device(&dev) != TT_OK || kv8::setup(dev) != TT_OK) return 0;
+  return kv8::workspace_bytes(dim, kv8::g_sms[dev]);
+}
+
+int tt_kv8_attention(const void* q, int type, long long q_stride_b, long long q_stride_s, long long q_stride_h,
+                     const void* k_codes, const void* v_codes, const float* k_scales, const float* v_scales,
+                     const int* block_table, long long table_stride, int columns, const int* lengths,
+                     const int* n_query, const float* scale, int causal, void* out, void* workspace,
+                     size_t workspace_bytes, int* status, int batch, int S, int heads_q, int heads, int dim,
+                     int page, int pages, void* stream) {
+  using namespace tt;
+  if (!q || !k_codes || !v_codes || !k_scales || !v_scales || !block_table || !lengths || !scale || !out ||
+      !workspace || !status)
+    return TT_ERR_NULL;
+  if (batch <= 0 || S <= 0 || columns <= 0 || heads <= 0 || heads_q <= 0 || heads_q % heads) return TT_ERR_SHAPE;
+  if (type < 0 || type > 2 || pages <= 0 || dim < 16 || dim > 256 || dim % 16) return TT_ERR_SHAPE;
+  if (page != 16 && page != 32 && page != 64 && page != 128) return TT_ERR_SHAPE;
+  const long long rows = (long long)S * (heads_q / heads);
+  if (rows > 0x7fffff00LL || (long long)columns * page > 0x7fffff00LL) return TT_ERR_SHAPE;
+  const int per = type == q4::kF32 ? 4 : 8;  // values in 16 bytes
+  if (!aligned16(q) || !aligned16(out) || !aligned16(k_codes) || !aligned16(v_codes) || !aligned16(workspace) ||
+      q_stride_b % per || q_stride_s % per || q_stride_h % per)
+    return TT_ERR_ALIGN;
+  int dev = 0;
+  int st = check_device(&dev);
+  if (st != TT_OK) return st;
+  if ((st = kv8::setup(dev)) != TT_OK) return st;
+  const int sms = kv8::g_sms[dev];
+  if (workspace_bytes < kv8::workspace_bytes(dim, sms)) return TT_ERR_WORKSPACE;
+  kv8::Attend p;
+  p.q = q; p.q_b = q_stride_b; p.q_s = q_stride_s; p.q_h = q_stride_h;
+  p.o = out;
+  p.kc = (const unsigned char*)k_codes; p.vc = (const unsigned char*)v_codes;
+  p.ks = k_scales; p.vs = v_scales;
+  p.table = block_table; p.table_b = table_stride; p.lengths = lengths; p.n_query = n_query;
+  p.warps = kv8::warps_of(dim, sms);
+  p.meta = (int4*)workspace;
+  p.part = (float*)((char*)workspace + (size_t)p.warps * 16);
+  p.status = status;
+  p.scale = *scale * 1.4426950408889634f;
+  p.causal = causal;
+  p.batch = batch; p.S = S; p.heads_q = heads_q; p.heads = heads; p.dim = dim; p.page = page; p.pages = pages;
+  p.cols = columns;
+  p.rows = (int)rows;
+  p.tiles = (int)((rows + 15) / 16);
+  cudaStream_t s = (cudaStream_t)stream;
+  if (type == q4::kF32) return kv8::launch_dim<float>(p, sms, s);
+  if (type == q4::kBF16) return kv8::launch_dim<__nv_bfloat16>(p, sms, s);
+  return kv8::launch_dim<__half>(p, sms, s);
+}
+
+}  // extern "C"

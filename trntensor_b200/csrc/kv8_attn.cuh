@@ -1,0 +1,653 @@
+// Attention of few query rows over a paged 8-bit cache (csrc/kv8.cuh).
+//
+//   o = sum_t softmax_t(scale q.K^[t]) V^[t],  K^[t] = sk[page,h] ck[t]
+//
+// Two contractions with a softmax between; the scores stay in registers. A
+// kv head's query rows (tokens x heads of its group) make tiles of 16, and the
+// work is cut into chunks of 64 tokens of one tile. The chunks of all
+// sequences, heads and tiles form one line, of which every warp takes an equal
+// piece, so that ragged lengths and a lone long sequence both fill the GPU; a
+// tile whose chunks lie with several warps is joined by a second small kernel,
+// always in the same order.
+//
+// What bounds it: the cache's bytes. Each warp keeps its own ring of shared
+// memory slots (one unit quartet of keys or of values each) filled by bulk
+// copies two to three slots ahead, across tile borders. Tensor-core operands:
+// the codes are exact in fp16; a row of q is scaled by a power of two to below
+// 2^14 and rounded to fp16 (exact for 16-bit types down to 2^-27 of the row's
+// largest value, 2^-39 of that below) or, for fp32, kept as two fp16 terms.
+// The softmax weights are fp16 (2^-12, below the rounding of a bf16 result and
+// at that of an fp16 one; again held up by 2^14), two terms for fp32. Page
+// scales multiply scores and weights in fp32; weights are held relative to the
+// largest value scale seen.
+//
+// Order of tokens in a chunk: lane 4 g + t of a fragment owns unit t's sixteen
+// tokens as score columns (tile j, column 2 t + e: token 16 t + 2 j + e), which
+// is also how a lane reads sixteen tokens of a value row at once.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "kv8.cuh"
+#include "ptx.cuh"
+#include "q4.cuh"
+
+namespace tt {
+namespace kv8 {
+
+constexpr int kChunk = 64;
+constexpr float kUp = 16384.f;  // the largest fp16 weight of a chunk
+
+struct Attend {
+  const void* q;
+  long long q_b, q_s, q_h;
+  void* o;  // (batch, S, heads_q, dim) contiguous
+  const unsigned char* kc;
+  const unsigned char* vc;
+  const float* ks;
+  const float* vs;
+  const int* table;
+  long long table_b;
+  const int* lengths;
+  const int* n_query;  // nullable: S
+  float* part;         // partial sums: [warp][2][16][2 + dim] (maximum, sum, values)
+  int4* meta;          // [warp]: (b, h * tiles + tile, last warp, 1) of a tile that others finish
+  int* status;
+  float scale;  // times log2(e)
+  int causal;
+  int batch, S, heads_q, heads, dim, page, pages, cols, rows, tiles;
+  int warps;  // of the whole grid
+};
+
+template <int DP, int kTerms>
+struct Shape {
+  static constexpr bool kQRegs = DP <= 128 && kTerms == 1;
+  static constexpr int kWarps = DP <= 128 ? 8 : 4;
+  static constexpr int kUnit = 16 * DP;
+  static constexpr int kSlot = 4 * (kUnit + 32);
+  static constexpr int kSlots = DP == 64 ? 5 : DP == 192 ? 3 : kTerms == 1 ? 3 : 2;
+  static constexpr int kQBytes = kQRegs ? 0 : kTerms * 16 * DP * 2;
+  static constexpr int kSmem = kWarps * (kSlots * kSlot + kQBytes);
+  static_assert(kSmem + 1024 <= 227 * 1024, "shared memory of an SM");
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+// Bounded wait: false when the copy has not arrived within the budget.
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_drain(bar, parity);
+}
+// Sixteen neighbouring values, 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load16(const T* at, float (&x)[16]) {
+  constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 16 / kPer; ++i) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + i);
+    const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[i * kPer + j] = q4::to_f(e[j]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store2(T* at, float a, float b) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float2*>(at) = make_float2(a, b);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    *reinterpret_cast<uint32_t*>(at) = q4::pack_f16(a, b);
+  } else {
+    *reinterpret_cast<uint32_t*>(at) = q4::pack_bf16(a, b);
+  }
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+// Four biased codes as two fp16 pairs.
+__device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 ra = __hsub2(reinterpret_cast<const __half2&>(a), bias);
+  const __half2 rb = __hsub2(reinterpret_cast<const __half2&>(b), bias);
+  lo = reinterpret_cast<const uint32_t&>(ra);
+  hi = reinterpret_cast<const uint32_t&>(rb);
+}
+// Two floats (below 65504) as kTerms fp16 pairs.
+template <int kTerms>
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t (&out)[kTerms]) {
+#pragma unroll
+  for (int i = 0; i < kTerms; ++i) {
+    const __half2 v = __floats2half2_rn(a, b);
+    out[i] = reinterpret_cast<const uint32_t&>(v);
+    a -= __low2float(v);
+    b -= __high2float(v);
+  }
+}
+
+__device__ __forceinline__ long long clamp_length(const Attend& p, int b, bool report) {
+  long long n = p.lengths[b];
+  const long long most = (long long)p.cols * p.page;
+  if (n < 0 || n > most) {
+    if (report) raise(p.status, kBadLength);
+    n = n < 0 ? 0 : most;
+  }
+  return n;
+}
+__device__ __forceinline__ int clamp_count(const Attend& p, int b, bool report) {
+  int n = p.n_query ? p.n_query[b] : p.S;
+  if (n < 0 || n > p.S) {
+    if (report) raise(p.status, kBadLength);
+    n = n < 0 ? 0 : p.S;
+  }
+  return n;
+}
+__device__ __forceinline__ long long chunks_of(long long n) { return (n + kChunk - 1) / kChunk; }
+
+// Chunks of the sequences before `b_end`, summed by a warp.
+__device__ __forceinline__ long long chunk_sum(const Attend& p, int b_end, int lane) {
+  long long s = 0;
+  for (int b = lane; b < b_end; b += 32) s += chunks_of(clamp_length(p, b, false));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s * p.heads * p.tiles;
+}
+
+// A place in the line of chunks.
+struct Place {
+  int b, h, tile;
+  long long length;
+  int chunk, chunks;
+};
+
+__device__ __forceinline__ void next_sequence(const Attend& p, Place& x) {
+  x.h = x.tile = x.chunk = 0;
+  do {
+    ++x.b;
+    x.length = x.b < p.batch ? clamp_length(p, x.b, false) : 0;
+  } while (x.b < p.batch && x.length == 0);
+  x.chunks = (int)chunks_of(x.length);
+}
+__device__ __forceinline__ void advance(const Attend& p, Place& x) {
+  if (++x.chunk < x.chunks) return;
+  x.chunk = 0;
+  if (++x.tile < p.tiles) return;
+  x.tile = 0;
+  if (++x.h < p.heads) return;
+  next_sequence(p, x);
+}
+
+template <typename T, int DP, int kTerms>
+__global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kernel(const Attend p) {
+  using S = Shape<DP, kTerms>;
+  using q4::from_f;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint64_t bars[S::kWarps * S::kSlots];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int worker = warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
+  unsigned char* mine = smem + warp * S::kSlots * S::kSlot;
+  uint64_t* bar = bars + warp * S::kSlots;
+  const int dim = p.dim;
+  const uint32_t unit_bytes = 16 * dim;
+
+  if (lane < S::kSlots) mbar_init(bar + lane, 1);
+  fence_mbar_init();
+  __syncwarp();
+
+  // sequences without a token, and what is wrong with the lengths
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    const long long n = clamp_length(p, b, threadIdx.x == 0);
+    if (threadIdx.x == 0) clamp_count(p, b, true);
+    if (n == 0) {
+      const long long all = (long long)p.S * p.heads_q * dim;
+      for (long long i = threadIdx.x; i < all; i += blockDim.x)
+        static_cast<T*>(p.o)[b * all + i] = from_f<T>(0.f);
+    }
+  }
+  if (lane == 0) p.meta[worker] = make_int4(0, 0, 0, 0);
+
+  // this warp's piece of the line
+  const long long total = chunk_sum(p, p.batch, lane);
+  const long long workers = min((long long)p.warps, total);  // each has a chunk at least
+  if (worker >= workers) return;
+  const long long begin = total * worker / workers, end = total * (worker + 1) / workers;
+  Place at;
+  {
+    // the last sequence that starts at or before `begin`
+    long long before = 0;
+    int found = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 32) {
+      const int b = b0 + lane;
+      const long long c = b < p.batch ? chunks_of(clamp_length(p, b, false)) * p.heads * p.tiles : 0;
+      long long sum = c;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      const unsigned in = __ballot_sync(0xffffffffu, before + sum > begin);
+      if (in) {
+        const int first = __ffs(in) - 1;
+        before += __shfl_sync(0xffffffffu, sum - c, first);
+        found = b0 + first;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    at.b = found;
+    at.length = clamp_length(p, found, false);
+    at.chunks = (int)chunks_of(at.length);
+    const long long in = begin - before;
+    at.chunk = (int)(in % at.chunks);
+    at.tile = (int)(in / at.chunks % p.tiles);
+    at.h = (int)(in / at.chunks / p.tiles);
+  }
+
+  // ---- copies: lane t (t < 4 of the warp) stands for unit t of a chunk
+  Place ahead = at;              // the chunk whose keys are asked for next
+  long long left = end - begin;  // chunks not yet asked for
+  // page of this lane's unit of a place; -1 behind the sequence's end
+  auto page_at = [&](const Place& x) -> int {
+    const long long tok = (long long)x.chunk * kChunk + 16 * t;
+    if (tok >= x.length) return -1;
+    const int page = p.table[x.b * p.table_b + tok / p.page];
+    if (page < 0 || page >= p.pages) {
+      if (g == 0) raise(p.status, kBadPage);
+      return -1;
+    }
+    return page;
+  };
+  auto offset_of = [&](const Place& x, int page) -> long long {
+    const long long tok = (long long)x.chunk * kChunk + 16 * t;
+    return (((long long)page * p.heads + x.h) * p.page + tok % p.page) * dim;
+  };
+  uint32_t slot_in = 0;
+  auto ask = [&](const unsigned char* codes, int page, long long offset) {
+    const unsigned has = __ballot_sync(0xffffffffu, page >= 0) & 15u;
+    uint64_t* b = bar + slot_in;
+    if (lane == 0) mbar_arrive_expect_tx(b, __popc(has) * unit_bytes);
+    __syncwarp();
+    if (lane < 4 && page >= 0)
+      bulk_load(smem_u32(mine + slot_in * S::kSlot + t * (S::kUnit + 32)), codes + offset, unit_bytes, smem_u32(b));
+    slot_in = slot_in + 1 == S::kSlots ? 0 : slot_in + 1;
+  };
+
+  // Copies are asked for in the order K0 V0 K1 V1 ..., always kSlots ahead.
+  // page_k is the page of the chunk whose keys come next, page_v and off_v of
+  // the one whose keys were asked for last.
+  int page_k = page_at(ahead), page_v = -1;
+  long long off_v = 0;
+  bool want_values = false;  // the next copy is of values
+  int asked = 0;             // chunks whose keys are asked for and not consumed, and their scales
+  float fsk[3] = {0.f, 0.f, 0.f}, fsv[3] = {0.f, 0.f, 0.f};
+  auto ask_next = [&]() {
+    if (want_values) {
+      ask(p.vc, page_v, off_v);
+      want_values = false;
+      return;
+    }
+    if (left == 0) return;
+    --left;
+    page_v = page_k;
+    off_v = page_k >= 0 ? offset_of(ahead, page_k) : 0;
+    const long long at_scale = (long long)page_k * p.heads + ahead.h;
+    const float nsk = page_k >= 0 ? p.ks[at_scale] : 0.f, nsv = page_k >= 0 ? p.vs[at_scale] : 0.f;
+    if (asked == 0) { fsk[0] = nsk; fsv[0] = nsv; }
+    else if (asked == 1) { fsk[1] = nsk; fsv[1] = nsv; }
+    else { fsk[2] = nsk; fsv[2] = nsv; }
+    ++asked;
+    ask(p.kc, page_k, off_v);
+    want_values = true;
+    if (left > 0) {
+      advance(p, ahead);
+      page_k = page_at(ahead);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < S::kSlots; ++i) ask_next();
+
+  uint32_t slot = 0, parity = 0;
+  bool alive = true;
+  auto arrive = [&]() {
+    alive = __all_sync(0xffffffffu, wait_full(bar + slot, parity));
+    if (!alive) {  // give up, but not before the other copies are in or the wait for them is over
+      if (lane == 0) raise(p.status, kTimeout);
+      for (uint32_t i = 0; i < S::kSlots; ++i) mbar_wait_drain(bar + i, i < slot ? parity ^ 1 : parity);
+    }
+  };
+  auto release = [&]() {  // this slot's reads are done: the next copy goes into it
+    fence_proxy_async_smem();
+    __syncwarp();
+    ask_next();
+    slot = slot + 1 == S::kSlots ? 0 : slot + 1;
+    if (slot == 0) parity ^= 1;
+  };
+
+  const int group = p.heads_q / p.heads;
+  float acc[DP / 8][4];
+  uint32_t qf[S::kQRegs ? DP / 16 : 1][4];
+  unsigned char* qs = smem + S::kWarps * S::kSlots * S::kSlot + warp * S::kQBytes;  // [step][term][lane][4]
+  float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f, top_v = 0.f, qs0 = 0.f, qs1 = 0.f;
+  long long lim0 = 0, lim1 = 0, lim_min = 0;
+  bool fresh = true, whole = true;
+
+  for (long long i = begin; i < end; ++i) {
+    if (fresh) {  // a tile begins: its queries
+      fresh = false;
+      whole = at.chunk == 0;
+      const int count = clamp_count(p, at.b, false);
+      float top[2], x[2][DP / 64][16];
+      long long lim[2];
+      bool has[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = at.tile * 16 + g + 8 * h;
+        const int tok = r / group, head = at.h * group + r % group;
+        has[h] = r < p.rows && tok < count;
+        const T* row = static_cast<const T*>(p.q) + at.b * p.q_b + (has[h] ? tok * p.q_s + head * p.q_h : 0);
+        lim[h] = !has[h] ? 0 : p.causal ? at.length - count + tok + 1 : at.length;
+        if (lim[h] < 0) lim[h] = 0;
+        float m = 0.f;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          const int d = 16 * (t + 4 * c);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[h][c][e] = 0.f;
+          if (has[h] && d < dim) load16(row + d, x[h][c]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[h][c][e]));
+        }
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        top[h] = m;
+      }
+      // a row's power of two: its largest value comes to 2^13 .. 2^14
+      float up[2], down[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int ex = (int)((__float_as_uint(top[h]) >> 23) & 255);
+        ex = ex < 14 ? 14 : ex;  // up = 2^(140 - ex), down = 1 / up
+        up[h] = __uint_as_float((uint32_t)(267 - ex) << 23);
+        down[h] = __uint_as_float((uint32_t)(ex - 13) << 23);
+      }
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t f[4][kTerms];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* y = x[h][c] + 4 * w;
+            split_f16<kTerms>(y[0] * up[h], y[1] * up[h], f[h]);
+            split_f16<kTerms>(y[2] * up[h], y[3] * up[h], f[2 + h]);
+          }
+          const int step = c * 4 + w;
+          if constexpr (S::kQRegs) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) qf[step][r] = f[r][0];
+          } else {
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k)
+              *reinterpret_cast<uint4*>(qs + ((step * kTerms + k) * 32 + lane) * 16) =
+                  make_uint4(f[0][k], f[1][k], f[2][k], f[3][k]);
+          }
+        }
+      qs0 = down[0] * p.scale;
+      qs1 = down[1] * p.scale;
+      lim0 = lim[0];
+      lim1 = lim[1];
+      lim_min = min(has[0] ? lim0 : at.length, has[1] ? lim1 : at.length);
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
+      m0 = m1 = -INFINITY;
+      l0 = l1 = top_v = 0.f;
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+    }
+
+    // scores: 16 rows x 64 tokens
+    float s[8][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+    arrive();
+    if (!alive) return;
+    {
+      const uint32_t keys = smem_u32(mine + slot * S::kSlot) + (g >> 1) * (S::kUnit + 32) + (g & 1) * dim + t * 16;
+#pragma unroll
+      for (int c = 0; c < DP / 64; ++c) {
+        uint32_t qa[4][kTerms][4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) {
+            if constexpr (S::kQRegs) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) qa[w][k][r] = qf[c * 4 + w][r];
+            } else {
+              const uint4 v = *reinterpret_cast<const uint4*>(qs + (((c * 4 + w) * kTerms + k) * 32 + lane) * 16);
+              qa[w][k][0] = v.x; qa[w][k][1] = v.y; qa[w][k][2] = v.z; qa[w][k][3] = v.w;
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint4 v = lds128(keys + 2 * j * dim + c * 64);
+          const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            uint32_t lo, hi;
+            decode4(word[w], lo, hi);
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k)
+              q4::mma16816<true>(s[j], qa[w][k][0], qa[w][k][1], qa[w][k][2], qa[w][k][3], lo, hi);
+          }
+        }
+      }
+    }
+    const float sk = fsk[0], sv = fsv[0];
+    // the ring of scales moves on before the next chunk is asked for
+    fsk[0] = fsk[1]; fsk[1] = fsk[2];
+    fsv[0] = fsv[1]; fsv[1] = fsv[2];
+    --asked;
+    release();
+
+    const float f0 = qs0 * sk, f1 = qs1 * sk;
+    const long long tok0 = (long long)at.chunk * kChunk + 16 * t;
+    const bool mask = (long long)(at.chunk + 1) * kChunk > lim_min;
+    float n0 = m0, n1 = m1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[j][e] *= f0;
+        s[j][2 + e] *= f1;
+        if (mask) {
+          if (tok0 + 2 * j + e >= lim0) s[j][e] = -INFINITY;
+          if (tok0 + 2 * j + e >= lim1) s[j][2 + e] = -INFINITY;
+        }
+        n0 = fmaxf(n0, s[j][e]);
+        n1 = fmaxf(n1, s[j][2 + e]);
+      }
+    }
+    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
+    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
+    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
+    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+    // largest value scale so far; a NaN stays in its own page's weights
+    float nv = fmaxf(top_v, sv);
+    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 1));
+    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 2));
+    nv = fmaxf(nv, 1e-30f);
+    const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+    const float old0 = exp2_approx(m0 - z0), old1 = exp2_approx(m1 - z1);
+    const float shrink = __fdividef(top_v, nv), rel = __fdividef(sv, nv) * kUp;
+    l0 *= old0;
+    l1 *= old1;
+    const float a0 = old0 * shrink, a1 = old1 * shrink;
+    if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) {
+        acc[n][0] *= a0;
+        acc[n][1] *= a0;
+        acc[n][2] *= a1;
+        acc[n][3] *= a1;
+      }
+    }
+    m0 = n0;
+    m1 = n1;
+    top_v = nv;
+    // a NaN scale reaches no row that its page is hidden from
+    const bool odd = mask && rel != rel;
+    uint32_t w[4][4][kTerms];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float* x = s[2 * kk + half];
+        x[0] = exp2_approx(x[0] - z0);
+        x[1] = exp2_approx(x[1] - z0);
+        x[2] = exp2_approx(x[2] - z1);
+        x[3] = exp2_approx(x[3] - z1);
+        l0 += x[0] + x[1];
+        l1 += x[2] + x[3];
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = odd && x[e] == 0.f ? 0.f : x[e] * rel;
+        split_f16<kTerms>(y[0], y[1], w[kk][2 * half]);
+        split_f16<kTerms>(y[2], y[3], w[kk][2 * half + 1]);
+      }
+    arrive();
+    if (!alive) return;
+    {
+      const uint32_t vals = smem_u32(mine + slot * S::kSlot) + t * (S::kUnit + 32) + g * 16;
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) {
+        const uint4 v = lds128(vals + n * 128);
+        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          uint32_t lo, hi;
+          decode4(word[kk], lo, hi);
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k)
+            q4::mma16816<true>(acc[n], w[kk][0][k], w[kk][1][k], w[kk][2][k], w[kk][3][k], lo, hi);
+        }
+      }
+    }
+    release();
+
+    const bool last = at.chunk + 1 == at.chunks;
+    if (last || i + 1 == end) {  // the tile's sums leave the warp
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = at.tile * 16 + g + 8 * h;
+        const bool none = (h ? lim1 : lim0) == 0;  // a row that sees nothing
+        const float l = none ? 0.f : h ? l1 : l0;
+        if (r < p.rows) {
+          if (whole && last) {
+            const float inv = l > 0.f || l != l ? top_v / (l * kUp) : 0.f;
+            T* o = static_cast<T*>(p.o) +
+                   (((long long)at.b * p.S + r / group) * p.heads_q + at.h * group + r % group) * dim;
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+              const int d = n * 8 + 2 * t;
+              if (d < dim) store2(o + d, none ? 0.f : acc[n][2 * h] * inv, none ? 0.f : acc[n][2 * h + 1] * inv);
+            }
+          } else {
+            // second half of a tile that began before this piece, or first of one that goes on
+            const float back = top_v / kUp;
+            float* out = p.part + (((long long)worker * 2 + (whole ? 1 : 0)) * 16 + g + 8 * h) * (dim + 2);
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n) {
+              const int d = n * 8 + 2 * t;
+              if (d < dim)
+                *reinterpret_cast<float2*>(out + 2 + d) =
+                    make_float2(none ? 0.f : acc[n][2 * h] * back, none ? 0.f : acc[n][2 * h + 1] * back);
+            }
+            if (t == 0) *reinterpret_cast<float2*>(out) = make_float2(none ? -INFINITY : h ? m1 : m0, l);
+          }
+        }
+      }
+      if (whole && !last && lane == 0) {  // those after this warp have the rest
+        const long long c1 = i + (at.chunks - 1 - at.chunk);
+        p.meta[worker] = make_int4(at.b, at.h * p.tiles + at.tile, (int)(((c1 + 1) * workers - 1) / total), 1);
+      }
+      fresh = true;
+    }
+    if (i + 1 < end) advance(p, at);
+  }
+}
+
+// Joins the pieces of the tiles that several warps had: one CTA for each warp
+// that began such a tile; its warps share the pieces, row by row.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const Attend p) {
+  using q4::from_f;
+  __shared__ float sum[8][256];
+  __shared__ float mx[8], ls[8];
+  const int w0 = blockIdx.x;
+  const int4 meta = p.meta[w0];
+  if (meta.w == 0) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int b = meta.x, h = meta.y / p.tiles, tile = meta.y % p.tiles, w1 = meta.z;
+  const int group = p.heads_q / p.heads, dim = p.dim;
+  for (int r = tile * 16; r < min(p.rows, tile * 16 + 16); ++r) {
+    float m = -INFINITY, l = 0.f, a[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = 0.f;
+    for (int w = w0 + warp; w <= w1; w += 8) {
+      const float* in = p.part + (((long long)w * 2 + (w == w0 ? 1 : 0)) * 16 + r % 16) * (dim + 2);
+      const float mi = in[0], li = in[1];
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = lane + 32 * e < dim ? in[2 + lane + 32 * e] : 0.f;
+      const float n = fmaxf(m, mi), z = n == -INFINITY ? 0.f : n;
+      const float fa = exp2_approx(m - z), fb = exp2_approx(mi - z);
+      l = l * fa + li * fb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = a[e] * fa + x[e] * fb;
+      m = n;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[warp][lane + 32 * e] = a[e];
+    if (lane == 0) {
+      mx[warp] = m;
+      ls[warp] = l;
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int w = 0; w < 8; ++w) top = fmaxf(top, mx[w]);
+    if (top == -INFINITY) top = 0.f;
+    float den = 0.f;
+    for (int w = 0; w < 8; ++w) den += ls[w] * exp2_approx(mx[w] - top);
+    const float inv = den > 0.f || den != den ? 1.f / den : 0.f;
+    T* o = static_cast<T*>(p.o) + (((long long)b * p.S + r / group) * p.heads_q + h * group + r % group) * dim;
+    for (int d = threadIdx.x; d < dim; d += blockDim.x) {
+      float v = 0.f;
+      for (int w = 0; w < 8; ++w) v += sum[w][d] * exp2_approx(mx[w] - top);
+      o[d] = from_f<T>(v * inv);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace kv8
+}  // namespace tt
