@@ -326,15 +326,24 @@ int tt_q4_quantize(const void* W, int type, long long ldw, int scale_type, int N
 /* out (N, K) contiguous = s c, rounded once. */
 int tt_q4_dequantize(const void* packed, const void* packed_scales, int scale_type, int N, int K,
                      int group, void* out, int type, void* stream);
+/* row_scale (N fp32): the power of two by which each row's scales are brought
+ * into fp16's range in products of more than 16 rows. */
+int tt_q4_row_scale(const void* packed_scales, int scale_type, int N, int K, int group,
+                    float* row_scale, void* stream);
+/* Bytes of workspace for a product (0 up to 16 rows, where it may be NULL). */
+size_t tt_q4_matmul_workspace_bytes(int type, int scale_type, int transposed, int M, int N, int K);
 /* y (M, N; row stride ldy) = x (M, K; row stride ldx) W^T: fp32 sums, rounded
- * once to x's type. */
+ * once to x's type. dev_status as in the file's head; unlike other calls these
+ * do not clear it. */
 int tt_q4_matmul(const void* x, int type, long long ldx, const void* packed,
-                 const void* packed_scales, int scale_type, int M, int N, int K, int group, void* y,
-                 long long ldy, void* stream);
+                 const void* packed_scales, int scale_type, const float* row_scale, int M, int N,
+                 int K, int group, void* y, long long ldy, void* workspace, size_t workspace_bytes,
+                 int* dev_status, void* stream);
 /* dx (M, K; row stride lddx) = dy (M, N; row stride lddy) W. */
 int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed,
-                   const void* packed_scales, int scale_type, int M, int N, int K, int group,
-                   void* dx, long long lddx, void* stream);
+                   const void* packed_scales, int scale_type, const float* row_scale, int M, int N,
+                   int K, int group, void* dx, long long lddx, void* workspace,
+                   size_t workspace_bytes, int* dev_status, void* stream);
 
 /*
  * Paged key-value cache held in 8 bits: x^ = s c, c in -127..127 stored biased

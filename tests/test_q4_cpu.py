@@ -108,14 +108,19 @@ def test_library_refuses_bad_arguments():
     """Argument checks of the C ABI come before any CUDA call."""
     lib = _lib.load()
     p = 16  # never dereferenced: a shape or NULL check answers first
-    assert lib.tt_q4_matmul(None, 0, 8, p, p, 0, 1, 8, 8, 32, p, 8, None) == _lib.TT_ERR_NULL
+    assert lib.tt_q4_matmul(None, 0, 8, p, p, 0, p, 1, 8, 8, 32, p, 8, None, 0, p, None) == _lib.TT_ERR_NULL
+    # more than 16 rows need a workspace
+    assert lib.tt_q4_matmul_workspace_bytes(1, 1, 0, 16, 8, 8) == 0
+    assert lib.tt_q4_matmul_workspace_bytes(1, 1, 0, 17, 8, 8) >= 17 * (64 * 2 + 4)
+    assert lib.tt_q4_matmul(p, 0, 8, p, p, 0, p, 17, 8, 8, 32, p, 8, None, 0, p, None) == _lib.TT_ERR_NULL
+    assert lib.tt_q4_row_scale(p, 0, 8, 8, 33, p, None) == _lib.TT_ERR_SHAPE
     for bad in (dict(m=0), dict(n=0), dict(k=0), dict(group=16), dict(type=3), dict(st=2),
                 dict(ldx=7), dict(ldy=7)):
         a = dict(m=1, n=8, k=8, group=32, type=0, st=0, ldx=8, ldy=8) | bad
         for fn in (lib.tt_q4_matmul, lib.tt_q4_matmul_t):
-            assert fn(p, a["type"], a["ldx"], p, p, a["st"], a["m"], a["n"], a["k"], a["group"], p,
-                      a["ldy"], None) == _lib.TT_ERR_SHAPE, bad
-    assert lib.tt_q4_matmul(p, 0, 8, 8, p, 0, 1, 8, 8, 32, p, 8, None) == _lib.TT_ERR_ALIGN
+            assert fn(p, a["type"], a["ldx"], p, p, a["st"], p, a["m"], a["n"], a["k"], a["group"], p,
+                      a["ldy"], p, 0, p, None) == _lib.TT_ERR_SHAPE, bad
+    assert lib.tt_q4_matmul(p, 0, 8, 8, p, 0, p, 1, 8, 8, 32, p, 8, None, 0, p, None) == _lib.TT_ERR_ALIGN
     assert lib.tt_q4_quantize(p, 0, 7, 0, 8, 8, 32, p, p, None) == _lib.TT_ERR_SHAPE
     assert lib.tt_q4_pack(p, p, 2, 8, 8, 32, p, p, None) == _lib.TT_ERR_SHAPE
     assert lib.tt_q4_dequantize(p, p, 0, 8, 8, 33, p, 0, None) == _lib.TT_ERR_SHAPE

@@ -75,8 +75,10 @@ SIGNATURES: dict[str, tuple] = {
     "tt_q4_pack": (_I, [_P, _P, _I, _I, _I, _I, _P, _P, _P]),
     "tt_q4_quantize": (_I, [_P, _I, _LL, _I, _I, _I, _I, _P, _P, _P]),
     "tt_q4_dequantize": (_I, [_P, _P, _I, _I, _I, _I, _P, _I, _P]),
-    "tt_q4_matmul": (_I, [_P, _I, _LL, _P, _P, _I, _I, _I, _I, _I, _P, _LL, _P]),
-    "tt_q4_matmul_t": (_I, [_P, _I, _LL, _P, _P, _I, _I, _I, _I, _I, _P, _LL, _P]),
+    "tt_q4_row_scale": (_I, [_P, _I, _I, _I, _I, _P, _P]),
+    "tt_q4_matmul_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "tt_q4_matmul": (_I, [_P, _I, _LL, _P, _P, _I, _P, _I, _I, _I, _I, _P, _LL, _P, _SZ, _P, _P]),
+    "tt_q4_matmul_t": (_I, [_P, _I, _LL, _P, _P, _I, _P, _I, _I, _I, _I, _P, _LL, _P, _SZ, _P, _P]),
 }
 
 

@@ -13,6 +13,7 @@
 
 #include "common.cuh"
 #include "q4.cuh"
+#include "q4_host.cuh"
 
 namespace tt {
 namespace q4 {
@@ -22,6 +23,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;
+constexpr int kFewRows = 16;  // above, the products go to csrc/q4_gemm.cuh
 
 // ------------------------------------------------------- packing and decoding
 
@@ -469,14 +471,6 @@ int launch_cluster(F kernel, dim3 grid, int threads, int smem, int cluster, cuda
   return cuda_status(cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), args));
 }
 
-// tiles as (y, z) with y <= 65535; false when there are too many.
-bool grid_of(long long tiles, int splits, dim3* grid) {
-  const long long y = tiles < 65535 ? tiles : 65535, z = (tiles + y - 1) / y;
-  if (z > 65535) return false;
-  *grid = dim3((unsigned)splits, (unsigned)y, (unsigned)z);
-  return true;
-}
-
 // CTAs of a cluster: as many (a power of two) as leave each warp a block and
 // the GPU no more than about two CTAs an SM.
 int pick_splits(long long tiles, long long steps, int sms) {
@@ -568,9 +562,10 @@ int matmul_scaled(bool transposed, const void* x, long long ldx, const void* pac
 }
 
 int matmul(bool transposed, const void* x, int type, long long ldx, const void* packed,
-           const void* scales, int scale_type, int M, int N, int K, int group, void* y,
-           long long ldy, void* stream) {
-  if (!x || !packed || !scales || !y) return TT_ERR_NULL;
+           const void* scales, int scale_type, const float* row_scale, int M, int N, int K, int group,
+           void* y, long long ldy, void* workspace, size_t workspace_bytes, int* dev_status, void* stream) {
+  if (!x || !packed || !scales || !row_scale || !y || !dev_status) return TT_ERR_NULL;
+  if (M > kFewRows && !workspace) return TT_ERR_NULL;
   if (M <= 0 || N <= 0 || K <= 0 || !good_group(group)) return TT_ERR_SHAPE;
   if (type < 0 || type > 2 || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
   if (ldx < (transposed ? N : K) || ldy < (transposed ? K : N)) return TT_ERR_SHAPE;
@@ -581,6 +576,9 @@ int matmul(bool transposed, const void* x, int type, long long ldx, const void* 
   if ((st = setup(dev)) != TT_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
   const int sms = g_sms[dev];
+  if (M > kFewRows)
+    return run_gemm(transposed, x, type, ldx, packed, scales, scale_type, row_scale, M, N, K, group, y, ldy,
+                    workspace, workspace_bytes, dev_status, dev, s);
   if (type == kF32)
     return matmul_scaled<float>(transposed, x, ldx, packed, scales, scale_type, M, N, K, group, y, ldy, sms, s);
   if (type == kBF16)
@@ -693,14 +691,33 @@ int tt_q4_dequantize(const void* packed, const void* packed_scales, int scale_ty
                                 : q4::run_dequantize<__half, BF>(packed, packed_scales, N, K, group, out, s);
 }
 
+int tt_q4_row_scale(const void* packed_scales, int scale_type, int N, int K, int group, float* row_scale,
+                    void* stream) {
+  using namespace tt;
+  if (!packed_scales || !row_scale) return TT_ERR_NULL;
+  if (N <= 0 || K <= 0 || !q4::good_group(group) || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
+  int st = check_device(nullptr);
+  if (st != TT_OK) return st;
+  return q4::run_row_scale(packed_scales, scale_type, N, K, group, row_scale, (cudaStream_t)stream);
+}
+
+size_t tt_q4_matmul_workspace_bytes(int type, int scale_type, int transposed, int M, int N, int K) {
+  if (M <= tt::q4::kFewRows || N <= 0 || K <= 0 || type < 0 || type > 2) return 0;
+  return tt::q4::gemm_workspace_bytes(type, scale_type, transposed != 0, M, N, K);
+}
+
 int tt_q4_matmul(const void* x, int type, long long ldx, const void* packed, const void* packed_scales,
-                 int scale_type, int M, int N, int K, int group, void* y, long long ldy, void* stream) {
-  return tt::q4::matmul(false, x, type, ldx, packed, packed_scales, scale_type, M, N, K, group, y, ldy, stream);
+                 int scale_type, const float* row_scale, int M, int N, int K, int group, void* y, long long ldy,
+                 void* workspace, size_t workspace_bytes, int* dev_status, void* stream) {
+  return tt::q4::matmul(false, x, type, ldx, packed, packed_scales, scale_type, row_scale, M, N, K, group, y, ldy,
+                        workspace, workspace_bytes, dev_status, stream);
 }
 
 int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed, const void* packed_scales,
-                   int scale_type, int M, int N, int K, int group, void* dx, long long lddx, void* stream) {
-  return tt::q4::matmul(true, dy, type, lddy, packed, packed_scales, scale_type, M, N, K, group, dx, lddx, stream);
+                   int scale_type, const float* row_scale, int M, int N, int K, int group, void* dx,
+                   long long lddx, void* workspace, size_t workspace_bytes, int* dev_status, void* stream) {
+  return tt::q4::matmul(true, dy, type, lddy, packed, packed_scales, scale_type, row_scale, M, N, K, group, dx,
+                        lddx, workspace, workspace_bytes, dev_status, stream);
 }
 
 }  // extern "C"

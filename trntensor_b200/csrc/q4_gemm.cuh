@@ -1,0 +1,428 @@
+// Products of many rows with a 4-bit matrix on the fifth-generation tensor
+// cores (csrc/q4.cuh has the storage).
+//
+//   y[m,n]  = sum_k x[m,k] W^[n,k]        (rows of the tile: n, sum over k)
+//   dx[m,k] = sum_n dy[m,n] W^[n,k]       (kTrans: rows k, sum over n)
+//
+// tcgen05.mma with fp16 operands: the matrix is decoded on the way into shared
+// memory (operand A, 128 or 256 rows of a tile), the dense operand comes as
+// fp16 through TMA (operand B, 32 to 256 tokens) and D = A B^T stays in TMEM.
+// In fp16 nothing of a bf16-scaled matrix is lost: a code has at most 3
+// significant bits (|c| <= 8), a bf16 scale 8, an fp16 number 11. Ranges are
+// brought into fp16's by powers of two: each row n of W by e_n (its largest
+// scale comes to 2^11..2^12), each row of the dense operand by f_m (to
+// 2^13..2^14); they come off in the epilogue, or for the sum over n, e_n goes
+// into dy. fp32 scales are taken as 8-bit terms and fp32 rows as two fp16
+// terms, one pass over the sum for each pair of terms that matters.
+//
+// What bounds it: the tensor cores for many tokens (256 x 256 tiles, so that
+// the L2 has to deliver only 40 bytes a clock and SM), the matrix's bytes for
+// few (the decoding warps then keep four blocks in flight each, and CTAs of a
+// cluster share the sum when there are too few tiles for all SMs).
+// Roles: warps 0-7 decode (registers to swizzled shared memory, then, at the
+// end, D to global memory), warp 8 issues the TMA loads, warp 9 the MMAs.
+#pragma once
+#include "ptx.cuh"
+#include "ptx2sm.cuh"
+#include "q4.cuh"
+
+namespace tt {
+namespace q4 {
+
+constexpr int kGemmThreads = 320;
+constexpr int kStageK = 64;  // terms of the sum in a stage: 128 bytes of fp16
+
+struct Gemm {
+  const uint4* packed;
+  const void* scales;
+  int scales_f32;          // fp32, else bf16
+  const float* row_scale;  // 2^e_n
+  const float* f;          // f_m, nullable: 1
+  void* out;
+  int type;                // of out
+  long long ldo;
+  int M, N, K, kblocks;
+  int steps;               // 128-wide steps of the sum
+  int passes;              // of the sum, one for each pair of terms:
+  int scale_term[4], x_term[4];
+  int tiles_m;
+  int* err;
+};
+
+template <int R, int MT>
+struct GemmShape {
+  static constexpr int kA = R * 128 * 128;  // bytes of operand A in a stage
+  static constexpr int kB = MT * 128;
+  static constexpr int kStageBytes = kA + kB;
+  static constexpr int kStages = R == 2 ? 3 : MT == 256 ? 4 : MT == 128 ? 6 : 8;
+  static constexpr int kSmem = kStages * kStageBytes + 1024;
+  static constexpr int kColumns = R * MT;
+  // blocks that a decoding warp keeps in flight, for each of its R
+  static constexpr int kDepth = R == 2 ? 2 : 4;
+  static_assert(kSmem <= 226 * 1024, "shared memory of an SM");
+  static_assert(R == 2 || 128 * MT * 4 <= kStages * kStageBytes, "D fits where the stages were");
+};
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// fp16 operands, fp32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn) {
+  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ float load_scale(const Gemm& p, long long i) {
+  return p.scales_f32 ? __ldg(static_cast<const float*>(p.scales) + i)
+                      : to_f(__ldg(static_cast<const __nv_bfloat16*>(p.scales) + i));
+}
+__device__ __forceinline__ void store_out(const Gemm& p, long long i, float v) {
+  if (p.type == kF32) static_cast<float*>(p.out)[i] = v;
+  else if (p.type == kBF16) static_cast<__nv_bfloat16*>(p.out)[i] = from_f<__nv_bfloat16>(v);
+  else static_cast<__half*>(p.out)[i] = from_f<__half>(v);
+}
+// The i-th 8-bit term of a scale.
+__device__ __forceinline__ float scale_term(float s, int i) {
+  const float a = __bfloat162float(__float2bfloat16_rn(s));
+  if (i == 0) return a;
+  const float r = s - a, b = __bfloat162float(__float2bfloat16_rn(r));
+  return i == 1 ? b : r - b;
+}
+
+template <int R, int MT, int kGroups, bool kTrans>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
+  using S = GemmShape<R, MT>;
+  constexpr int kArrive = kTrans ? 4 : 8;  // decoding warps that fill a stage
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full_a[S::kStages], full_b[S::kStages], empty[S::kStages], done;
+  __shared__ uint32_t tmem_slot;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = gridDim.x, rank = blockIdx.x;
+  const long long tile = blockIdx.y + (long long)blockIdx.z * gridDim.y;
+  const int m0 = (int)(tile % p.tiles_m) * MT;
+  const long long row0 = tile / p.tiles_m * (R * 128);
+  const long long rows = kTrans ? p.K : p.N;
+  const bool active = row0 < rows;
+  // this CTA's steps of the sum
+  const int s0 = (int)((long long)p.steps * rank / splits), s1 = (int)((long long)p.steps * (rank + 1) / splits);
+  const int count = active ? (s1 - s0) * p.passes : 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&full_a[s], kArrive);
+      mbar_init(&full_b[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&done, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&mapB);
+  }
+  if (warp == 9) {
+    tmem_alloc(&tmem_slot, S::kColumns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  bool ok = true;
+
+  if (warp == 8) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      for (int i = 0; i < count && ok; ++i) {
+        const int pass = i / (s1 - s0), step = s0 + i % (s1 - s0);
+        for (int sub = 0; sub < 2; ++sub, ++it) {
+          const int s = it % S::kStages;
+          if (!mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full_b[s], S::kB);
+          tma_load_3d(smem + s * S::kStageBytes + S::kA, &mapB, &full_b[s], step * 128 + sub * 64, m0,
+                      p.x_term[pass]);
+        }
+      }
+      for (uint32_t k = it > S::kStages ? it - S::kStages : 0; k < it; ++k)
+        mbar_wait_drain(&full_b[k % S::kStages], (k / S::kStages) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_f16(128, MT, kTrans ? 1 : 0);
+      uint32_t it = 0;
+      for (; it < 2u * count; ++it) {
+        const int s = it % S::kStages;
+        const uint32_t ph = (it / S::kStages) & 1u;
+        if (!mbar_wait(&full_b[s], ph, p.err, kDevTimeoutFull) ||
+            !mbar_wait(&full_a[s], ph, p.err, kDevTimeoutFull))
+          break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kA;
+#pragma unroll
+        for (int ks = 0; ks < kStageK / 16; ++ks) {
+          const uint64_t b = smem_desc(sb + ks * 32, 16, 1024, 2);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            // sum-major: 128-byte rows of 64 terms; row-major (kTrans): two
+            // columns of 64 rows, 8 KB apart, one term to a 128-byte line
+            const uint64_t a = kTrans ? smem_desc(sa + r * 16384 + ks * 2048, 8192, 1024, 2)
+                                      : smem_desc(sa + r * 16384 + ks * 32, 16, 1024, 2);
+            mma_f16(tmem + r * MT, a, b, idesc, (it | ks) != 0);
+          }
+        }
+        mma_commit(&empty[s]);
+      }
+      mma_commit(&done);
+      mbar_wait_drain(&done, 0);
+    }
+    __syncwarp();
+  } else {
+    const int g = lane >> 2, t = lane & 3, odd = g & 1;
+    const long long rtiles = ((long long)p.N + kRows - 1) / kRows;
+    struct Piece {
+      uint4 q[R][2];
+      float s[R][2][kGroups];
+    };
+    Piece ring[S::kDepth];
+    float down[R][2];  // 2^-e_n of this lane's rows
+    auto norm = [&](long long n) -> float {
+      const float e = n < p.N ? __ldg(p.row_scale + n) : 1.f;
+      return __uint_as_float(0x7f000000u - __float_as_uint(e));  // exact: e is a power of two
+    };
+    if constexpr (!kTrans) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) down[r][h] = norm(row0 + r * 128 + warp * 16 + g + 8 * h);
+    }
+    auto fetch = [&](int i, Piece& x) {
+      const bool in = i < count;
+      const int step = in ? s0 + i % (s1 - s0) : 0;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const long long rt = kTrans ? step * 8LL + warp : row0 / 16 + r * 8 + warp;
+        const long long kb = kTrans ? row0 / 128 + r : step;
+        const bool there = in && rt < rtiles && kb < p.kblocks;
+        const long long blk = rt * p.kblocks + kb;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          x.q[r][h] = there ? ldg_stream(p.packed + blk * 64 + h * 32 + lane)
+                            : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+#pragma unroll
+          for (int k = 0; k < kGroups; ++k)
+            x.s[r][h][k] = there ? load_scale(p, (blk * kGroups + k) * kRows + g + 8 * h) : 0.f;
+        }
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < S::kDepth; ++d) fetch(d, ring[d]);
+    for (int i0 = 0; i0 < count && ok; i0 += S::kDepth) {
+#pragma unroll
+      for (int d = 0; d < S::kDepth; ++d) {
+        const int i = i0 + d;
+        if (i >= count || !ok) break;
+        Piece& x = ring[d];
+        const int term = p.passes == 1 ? 0 : p.scale_term[i / (s1 - s0)];
+        if constexpr (kTrans) {
+          const long long n = (s0 + i % (s1 - s0)) * 128LL + warp * 16 + g;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            down[0][h] = norm(n + 8 * h);
+#pragma unroll
+            for (int r = 1; r < R; ++r) down[r][h] = down[0][h];
+          }
+        }
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          if (kTrans && sub != warp >> 2) continue;  // four warps a stage
+          const uint32_t it = 2u * i + sub;
+          const int s = it % S::kStages;
+          ok = mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint32_t base = smem_u32(smem + s * S::kStageBytes);
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t word[4] = {x.q[r][h].x, x.q[r][h].y, x.q[r][h].z, x.q[r][h].w};
+              __half2 sc[kGroups];
+#pragma unroll
+              for (int k = 0; k < kGroups; ++k) {
+                const float v = x.s[r][h][k] * down[r][h];
+                sc[k] = __float2half2_rn(p.scales_f32 ? scale_term(v, term) : v);
+              }
+#pragma unroll
+              for (int pair = kTrans ? 0 : sub; pair < (kTrans ? 2 : sub + 1); ++pair)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  // odd rows take the pair's words the other way round: eight
+                  // lanes then meet all 32 banks
+                  const uint32_t wd = odd ? word[2 * pair + (e ^ 1)] : word[2 * pair + e];
+                  constexpr int kPer = 4 / kGroups;
+                  const __half2 sh =
+                      kGroups < 4 ? sc[2 * pair / kPer]
+                                  : (odd ? sc[(2 * pair + (e ^ 1)) / kPer] : sc[(2 * pair + e) / kPer]);
+                  uint32_t v[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const uint32_t c = decode_pair<true>(wd >> (4 * j));
+                    const __half2 y = __hmul2(reinterpret_cast<const __half2&>(c), sh);
+                    v[j] = reinterpret_cast<const uint32_t&>(y);
+                  }
+                  const uint32_t chunk = (uint32_t)((e ^ odd) * 4 + t);
+                  uint32_t at;
+                  if constexpr (kTrans) {
+                    const uint32_t n = (warp & 3) * 16 + g + 8 * h;
+                    at = base + (2 * r + pair) * 8192 + n * 128 + ((chunk ^ (n & 7)) << 4);
+                  } else {
+                    const uint32_t n = r * 128 + warp * 16 + g + 8 * h;
+                    at = base + n * 128 + ((chunk ^ (n & 7)) << 4);
+                  }
+                  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]),
+                               "r"(v[2]), "r"(v[3])
+                               : "memory");
+                }
+            }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full_a[s]);
+        }
+        fetch(i + S::kDepth, x);
+      }
+    }
+    // D: lanes are rows of the tile, columns are tokens
+    ok = mbar_wait(&done, 0, p.err, kDevTimeoutAcc) && ok;
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    if (ok && active) {
+      const int quad = warp & 3, half = warp >> 2;
+      const long long row = row0 + (R == 2 ? half * 128 : 0) + quad * 32 + lane;
+      const int c0 = R == 2 ? 0 : half * (MT / 2), c1 = R == 2 ? MT : c0 + MT / 2;
+      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (R == 2 ? half * MT : 0);
+      const float up = !kTrans && row < rows ? __ldg(p.row_scale + row) : 1.f;
+      float* dsm = reinterpret_cast<float*>(smem);
+      for (int c = c0; c < c1; c += 16) {
+        if (m0 + c >= p.M) break;
+        float v[16];
+        tmem_ld16(from + c, v);
+        tmem_ld_wait();
+        if (splits > 1) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) dsm[(c + k) * 128 + quad * 32 + lane] = v[k];
+        } else if (row < rows) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int m = m0 + c + k;
+            if (m < p.M)
+              store_out(p, m * p.ldo + row, v[k] * up * (p.f ? __ldg(p.f + m) : 1.f));
+          }
+        }
+      }
+    }
+  }
+  if (splits > 1) {  // the CTAs' parts, added in rank order, a share of the tokens each
+    cluster_sync();
+    if (R == 1 && active && threadIdx.x < 256) {
+      const int r = threadIdx.x & 127;
+      const long long row = row0 + r;
+      const float up = !kTrans && row < rows ? __ldg(p.row_scale + row) : 1.f;
+      const uint32_t base = smem_u32(smem);
+      for (int c = rank + splits * (threadIdx.x >> 7); c < MT && m0 + c < p.M; c += 2 * splits) {
+        float v = 0.f;
+        for (int k = 0; k < splits; ++k) {
+          float w;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(mapa(base + (c * 128 + r) * 4, k)));
+          v += w;
+        }
+        const int m = m0 + c;
+        if (row < rows)
+          store_out(p, m * p.ldo + row, v * up * (p.f ? __ldg(p.f + m) : 1.f));
+      }
+    }
+    cluster_sync();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kColumns);
+  }
+}
+
+// 2^e_n of each row: the exponent that brings its largest finite |s| to
+// 2^11 .. 2^12 when divided by. A row of zeros gets 1.
+template <typename ST>
+__global__ void row_scale_kernel(const ST* __restrict__ scales, int N, int kblocks, int gpb,
+                                 float* __restrict__ out) {
+  // a warp a row tile: lanes 0-15 and 16-31 are its rows, taking turns
+  const long long rt = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+  const int lane = threadIdx.x & 31;
+  const long long rtiles = ((long long)N + kRows - 1) / kRows;
+  if (rt >= rtiles) return;
+  const long long lines = (long long)kblocks * gpb;
+  const ST* at = scales + rt * lines * kRows;
+  uint32_t top = 0;
+  for (long long i = lane; i < lines * kRows; i += 32) {
+    const uint32_t b = __float_as_uint(fabsf(to_f(at[i])));
+    if (b < 0x7f800000u) top = max(top, b);
+  }
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+  int e = (int)(top >> 23) - 11;  // biased exponent of 2^e
+  e = top == 0 ? 127 : e < 1 ? 1 : e > 253 ? 253 : e;
+  const long long n = rt * kRows + (lane & 15);
+  if (lane < 16 && n < N) out[n] = __uint_as_float((uint32_t)e << 23);
+}
+
+// Rows of the dense operand as fp16: x 2^e (e by column, or none), times the
+// power of two that brings the row's largest finite value to 2^13 .. 2^14,
+// rounded (kTerms 1) or as two terms; zeros behind the row's end. f gets the
+// power's reciprocal. `finite`: one more copy of the first term, without
+// infinities and NaN, for the passes of a scale's smaller terms (an infinity
+// enters the sum once).
+template <typename XT, int kTerms>
+__global__ void __launch_bounds__(256)
+convert_kernel(const XT* __restrict__ x, long long ldx, const float* __restrict__ col, int M, int C, int Cp,
+               __half* __restrict__ out, float* __restrict__ f, int finite) {
+  __shared__ uint32_t tops[8];
+  const int m = blockIdx.x;
+  const XT* row = x + m * ldx;
+  uint32_t top = 0;
+  for (int i = threadIdx.x; i < C; i += 256) {
+    const float v = to_f(row[i]) * (col ? __ldg(col + i) : 1.f);
+    const uint32_t b = __float_as_uint(fabsf(v));
+    if (b < 0x7f800000u) top = max(top, b);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = max(top, tops[w]);
+  int e = (int)(top >> 23);
+  e = e < 14 ? 14 : e;
+  const float up = __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(140 - e)
+  if (threadIdx.x == 0) f[m] = __uint_as_float((uint32_t)(e - 13) << 23);
+  __half* hi = out + (long long)m * Cp;
+  __half* lo = hi + (long long)M * Cp;
+  __half* fin = lo + (kTerms == 2 ? (long long)M * Cp : 0);
+  for (int i = threadIdx.x; i < Cp; i += 256) {
+    const float v = i < C ? to_f(row[i]) * (col ? __ldg(col + i) : 1.f) * up : 0.f;
+    const __half h = __float2half_rn(v);
+    hi[i] = h;
+    if (finite) fin[i] = isfinite(v) ? h : __float2half_rn(0.f);
+    if (kTerms == 2) {
+      const float r = v - __half2float(h);
+      lo[i] = __float2half_rn(isfinite(v) ? r : 0.f);
+    }
+  }
+}
+
+}  // namespace q4
+}  // namespace tt

@@ -23,12 +23,17 @@ import math
 import torch
 
 from . import _lib
-from .dispatch import _device, _ptr
-from .quantized import _TYPES, _stream_of
+from .dispatch import _device
+from .quantized import _TYPES, _on, _stream_of
 
+_WORKSPACE: dict[tuple[int, int], int] = {}  # bytes by (device, head_dim)
 _PAGES = (16, 32, 64, 128)
 _WRONG = ((1, "a page id outside the cache"), (2, "a length or count out of range"),
           (4, "one append wrote a page for two places"), (8, "a device copy never arrived"))
+
+
+def _at(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _check_geometry(num_pages: int, kv_heads: int, head_dim: int, page_size: int) -> None:
@@ -114,10 +119,10 @@ class KVCache8:
                         device=self.device)
         v = torch.empty_like(k)
         if n:
-            with torch.cuda.device(self.device):
+            with _on(self.device):
                 _lib.check(_lib.load().tt_kv8_read(
-                    _ptr(self._k), _ptr(self._v), _ptr(self.k_scales), _ptr(self.v_scales),
-                    _ptr(pages), n, _ptr(k), _ptr(v), _TYPES[dtype], _ptr(self.status),
+                    _at(self._k), _at(self._v), _at(self.k_scales), _at(self.v_scales),
+                    _at(pages), n, _at(k), _at(v), _TYPES[dtype], _at(self.status),
                     self.num_pages, self.kv_heads, self.page_size, self.head_dim,
                     _stream_of(self.device)), "tt_kv8_read")
         return k, v
@@ -136,7 +141,7 @@ class KVCache8:
 def _int32(t: torch.Tensor | None, name: str, shape: tuple, dev: torch.device):
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != dev:
+    if t.dtype != torch.int32 or t.shape != shape or t.device != dev:
         raise ValueError(f"{name} must be int32 {shape} on {dev}, got {t.dtype} {tuple(t.shape)} "
                          f"on {t.device}")
     return t.contiguous()
@@ -156,7 +161,8 @@ def _check_tokens(x: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor
                          f"got {x.dtype} {tuple(x.shape)}")
     if x.device != dev:
         raise ValueError(f"{name} must be on {dev}, got {x.device}")
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     return x if x.stride(3) == 1 else x.contiguous()
 
 
@@ -187,7 +193,7 @@ def kv_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
     if k.shape != v.shape or k.dtype != v.dtype or tuple(k.shape[2:]) != (cache.kv_heads, cache.head_dim):
         raise ValueError(f"k and v must be alike and end in {(cache.kv_heads, cache.head_dim)}, got "
                          f"{tuple(k.shape)} {k.dtype} and {tuple(v.shape)} {v.dtype}")
-    batch, new = int(k.shape[0]), int(k.shape[1])
+    batch, new = k.shape[:2]
     table = _check_table(block_table, batch, dev)
     lengths = _int32(lengths, "lengths", (batch,), dev)
     n_new = _int32(n_new, "n_new", (batch,), dev)
@@ -195,13 +201,13 @@ def kv_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
         inv_freq = _check_freq(inv_freq, cache.head_dim, dev)
     if batch == 0 or new == 0:
         return
-    with torch.cuda.device(dev):
+    with _on(dev):
         _lib.check(_lib.load().tt_kv8_append(
-            _ptr(k), _ptr(v), _TYPES[k.dtype], k.stride(0), k.stride(1), k.stride(2), v.stride(0),
-            v.stride(1), v.stride(2), _ptr(table), table.stride(0), int(table.shape[1]),
-            _ptr(lengths), _ptr(n_new), _ptr(inv_freq),
-            0 if inv_freq is None else int(inv_freq.shape[0]), int(interleaved), _ptr(cache._k),
-            _ptr(cache._v), _ptr(cache.k_scales), _ptr(cache.v_scales), _ptr(cache.status), batch,
+            _at(k), _at(v), _TYPES[k.dtype], k.stride(0), k.stride(1), k.stride(2), v.stride(0),
+            v.stride(1), v.stride(2), _at(table), table.stride(0), int(table.shape[1]),
+            _at(lengths), _at(n_new), _at(inv_freq),
+            0 if inv_freq is None else int(inv_freq.shape[0]), int(interleaved), _at(cache._k),
+            _at(cache._v), _at(cache.k_scales), _at(cache.v_scales), _at(cache.status), batch,
             new, cache.kv_heads, cache.head_dim, cache.page_size, cache.num_pages,
             _stream_of(dev)), "tt_kv8_append")
 
@@ -214,15 +220,15 @@ def kv_rotate(x: torch.Tensor, lengths: torch.Tensor, inv_freq: torch.Tensor, *,
     if dev.type != "cuda":
         raise ValueError(f"kv_rotate: x must be on a CUDA device, got {dev}")
     x = _check_tokens(x, "x", dev)
-    batch, new, heads, dim = (int(s) for s in x.shape)
+    batch, new, heads, dim = x.shape
     lengths = _int32(lengths, "lengths", (batch,), dev)
     inv_freq = _check_freq(inv_freq, dim, dev)
     out = torch.empty((batch, new, heads, dim), dtype=x.dtype, device=dev)
     if out.numel():
-        with torch.cuda.device(dev):
+        with _on(dev):
             _lib.check(_lib.load().tt_kv8_rotate(
-                _ptr(x), _TYPES[x.dtype], x.stride(0), x.stride(1), x.stride(2), _ptr(lengths),
-                _ptr(inv_freq), int(inv_freq.shape[0]), int(interleaved), _ptr(out), batch, new,
+                _at(x), _TYPES[x.dtype], x.stride(0), x.stride(1), x.stride(2), _at(lengths),
+                _at(inv_freq), int(inv_freq.shape[0]), int(interleaved), _at(out), batch, new,
                 heads, dim, _stream_of(dev)), "tt_kv8_rotate")
     return out
 
@@ -242,7 +248,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, le
     """
     dev = cache.device
     q = _check_tokens(q, "q", dev)
-    batch, new, heads, dim = (int(s) for s in q.shape)
+    batch, new, heads, dim = q.shape
     if dim != cache.head_dim or heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"q must end in (a multiple of {cache.kv_heads} heads, {cache.head_dim}), "
                          f"got {tuple(q.shape)}")
@@ -256,17 +262,22 @@ def kv_attention(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, le
     if out.numel() == 0:
         return out
     per = 16 // q.element_size()
-    if q.data_ptr() % 16 or any(q.stride(i) % per for i in range(3)):
+    sb, ss, sh, _ = q.stride()
+    if q.data_ptr() % 16 or sb % per or ss % per or sh % per:
         q = q.clone(memory_format=torch.contiguous_format)
+        sb, ss, sh, _ = q.stride()
     lib = _lib.load()
-    with torch.cuda.device(dev):
-        ws_bytes = int(lib.tt_kv8_attention_workspace_bytes(dim))
+    with _on(dev):
+        ws_bytes = _WORKSPACE.get((dev.index, dim))
+        if ws_bytes is None:
+            ws_bytes = int(lib.tt_kv8_attention_workspace_bytes(dim))
+            _WORKSPACE[dev.index, dim] = ws_bytes
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _lib.check(lib.tt_kv8_attention(
-            _ptr(q), _TYPES[q.dtype], q.stride(0), q.stride(1), q.stride(2), _ptr(cache._k),
-            _ptr(cache._v), _ptr(cache.k_scales), _ptr(cache.v_scales), _ptr(table),
-            table.stride(0), int(table.shape[1]), _ptr(lengths), _ptr(n_query),
-            ctypes.byref(ctypes.c_float(scale)), int(causal), _ptr(out), _ptr(ws), ws_bytes, _ptr(cache.status),
+            _at(q), _TYPES[q.dtype], sb, ss, sh, _at(cache._k),
+            _at(cache._v), _at(cache.k_scales), _at(cache.v_scales), _at(table),
+            table.stride(0), int(table.shape[1]), _at(lengths), _at(n_query),
+            ctypes.byref(ctypes.c_float(scale)), int(causal), _at(out), _at(ws), ws_bytes, _at(cache.status),
             batch, new, heads, cache.kv_heads, dim, cache.page_size, cache.num_pages,
             _stream_of(dev)), "tt_kv8_attention")
     return out

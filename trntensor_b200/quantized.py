@@ -12,7 +12,7 @@ gradient. Nothing here has a counterpart in the reference.
 
 from __future__ import annotations
 
-import ctypes
+import contextlib
 
 import torch
 
@@ -21,17 +21,30 @@ from .dispatch import _device, _ptr
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GROUPS = (32, 64, 128)
+_FEW_ROWS = 16  # up to here a product needs no workspace
 
 
-def _stream_of(dev: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """Context in which ``dev`` is the current CUDA device."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream_of(dev: torch.device) -> int:
+    """Handle of ``dev``'s current stream (the raw query: a Stream object costs
+    more than a small launch)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 class Q4Matrix:
     """An (N, K) matrix of 4-bit codes with group scales, in kernel order.
 
     Made by :func:`quantize_q4` or :func:`pack_q4`; ``packed`` and ``scales``
-    are the stored bytes and scales (bf16 or fp32), padded to 16 x 128 blocks.
+    are the stored bytes and scales (bf16 or fp32), padded to 16 x 128 blocks,
+    ``row_scale`` a power of two a row. ``status`` is a device word in which a
+    product notes a device wait that ran out; :meth:`check` reads it.
     """
 
     ndim = 2
@@ -40,6 +53,21 @@ class Q4Matrix:
                  group: int):
         self.packed, self.scales, self.group = packed, scales, group
         self.shape = torch.Size(shape)
+        self.status = torch.zeros((), dtype=torch.int32, device=packed.device)
+        n, k = self.shape
+        self.row_scale = torch.ones(n, dtype=torch.float32, device=packed.device)
+        if n and k and packed.device.type == "cuda":
+            with _on(packed.device):
+                _lib.check(_lib.load().tt_q4_row_scale(
+                    _ptr(scales), _TYPES[scales.dtype], n, k, group, _ptr(self.row_scale),
+                    _stream_of(packed.device)), "tt_q4_row_scale")
+
+    def check(self) -> None:
+        """Raise if a device wait of a product ran out (waits for the device)."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            raise _lib.DeviceError(f"Q4Matrix: device wait ran out (status 0x{code:x})")
 
     @property
     def device(self) -> torch.device:
@@ -62,7 +90,7 @@ class Q4Matrix:
         out = torch.empty((n, k), dtype=kind, device=self.device)
         if out.numel():
             lib = _lib.load()
-            with torch.cuda.device(self.device):
+            with _on(self.device):
                 _lib.check(lib.tt_q4_dequantize(
                     _ptr(self.packed), _ptr(self.scales), _TYPES[self.scales.dtype], n, k,
                     self.group, _ptr(out), _TYPES[kind], _stream_of(self.device)),
@@ -129,7 +157,7 @@ def quantize_q4(weight: torch.Tensor, *, group: int = 128,
     n, k = (int(s) for s in w.shape)
     packed, scales = _empty_q4(n, k, group, scale_dtype, w.device)
     if n and k:
-        with torch.cuda.device(w.device):
+        with _on(w.device):
             _lib.check(_lib.load().tt_q4_quantize(
                 _ptr(w), _TYPES[w.dtype], int(w.stride(0)) if n > 1 else k, _TYPES[scale_dtype],
                 n, k, group, _ptr(packed), _ptr(scales), _stream_of(w.device)), "tt_q4_quantize")
@@ -153,7 +181,7 @@ def pack_q4(codes: torch.Tensor, scales: torch.Tensor, *, group: int = 128) -> Q
     s = (s.float() if s.dtype == torch.float16 else s).contiguous()
     packed, out = _empty_q4(n, k, group, s.dtype, c.device)
     if n and k:
-        with torch.cuda.device(c.device):
+        with _on(c.device):
             _lib.check(_lib.load().tt_q4_pack(
                 _ptr(c), _ptr(s), _TYPES[s.dtype], n, k, group, _ptr(packed), _ptr(out),
                 _stream_of(c.device)), "tt_q4_pack")
@@ -163,21 +191,32 @@ def pack_q4(codes: torch.Tensor, scales: torch.Tensor, *, group: int = 128) -> Q
 def _product(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
     """(M, K) -> (M, N) or, over_n, (M, N) -> (M, K) on the matrix's device."""
     n, k = w.shape
-    m, cols = int(x.shape[0]), (k if over_n else n)
-    out = torch.empty((m, cols), dtype=x.dtype, device=x.device)
-    if out.numel() == 0:
+    m, have = x.shape
+    cols = k if over_n else n
+    out = x.new_empty((m, cols))
+    if m == 0 or cols == 0:
         return out
-    if n == 0 or k == 0:
+    if have == 0:
         return out.zero_()
-    if x.stride(1) != 1 or (m > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
+    ldx, inner = x.stride()
+    if inner != 1 or ldx < have:
+        if m > 1 or inner != 1:
+            x = x.contiguous()
+        ldx = have
     lib = _lib.load()
     fn = lib.tt_q4_matmul_t if over_n else lib.tt_q4_matmul
-    with torch.cuda.device(x.device):
-        _lib.check(fn(_ptr(x), _TYPES[x.dtype], int(x.stride(0)) if m > 1 else int(x.shape[1]),
-                      _ptr(w.packed), _ptr(w.scales), _TYPES[w.scales.dtype], m, n, k, w.group,
-                      _ptr(out), cols, _stream_of(x.device)),
-                   "tt_q4_matmul_t" if over_n else "tt_q4_matmul")
+    dev, kind = x.device, _TYPES[x.dtype]
+    ws, ws_bytes = None, 0
+    if m > _FEW_ROWS:
+        ws_bytes = lib.tt_q4_matmul_workspace_bytes(kind, _TYPES[w.scales.dtype], over_n, m, n, k)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        st = fn(x.data_ptr(), kind, ldx, w.packed.data_ptr(), w.scales.data_ptr(),
+                _TYPES[w.scales.dtype], w.row_scale.data_ptr(), m, n, k, w.group, out.data_ptr(),
+                cols, None if ws is None else ws.data_ptr(), ws_bytes, w.status.data_ptr(),
+                _stream_of(dev))
+    if st:
+        _lib.check(st, "tt_q4_matmul_t" if over_n else "tt_q4_matmul")
     return out
 
 
@@ -192,14 +231,23 @@ class _Q4Product(torch.autograd.Function):
         return _Q4Product.apply(dy, ctx.w, not ctx.over_n), None, None
 
 
+def _dispatch(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Q4Product.apply(x, w, over_n)
+    return _product(x.detach() if x.requires_grad else x, w, over_n)
+
+
 def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> torch.Tensor:
     """``x @ W^T``: (..., K) -> (..., N); with ``over_n`` ``x @ W``: (..., N) -> (..., K).
 
-    x is fp32, bf16 or fp16; products are exact, sums are fp32, and the result
-    is rounded once to x's type (over n the scaled operand is split into bf16
-    terms, which keeps 2^-16 of each product for 16-bit types and fp32's own
-    bits for fp32). Differentiable in x, any number of times. A host x is
-    copied to the matrix's device and the result comes back.
+    x is fp32, bf16 or fp16; sums are fp32 and the result is rounded once to
+    x's type. Up to 16 rows products over k are exact, and over n they keep
+    2^-16 (fp32: all bits). With more rows both operands are brought to fp16's
+    range by powers of two a row: products are exact where scales are bf16 and
+    x is of 16 bits and no smaller than 2^-27 of its row's largest value, else
+    they keep 2^-18 (fp32: 2^-20) of themselves and 2^-38 of the largest.
+    Differentiable in x, any number of times. A host x is copied to the
+    matrix's device and the result comes back.
     """
     if not isinstance(weight, Q4Matrix):
         raise ValueError(f"q4_matmul: weight must be a Q4Matrix, got {type(weight).__name__}")
@@ -210,31 +258,29 @@ def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> tor
         raise ValueError(f"q4_matmul: x must end in {want} for {weight!r}, got {tuple(x.shape)}")
     if x.device.type == "cuda" and x.device != weight.device:
         raise ValueError(f"q4_matmul: x is on {x.device}, the matrix on {weight.device}")
+    if x.dim() == 2 and x.device == weight.device:
+        return _dispatch(x, weight, over_n)
     lead = x.shape[:-1]
     rows = 1
     for s in lead:
         rows *= int(s)
-    flat = x.to(weight.device).reshape(rows, want)
-    y = _Q4Product.apply(flat, weight, over_n)
+    y = _dispatch(x.to(weight.device).reshape(rows, want), weight, over_n)
     return y.reshape(*lead, y.shape[-1]).to(x.device)
 
 
-def einsum_q4(subscripts: str, operands: tuple, precision: str) -> torch.Tensor:
-    """Two-operand einsum with one :class:`Q4Matrix`: a product over k or over n
-    with the dense operand's other indices kept."""
-    from .plan import _check_precision, _parse_subscripts, _validate_subscripts
+# (subscripts, place of the matrix, dimensions of the dense operand) -> how it runs
+_FORMS: dict[tuple, tuple] = {}
+
+
+def _form(subscripts: str, operands: tuple, held: int) -> tuple:
+    """(axis of x that is contracted, its permutation or None, over_n, the
+    result's permutation or None) of a contraction with one Q4Matrix."""
+    from .plan import _parse_subscripts, _validate_subscripts
 
     _validate_subscripts(subscripts, operands)
-    _check_precision(precision)
     lhs, out = _parse_subscripts(subscripts)
     terms = lhs.split(",")
-    held = [i for i, op in enumerate(operands) if isinstance(op, Q4Matrix)]
-    if len(operands) != 2 or len(held) != 1:
-        raise ValueError(
-            f"einsum {subscripts!r}: a Q4Matrix contracts with one dense operand; "
-            "use dequantize() for other forms")
-    w, x = operands[held[0]], operands[1 - held[0]]
-    tw, tx = terms[held[0]], terms[1 - held[0]]
+    tw, tx = terms[held], terms[1 - held]
     shared = [c for c in tw if c in tx]
     if (len(set(tw)) != 2 or len(set(tx)) != len(tx) or len(set(out)) != len(out)
             or len(shared) != 1 or shared[0] in out):
@@ -246,12 +292,38 @@ def einsum_q4(subscripts: str, operands: tuple, precision: str) -> torch.Tensor:
     rest = [ch for ch in tx if ch != c]
     if set(out) != set(rest) | {free}:
         raise ValueError(f"einsum {subscripts!r}: every uncontracted index must be in the output")
+    into = [tx.index(ch) for ch in rest + [c]]
+    order = [(rest + [free]).index(ch) for ch in out]
+    plain = list(range(len(into)))
+    return (tx.index(c), None if into == plain else into, c == tw[0],
+            None if order == list(range(len(order))) else order)
+
+
+def einsum_q4(subscripts: str, operands: tuple, precision: str) -> torch.Tensor:
+    """Two-operand einsum with one :class:`Q4Matrix`: a product over k or over n
+    with the dense operand's other indices kept."""
+    from .plan import _check_precision, _validate_subscripts
+
+    if len(operands) != 2 or isinstance(operands[0], Q4Matrix) == isinstance(operands[1], Q4Matrix):
+        _validate_subscripts(subscripts, operands)
+        raise ValueError(
+            f"einsum {subscripts!r}: a Q4Matrix contracts with one dense operand; "
+            "use dequantize() for other forms")
+    held = 0 if isinstance(operands[0], Q4Matrix) else 1
+    w, x = operands[held], operands[1 - held]
+    key = (subscripts, held, x.dim())
+    form = _FORMS.get(key)
+    if form is None:
+        form = _FORMS[key] = _form(subscripts, operands, held)
+    axis, into, over_n, order = form
+    if x.shape[axis] != w.shape[0 if over_n else 1]:
+        _validate_subscripts(subscripts, operands)
     if precision != "fast":
         from .einsum import einsum
 
-        ops = [w.dequantize(torch.float64), x]
-        return einsum(f"{tw},{tx}->{out}", ops[0].to(x.device), x.double(),
-                      precision=precision).to(x.dtype)
-    y = q4_matmul(x.permute([tx.index(ch) for ch in rest + [c]]), w, over_n=c == tw[0])
-    order = [(rest + [free]).index(ch) for ch in out]
-    return y if order == list(range(len(order))) else y.permute(order).contiguous()
+        _check_precision(precision)
+        ops = [x.double(), x.double()]
+        ops[held] = w.dequantize(torch.float64).to(x.device)
+        return einsum(subscripts, *ops, precision=precision).to(x.dtype)
+    y = q4_matmul(x if into is None else x.permute(into), w, over_n=over_n)
+    return y if order is None else y.permute(order).contiguous()
