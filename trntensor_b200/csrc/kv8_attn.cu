@@ -38,13 +38,10 @@ int setup(int dev) {
   });
 }
 
-// Warps of the grid: one CTA an SM.
-int warps_of(int dim, int sms) { return sms * (dim <= 128 ? 8 : 4); }
-
-size_t workspace_bytes(int dim, int sms) {
-  const size_t warps = warps_of(dim, sms);
-  return warps * 16 + warps * 2 * 16 * (dim + 2) * 4;
-}
+// One CTA an SM; for each a word of meta, two pieces a warp, and two joined.
+int warps_of(int dim) { return dim <= 128 ? 8 : 4; }
+size_t piece_bytes(int dim) { return (size_t)2 * 16 * (dim + 2) * 4; }
+size_t workspace_bytes(int dim, int sms) { return sms * (16 + (warps_of(dim) + 1) * piece_bytes(dim)); }
 
 template <typename T, int DP>
 int launch(const Attend& p, int sms, cudaStream_t s) {
@@ -53,7 +50,7 @@ int launch(const Attend& p, int sms, cudaStream_t s) {
   attend_kernel<T, DP, kTerms><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
   int st = cuda_status(cudaGetLastError());
   if (st != TT_OK) return st;
-  join_kernel<T><<<p.warps, 256, 0, s>>>(p);
+  join_kernel<T><<<dim3(sms, p.rows < 16 ? p.rows : 16), 256, 0, s>>>(p);
   return cuda_status(cudaGetLastError());
 }
 template <typename T>
@@ -108,9 +105,9 @@ int tt_kv8_attention(const void* q, int type, long long q_stride_b, long long q_
   p.kc = (const unsigned char*)k_codes; p.vc = (const unsigned char*)v_codes;
   p.ks = k_scales; p.vs = v_scales;
   p.table = block_table; p.table_b = table_stride; p.lengths = lengths; p.n_query = n_query;
-  p.warps = kv8::warps_of(dim, sms);
   p.meta = (int4*)workspace;
-  p.part = (float*)((char*)workspace + (size_t)p.warps * 16);
+  p.joint = (float*)((char*)workspace + (size_t)sms * 16);
+  p.part = (float*)((char*)p.joint + sms * kv8::piece_bytes(dim));
   p.status = status;
   p.scale = *scale * 1.4426950408889634f;
   p.causal = causal;

@@ -6,9 +6,10 @@
 // kv head's query rows (tokens x heads of its group) make tiles of 16, and the
 // work is cut into chunks of 64 tokens of one tile. The chunks of all
 // sequences, heads and tiles form one line, of which every warp takes an equal
-// piece, so that ragged lengths and a lone long sequence both fill the GPU; a
-// tile whose chunks lie with several warps is joined by a second small kernel,
-// always in the same order.
+// piece, so that ragged lengths and a lone long sequence both fill the GPU. A
+// tile whose chunks lie with several warps is joined in shared memory when
+// they are of one CTA, and by a second small kernel when they are not, always
+// in the same order.
 //
 // What bounds it: the cache's bytes. Each warp keeps its own ring of shared
 // memory slots (one unit quartet of keys or of values each) filled by bulk
@@ -51,13 +52,13 @@ struct Attend {
   long long table_b;
   const int* lengths;
   const int* n_query;  // nullable: S
-  float* part;         // partial sums: [warp][2][16][2 + dim] (maximum, sum, values)
-  int4* meta;          // [warp]: (b, h * tiles + tile, last warp, 1) of a tile that others finish
+  float* part;         // pieces: [CTA][warp][2][16][2 + dim] (maximum, sum, values)
+  float* joint;        // and joined: [CTA][2][16][2 + dim]
+  int4* meta;          // [CTA]: (b, h * tiles + tile, last CTA, 1) of a tile that others finish
   int* status;
   float scale;  // times log2(e)
   int causal;
   int batch, S, heads_q, heads, dim, page, pages, cols, rows, tiles;
-  int warps;  // of the whole grid
 };
 
 template <int DP, int kTerms>
@@ -188,6 +189,60 @@ __device__ __forceinline__ void advance(const Attend& p, Place& x) {
   next_sequence(p, x);
 }
 
+// Pieces of a row (maximum, sum, values) made one by a warp: first the largest
+// maximum, then the sums, so that the loads do not wait for one another.
+template <int DP>
+struct Joined {
+  static constexpr int kPer = DP / 32;
+  float m, l, a[kPer];
+  // Pieces first, first + step, .. last, each `stride` floats behind the one
+  // before; those that `there` marks as missing are left out. `head`: what
+  // piece 0 lies behind its place.
+  __device__ __forceinline__ void join(const float* in, int stride, int first, int last, int step, int dim, int lane,
+                                       const int4* there, int head = 0) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) a[e] = 0.f;
+    for (int k = first + step * lane; k <= last; k += step * 32)
+      if (there == nullptr || there[k].x >= 0) m = fmaxf(m, in[(long long)k * stride + (k == 0 ? head : 0)]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float z = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int k = first; k <= last; k += step) {
+      if (there != nullptr && there[k].x < 0) continue;
+      const float* at = in + (long long)k * stride + (k == 0 ? head : 0);
+      const float f = exp2_approx(at[0] - z);
+      l += at[1] * f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (lane + 32 * e < dim) a[e] += at[2 + lane + 32 * e] * f;
+    }
+  }
+  __device__ __forceinline__ void keep(float* out, int dim, int lane) const {
+    if (lane == 0) {
+      out[0] = m;
+      out[1] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (lane + 32 * e < dim) out[2 + lane + 32 * e] = a[e];
+  }
+  template <typename T>
+  __device__ __forceinline__ void finish(T* o, int dim, int lane) const {
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (lane + 32 * e < dim) o[lane + 32 * e] = q4::from_f<T>(a[e] * inv);
+  }
+};
+// Where row r of kv head h's rows stands in the result.
+__device__ __forceinline__ long long row_offset(const Attend& p, int b, int h, int r) {
+  const int group = p.heads_q / p.heads;
+  return (((long long)b * p.S + r / group) * p.heads_q + h * group + r % group) * p.dim;
+}
+
 template <typename T, int DP, int kTerms>
 __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kernel(const Attend p) {
   using S = Shape<DP, kTerms>;
@@ -195,7 +250,9 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t bars[S::kWarps * S::kSlots];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int worker = warp * gridDim.x + blockIdx.x;  // neighbours on different SMs
+  // pieces of tiles that this CTA's warps leave: tile, whether it began and ended here
+  __shared__ int4 left_at[S::kWarps * 2];
+  if (threadIdx.x < S::kWarps * 2) left_at[threadIdx.x] = make_int4(-1, 0, 0, 0);
   unsigned char* mine = smem + warp * S::kSlots * S::kSlot;
   uint64_t* bar = bars + warp * S::kSlots;
   const int dim = p.dim;
@@ -215,13 +272,21 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
         static_cast<T*>(p.o)[b * all + i] = from_f<T>(0.f);
     }
   }
-  if (lane == 0) p.meta[worker] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  __syncthreads();
 
   // this warp's piece of the line
   const long long total = chunk_sum(p, p.batch, lane);
-  const long long workers = min((long long)p.warps, total);  // each has a chunk at least
-  if (worker >= workers) return;
-  const long long begin = total * worker / workers, end = total * (worker + 1) / workers;
+  // Warps of a CTA that work: one while there are no more chunks than CTAs, so
+  // that a little work spreads over the SMs; each has a chunk at least.
+  const int per_cta = (int)max(1LL, min((long long)S::kWarps, (total + gridDim.x - 1) / gridDim.x));
+  const long long workers = min((long long)gridDim.x * per_cta, total);
+  const long long worker = (long long)blockIdx.x * per_cta + warp;
+  const bool works = warp < per_cta && worker < workers;
+  const long long begin = works ? total * worker / workers : 0, end = works ? total * (worker + 1) / workers : 0;
+  const int group = p.heads_q / p.heads;
+  const int rows_of = dim + 2;
+  if (works) {
   Place at;
   {
     // the last sequence that starts at or before `begin`
@@ -334,7 +399,6 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     if (slot == 0) parity ^= 1;
   };
 
-  const int group = p.heads_q / p.heads;
   float acc[DP / 8][4];
   uint32_t qf[S::kQRegs ? DP / 16 : 1][4];
   unsigned char* qs = smem + S::kWarps * S::kSlots * S::kSlot + warp * S::kQBytes;  // [step][term][lane][4]
@@ -425,7 +489,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
     arrive();
-    if (!alive) return;
+    if (!alive) break;
     {
       const uint32_t keys = smem_u32(mine + slot * S::kSlot) + (g >> 1) * (S::kUnit + 32) + (g & 1) * dim + t * 16;
 #pragma unroll
@@ -531,7 +595,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
         split_f16<kTerms>(y[2], y[3], w[kk][2 * half + 1]);
       }
     arrive();
-    if (!alive) return;
+    if (!alive) break;
     {
       const uint32_t vals = smem_u32(mine + slot * S::kSlot) + t * (S::kUnit + 32) + g * 16;
 #pragma unroll
@@ -564,17 +628,17 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
         if (r < p.rows) {
           if (whole && last) {
             const float inv = l > 0.f || l != l ? top_v / (l * kUp) : 0.f;
-            T* o = static_cast<T*>(p.o) +
-                   (((long long)at.b * p.S + r / group) * p.heads_q + at.h * group + r % group) * dim;
+            T* o = static_cast<T*>(p.o) + row_offset(p, at.b, at.h, r);
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) {
               const int d = n * 8 + 2 * t;
               if (d < dim) store2(o + d, none ? 0.f : acc[n][2 * h] * inv, none ? 0.f : acc[n][2 * h + 1] * inv);
             }
           } else {
-            // second half of a tile that began before this piece, or first of one that goes on
-            const float back = top_v / kUp;
-            float* out = p.part + (((long long)worker * 2 + (whole ? 1 : 0)) * 16 + g + 8 * h) * (dim + 2);
+            // a piece for the joining: slot 0 of a tile that began before, 1 of one that goes on
+            const float back = none ? 0.f : top_v / kUp;
+            float* out = p.part + (((long long)blockIdx.x * S::kWarps + warp) * 2 + (whole ? 1 : 0)) * 16 * rows_of +
+                         (g + 8 * h) * rows_of;
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n) {
               const int d = n * 8 + 2 * t;
@@ -586,67 +650,72 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
           }
         }
       }
-      if (whole && !last && lane == 0) {  // those after this warp have the rest
-        const long long c1 = i + (at.chunks - 1 - at.chunk);
-        p.meta[worker] = make_int4(at.b, at.h * p.tiles + at.tile, (int)(((c1 + 1) * workers - 1) / total), 1);
+      if (!(whole && last) && lane == 0) {
+        const long long c1 = i + (at.chunks - 1 - at.chunk);  // the tile's last chunk, and who has it
+        const int who = (int)((((c1 + 1) * workers - 1) / total) / per_cta);
+        left_at[warp * 2 + (whole ? 1 : 0)] =
+            make_int4(at.b, at.h * p.tiles + at.tile, (whole ? 1 : 0) | (last ? 2 : 0), who);
       }
       fresh = true;
     }
     if (i + 1 < end) advance(p, at);
   }
+  }  // works
+  __syncthreads();
+  // this CTA's pieces of a tile, one after the other in left_at, become one
+  for (int i = 0; i < S::kWarps * 2;) {
+    const int4 own = left_at[i];
+    if (own.x < 0) {
+      ++i;
+      continue;
+    }
+    int j = i, flags = own.z;  // the first piece says whether it began here, the last whether it ended
+    for (int k = i + 1; k < S::kWarps * 2; ++k) {
+      const int4 o = left_at[k];
+      if (o.x < 0) continue;
+      if (o.x != own.x || o.y != own.y) break;
+      j = k;
+      flags |= o.z & 2;
+    }
+    const int h = own.y / p.tiles, tile = own.y % p.tiles;
+    const bool begins = flags & 1, ends = flags & 2;
+    for (int r = warp; r < 16 && tile * 16 + r < p.rows; r += S::kWarps) {
+      const float* in = p.part + ((long long)blockIdx.x * S::kWarps * 2 * 16 + r) * rows_of;
+      Joined<DP> x;
+      x.join(in, 16 * rows_of, i, j, 1, dim, lane, left_at);
+      if (begins && ends) {
+        x.finish(static_cast<T*>(p.o) + row_offset(p, own.x, h, tile * 16 + r), dim, lane);
+      } else {
+        float* out = p.joint + (((long long)blockIdx.x * 2 + (begins ? 1 : 0)) * 16 + r) * rows_of;
+        x.keep(out, dim, lane);
+      }
+    }
+    if (begins && !ends && threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(own.x, own.y, own.w, 1);
+    i = j + 1;
+  }
 }
 
-// Joins the pieces of the tiles that several warps had: one CTA for each warp
-// that began such a tile; its warps share the pieces, row by row.
+// Joins the pieces of the tiles that several CTAs had: one CTA for each that
+// began such a tile, and each row of it; its warps share the pieces.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const Attend p) {
-  using q4::from_f;
-  __shared__ float sum[8][256];
-  __shared__ float mx[8], ls[8];
-  const int w0 = blockIdx.x;
-  const int4 meta = p.meta[w0];
-  if (meta.w == 0) return;
+  constexpr int kW = 8;
+  __shared__ float sums[kW][258];
+  const int c0 = blockIdx.x;
+  const int4 meta = p.meta[c0];
+  const int tile = meta.y % p.tiles, r = blockIdx.y;
+  if (meta.w == 0 || tile * 16 + r >= p.rows) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int b = meta.x, h = meta.y / p.tiles, tile = meta.y % p.tiles, w1 = meta.z;
-  const int group = p.heads_q / p.heads, dim = p.dim;
-  for (int r = tile * 16; r < min(p.rows, tile * 16 + 16); ++r) {
-    float m = -INFINITY, l = 0.f, a[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a[e] = 0.f;
-    for (int w = w0 + warp; w <= w1; w += 8) {
-      const float* in = p.part + (((long long)w * 2 + (w == w0 ? 1 : 0)) * 16 + r % 16) * (dim + 2);
-      const float mi = in[0], li = in[1];
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = lane + 32 * e < dim ? in[2 + lane + 32 * e] : 0.f;
-      const float n = fmaxf(m, mi), z = n == -INFINITY ? 0.f : n;
-      const float fa = exp2_approx(m - z), fb = exp2_approx(mi - z);
-      l = l * fa + li * fb;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) a[e] = a[e] * fa + x[e] * fb;
-      m = n;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum[warp][lane + 32 * e] = a[e];
-    if (lane == 0) {
-      mx[warp] = m;
-      ls[warp] = l;
-    }
-    __syncthreads();
-    float top = -INFINITY;
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, mx[w]);
-    if (top == -INFINITY) top = 0.f;
-    float den = 0.f;
-    for (int w = 0; w < 8; ++w) den += ls[w] * exp2_approx(mx[w] - top);
-    const float inv = den > 0.f || den != den ? 1.f / den : 0.f;
-    T* o = static_cast<T*>(p.o) + (((long long)b * p.S + r / group) * p.heads_q + h * group + r % group) * dim;
-    for (int d = threadIdx.x; d < dim; d += blockDim.x) {
-      float v = 0.f;
-      for (int w = 0; w < 8; ++w) v += sum[w][d] * exp2_approx(mx[w] - top);
-      o[d] = from_f<T>(v * inv);
-    }
-    __syncthreads();
-  }
+  const int rows_of = p.dim + 2;
+  // slot 1 of the first CTA, slot 0 of those after it
+  const float* in = p.joint + ((long long)c0 * 2 * 16 + r) * rows_of;
+  Joined<256> x;
+  x.join(in, 2 * 16 * rows_of, warp, meta.z - c0, kW, p.dim, lane, nullptr, 16 * rows_of);
+  x.keep(sums[warp], p.dim, lane);
+  __syncthreads();
+  if (warp != 0) return;
+  x.join(sums[0], 258, 0, kW - 1, 1, p.dim, lane, nullptr);
+  x.finish(static_cast<T*>(p.o) + row_offset(p, meta.x, meta.y / p.tiles, tile * 16 + r), p.dim, lane);
 }
 
 }  // namespace kv8

@@ -242,7 +242,7 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
       has[j] = m0 + 8 * j + g < M;
       xr[j] = x + (has[j] ? (m0 + 8 * j + g) * ldx : 0);
     }
-#pragma unroll 2
+#pragma unroll 4
     for (int kb = blockIdx.x * warps + warp; kb < kblocks; kb += splits * warps) {
       const long long blk = row_tile * kblocks + kb;
       const uint4 qa = ldg_stream(packed + blk * 64 + lane);
@@ -357,6 +357,7 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
 
   if (active) {
+#pragma unroll 2
     for (long long rt = blockIdx.x * warps + warp; rt < rtiles; rt += splits * warps) {
       const long long blk = rt * kblocks + kb;
       const long long n0 = rt * kRows;
@@ -472,7 +473,8 @@ int launch_cluster(F kernel, dim3 grid, int threads, int smem, int cluster, cuda
 }
 
 // CTAs of a cluster: as many (a power of two) as leave each warp a block and
-// the GPU no more than about two CTAs an SM.
+// the GPU no more than about two CTAs an SM (a cluster's barriers cost more
+// than a third CTA gains).
 int pick_splits(long long tiles, long long steps, int sms) {
   int s = 1;
   while (s < kMaxCluster && tiles * s * 2 <= 2LL * sms + sms / 2 && steps >= (long long)s * 2 * kWarps) s *= 2;

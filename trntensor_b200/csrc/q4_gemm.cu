@@ -81,10 +81,11 @@ int launch_tile(const CUtensorMap& map, const Gemm& p, int group, int R, int MT,
 template <typename XT>
 int convert(const void* x, long long ldx, const float* col, int M, int C, int Cp, int terms, int finite, void* out,
             float* f, cudaStream_t s) {
+  const int wide = aligned16(x) && ldx % (16 / (int)sizeof(XT)) == 0;
   if (terms == 2)
-    convert_kernel<XT, 2><<<M, 256, 0, s>>>((const XT*)x, ldx, col, M, C, Cp, (__half*)out, f, finite);
+    convert_kernel<XT, 2><<<M, 256, 0, s>>>((const XT*)x, ldx, col, M, C, Cp, wide, (__half*)out, f, finite);
   else
-    convert_kernel<XT, 1><<<M, 256, 0, s>>>((const XT*)x, ldx, col, M, C, Cp, (__half*)out, f, finite);
+    convert_kernel<XT, 1><<<M, 256, 0, s>>>((const XT*)x, ldx, col, M, C, Cp, wide, (__half*)out, f, finite);
   return cuda_status(cudaGetLastError());
 }
 

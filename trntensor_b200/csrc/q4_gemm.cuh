@@ -19,8 +19,8 @@
 // the L2 has to deliver only 40 bytes a clock and SM), the matrix's bytes for
 // few (the decoding warps then keep four blocks in flight each, and CTAs of a
 // cluster share the sum when there are too few tiles for all SMs).
-// Roles: warps 0-7 decode (registers to swizzled shared memory, then, at the
-// end, D to global memory), warp 8 issues the TMA loads, warp 9 the MMAs.
+// Roles: warps 0-15 decode (registers to swizzled shared memory, then, at the
+// end, D to global memory), warp 16 issues the TMA loads, warp 17 the MMAs.
 #pragma once
 #include "ptx.cuh"
 #include "ptx2sm.cuh"
@@ -29,7 +29,8 @@
 namespace tt {
 namespace q4 {
 
-constexpr int kGemmThreads = 320;
+constexpr int kDecodeWarps = 16;
+constexpr int kGemmThreads = (kDecodeWarps + 2) * 32;
 constexpr int kStageK = 64;  // terms of the sum in a stage: 128 bytes of fp16
 
 struct Gemm {
@@ -57,8 +58,10 @@ struct GemmShape {
   static constexpr int kStages = R == 2 ? 3 : MT == 256 ? 4 : MT == 128 ? 6 : 8;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
   static constexpr int kColumns = R * MT;
-  // blocks that a decoding warp keeps in flight, for each of its R
+  // half blocks that a decoding warp keeps in flight, for each of its R
   static constexpr int kDepth = R == 2 ? 2 : 4;
+  // TMEM columns that a warp brings out at the end
+  static constexpr int kOut = R * MT / 4 < 16 ? 16 : R * MT / 4;
   static_assert(kSmem <= 226 * 1024, "shared memory of an SM");
   static_assert(R == 2 || 128 * MT * 4 <= kStages * kStageBytes, "D fits where the stages were");
 };
@@ -76,9 +79,16 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-__device__ __forceinline__ float load_scale(const Gemm& p, long long i) {
-  return p.scales_f32 ? __ldg(static_cast<const float*>(p.scales) + i)
-                      : to_f(__ldg(static_cast<const __nv_bfloat16*>(p.scales) + i));
+// A scale's bits, and their value: apart, so that nothing waits for the load
+// before the value is wanted.
+__device__ __forceinline__ uint32_t load_scale(const Gemm& p, long long i) {
+  uint32_t v;
+  if (p.scales_f32) v = __ldg(static_cast<const uint32_t*>(p.scales) + i);
+  else v = __ldg(static_cast<const unsigned short*>(p.scales) + i);
+  return v;
+}
+__device__ __forceinline__ float scale_value(const Gemm& p, uint32_t bits) {
+  return __uint_as_float(p.scales_f32 ? bits : bits << 16);
 }
 __device__ __forceinline__ void store_out(const Gemm& p, long long i, float v) {
   if (p.type == kF32) static_cast<float*>(p.out)[i] = v;
@@ -97,7 +107,7 @@ template <int R, int MT, int kGroups, bool kTrans>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
   using S = GemmShape<R, MT>;
-  constexpr int kArrive = kTrans ? 4 : 8;  // decoding warps that fill a stage
+  constexpr int kArrive = 8;  // decoding warps that fill a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t full_a[S::kStages], full_b[S::kStages], empty[S::kStages], done;
@@ -123,7 +133,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     fence_mbar_init();
     tma_prefetch_desc(&mapB);
   }
-  if (warp == 9) {
+  if (warp == 17) {
     tmem_alloc(&tmem_slot, S::kColumns);
     tmem_relinquish();
   }
@@ -133,11 +143,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
   const uint32_t tmem = tmem_slot;
   bool ok = true;
 
-  if (warp == 8) {
+  if (warp == 16) {
     if (lane == 0) {
       uint32_t it = 0;
-      for (int i = 0; i < count && ok; ++i) {
-        const int pass = i / (s1 - s0), step = s0 + i % (s1 - s0);
+      for (int i = 0, pass = 0, step = s0; i < count && ok; ++i) {
         for (int sub = 0; sub < 2; ++sub, ++it) {
           const int s = it % S::kStages;
           if (!mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty)) {
@@ -148,12 +157,16 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
           tma_load_3d(smem + s * S::kStageBytes + S::kA, &mapB, &full_b[s], step * 128 + sub * 64, m0,
                       p.x_term[pass]);
         }
+        if (++step == s1) {
+          step = s0;
+          ++pass;
+        }
       }
       for (uint32_t k = it > S::kStages ? it - S::kStages : 0; k < it; ++k)
         mbar_wait_drain(&full_b[k % S::kStages], (k / S::kStages) & 1u);
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_f16(128, MT, kTrans ? 1 : 0);
       uint32_t it = 0;
@@ -184,118 +197,130 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     }
     __syncwarp();
   } else {
-    const int g = lane >> 2, t = lane & 3, odd = g & 1;
+    // A warp has row tile w8 of a step (or R of them) and the words 2 pair, 2
+    // pair + 1 of its blocks: 64 columns. Those are a stage of the sum over k,
+    // of which the step has two, or a column half of the sum over n, where
+    // four row tiles make a stage.
+    const int g = lane >> 2, t = lane & 3, odd = g & 1, w8 = warp & 7, pair = warp >> 3;
+    const uint32_t sub = kTrans ? w8 >> 2 : pair;
     const long long rtiles = ((long long)p.N + kRows - 1) / kRows;
+    constexpr int kScales = kGroups == 4 ? 2 : 1;  // of a word pair
     struct Piece {
-      uint4 q[R][2];
-      float s[R][2][kGroups];
+      uint2 q[R][2];
+      uint32_t s[R][2][kScales];
+      float e[2];  // kTrans: 2^e_n of the two rows
     };
     Piece ring[S::kDepth];
     float down[R][2];  // 2^-e_n of this lane's rows
-    auto norm = [&](long long n) -> float {
-      const float e = n < p.N ? __ldg(p.row_scale + n) : 1.f;
-      return __uint_as_float(0x7f000000u - __float_as_uint(e));  // exact: e is a power of two
-    };
+    auto inverse = [](float e) { return __uint_as_float(0x7f000000u - __float_as_uint(e)); };  // of a power of two
     if constexpr (!kTrans) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) down[r][h] = norm(row0 + r * 128 + warp * 16 + g + 8 * h);
+        for (int h = 0; h < 2; ++h) {
+          const long long n = row0 + r * 128 + w8 * 16 + g + 8 * h;
+          down[r][h] = n < p.N ? inverse(__ldg(p.row_scale + n)) : 1.f;
+        }
     }
-    auto fetch = [&](int i, Piece& x) {
-      const bool in = i < count;
-      const int step = in ? s0 + i % (s1 - s0) : 0;
+    int next = s0, left = count;  // step to fetch
+    auto fetch = [&](Piece& x) {
+      const bool in = left > 0;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const long long rt = kTrans ? step * 8LL + warp : row0 / 16 + r * 8 + warp;
-        const long long kb = kTrans ? row0 / 128 + r : step;
+        const long long rt = kTrans ? next * 8LL + w8 : row0 / 16 + r * 8 + w8;
+        const long long kb = kTrans ? row0 / 128 + r : next;
         const bool there = in && rt < rtiles && kb < p.kblocks;
         const long long blk = rt * p.kblocks + kb;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x.q[r][h] = there ? ldg_stream(p.packed + blk * 64 + h * 32 + lane)
-                            : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+          x.q[r][h] = there ? ldg_stream2(reinterpret_cast<const uint2*>(p.packed + blk * 64 + h * 32 + lane) + pair)
+                            : make_uint2(0x88888888u, 0x88888888u);
 #pragma unroll
-          for (int k = 0; k < kGroups; ++k)
-            x.s[r][h][k] = there ? load_scale(p, (blk * kGroups + k) * kRows + g + 8 * h) : 0.f;
+          for (int k = 0; k < kScales; ++k)
+            x.s[r][h][k] =
+                there ? load_scale(p, (blk * kGroups + pair * kGroups / 2 + k) * kRows + g + 8 * h) : 0u;
         }
       }
+      if constexpr (kTrans) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const long long n = next * 128LL + w8 * 16 + g + 8 * h;
+          x.e[h] = in && n < p.N ? __ldg(p.row_scale + n) : 1.f;
+        }
+      }
+      --left;
+      if (++next == s1) next = s0;
     };
 #pragma unroll
-    for (int d = 0; d < S::kDepth; ++d) fetch(d, ring[d]);
+    for (int d = 0; d < S::kDepth; ++d) fetch(ring[d]);
+    int pass = 0, step = s0, term = p.scale_term[0];
+    uint32_t it = sub;  // stage number
     for (int i0 = 0; i0 < count && ok; i0 += S::kDepth) {
 #pragma unroll
       for (int d = 0; d < S::kDepth; ++d) {
-        const int i = i0 + d;
-        if (i >= count || !ok) break;
+        if (i0 + d >= count || !ok) break;
         Piece& x = ring[d];
-        const int term = p.passes == 1 ? 0 : p.scale_term[i / (s1 - s0)];
         if constexpr (kTrans) {
-          const long long n = (s0 + i % (s1 - s0)) * 128LL + warp * 16 + g;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int r = 0; r < R; ++r) down[r][h] = inverse(x.e[h]);
+        }
+        uint4 v[R][2][2];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            down[0][h] = norm(n + 8 * h);
+            __half2 sc[kScales];
 #pragma unroll
-            for (int r = 1; r < R; ++r) down[r][h] = down[0][h];
-          }
-        }
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          if (kTrans && sub != warp >> 2) continue;  // four warps a stage
-          const uint32_t it = 2u * i + sub;
-          const int s = it % S::kStages;
-          ok = mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const uint32_t base = smem_u32(smem + s * S::kStageBytes);
-#pragma unroll
-          for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint32_t word[4] = {x.q[r][h].x, x.q[r][h].y, x.q[r][h].z, x.q[r][h].w};
-              __half2 sc[kGroups];
-#pragma unroll
-              for (int k = 0; k < kGroups; ++k) {
-                const float v = x.s[r][h][k] * down[r][h];
-                sc[k] = __float2half2_rn(p.scales_f32 ? scale_term(v, term) : v);
-              }
-#pragma unroll
-              for (int pair = kTrans ? 0 : sub; pair < (kTrans ? 2 : sub + 1); ++pair)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  // odd rows take the pair's words the other way round: eight
-                  // lanes then meet all 32 banks
-                  const uint32_t wd = odd ? word[2 * pair + (e ^ 1)] : word[2 * pair + e];
-                  constexpr int kPer = 4 / kGroups;
-                  const __half2 sh =
-                      kGroups < 4 ? sc[2 * pair / kPer]
-                                  : (odd ? sc[(2 * pair + (e ^ 1)) / kPer] : sc[(2 * pair + e) / kPer]);
-                  uint32_t v[4];
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) {
-                    const uint32_t c = decode_pair<true>(wd >> (4 * j));
-                    const __half2 y = __hmul2(reinterpret_cast<const __half2&>(c), sh);
-                    v[j] = reinterpret_cast<const uint32_t&>(y);
-                  }
-                  const uint32_t chunk = (uint32_t)((e ^ odd) * 4 + t);
-                  uint32_t at;
-                  if constexpr (kTrans) {
-                    const uint32_t n = (warp & 3) * 16 + g + 8 * h;
-                    at = base + (2 * r + pair) * 8192 + n * 128 + ((chunk ^ (n & 7)) << 4);
-                  } else {
-                    const uint32_t n = r * 128 + warp * 16 + g + 8 * h;
-                    at = base + n * 128 + ((chunk ^ (n & 7)) << 4);
-                  }
-                  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[0]), "r"(v[1]),
-                               "r"(v[2]), "r"(v[3])
-                               : "memory");
-                }
+            for (int k = 0; k < kScales; ++k) {
+              const float f = scale_value(p, x.s[r][h][k]) * down[r][h];
+              sc[k] = __float2half2_rn(p.scales_f32 ? scale_term(f, term) : f);
             }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full_a[s]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // odd rows take the pair's words the other way round: eight
+              // lanes then meet all 32 banks
+              const uint32_t wd = (e == odd) ? x.q[r][h].x : x.q[r][h].y;
+              const __half2 sh = kScales == 1 ? sc[0] : (e == odd ? sc[0] : sc[kScales - 1]);
+              uint32_t y[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t c = decode_pair<true>(wd >> (4 * j));
+                const __half2 z = __hmul2(reinterpret_cast<const __half2&>(c), sh);
+                y[j] = reinterpret_cast<const uint32_t&>(z);
+              }
+              v[r][h][e] = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+          }
+        fetch(x);
+        const int s = it % S::kStages;
+        ok = mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t base = smem_u32(smem + s * S::kStageBytes);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t n = kTrans ? (w8 & 3) * 16 + g + 8 * h : r * 128 + w8 * 16 + g + 8 * h;
+              const uint32_t chunk = (uint32_t)((e ^ odd) * 4 + t);
+              const uint32_t at = base + (kTrans ? (2 * r + pair) * 8192 : 0) + n * 128 + ((chunk ^ (n & 7)) << 4);
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v[r][h][e].x), "r"(v[r][h][e].y),
+                           "r"(v[r][h][e].z), "r"(v[r][h][e].w)
+                           : "memory");
+            }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full_a[s]);
+        it += 2;
+        if (++step == s1) {
+          step = s0;
+          ++pass;
+          if (pass < p.passes) term = p.scale_term[pass];
         }
-        fetch(i + S::kDepth, x);
       }
     }
     // D: lanes are rows of the tile, columns are tokens
@@ -303,10 +328,12 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     if (ok && active) {
-      const int quad = warp & 3, half = warp >> 2;
-      const long long row = row0 + (R == 2 ? half * 128 : 0) + quad * 32 + lane;
-      const int c0 = R == 2 ? 0 : half * (MT / 2), c1 = R == 2 ? MT : c0 + MT / 2;
-      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + (R == 2 ? half * MT : 0);
+      // a quarter of the columns each: of all 2 MT, rows 128 and up behind MT
+      const int quad = warp & 3, first = (warp >> 2) * S::kOut;
+      const int half = R == 2 ? first / MT : 0;
+      const long long row = row0 + half * 128 + quad * 32 + lane;
+      const int c0 = first - half * MT, c1 = first < S::kColumns ? c0 + S::kOut : c0;
+      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * MT;
       const float up = !kTrans && row < rows ? __ldg(p.row_scale + row) : 1.f;
       float* dsm = reinterpret_cast<float*>(smem);
       for (int c = c0; c < c1; c += 16) {
@@ -351,7 +378,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kColumns);
   }
@@ -389,16 +416,41 @@ __global__ void row_scale_kernel(const ST* __restrict__ scales, int N, int kbloc
 // enters the sum once).
 template <typename XT, int kTerms>
 __global__ void __launch_bounds__(256)
-convert_kernel(const XT* __restrict__ x, long long ldx, const float* __restrict__ col, int M, int C, int Cp,
+convert_kernel(const XT* __restrict__ x, long long ldx, const float* __restrict__ col, int M, int C, int Cp, int wide,
                __half* __restrict__ out, float* __restrict__ f, int finite) {
   __shared__ uint32_t tops[8];
   const int m = blockIdx.x;
   const XT* row = x + m * ldx;
+  // eight neighbouring values of the row, zeros behind its end
+  auto eight = [&](int i, float (&v)[8]) {
+    constexpr int kPer = 16 / sizeof(XT);
+    if (wide && i + 8 <= C) {
+#pragma unroll
+      for (int j = 0; j < 8 / kPer; ++j) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + i) + j);
+        const XT* e = reinterpret_cast<const XT*>(&u);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) v[j * kPer + k] = to_f(e[k]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j < C ? to_f(__ldg(row + i + j)) : 0.f;
+    }
+    if (col) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= i + j < C ? __ldg(col + i + j) : 1.f;
+    }
+  };
   uint32_t top = 0;
-  for (int i = threadIdx.x; i < C; i += 256) {
-    const float v = to_f(row[i]) * (col ? __ldg(col + i) : 1.f);
-    const uint32_t b = __float_as_uint(fabsf(v));
-    if (b < 0x7f800000u) top = max(top, b);
+#pragma unroll 2
+  for (int i = threadIdx.x * 8; i < C; i += 2048) {
+    float v[8];
+    eight(i, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = __float_as_uint(fabsf(v[j]));
+      top = max(top, b < 0x7f800000u ? b : 0u);
+    }
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
@@ -410,16 +462,28 @@ convert_kernel(const XT* __restrict__ x, long long ldx, const float* __restrict_
   const float up = __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(140 - e)
   if (threadIdx.x == 0) f[m] = __uint_as_float((uint32_t)(e - 13) << 23);
   __half* hi = out + (long long)m * Cp;
-  __half* lo = hi + (long long)M * Cp;
-  __half* fin = lo + (kTerms == 2 ? (long long)M * Cp : 0);
-  for (int i = threadIdx.x; i < Cp; i += 256) {
-    const float v = i < C ? to_f(row[i]) * (col ? __ldg(col + i) : 1.f) * up : 0.f;
-    const __half h = __float2half_rn(v);
-    hi[i] = h;
-    if (finite) fin[i] = isfinite(v) ? h : __float2half_rn(0.f);
+  const long long plane = (long long)M * Cp;
+  auto put = [&](__half* at, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(at) =
+        make_uint4(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]), pack_f16(v[4], v[5]), pack_f16(v[6], v[7]));
+  };
+#pragma unroll 2
+  for (int i = threadIdx.x * 8; i < Cp; i += 2048) {
+    float v[8];
+    eight(i, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= up;
+    put(hi + i, v);
     if (kTerms == 2) {
-      const float r = v - __half2float(h);
-      lo[i] = __float2half_rn(isfinite(v) ? r : 0.f);
+      float lo[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) lo[j] = isfinite(v[j]) ? v[j] - __half2float(__float2half_rn(v[j])) : 0.f;
+      put(hi + plane + i, lo);
+    }
+    if (finite) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = isfinite(v[j]) ? v[j] : 0.f;
+      put(hi + kTerms * plane + i, v);
     }
   }
 }
