@@ -50,8 +50,16 @@ int launch(const Attend& p, int sms, cudaStream_t s) {
   attend_kernel<T, DP, kTerms><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
   int st = cuda_status(cudaGetLastError());
   if (st != TT_OK) return st;
-  join_kernel<T><<<dim3(sms, p.rows < 16 ? p.rows : 16), 256, 0, s>>>(p);
-  return cuda_status(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sms, p.rows < 16 ? p.rows : 16);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, join_kernel<T>, p));
 }
 template <typename T>
 int launch_dim(const Attend& p, int sms, cudaStream_t s) {
@@ -112,6 +120,7 @@ int tt_kv8_attention(const void* q, int type, long long q_stride_b, long long q_
   p.scale = *scale * 1.4426950408889634f;
   p.causal = causal;
   p.batch = batch; p.S = S; p.heads_q = heads_q; p.heads = heads; p.dim = dim; p.page = page; p.pages = pages;
+  p.page_log = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   p.cols = columns;
   p.rows = (int)rows;
   p.tiles = (int)((rows + 15) / 16);

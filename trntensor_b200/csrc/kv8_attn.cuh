@@ -58,7 +58,7 @@ struct Attend {
   int* status;
   float scale;  // times log2(e)
   int causal;
-  int batch, S, heads_q, heads, dim, page, pages, cols, rows, tiles;
+  int batch, S, heads_q, heads, dim, page, page_log, pages, cols, rows, tiles;
 };
 
 template <int DP, int kTerms>
@@ -66,7 +66,7 @@ struct Shape {
   static constexpr bool kQRegs = DP <= 128 && kTerms == 1;
   static constexpr int kWarps = DP <= 128 ? 8 : 4;
   static constexpr int kUnit = 16 * DP;
-  static constexpr int kSlot = 4 * (kUnit + 32);
+  static constexpr int kSlot = 4 * (kUnit + 32) + 16;  // four units, and their scales
   static constexpr int kSlots = DP == 64 ? 5 : DP == 192 ? 3 : kTerms == 1 ? 3 : 2;
   static constexpr int kQBytes = kQRegs ? 0 : kTerms * 16 * DP * 2;
   static constexpr int kSmem = kWarps * (kSlots * kSlot + kQBytes);
@@ -78,6 +78,17 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
+}
+// Four bytes into shared memory (zeros where not `on`), noted on the barrier
+// when they and all of this lane's earlier ones are there.
+__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool on, uint32_t bar) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float lds32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
 }
 // Bounded wait: false when the copy has not arrived within the budget.
 __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity) {
@@ -258,7 +269,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
   const int dim = p.dim;
   const uint32_t unit_bytes = 16 * dim;
 
-  if (lane < S::kSlots) mbar_init(bar + lane, 1);
+  if (lane < S::kSlots) mbar_init(bar + lane, 1 + 4);  // the units' bytes, and a scale each
   fence_mbar_init();
   __syncwarp();
 
@@ -274,6 +285,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
   }
   if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
   __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // this warp's piece of the line
   const long long total = chunk_sum(p, p.batch, lane);
@@ -324,55 +336,49 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
   long long left = end - begin;  // chunks not yet asked for
   // page of this lane's unit of a place; -1 behind the sequence's end
   auto page_at = [&](const Place& x) -> int {
-    const long long tok = (long long)x.chunk * kChunk + 16 * t;
-    if (tok >= x.length) return -1;
-    const int page = p.table[x.b * p.table_b + tok / p.page];
-    if (page < 0 || page >= p.pages) {
-      if (g == 0) raise(p.status, kBadPage);
-      return -1;
-    }
-    return page;
-  };
-  auto offset_of = [&](const Place& x, int page) -> long long {
-    const long long tok = (long long)x.chunk * kChunk + 16 * t;
-    return (((long long)page * p.heads + x.h) * p.page + tok % p.page) * dim;
+    const int tok = x.chunk * kChunk + 16 * t;
+    if (tok >= (int)x.length) return -1;
+    return p.table[x.b * p.table_b + (tok >> p.page_log)];
   };
   uint32_t slot_in = 0;
-  auto ask = [&](const unsigned char* codes, int page, long long offset) {
+  auto ask = [&](const unsigned char* codes, const float* scales, int page, int h, int tok) {
     const unsigned has = __ballot_sync(0xffffffffu, page >= 0) & 15u;
     uint64_t* b = bar + slot_in;
+    unsigned char* to = mine + slot_in * S::kSlot;
     if (lane == 0) mbar_arrive_expect_tx(b, __popc(has) * unit_bytes);
     __syncwarp();
-    if (lane < 4 && page >= 0)
-      bulk_load(smem_u32(mine + slot_in * S::kSlot + t * (S::kUnit + 32)), codes + offset, unit_bytes, smem_u32(b));
+    if (lane < 4) {
+      const long long head = (long long)max(page, 0) * p.heads + h;
+      if (page >= 0)
+        bulk_load(smem_u32(to + t * (S::kUnit + 32)),
+                  codes + (head * p.page + (tok & (p.page - 1))) * dim, unit_bytes, smem_u32(b));
+      copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 4 * t), scales + head, page >= 0, smem_u32(b));
+    }
     slot_in = slot_in + 1 == S::kSlots ? 0 : slot_in + 1;
   };
 
   // Copies are asked for in the order K0 V0 K1 V1 ..., always kSlots ahead.
-  // page_k is the page of the chunk whose keys come next, page_v and off_v of
-  // the one whose keys were asked for last.
-  int page_k = page_at(ahead), page_v = -1;
-  long long off_v = 0;
+  // page_k is the page of the chunk whose keys come next (read from the table
+  // one chunk before it is used), the others are of the one whose keys were
+  // asked for last.
+  int page_k = page_at(ahead), page_v = -1, head_v = 0, tok_v = 0;
   bool want_values = false;  // the next copy is of values
-  int asked = 0;             // chunks whose keys are asked for and not consumed, and their scales
-  float fsk[3] = {0.f, 0.f, 0.f}, fsv[3] = {0.f, 0.f, 0.f};
   auto ask_next = [&]() {
     if (want_values) {
-      ask(p.vc, page_v, off_v);
+      ask(p.vc, p.vs, page_v, head_v, tok_v);
       want_values = false;
       return;
     }
     if (left == 0) return;
     --left;
+    if (page_k >= p.pages || (page_k < 0 && ahead.chunk * kChunk + 16 * t < (int)ahead.length)) {
+      if (g == 0) raise(p.status, kBadPage);
+      page_k = -1;
+    }
     page_v = page_k;
-    off_v = page_k >= 0 ? offset_of(ahead, page_k) : 0;
-    const long long at_scale = (long long)page_k * p.heads + ahead.h;
-    const float nsk = page_k >= 0 ? p.ks[at_scale] : 0.f, nsv = page_k >= 0 ? p.vs[at_scale] : 0.f;
-    if (asked == 0) { fsk[0] = nsk; fsv[0] = nsv; }
-    else if (asked == 1) { fsk[1] = nsk; fsv[1] = nsv; }
-    else { fsk[2] = nsk; fsv[2] = nsv; }
-    ++asked;
-    ask(p.kc, page_k, off_v);
+    head_v = ahead.h;
+    tok_v = ahead.chunk * kChunk + 16 * t;
+    ask(p.kc, p.ks, page_v, head_v, tok_v);
     want_values = true;
     if (left > 0) {
       advance(p, ahead);
@@ -403,7 +409,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
   uint32_t qf[S::kQRegs ? DP / 16 : 1][4];
   unsigned char* qs = smem + S::kWarps * S::kSlots * S::kSlot + warp * S::kQBytes;  // [step][term][lane][4]
   float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f, top_v = 0.f, qs0 = 0.f, qs1 = 0.f;
-  long long lim0 = 0, lim1 = 0, lim_min = 0;
+  int lim0 = 0, lim1 = 0, lim_min = 0;
   bool fresh = true, whole = true;
 
   for (long long i = begin; i < end; ++i) {
@@ -412,7 +418,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
       whole = at.chunk == 0;
       const int count = clamp_count(p, at.b, false);
       float top[2], x[2][DP / 64][16];
-      long long lim[2];
+      int lim[2];
       bool has[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
         const int tok = r / group, head = at.h * group + r % group;
         has[h] = r < p.rows && tok < count;
         const T* row = static_cast<const T*>(p.q) + at.b * p.q_b + (has[h] ? tok * p.q_s + head * p.q_h : 0);
-        lim[h] = !has[h] ? 0 : p.causal ? at.length - count + tok + 1 : at.length;
+        lim[h] = !has[h] ? 0 : p.causal ? (int)at.length - count + tok + 1 : (int)at.length;
         if (lim[h] < 0) lim[h] = 0;
         float m = 0.f;
 #pragma unroll
@@ -471,7 +477,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
       qs1 = down[1] * p.scale;
       lim0 = lim[0];
       lim1 = lim[1];
-      lim_min = min(has[0] ? lim0 : at.length, has[1] ? lim1 : at.length);
+      lim_min = min(has[0] ? lim0 : (int)at.length, has[1] ? lim1 : (int)at.length);
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
       m0 = m1 = -INFINITY;
@@ -507,31 +513,31 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
               qa[w][k][0] = v.x; qa[w][k][1] = v.y; qa[w][k][2] = v.z; qa[w][k][3] = v.w;
             }
           }
+        // four tiles at a time, so that neighbouring products are of different sums
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint4 v = lds128(keys + 2 * j * dim + c * 64);
-          const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+        for (int j0 = 0; j0 < 8; j0 += 4) {
+          uint4 v[4];
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            uint32_t lo, hi;
-            decode4(word[w], lo, hi);
+          for (int j = 0; j < 4; ++j) v[j] = lds128(keys + 2 * (j0 + j) * dim + c * 64);
 #pragma unroll
-            for (int k = 0; k < kTerms; ++k)
-              q4::mma16816<true>(s[j], qa[w][k][0], qa[w][k][1], qa[w][k][2], qa[w][k][3], lo, hi);
-          }
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t lo, hi;
+              decode4(w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w, lo, hi);
+#pragma unroll
+              for (int k = 0; k < kTerms; ++k)
+                q4::mma16816<true>(s[j0 + j], qa[w][k][0], qa[w][k][1], qa[w][k][2], qa[w][k][3], lo, hi);
+            }
         }
       }
     }
-    const float sk = fsk[0], sv = fsv[0];
-    // the ring of scales moves on before the next chunk is asked for
-    fsk[0] = fsk[1]; fsk[1] = fsk[2];
-    fsv[0] = fsv[1]; fsv[1] = fsv[2];
-    --asked;
+    const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * t);
     release();
 
     const float f0 = qs0 * sk, f1 = qs1 * sk;
-    const long long tok0 = (long long)at.chunk * kChunk + 16 * t;
-    const bool mask = (long long)(at.chunk + 1) * kChunk > lim_min;
+    const int tok0 = at.chunk * kChunk + 16 * t;
+    const bool mask = (at.chunk + 1) * kChunk > lim_min;
     float n0 = m0, n1 = m1;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -551,6 +557,9 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
     n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
     n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+    arrive();
+    if (!alive) break;
+    const float sv = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * t);
     // largest value scale so far; a NaN stays in its own page's weights
     float nv = fmaxf(top_v, sv);
     nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 1));
@@ -594,22 +603,23 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
         split_f16<kTerms>(y[0], y[1], w[kk][2 * half]);
         split_f16<kTerms>(y[2], y[3], w[kk][2 * half + 1]);
       }
-    arrive();
-    if (!alive) break;
     {
       const uint32_t vals = smem_u32(mine + slot * S::kSlot) + t * (S::kUnit + 32) + g * 16;
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        const uint4 v = lds128(vals + n * 128);
-        const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+      for (int n0 = 0; n0 < DP / 8; n0 += 4) {
+        uint4 v[4];
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          uint32_t lo, hi;
-          decode4(word[kk], lo, hi);
+        for (int n = 0; n < 4; ++n) v[n] = lds128(vals + (n0 + n) * 128);
 #pragma unroll
-          for (int k = 0; k < kTerms; ++k)
-            q4::mma16816<true>(acc[n], w[kk][0][k], w[kk][1][k], w[kk][2][k], w[kk][3][k], lo, hi);
-        }
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            uint32_t lo, hi;
+            decode4(kk == 0 ? v[n].x : kk == 1 ? v[n].y : kk == 2 ? v[n].z : v[n].w, lo, hi);
+#pragma unroll
+            for (int k = 0; k < kTerms; ++k)
+              q4::mma16816<true>(acc[n0 + n], w[kk][0][k], w[kk][1][k], w[kk][2][k], w[kk][3][k], lo, hi);
+          }
       }
     }
     release();
@@ -701,6 +711,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const Attend p) {
   constexpr int kW = 8;
   __shared__ float sums[kW][258];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early, runs after attend_kernel
   const int c0 = blockIdx.x;
   const int4 meta = p.meta[c0];
   const int tile = meta.y % p.tiles, r = blockIdx.y;

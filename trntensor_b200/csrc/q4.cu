@@ -242,48 +242,73 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
       has[j] = m0 + 8 * j + g < M;
       xr[j] = x + (has[j] ? (m0 + 8 * j + g) * ldx : 0);
     }
-#pragma unroll 4
-    for (int kb = blockIdx.x * warps + warp; kb < kblocks; kb += splits * warps) {
-      const long long blk = row_tile * kblocks + kb;
-      const uint4 qa = ldg_stream(packed + blk * 64 + lane);
-      const uint4 qb = ldg_stream(packed + blk * 64 + 32 + lane);
-      const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
-      uint32_t xp[kTiles][4][kTerms][4];
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          load_eight<XT, kTerms>(xr[j], (long long)kb * kCols + 32 * w + 8 * t, has[j] ? K : 0,
-                                 wide != 0, xp[j][w]);
+    // A ring of blocks in registers: codes, scales and the tokens' values are
+    // asked for kDepth blocks ahead.
+    constexpr int kDepth = kTerms == 1 ? (kTiles == 1 ? 4 : 2) : 2;
+    constexpr bool kF32Scale = sizeof(ST) == 4;
+    struct Piece {
+      uint4 qa, qb;
+      uint32_t s[kGroups][2];
+    };
+    Piece ring[kDepth];
+    const int stride = splits * warps;
+    int next = blockIdx.x * warps + warp;
+    auto fetch = [&](Piece& f) {  // behind the last block: the last again, for nothing
+      const long long blk = row_tile * kblocks + min(next, kblocks - 1);
+      f.qa = ldg128(packed + blk * 64 + lane);
+      f.qb = ldg128(packed + blk * 64 + 32 + lane);
 #pragma unroll
       for (int gi = 0; gi < kGroups; ++gi) {
-        float c[kTiles][4];
+        f.s[gi][0] = scale_word(scales, kF32Scale, (blk * kGroups + gi) * kRows + g);
+        f.s[gi][1] = scale_word(scales, kF32Scale, (blk * kGroups + gi) * kRows + g + 8);
+      }
+      next += stride;
+    };
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) fetch(ring[d]);
+    for (int kb0 = blockIdx.x * warps + warp; kb0 < kblocks; kb0 += stride * kDepth) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d) {
+        const int kb = kb0 + d * stride;
+        if (kb >= kblocks) break;
+        uint32_t xp[kTiles][4][kTerms][4];
 #pragma unroll
         for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+          for (int w = 0; w < 4; ++w)
+            load_eight<XT, kTerms>(xr[j], (long long)kb * kCols + 32 * w + 8 * t, has[j] ? K : 0, wide != 0, xp[j][w]);
+        const Piece f = ring[d];
+        fetch(ring[d]);
+        const uint32_t wa[4] = {f.qa.x, f.qa.y, f.qa.z, f.qa.w}, wb[4] = {f.qb.x, f.qb.y, f.qb.z, f.qb.w};
 #pragma unroll
-        for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w)
+        for (int gi = 0; gi < kGroups; ++gi) {
+          float c[kTiles][4];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t a0 = decode_pair<kHalf>(wa[w] >> (8 * half));
-            const uint32_t a1 = decode_pair<kHalf>(wb[w] >> (8 * half));
-            const uint32_t a2 = decode_pair<kHalf>(wa[w] >> (8 * half + 4));
-            const uint32_t a3 = decode_pair<kHalf>(wb[w] >> (8 * half + 4));
+          for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j)
+            for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
 #pragma unroll
-              for (int i = 0; i < kTerms; ++i)
-                mma16816<kHalf>(c[j], a0, a1, a2, a3, xp[j][w][i][2 * half], xp[j][w][i][2 * half + 1]);
+          for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t a0 = decode_pair<kHalf>(wa[w] >> (8 * half));
+              const uint32_t a1 = decode_pair<kHalf>(wb[w] >> (8 * half));
+              const uint32_t a2 = decode_pair<kHalf>(wa[w] >> (8 * half + 4));
+              const uint32_t a3 = decode_pair<kHalf>(wb[w] >> (8 * half + 4));
+#pragma unroll
+              for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                for (int i = 0; i < kTerms; ++i)
+                  mma16816<kHalf>(c[j], a0, a1, a2, a3, xp[j][w][i][2 * half], xp[j][w][i][2 * half + 1]);
+            }
+          const float s0 = scale_value(f.s[gi][0], kF32Scale, g & 1), s1 = scale_value(f.s[gi][1], kF32Scale, g & 1);
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j) {
+            acc[j][0] += s0 * c[j][0];
+            acc[j][1] += s0 * c[j][1];
+            acc[j][2] += s1 * c[j][2];
+            acc[j][3] += s1 * c[j][3];
           }
-        const ST* sp = scales + (blk * kGroups + gi) * kRows + g;
-        const float s0 = to_f(sp[0]), s1 = to_f(sp[8]);
-#pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          acc[j][0] += s0 * c[j][0];
-          acc[j][1] += s0 * c[j][1];
-          acc[j][2] += s1 * c[j][2];
-          acc[j][3] += s1 * c[j][3];
         }
       }
     }
@@ -324,6 +349,14 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
   }
 }
 
+// A value from its bits (16-bit types in the low half).
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t bits) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)bits));
+  else return __uint_as_float(bits << 16);
+}
+
 // ------------------------------------------------------------ dx = dy W, few rows
 
 // A CTA owns 128 columns of W and 16 tokens; the rows of W are shared among
@@ -357,50 +390,73 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
 
   if (active) {
-#pragma unroll 2
-    for (long long rt = blockIdx.x * warps + warp; rt < rtiles; rt += splits * warps) {
-      const long long blk = rt * kblocks + kb;
-      const long long n0 = rt * kRows;
-      // rows 2t, 2t+1 (half 0) and 8+2t, 9+2t (half 1); the words of t' = g / 2
-      uint4 q[4];
+    constexpr bool kF32Scale = sizeof(ST) == 4;
+    struct Piece {
+      uint4 q[4];               // rows 2t, 2t+1 (half 0) and 8+2t, 9+2t (half 1); the words of t' = g / 2
+      uint32_t d[2][4];         // token g / g + 8, rows as in q: bits of dy
+      uint32_t s[kGroups][4];
+    };
+    constexpr int kDepth = 2;
+    Piece ring[kDepth];
+    const long long stride = splits * warps;
+    long long next = blockIdx.x * warps + warp;
+    auto fetch = [&](Piece& f) {  // behind the last row tile: the last again, for nothing
+      const long long rt = min(next, rtiles - 1), blk = rt * kblocks + kb;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        q[r] = __ldg(packed + blk * 64 + (r >> 1) * 32 + (2 * t + (r & 1)) * 4 + (g >> 1));
-      float d[2][4];  // token g / g + 8, rows as in q
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long m = m0 + g + 8 * h;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const long long n = n0 + (r >> 1) * 8 + 2 * t + (r & 1);
-          d[h][r] = m < M && n < N ? to_f(dy[m * lddy + n]) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int gi = 0; gi < kGroups; ++gi) {
-        const ST* sp = scales + (blk * kGroups + gi) * kRows + 2 * t;
-        const float s[4] = {to_f(sp[0]), to_f(sp[1]), to_f(sp[8]), to_f(sp[9])};
-        uint32_t a[4][kTerms];  // a0: token g rows 0,1; a1: token g+8; a2, a3: rows 2,3
+      for (int r = 0; r < 4; ++r) {
+        f.q[r] = ldg128(packed + blk * 64 + (r >> 1) * 32 + (2 * t + (r & 1)) * 4 + (g >> 1));
+        const long long n = min(rt * kRows + (r >> 1) * 8 + 2 * t + (r & 1), (long long)N - 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          split_bf16<kTerms>(d[h][0] * s[0], d[h][1] * s[1], a[h]);
-          split_bf16<kTerms>(d[h][2] * s[2], d[h][3] * s[3], a[2 + h]);
+          const XT* at = dy + min(m0 + g + 8 * h, (long long)M - 1) * lddy + n;
+          f.d[h][r] = sizeof(XT) == 4 ? ldg32(at) : ldg16(at);
         }
 #pragma unroll
-        for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w) {
-          const uint32_t sel = g & 1 ? 0x7632 : 0x5410;
-          const uint32_t w0 = w == 0 ? q[0].x : w == 1 ? q[0].y : w == 2 ? q[0].z : q[0].w;
-          const uint32_t w1 = w == 0 ? q[1].x : w == 1 ? q[1].y : w == 2 ? q[1].z : q[1].w;
-          const uint32_t w2 = w == 0 ? q[2].x : w == 1 ? q[2].y : w == 2 ? q[2].z : q[2].w;
-          const uint32_t w3 = w == 0 ? q[3].x : w == 1 ? q[3].y : w == 2 ? q[3].z : q[3].w;
-          const uint32_t lo = __byte_perm(w0, w1, sel), hi = __byte_perm(w2, w3, sel);
+        for (int gi = 0; gi < kGroups; ++gi)
+          f.s[gi][r] = scale_word(scales, kF32Scale, (blk * kGroups + gi) * kRows + (r >> 1) * 8 + 2 * t + (r & 1));
+      }
+      next += stride;
+    };
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t b0 = decode_pair<false>(lo >> (4 * j));
-            const uint32_t b1 = decode_pair<false>(hi >> (4 * j));
+    for (int d = 0; d < kDepth; ++d) fetch(ring[d]);
+    for (long long rt0 = blockIdx.x * warps + warp; rt0 < rtiles; rt0 += stride * kDepth) {
 #pragma unroll
-            for (int i = 0; i < kTerms; ++i)
-              mma16816<false>(acc[4 * w + j], a[0][i], a[1][i], a[2][i], a[3][i], b0, b1);
+      for (int dd = 0; dd < kDepth; ++dd) {
+        if (rt0 + dd * stride >= rtiles) break;
+        const Piece f = ring[dd];
+        fetch(ring[dd]);
+        float d[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const long long n = (rt0 + dd * stride) * kRows + (r >> 1) * 8 + 2 * t + (r & 1);
+            d[h][r] = m0 + g + 8 * h < M && n < N ? value_of<XT>(f.d[h][r]) : 0.f;
+          }
+#pragma unroll
+        for (int gi = 0; gi < kGroups; ++gi) {
+          float s[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[r] = scale_value(f.s[gi][r], kF32Scale, r & 1);
+          uint32_t a[4][kTerms];  // a0: token g rows 0,1; a1: token g+8; a2, a3: rows 2,3
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            split_bf16<kTerms>(d[h][0] * s[0], d[h][1] * s[1], a[h]);
+            split_bf16<kTerms>(d[h][2] * s[2], d[h][3] * s[3], a[2 + h]);
+          }
+#pragma unroll
+          for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w) {
+            const uint32_t sel = g & 1 ? 0x7632 : 0x5410;
+            auto word = [&](int r) { return w == 0 ? f.q[r].x : w == 1 ? f.q[r].y : w == 2 ? f.q[r].z : f.q[r].w; };
+            const uint32_t lo = __byte_perm(word(0), word(1), sel), hi = __byte_perm(word(2), word(3), sel);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t b0 = decode_pair<false>(lo >> (4 * j));
+              const uint32_t b1 = decode_pair<false>(hi >> (4 * j));
+#pragma unroll
+              for (int i = 0; i < kTerms; ++i)
+                mma16816<false>(acc[4 * w + j], a[0][i], a[1][i], a[2][i], a[3][i], b0, b1);
+            }
           }
         }
       }

@@ -112,18 +112,37 @@ __device__ __forceinline__ void split_bf16(float a, float b, uint32_t (&out)[kTe
   out[kTerms - 1] = pack_bf16(a, b);
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+// Plain loads, volatile: moved towards their use, or with a conversion beside
+// them, they would make the warp wait there and then. Callers give an address
+// that holds, and drop what they did not want when they use it.
+__device__ __forceinline__ uint4 ldg128(const void* p) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
   return v;
 }
-
-__device__ __forceinline__ uint2 ldg_stream2(const void* p) {
+__device__ __forceinline__ uint2 ldg64(const void* p) {
   uint2 v;
-  asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
+}
+__device__ __forceinline__ uint32_t ldg32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg16(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+// The word that holds scale i (bf16: with its neighbour), and the scale in it.
+__device__ __forceinline__ uint32_t scale_word(const void* scales, bool f32, long long i) {
+  return ldg32(static_cast<const char*>(scales) + (f32 ? 4 * i : (2 * i & ~3LL)));
+}
+__device__ __forceinline__ float scale_value(uint32_t word, bool f32, int odd) {
+  return __uint_as_float(f32 ? word : odd ? word & 0xffff0000u : word << 16);
 }
 
 }  // namespace q4

@@ -79,17 +79,6 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, int a_mn) {
   return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// A scale's bits, and their value: apart, so that nothing waits for the load
-// before the value is wanted.
-__device__ __forceinline__ uint32_t load_scale(const Gemm& p, long long i) {
-  uint32_t v;
-  if (p.scales_f32) v = __ldg(static_cast<const uint32_t*>(p.scales) + i);
-  else v = __ldg(static_cast<const unsigned short*>(p.scales) + i);
-  return v;
-}
-__device__ __forceinline__ float scale_value(const Gemm& p, uint32_t bits) {
-  return __uint_as_float(p.scales_f32 ? bits : bits << 16);
-}
 __device__ __forceinline__ void store_out(const Gemm& p, long long i, float v) {
   if (p.type == kF32) static_cast<float*>(p.out)[i] = v;
   else if (p.type == kBF16) static_cast<__nv_bfloat16*>(p.out)[i] = from_f<__nv_bfloat16>(v);
@@ -208,7 +197,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     struct Piece {
       uint2 q[R][2];
       uint32_t s[R][2][kScales];
-      float e[2];  // kTrans: 2^e_n of the two rows
+      uint32_t e[2];  // kTrans: 2^e_n of the two rows
     };
     Piece ring[S::kDepth];
     float down[R][2];  // 2^-e_n of this lane's rows
@@ -222,33 +211,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
           down[r][h] = n < p.N ? inverse(__ldg(p.row_scale + n)) : 1.f;
         }
     }
-    int next = s0, left = count;  // step to fetch
+    int next = s0;  // step to fetch
+    // Everything is fetched from somewhere: what lies behind the last row tile
+    // or block is dropped below, or never leaves the tile.
     auto fetch = [&](Piece& x) {
-      const bool in = left > 0;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const long long rt = kTrans ? next * 8LL + w8 : row0 / 16 + r * 8 + w8;
-        const long long kb = kTrans ? row0 / 128 + r : next;
-        const bool there = in && rt < rtiles && kb < p.kblocks;
+        const long long rt = min(kTrans ? next * 8LL + w8 : row0 / 16 + r * 8 + w8, rtiles - 1);
+        const long long kb = min(kTrans ? row0 / 128 + r : (long long)next, (long long)p.kblocks - 1);
         const long long blk = rt * p.kblocks + kb;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x.q[r][h] = there ? ldg_stream2(reinterpret_cast<const uint2*>(p.packed + blk * 64 + h * 32 + lane) + pair)
-                            : make_uint2(0x88888888u, 0x88888888u);
+          x.q[r][h] = ldg64(reinterpret_cast<const uint2*>(p.packed + blk * 64 + h * 32 + lane) + pair);
 #pragma unroll
           for (int k = 0; k < kScales; ++k)
             x.s[r][h][k] =
-                there ? load_scale(p, (blk * kGroups + pair * kGroups / 2 + k) * kRows + g + 8 * h) : 0u;
+                scale_word(p.scales, p.scales_f32, (blk * kGroups + pair * kGroups / 2 + k) * kRows + g + 8 * h);
         }
       }
       if constexpr (kTrans) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const long long n = next * 128LL + w8 * 16 + g + 8 * h;
-          x.e[h] = in && n < p.N ? __ldg(p.row_scale + n) : 1.f;
-        }
+        for (int h = 0; h < 2; ++h)
+          x.e[h] = ldg32(p.row_scale + min(next * 128LL + w8 * 16 + g + 8 * h, (long long)p.N - 1));
       }
-      --left;
       if (++next == s1) next = s0;
     };
 #pragma unroll
@@ -264,7 +249,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int r = 0; r < R; ++r) down[r][h] = inverse(x.e[h]);
+            for (int r = 0; r < R; ++r) down[r][h] = inverse(__uint_as_float(x.e[h]));
         }
         uint4 v[R][2][2];
 #pragma unroll
@@ -274,7 +259,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
             __half2 sc[kScales];
 #pragma unroll
             for (int k = 0; k < kScales; ++k) {
-              const float f = scale_value(p, x.s[r][h][k]) * down[r][h];
+              // a row tile behind the last adds nothing, whatever was fetched for it
+              const float f = !kTrans || step * 8LL + w8 < rtiles
+                                  ? scale_value(x.s[r][h][k], p.scales_f32, odd) * down[r][h] : 0.f;
               sc[k] = __float2half2_rn(p.scales_f32 ? scale_term(f, term) : f);
             }
 #pragma unroll
