@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
       for (int h = 0; h < 2; ++h) {
         int ex = (int)((__float_as_uint(top[h]) >> 23) & 255);
         ex = ex < 14 ? 14 : ex;  // up = 2^(140 - ex), down = 1 / up
-        up[h] = __uint_as_float((uint32_t)(267 - ex) << 23);
+        up[h] = __uint_as_float((uint32_t)(267 - ex) << 23) * (p.scale < 0.f ? -1.f : 1.f);
         down[h] = __uint_as_float((uint32_t)(ex - 13) << 23);
       }
 #pragma unroll
@@ -473,8 +473,8 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
                   make_uint4(f[0][k], f[1][k], f[2][k], f[3][k]);
           }
         }
-      qs0 = down[0] * p.scale;
-      qs1 = down[1] * p.scale;
+      qs0 = down[0] * fabsf(p.scale);
+      qs1 = down[1] * fabsf(p.scale);
       lim0 = lim[0];
       lim1 = lim[1];
       lim_min = min(has[0] ? lim0 : (int)at.length, has[1] ? lim1 : (int)at.length);
@@ -535,24 +535,28 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * t);
     release();
 
+    // The scores are used as they are: scaled by f (at least 0, the same for a
+    // lane's whole unit) only inside the exponent.
     const float f0 = qs0 * sk, f1 = qs1 * sk;
     const int tok0 = at.chunk * kChunk + 16 * t;
     const bool mask = (at.chunk + 1) * kChunk > lim_min;
-    float n0 = m0, n1 = m1;
+    if (mask) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        s[j][e] *= f0;
-        s[j][2 + e] *= f1;
-        if (mask) {
+        for (int e = 0; e < 2; ++e) {
           if (tok0 + 2 * j + e >= lim0) s[j][e] = -INFINITY;
           if (tok0 + 2 * j + e >= lim1) s[j][2 + e] = -INFINITY;
         }
-        n0 = fmaxf(n0, s[j][e]);
-        n1 = fmaxf(n1, s[j][2 + e]);
-      }
     }
+    float n0 = -INFINITY, n1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      n0 = fmaxf(n0, fmaxf(s[j][0], s[j][1]));
+      n1 = fmaxf(n1, fmaxf(s[j][2], s[j][3]));
+    }
+    n0 = fmaxf(m0, n0 * f0);  // a product that is not a number (a masked unit of scale 0) drops out
+    n1 = fmaxf(m1, n1 * f1);
     n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
     n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
     n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
@@ -568,8 +572,6 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
     const float old0 = exp2_approx(m0 - z0), old1 = exp2_approx(m1 - z1);
     const float shrink = __fdividef(top_v, nv), rel = __fdividef(sv, nv) * kUp;
-    l0 *= old0;
-    l1 *= old1;
     const float a0 = old0 * shrink, a1 = old1 * shrink;
     if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
 #pragma unroll
@@ -583,26 +585,53 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     m0 = n0;
     m1 = n1;
     top_v = nv;
-    // a NaN scale reaches no row that its page is hidden from
-    const bool odd = mask && rel != rel;
+    // Weights times the unit's value scale, 2^(s f - z + log2 rel). Where that
+    // has no logarithm (a unit of scale 0, NaN), or tokens are hidden, the
+    // weight is made first and multiplied after.
     uint32_t w[4][4][kTerms];
+    float sum0 = 0.f, sum1 = 0.f;
+    if (!mask && !__any_sync(0xffffffffu, !(rel > 1e-30f))) {
+      float lg;
+      asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
+      const float y0 = lg - z0, y1 = lg - z1, back = __fdividef(1.f, rel);
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
+      for (int kk = 0; kk < 4; ++kk)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float* x = s[2 * kk + half];
-        x[0] = exp2_approx(x[0] - z0);
-        x[1] = exp2_approx(x[1] - z0);
-        x[2] = exp2_approx(x[2] - z1);
-        x[3] = exp2_approx(x[3] - z1);
-        l0 += x[0] + x[1];
-        l1 += x[2] + x[3];
-        float y[4];
+        for (int half = 0; half < 2; ++half) {
+          float* x = s[2 * kk + half];
+          x[0] = exp2_approx(fmaf(x[0], f0, y0));
+          x[1] = exp2_approx(fmaf(x[1], f0, y0));
+          x[2] = exp2_approx(fmaf(x[2], f1, y1));
+          x[3] = exp2_approx(fmaf(x[3], f1, y1));
+          sum0 += x[0] + x[1];
+          sum1 += x[2] + x[3];
+          split_f16<kTerms>(x[0], x[1], w[kk][2 * half]);
+          split_f16<kTerms>(x[2], x[3], w[kk][2 * half + 1]);
+        }
+      sum0 *= back;
+      sum1 *= back;
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = odd && x[e] == 0.f ? 0.f : x[e] * rel;
-        split_f16<kTerms>(y[0], y[1], w[kk][2 * half]);
-        split_f16<kTerms>(y[2], y[3], w[kk][2 * half + 1]);
-      }
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float* x = s[2 * kk + half];
+          float y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool hidden = tok0 + 4 * kk + 2 * half + (e & 1) >= (e < 2 ? lim0 : lim1);
+            const float v = exp2_approx(fmaf(x[e], e < 2 ? f0 : f1, e < 2 ? -z0 : -z1));
+            x[e] = mask && hidden ? 0.f : v;
+            y[e] = mask && hidden ? 0.f : v * rel;
+          }
+          sum0 += x[0] + x[1];
+          sum1 += x[2] + x[3];
+          split_f16<kTerms>(y[0], y[1], w[kk][2 * half]);
+          split_f16<kTerms>(y[2], y[3], w[kk][2 * half + 1]);
+        }
+    }
+    l0 = l0 * old0 + sum0;
+    l1 = l1 * old1 + sum1;
     {
       const uint32_t vals = smem_u32(mine + slot * S::kSlot) + t * (S::kUnit + 32) + g * 16;
 #pragma unroll
