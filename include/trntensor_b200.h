@@ -327,10 +327,11 @@ int tt_q4_quantize(const void* W, int type, long long ldw, int scale_type, int N
 int tt_q4_dequantize(const void* packed, const void* packed_scales, int scale_type, int N, int K,
                      int group, void* out, int type, void* stream);
 /* row_scale (N fp32): the power of two by which each row's scales are brought
- * into fp16's range in products of more than 16 rows. */
+ * into fp16's range in products of many rows. */
 int tt_q4_row_scale(const void* packed_scales, int scale_type, int N, int K, int group,
                     float* row_scale, void* stream);
-/* Bytes of workspace for a product (0 up to 16 rows, where it may be NULL). */
+/* Bytes of workspace for a product (0 up to 16 rows, and up to 64 of 16-bit
+ * types over k, where it may be NULL). */
 size_t tt_q4_matmul_workspace_bytes(int type, int scale_type, int transposed, int M, int N, int K);
 /* y (M, N; row stride ldy) = x (M, K; row stride ldx) W^T: fp32 sums, rounded
  * once to x's type. dev_status as in the file's head; unlike other calls these

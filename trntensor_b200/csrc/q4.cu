@@ -23,7 +23,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;
-constexpr int kFewRows = 16;  // above, the products go to csrc/q4_gemm.cuh
+// Up to so many rows the products run here, above in csrc/q4_gemm.cuh.
+int few_rows(int type, bool transposed) { return !transposed && type != kF32 ? 64 : 16; }
 
 // ------------------------------------------------------- packing and decoding
 
@@ -155,39 +156,32 @@ __global__ void dequantize_kernel(const uint4* __restrict__ packed, const ST* __
 
 // ------------------------------------------------------------------ operands
 
-// Eight neighbouring k of a row as pairs for kTerms fragments; what lies
-// behind the row's end is zero. `wide`: rows start on 16 bytes and hold a
-// multiple of 8 values, so that eight values are all there or none is.
+// Eight neighbouring values as pairs for kTerms fragments. `wide`: all are
+// there and 16-byte aligned; else the first `left` are, and zeros follow.
 template <typename XT, int kTerms>
-__device__ __forceinline__ void load_eight(const XT* __restrict__ row, long long k0, int K, bool wide,
-                                           uint32_t (&out)[kTerms][4]) {
+__device__ __forceinline__ void load_eight(const XT* __restrict__ at, int left, bool wide, uint32_t (&out)[kTerms][4]) {
   if constexpr (sizeof(XT) == 2) {
     if (wide) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (k0 < K) v = __ldg(reinterpret_cast<const uint4*>(row + k0));
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
       out[0][0] = v.x; out[0][1] = v.y; out[0][2] = v.z; out[0][3] = v.w;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t lo = 0, hi = 0;
-        if (k0 + 2 * j < K) lo = __ldg(reinterpret_cast<const unsigned short*>(row) + k0 + 2 * j);
-        if (k0 + 2 * j + 1 < K) hi = __ldg(reinterpret_cast<const unsigned short*>(row) + k0 + 2 * j + 1);
+        if (2 * j < left) lo = __ldg(reinterpret_cast<const unsigned short*>(at) + 2 * j);
+        if (2 * j + 1 < left) hi = __ldg(reinterpret_cast<const unsigned short*>(at) + 2 * j + 1);
         out[0][j] = lo | hi << 16;
       }
     }
   } else {
     float f[8];
     if (wide) {
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-      if (k0 < K) {
-        a = __ldg(reinterpret_cast<const float4*>(row + k0));
-        b = __ldg(reinterpret_cast<const float4*>(row + k0) + 1);
-      }
+      const float4 a = __ldg(reinterpret_cast<const float4*>(at)), b = __ldg(reinterpret_cast<const float4*>(at) + 1);
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
       f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = k0 + i < K ? __ldg(row + k0 + i) : 0.f;
+      for (int i = 0; i < 8; ++i) f[i] = i < left ? __ldg(at + i) : 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -235,13 +229,10 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
     for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
 
   if (active) {
-    const XT* xr[kTiles];
-    bool has[kTiles];
+    const XT* xr[kTiles];  // a token that is not there reads another's values: its column is dropped
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) {
-      has[j] = m0 + 8 * j + g < M;
-      xr[j] = x + (has[j] ? (m0 + 8 * j + g) * ldx : 0);
-    }
+    for (int j = 0; j < kTiles; ++j) xr[j] = x + min(m0 + 8 * j + g, (long long)M - 1) * ldx + 8 * t;
+    const int whole = wide ? K / kCols : 0;  // blocks whose 128 columns can be read as they stand
     // A ring of blocks in registers: codes, scales and the tokens' values are
     // asked for kDepth blocks ahead.
     constexpr int kDepth = kTerms == 1 ? (kTiles == 1 ? 4 : 2) : 2;
@@ -276,7 +267,8 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
         for (int j = 0; j < kTiles; ++j)
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            load_eight<XT, kTerms>(xr[j], (long long)kb * kCols + 32 * w + 8 * t, has[j] ? K : 0, wide != 0, xp[j][w]);
+            load_eight<XT, kTerms>(xr[j] + (long long)kb * kCols + 32 * w, K - kb * kCols - 32 * w - 8 * t, kb < whole,
+                                   xp[j][w]);
         const Piece f = ring[d];
         fetch(ring[d]);
         const uint32_t wa[4] = {f.qa.x, f.qa.y, f.qa.z, f.qa.w}, wb[4] = {f.qb.x, f.qb.y, f.qb.z, f.qb.w};
@@ -359,90 +351,106 @@ __device__ __forceinline__ float value_of(uint32_t bits) {
 
 // ------------------------------------------------------------ dx = dy W, few rows
 
-// A CTA owns 128 columns of W and 16 tokens; the rows of W are shared among
-// its warps and the CTAs of its cluster. Here the scale varies along the sum,
-// so it goes into the other operand: dy s is split into bf16 terms (two for
-// 16-bit types: 2^-16 of each product, against 2^-9 or 2^-12 for the result's
-// own rounding; three for fp32). Tile (w, j) of a block takes the columns
-// k = 32 w + 8 (c / 2) + 2 j + c % 2, so that all its columns share a group.
-template <typename XT, typename ST, int kGroups>
+// A CTA owns 128 columns of W and 8 kTiles tokens; the rows of W are shared
+// among its warps and the CTAs of its cluster. Here the scale varies along the
+// sum, so it goes into the other operand: dy s is split into bf16 terms (two
+// for 16-bit types: 2^-16 of each product, against 2^-9 or 2^-12 for the
+// result's own rounding; three for fp32). A fragment of W takes the columns
+// k = 32 w + 8 (c / 2) + 2 j + c % 2 of a block, c = 0 .. 7, for two j, so that
+// all its columns share a group.
+template <typename XT, typename ST, int kTiles, int kGroups>
 __global__ void __launch_bounds__(kWarps * 32)
 matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restrict__ packed,
                 const ST* __restrict__ scales, int M, int N, int K, int kblocks,
                 XT* __restrict__ dx, long long lddx) {
   constexpr int kTerms = sizeof(XT) == 2 ? 2 : 3;
-  extern __shared__ float tpart[];  // [warp][16 tokens][128]
+  constexpr int kTok = 8 * kTiles, kRow = kCols + 4;  // a row's floats in shared memory
+  extern __shared__ float tpart[];  // [warp][token][kRow]
   cg::cluster_group cluster = cg::this_cluster();
   const int warp = threadIdx.x / 32, warps = blockDim.x / 32, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int splits = gridDim.x;
   const long long tile = blockIdx.y + (long long)blockIdx.z * gridDim.y;
-  const long long mtiles = ((long long)M + 15) / 16;
+  const long long mtiles = ((long long)M + kTok - 1) / kTok;
   const bool active = tile < (long long)kblocks * mtiles;
   const int kb = active ? (int)(tile % kblocks) : 0;
-  const long long m0 = active ? tile / kblocks * 16 : 0;
-  const long long rtiles = ((long long)N + kRows - 1) / kRows;
+  const long long m0 = active ? tile / kblocks * kTok : 0;
+  const int rtiles = (int)(((long long)N + kRows - 1) / kRows);
 
-  float acc[16][4];
+  float acc[kTiles][8][4];
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
+  for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][i][e] = 0.f;
 
   if (active) {
     constexpr bool kF32Scale = sizeof(ST) == 4;
     struct Piece {
-      uint4 q[4];               // rows 2t, 2t+1 (half 0) and 8+2t, 9+2t (half 1); the words of t' = g / 2
-      uint32_t d[2][4];         // token g / g + 8, rows as in q: bits of dy
-      uint32_t s[kGroups][4];
+      uint4 q[4];                // rows 2t, 2t+1, 8+2t, 9+2t; the words of t' = g / 2
+      uint32_t d[kTiles][4];     // token g, those rows: bits of dy
+      uint32_t s[kGroups][kF32Scale ? 4 : 2];  // bf16: two neighbours in a word
     };
     constexpr int kDepth = 2;
     Piece ring[kDepth];
-    const long long stride = splits * warps;
-    long long next = blockIdx.x * warps + warp;
+    const int stride = splits * warps;
+    int next = blockIdx.x * warps + warp;
+    const XT* row[kTiles];  // a token that is not there reads another's: its column is dropped
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j) row[j] = dy + min(m0 + 8 * j + g, (long long)M - 1) * lddy;
+    const uint4* at_q = packed + (long long)kb * 64 + 2 * t * 4 + (g >> 1);
     auto fetch = [&](Piece& f) {  // behind the last row tile: the last again, for nothing
-      const long long rt = min(next, rtiles - 1), blk = rt * kblocks + kb;
+      const int rt = min(next, rtiles - 1);
+      const uint4* q = at_q + (long long)rt * kblocks * 64;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) f.q[r] = ldg128(q + (r >> 1) * 32 + (r & 1) * 4);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        f.q[r] = ldg128(packed + blk * 64 + (r >> 1) * 32 + (2 * t + (r & 1)) * 4 + (g >> 1));
-        const long long n = min(rt * kRows + (r >> 1) * 8 + 2 * t + (r & 1), (long long)N - 1);
+        const int n = min(rt * kRows + (r >> 1) * 8 + 2 * t + (r & 1), N - 1);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const XT* at = dy + min(m0 + g + 8 * h, (long long)M - 1) * lddy + n;
-          f.d[h][r] = sizeof(XT) == 4 ? ldg32(at) : ldg16(at);
+        for (int j = 0; j < kTiles; ++j) f.d[j][r] = sizeof(XT) == 4 ? ldg32(row[j] + n) : ldg16(row[j] + n);
+      }
+#pragma unroll
+      for (int gi = 0; gi < kGroups; ++gi) {
+        const ST* s = scales + (((long long)rt * kblocks + kb) * kGroups + gi) * kRows + 2 * t;
+        if constexpr (kF32Scale) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) f.s[gi][r] = ldg32(s + (r >> 1) * 8 + (r & 1));
+        } else {
+          f.s[gi][0] = ldg32(s);
+          f.s[gi][1] = ldg32(s + 8);
         }
-#pragma unroll
-        for (int gi = 0; gi < kGroups; ++gi)
-          f.s[gi][r] = scale_word(scales, kF32Scale, (blk * kGroups + gi) * kRows + (r >> 1) * 8 + 2 * t + (r & 1));
       }
       next += stride;
     };
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) fetch(ring[d]);
-    for (long long rt0 = blockIdx.x * warps + warp; rt0 < rtiles; rt0 += stride * kDepth) {
+    for (int rt0 = blockIdx.x * warps + warp; rt0 < rtiles; rt0 += stride * kDepth) {
 #pragma unroll
       for (int dd = 0; dd < kDepth; ++dd) {
-        if (rt0 + dd * stride >= rtiles) break;
+        const int rt = rt0 + dd * stride;
+        if (rt >= rtiles) break;
         const Piece f = ring[dd];
         fetch(ring[dd]);
-        float d[2][4];
+        float d[kTiles][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int r = 0; r < 4; ++r) {
+          const bool in = rt * kRows + (r >> 1) * 8 + 2 * t + (r & 1) < N;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const long long n = (rt0 + dd * stride) * kRows + (r >> 1) * 8 + 2 * t + (r & 1);
-            d[h][r] = m0 + g + 8 * h < M && n < N ? value_of<XT>(f.d[h][r]) : 0.f;
-          }
+          for (int j = 0; j < kTiles; ++j) d[j][r] = in ? value_of<XT>(f.d[j][r]) : 0.f;
+        }
 #pragma unroll
         for (int gi = 0; gi < kGroups; ++gi) {
           float s[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[r] = scale_value(f.s[gi][r], kF32Scale, r & 1);
-          uint32_t a[4][kTerms];  // a0: token g rows 0,1; a1: token g+8; a2, a3: rows 2,3
+          for (int r = 0; r < 4; ++r)
+            s[r] = kF32Scale ? __uint_as_float(f.s[gi][r]) : scale_value(f.s[gi][r >> 1], false, r & 1);
+          uint32_t b[kTiles][2][kTerms];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            split_bf16<kTerms>(d[h][0] * s[0], d[h][1] * s[1], a[h]);
-            split_bf16<kTerms>(d[h][2] * s[2], d[h][3] * s[3], a[2 + h]);
+          for (int j = 0; j < kTiles; ++j) {
+            split_bf16<kTerms>(d[j][0] * s[0], d[j][1] * s[1], b[j][0]);
+            split_bf16<kTerms>(d[j][2] * s[2], d[j][3] * s[3], b[j][1]);
           }
 #pragma unroll
           for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w) {
@@ -450,42 +458,46 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
             auto word = [&](int r) { return w == 0 ? f.q[r].x : w == 1 ? f.q[r].y : w == 2 ? f.q[r].z : f.q[r].w; };
             const uint32_t lo = __byte_perm(word(0), word(1), sel), hi = __byte_perm(word(2), word(3), sel);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t b0 = decode_pair<false>(lo >> (4 * j));
-              const uint32_t b1 = decode_pair<false>(hi >> (4 * j));
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a0 = decode_pair<false>(lo >> (8 * i)), a1 = decode_pair<false>(lo >> (8 * i + 4));
+              const uint32_t a2 = decode_pair<false>(hi >> (8 * i)), a3 = decode_pair<false>(hi >> (8 * i + 4));
 #pragma unroll
-              for (int i = 0; i < kTerms; ++i)
-                mma16816<false>(acc[4 * w + j], a[0][i], a[1][i], a[2][i], a[3][i], b0, b1);
+              for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k)
+                  mma16816<false>(acc[j][2 * w + i], a0, a1, a2, a3, b[j][0][k], b[j][1][k]);
             }
           }
         }
       }
     }
   }
-  // columns of this lane: 32 w + 8 t + 2 j + {0, 1}
-  float* mine = tpart + warp * 16 * kCols;
+  // acc[j][2 w + i]: columns 32 w + 8 (g / 2) + 4 i + g % 2, and 2 on, tokens 8 j + 2 t, 2 t + 1
+  float* mine = tpart + warp * kTok * kRow;
 #pragma unroll
-  for (int w = 0; w < 4; ++w)
+  for (int j = 0; j < kTiles; ++j)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = 32 * w + 8 * t + 2 * j;
-      *reinterpret_cast<float2*>(mine + g * kCols + col) = make_float2(acc[4 * w + j][0], acc[4 * w + j][1]);
-      *reinterpret_cast<float2*>(mine + (g + 8) * kCols + col) = make_float2(acc[4 * w + j][2], acc[4 * w + j][3]);
-    }
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        mine[(8 * j + 2 * t + (e & 1)) * kRow + 32 * (i >> 1) + 8 * (g >> 1) + 4 * (i & 1) + (g & 1) + 2 * (e >> 1)] =
+            acc[j][i][e];
   __syncthreads();
-  constexpr int kOut = 16 * kCols;
+  constexpr int kOut = kTok * kCols;
   for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
-    float v = tpart[o];
-    for (int w = 1; w < warps; ++w) v += tpart[w * kOut + o];
-    tpart[o] = v;
+    const int at = o / kCols * kRow + o % kCols;
+    float v = tpart[at];
+    for (int w = 1; w < warps; ++w) v += tpart[w * kTok * kRow + at];
+    tpart[at] = v;
   }
   if (splits > 1) {
     cluster.sync();
     // every rank adds a share of the outputs, in rank order, and keeps it to itself
     if (active) {
       for (int o = threadIdx.x + blockIdx.x * blockDim.x; o < kOut; o += splits * blockDim.x) {
-        float v = cluster.map_shared_rank(tpart, 0)[o];
-        for (int r = 1; r < splits; ++r) v += cluster.map_shared_rank(tpart, r)[o];
+        const int at = o / kCols * kRow + o % kCols;
+        float v = cluster.map_shared_rank(tpart, 0)[at];
+        for (int r = 1; r < splits; ++r) v += cluster.map_shared_rank(tpart, r)[at];
         const long long m = m0 + o / kCols, k = (long long)kb * kCols + o % kCols;
         if (m < M && k < K) dx[m * lddx + k] = from_f<XT>(v);
       }
@@ -496,10 +508,171 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
     if (active) {
       for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
         const long long m = m0 + o / kCols, k = (long long)kb * kCols + o % kCols;
-        if (m < M && k < K) dx[m * lddx + k] = from_f<XT>(tpart[o]);
+        if (m < M && k < K) dx[m * lddx + k] = from_f<XT>(tpart[o / kCols * kRow + o % kCols]);
       }
     }
   }
+}
+
+// ------------------------------------------------- y = x W^T, up to 64 rows
+
+// As the first product, for 16-bit types and 9 to 64 tokens. There the tokens'
+// values are what a warp reads most of, so a CTA takes 128 rows of W, one row
+// tile a warp, and all its warps share the tokens' values from shared memory:
+// four blocks of k a stage, filled by cp.async one stage ahead, rows 64 bytes
+// off each other's banks. The CTAs of a cluster share the sum over k.
+// The alternative, tcgen05 with the matrix decoded into shared memory, took 64
+// us for 32 x 16384 x 8192: decoding with the scale and storing 16 bits a
+// weight is more than the SM can issue at the rate of the loads.
+constexpr int kMidBlocks = 4;                                // of k in a stage
+constexpr int kMidRow = kMidBlocks * kCols * 2 + 64;         // bytes of a token's row there
+constexpr int kMidStages = 2;
+
+template <int kTiles>
+constexpr int mid_smem() { return kMidStages * 8 * kTiles * kMidRow; }
+
+template <typename XT, typename ST, int kTiles, int kGroups>
+__global__ void __launch_bounds__(kWarps * 32, kTiles <= 4 ? 2 : 1)
+mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ packed, const ST* __restrict__ scales,
+           int M, int N, int K, int kblocks, int wide, XT* __restrict__ y, long long ldy) {
+  constexpr bool kHalf = !std::is_same<XT, __nv_bfloat16>::value;
+  constexpr bool kF32Scale = sizeof(ST) == 4;
+  constexpr int kTok = 8 * kTiles;
+  extern __shared__ __align__(16) unsigned char msm[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int splits = gridDim.x;
+  const long long group_of = blockIdx.y + (long long)blockIdx.z * gridDim.y;
+  const int rtiles = (int)(((long long)N + kRows - 1) / kRows);
+  const bool active = group_of * kWarps < rtiles;
+  const int rt = (int)min(group_of * kWarps + warp, (long long)rtiles - 1);  // behind the last: dropped at the end
+  const int b0 = (int)((long long)kblocks * blockIdx.x / splits), b1 = (int)((long long)kblocks * (blockIdx.x + 1) / splits);
+  const int stages = active ? (b1 - b0 + kMidBlocks - 1) / kMidBlocks : 0;
+
+  // a stage's values: token by token, 16 bytes a thread; zeros where there are none
+  auto fill = [&](int s) {
+    unsigned char* to = msm + (s % kMidStages) * kTok * kMidRow;
+    const int k0 = (b0 + s * kMidBlocks) * kCols;
+    for (int i = threadIdx.x; i < kTok * kMidBlocks * 16; i += kWarps * 32) {
+      const int m = i / (kMidBlocks * 16), c = i % (kMidBlocks * 16), k = k0 + 8 * c;
+      unsigned char* at = to + m * kMidRow + 16 * c;
+      const XT* from = x + (long long)min(m, M - 1) * ldx + k;
+      if (wide && k + 8 <= K) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(at)), "l"(from)
+                     : "memory");
+      } else {
+        uint32_t v[1][4];
+        load_eight<XT, 1>(from, K - k, false, v);
+        *reinterpret_cast<uint4*>(at) = make_uint4(v[0][0], v[0][1], v[0][2], v[0][3]);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  float acc[kTiles][4];
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+  struct Piece {
+    uint4 qa, qb;
+    uint32_t s[kGroups][2];
+  };
+  constexpr int kDepth = kTiles <= 4 ? kMidBlocks : 2;
+  Piece ring[kDepth];
+  int next = b0;
+  const uint4* at_q = packed + (long long)rt * kblocks * 64 + lane;
+  auto fetch = [&](Piece& f) {
+    const int kb = min(next, b1 - 1);
+    f.qa = ldg128(at_q + (long long)kb * 64);
+    f.qb = ldg128(at_q + (long long)kb * 64 + 32);
+#pragma unroll
+    for (int gi = 0; gi < kGroups; ++gi) {
+      f.s[gi][0] = scale_word(scales, kF32Scale, (((long long)rt * kblocks + kb) * kGroups + gi) * kRows + g);
+      f.s[gi][1] = scale_word(scales, kF32Scale, (((long long)rt * kblocks + kb) * kGroups + gi) * kRows + g + 8);
+    }
+    ++next;
+  };
+  if (stages > 0) {
+    fill(0);
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) fetch(ring[d]);
+  }
+  for (int s = 0; s < stages; ++s) {
+    if (s + 1 < stages) fill(s + 1);
+    else asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    const unsigned char* from = msm + (s % kMidStages) * kTok * kMidRow + g * kMidRow + t * 16;
+#pragma unroll
+    for (int i = 0; i < kMidBlocks; ++i) {
+      if (b0 + s * kMidBlocks + i >= b1) break;
+      const Piece f = ring[i % kDepth];
+      fetch(ring[i % kDepth]);
+      const uint32_t wa[4] = {f.qa.x, f.qa.y, f.qa.z, f.qa.w}, wb[4] = {f.qb.x, f.qb.y, f.qb.z, f.qb.w};
+#pragma unroll
+      for (int gi = 0; gi < kGroups; ++gi) {
+        float c[kTiles][4];
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[j][e] = 0.f;
+#pragma unroll
+        for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w) {
+          uint4 v[kTiles];
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j)
+            v[j] = *reinterpret_cast<const uint4*>(from + 8 * j * kMidRow + i * 256 + w * 64);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a0 = decode_pair<kHalf>(wa[w] >> (8 * half));
+            const uint32_t a1 = decode_pair<kHalf>(wb[w] >> (8 * half));
+            const uint32_t a2 = decode_pair<kHalf>(wa[w] >> (8 * half + 4));
+            const uint32_t a3 = decode_pair<kHalf>(wb[w] >> (8 * half + 4));
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j)
+              mma16816<kHalf>(c[j], a0, a1, a2, a3, half ? v[j].z : v[j].x, half ? v[j].w : v[j].y);
+          }
+        }
+        const float s0 = scale_value(f.s[gi][0], kF32Scale, g & 1), s1 = scale_value(f.s[gi][1], kF32Scale, g & 1);
+#pragma unroll
+        for (int j = 0; j < kTiles; ++j) {
+          acc[j][0] += s0 * c[j][0];
+          acc[j][1] += s0 * c[j][1];
+          acc[j][2] += s1 * c[j][2];
+          acc[j][3] += s1 * c[j][3];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  // [token][row], a row more to a token's line against bank conflicts
+  constexpr int kLine = kWarps * kRows + 1;
+  static_assert(kTok * kLine * 4 <= mid_smem<kTiles>(), "the sums fit where the stages were");
+  float* sums = reinterpret_cast<float*>(msm);
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      sums[(8 * j + 2 * t + (e & 1)) * kLine + warp * kRows + g + 8 * (e >> 1)] = acc[j][e];
+  __syncthreads();
+  if (splits > 1) cluster.sync();
+  if (active) {
+    for (int o = threadIdx.x + blockIdx.x * kWarps * 32; o < kTok * kWarps * kRows; o += splits * kWarps * 32) {
+      const int m = o / (kWarps * kRows), r = o % (kWarps * kRows);
+      const long long n = group_of * kWarps * kRows + r;
+      if (m >= M || n >= N) continue;
+      float v = 0.f;
+      if (splits > 1) {
+        for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(sums, k)[m * kLine + r];
+      } else {
+        v = sums[m * kLine + r];
+      }
+      y[m * ldy + n] = from_f<XT>(v);
+    }
+  }
+  if (splits > 1) cluster.sync();
 }
 
 // ---------------------------------------------------------------------- host
@@ -552,28 +725,61 @@ int run_matvec(const void* x, long long ldx, const void* packed, const void* sca
   return launch_cluster(matvec_kernel<XT, ST, kTiles, kGroups>, grid, kWarps * 32, 0, splits, s, args);
 }
 
-template <typename XT, typename ST, int kGroups>
+template <typename XT, typename ST, int kTiles, int kGroups>
+int run_mid(const void* x, long long ldx, const void* packed, const void* scales, int M, int N, int K, void* y,
+            long long ldy, int sms, cudaStream_t s) {
+  int kblocks = (int)(((long long)K + kCols - 1) / kCols);
+  const long long groups = ((long long)N + kRows * kWarps - 1) / (kRows * kWarps);
+  int splits = 1;  // two CTAs an SM, four blocks for each
+  while (splits < kMaxCluster && groups * splits * 2 <= 2LL * sms && kblocks >= splits * 2 * kMidBlocks) splits *= 2;
+  dim3 grid;
+  if (!grid_of(groups, splits, &grid)) return TT_ERR_SHAPE;
+  int wide = ldx % 8 == 0 && aligned16(x);
+  void* args[] = {&x, &ldx, &packed, &scales, &M, &N, &K, &kblocks, &wide, &y, &ldy};
+  return launch_cluster(mid_kernel<XT, ST, kTiles, kGroups>, grid, kWarps * 32, mid_smem<kTiles>(), splits, s, args);
+}
+template <typename XT, typename ST, int kTiles>
+int run_mid_group(const void* x, long long ldx, const void* packed, const void* scales, int M, int N, int K, int group,
+                  void* y, long long ldy, int sms, cudaStream_t s) {
+  if (group == 128) return run_mid<XT, ST, kTiles, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  if (group == 64) return run_mid<XT, ST, kTiles, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  return run_mid<XT, ST, kTiles, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+}
+
+template <int kTiles>
+constexpr int t_smem() { return kWarps * 8 * kTiles * (kCols + 4) * 4; }
+
+template <typename XT, typename ST, int kTiles, int kGroups>
 int run_matvec_t(const void* dy, long long lddy, const void* packed, const void* scales, int M,
                  int N, int K, void* dx, long long lddx, int sms, cudaStream_t s) {
   int kblocks = (int)(((long long)K + kCols - 1) / kCols);
   const long long rtiles = ((long long)N + kRows - 1) / kRows;
-  const long long tiles = (long long)kblocks * (((long long)M + 15) / 16);
+  const long long tiles = (long long)kblocks * (((long long)M + 8 * kTiles - 1) / (8 * kTiles));
   const int splits = pick_splits(tiles, rtiles, sms);
   dim3 grid;
   if (!grid_of(tiles, splits, &grid)) return TT_ERR_SHAPE;
   void* args[] = {&dy, &lddy, &packed, &scales, &M, &N, &K, &kblocks, &dx, &lddx};
-  return launch_cluster(matvec_t_kernel<XT, ST, kGroups>, grid, kWarps * 32,
-                        kWarps * 16 * kCols * 4, splits, s, args);
+  return launch_cluster(matvec_t_kernel<XT, ST, kTiles, kGroups>, grid, kWarps * 32, t_smem<kTiles>(), splits, s,
+                        args);
 }
 
+template <typename F>
+bool set_smem(F kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
+}
+template <typename XT, typename ST, int kGroups>
+bool set_group() {
+  bool ok = set_smem(matvec_t_kernel<XT, ST, 1, kGroups>, t_smem<1>()) &&
+            set_smem(matvec_t_kernel<XT, ST, 2, kGroups>, t_smem<2>());
+  if constexpr (sizeof(XT) == 2)
+    ok = ok && set_smem(mid_kernel<XT, ST, 2, kGroups>, mid_smem<2>()) &&
+         set_smem(mid_kernel<XT, ST, 4, kGroups>, mid_smem<4>()) &&
+         set_smem(mid_kernel<XT, ST, 8, kGroups>, mid_smem<8>());
+  return ok;
+}
 template <typename XT, typename ST>
 int set_attrs() {
-  const int bytes = kWarps * 16 * kCols * 4;
-  if (cudaFuncSetAttribute(matvec_t_kernel<XT, ST, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-      cudaFuncSetAttribute(matvec_t_kernel<XT, ST, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-      cudaFuncSetAttribute(matvec_t_kernel<XT, ST, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return TT_ERR_CUDA;
-  return TT_OK;
+  return set_group<XT, ST, 1>() && set_group<XT, ST, 2>() && set_group<XT, ST, 4>() ? TT_OK : TT_ERR_CUDA;
 }
 
 int setup(int dev) {
@@ -596,18 +802,29 @@ int matmul_typed(bool transposed, const void* x, long long ldx, const void* pack
                  int sms, cudaStream_t s) {
   const int gpb = kCols / group;
   if (transposed) {
-    if (gpb == 1) return run_matvec_t<XT, ST, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    if (gpb == 2) return run_matvec_t<XT, ST, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    return run_matvec_t<XT, ST, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (M <= 8) {
+      if (gpb == 1) return run_matvec_t<XT, ST, 1, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+      if (gpb == 2) return run_matvec_t<XT, ST, 1, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+      return run_matvec_t<XT, ST, 1, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    }
+    if (gpb == 1) return run_matvec_t<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (gpb == 2) return run_matvec_t<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    return run_matvec_t<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
   }
   if (M <= 8) {
     if (gpb == 1) return run_matvec<XT, ST, 1, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
     if (gpb == 2) return run_matvec<XT, ST, 1, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
     return run_matvec<XT, ST, 1, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
   }
-  if (gpb == 1) return run_matvec<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-  if (gpb == 2) return run_matvec<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-  return run_matvec<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  if constexpr (sizeof(XT) == 2) {
+    if (M <= 16) return run_mid_group<XT, ST, 2>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
+    if (M <= 32) return run_mid_group<XT, ST, 4>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
+    return run_mid_group<XT, ST, 8>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
+  } else {
+    if (gpb == 1) return run_matvec<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (gpb == 2) return run_matvec<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    return run_matvec<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  }
 }
 
 template <typename XT>
@@ -623,7 +840,8 @@ int matmul(bool transposed, const void* x, int type, long long ldx, const void* 
            const void* scales, int scale_type, const float* row_scale, int M, int N, int K, int group,
            void* y, long long ldy, void* workspace, size_t workspace_bytes, int* dev_status, void* stream) {
   if (!x || !packed || !scales || !row_scale || !y || !dev_status) return TT_ERR_NULL;
-  if (M > kFewRows && !workspace) return TT_ERR_NULL;
+  const bool few = M <= few_rows(type, transposed);
+  if (!few && !workspace) return TT_ERR_NULL;
   if (M <= 0 || N <= 0 || K <= 0 || !good_group(group)) return TT_ERR_SHAPE;
   if (type < 0 || type > 2 || scale_type < 0 || scale_type > 1) return TT_ERR_SHAPE;
   if (ldx < (transposed ? N : K) || ldy < (transposed ? K : N)) return TT_ERR_SHAPE;
@@ -634,7 +852,7 @@ int matmul(bool transposed, const void* x, int type, long long ldx, const void* 
   if ((st = setup(dev)) != TT_OK) return st;
   cudaStream_t s = (cudaStream_t)stream;
   const int sms = g_sms[dev];
-  if (M > kFewRows)
+  if (!few)
     return run_gemm(transposed, x, type, ldx, packed, scales, scale_type, row_scale, M, N, K, group, y, ldy,
                     workspace, workspace_bytes, dev_status, dev, s);
   if (type == kF32)
@@ -760,7 +978,7 @@ int tt_q4_row_scale(const void* packed_scales, int scale_type, int N, int K, int
 }
 
 size_t tt_q4_matmul_workspace_bytes(int type, int scale_type, int transposed, int M, int N, int K) {
-  if (M <= tt::q4::kFewRows || N <= 0 || K <= 0 || type < 0 || type > 2) return 0;
+  if (type < 0 || type > 2 || N <= 0 || K <= 0 || M <= tt::q4::few_rows(type, transposed != 0)) return 0;
   return tt::q4::gemm_workspace_bytes(type, scale_type, transposed != 0, M, N, K);
 }
 

@@ -21,7 +21,7 @@ from .dispatch import _device, _ptr
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GROUPS = (32, 64, 128)
-_FEW_ROWS = 16  # up to here a product needs no workspace
+_FEW_ROWS = 16  # up to here no product needs a workspace
 
 
 _HERE = contextlib.nullcontext()
@@ -209,7 +209,8 @@ def _product(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
     ws, ws_bytes = None, 0
     if m > _FEW_ROWS:
         ws_bytes = lib.tt_q4_matmul_workspace_bytes(kind, _TYPES[w.scales.dtype], over_n, m, n, k)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with _on(dev):
         st = fn(x.data_ptr(), kind, ldx, w.packed.data_ptr(), w.scales.data_ptr(),
                 _TYPES[w.scales.dtype], w.row_scale.data_ptr(), m, n, k, w.group, out.data_ptr(),
@@ -241,8 +242,8 @@ def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> tor
     """``x @ W^T``: (..., K) -> (..., N); with ``over_n`` ``x @ W``: (..., N) -> (..., K).
 
     x is fp32, bf16 or fp16; sums are fp32 and the result is rounded once to
-    x's type. Up to 16 rows products over k are exact, and over n they keep
-    2^-16 (fp32: all bits). With more rows both operands are brought to fp16's
+    x's type. Up to 16 rows (64 of 16-bit types over k) products over k are
+    exact, and over n they keep 2^-16 (fp32: all bits). With more both operands are brought to fp16's
     range by powers of two a row: products are exact where scales are bf16 and
     x is of 16 bits and no smaller than 2^-27 of its row's largest value, else
     they keep 2^-18 (fp32: 2^-20) of themselves and 2^-38 of the largest.
