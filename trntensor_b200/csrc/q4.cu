@@ -202,7 +202,7 @@ __device__ __forceinline__ void load_eight(const XT* __restrict__ at, int left, 
 // are added in a fixed order: warps through shared memory, CTAs through the
 // cluster's.
 template <typename XT, typename ST, int kTiles, int kGroups>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && sizeof(XT) == 2 ? 3 : 1)
 matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ packed,
               const ST* __restrict__ scales, int M, int N, int K, int kblocks, int wide,
               XT* __restrict__ y, long long ldy) {
@@ -235,7 +235,7 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
     const int whole = wide ? K / kCols : 0;  // blocks whose 128 columns can be read as they stand
     // A ring of blocks in registers: codes, scales and the tokens' values are
     // asked for kDepth blocks ahead.
-    constexpr int kDepth = kTerms == 1 ? (kTiles == 1 ? 4 : 2) : 2;
+    constexpr int kDepth = 2;
     constexpr bool kF32Scale = sizeof(ST) == 4;
     struct Piece {
       uint4 qa, qb;
@@ -260,8 +260,9 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
     for (int kb0 = blockIdx.x * warps + warp; kb0 < kblocks; kb0 += stride * kDepth) {
 #pragma unroll
       for (int d = 0; d < kDepth; ++d) {
-        const int kb = kb0 + d * stride;
-        if (kb >= kblocks) break;
+        // past the end the last block is fetched again, and counts for nothing
+        const int kb = min(kb0 + d * stride, kblocks - 1);
+        const bool on = kb0 + d * stride < kblocks;
         uint32_t xp[kTiles][4][kTerms][4];
 #pragma unroll
         for (int j = 0; j < kTiles; ++j)
@@ -283,10 +284,9 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
           for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              const uint32_t a0 = decode_pair<kHalf>(wa[w] >> (8 * half));
-              const uint32_t a1 = decode_pair<kHalf>(wb[w] >> (8 * half));
-              const uint32_t a2 = decode_pair<kHalf>(wa[w] >> (8 * half + 4));
-              const uint32_t a3 = decode_pair<kHalf>(wb[w] >> (8 * half + 4));
+              uint32_t a0, a1, a2, a3;
+              decode_four<kHalf>(wa[w] >> (8 * half), a0, a2);
+              decode_four<kHalf>(wb[w] >> (8 * half), a1, a3);
 #pragma unroll
               for (int j = 0; j < kTiles; ++j)
 #pragma unroll
@@ -295,12 +295,13 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
             }
           const float s0 = scale_value(f.s[gi][0], kF32Scale, g & 1), s1 = scale_value(f.s[gi][1], kF32Scale, g & 1);
 #pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            acc[j][0] += s0 * c[j][0];
-            acc[j][1] += s0 * c[j][1];
-            acc[j][2] += s1 * c[j][2];
-            acc[j][3] += s1 * c[j][3];
-          }
+          for (int j = 0; j < kTiles; ++j)
+            if (on) {
+              acc[j][0] += s0 * c[j][0];
+              acc[j][1] += s0 * c[j][1];
+              acc[j][2] += s1 * c[j][2];
+              acc[j][3] += s1 * c[j][3];
+            }
         }
       }
     }
@@ -429,8 +430,7 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
     for (int rt0 = blockIdx.x * warps + warp; rt0 < rtiles; rt0 += stride * kDepth) {
 #pragma unroll
       for (int dd = 0; dd < kDepth; ++dd) {
-        const int rt = rt0 + dd * stride;
-        if (rt >= rtiles) break;
+        const int rt = rt0 + dd * stride;  // behind the last: dy counts as zero, and the scale too
         const Piece f = ring[dd];
         fetch(ring[dd]);
         float d[kTiles][4];
@@ -445,7 +445,7 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
           float s[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            s[r] = kF32Scale ? __uint_as_float(f.s[gi][r]) : scale_value(f.s[gi][r >> 1], false, r & 1);
+            s[r] = rt >= rtiles ? 0.f : kF32Scale ? __uint_as_float(f.s[gi][r]) : scale_value(f.s[gi][r >> 1], false, r & 1);
           uint32_t b[kTiles][2][kTerms];
 #pragma unroll
           for (int j = 0; j < kTiles; ++j) {
@@ -606,7 +606,7 @@ mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ pa
     const unsigned char* from = msm + (s % kMidStages) * kTok * kMidRow + g * kMidRow + t * 16;
 #pragma unroll
     for (int i = 0; i < kMidBlocks; ++i) {
-      if (b0 + s * kMidBlocks + i >= b1) break;
+      const bool on = b0 + s * kMidBlocks + i < b1;  // else the last block again, for nothing
       const Piece f = ring[i % kDepth];
       fetch(ring[i % kDepth]);
       const uint32_t wa[4] = {f.qa.x, f.qa.y, f.qa.z, f.qa.w}, wb[4] = {f.qb.x, f.qb.y, f.qb.z, f.qb.w};
@@ -625,10 +625,9 @@ mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ pa
             v[j] = *reinterpret_cast<const uint4*>(from + 8 * j * kMidRow + i * 256 + w * 64);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const uint32_t a0 = decode_pair<kHalf>(wa[w] >> (8 * half));
-            const uint32_t a1 = decode_pair<kHalf>(wb[w] >> (8 * half));
-            const uint32_t a2 = decode_pair<kHalf>(wa[w] >> (8 * half + 4));
-            const uint32_t a3 = decode_pair<kHalf>(wb[w] >> (8 * half + 4));
+            uint32_t a0, a1, a2, a3;
+            decode_four<kHalf>(wa[w] >> (8 * half), a0, a2);
+            decode_four<kHalf>(wb[w] >> (8 * half), a1, a3);
 #pragma unroll
             for (int j = 0; j < kTiles; ++j)
               mma16816<kHalf>(c[j], a0, a1, a2, a3, half ? v[j].z : v[j].x, half ? v[j].w : v[j].y);
@@ -636,12 +635,13 @@ mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ pa
         }
         const float s0 = scale_value(f.s[gi][0], kF32Scale, g & 1), s1 = scale_value(f.s[gi][1], kF32Scale, g & 1);
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j) {
-          acc[j][0] += s0 * c[j][0];
-          acc[j][1] += s0 * c[j][1];
-          acc[j][2] += s1 * c[j][2];
-          acc[j][3] += s1 * c[j][3];
-        }
+        for (int j = 0; j < kTiles; ++j)
+          if (on) {
+            acc[j][0] += s0 * c[j][0];
+            acc[j][1] += s0 * c[j][1];
+            acc[j][2] += s1 * c[j][2];
+            acc[j][3] += s1 * c[j][3];
+          }
       }
     }
     __syncthreads();

@@ -68,7 +68,30 @@ __device__ __forceinline__ uint32_t decode_pair(uint32_t x) {
   }
 }
 
-// Not volatile, like the loads below: the compiler moves them past each other.
+// Two fp16 pairs at a time, from nibbles 0 and 1 of each half of x: the second
+// stands 16 times too high in the mantissa, which the fused multiply-add that
+// takes the bias off puts right, instead of a shift.
+__device__ __forceinline__ void decode_two_pairs(uint32_t x, uint32_t& first, uint32_t& second) {
+  const uint32_t a = and_or(x, 0x000f000fu, 0x64006400u), b = and_or(x, 0x00f000f0u, 0x64006400u);
+  const __half2 ra = __hsub2(reinterpret_cast<const __half2&>(a), __half2half2(__ushort_as_half(0x6408)));  // 1032
+  const __half2 rb = __hfma2(reinterpret_cast<const __half2&>(b), __half2half2(__ushort_as_half(0x2c00)),   // 1 / 16
+                             __half2half2(__ushort_as_half(0xd480)));                                       // -72
+  first = reinterpret_cast<const uint32_t&>(ra);
+  second = reinterpret_cast<const uint32_t&>(rb);
+}
+
+// The same for either type (bf16's mantissa is too short for the second form).
+template <bool kHalf>
+__device__ __forceinline__ void decode_four(uint32_t x, uint32_t& first, uint32_t& second) {
+  if constexpr (kHalf) {
+    decode_two_pairs(x, first, second);
+  } else {
+    first = decode_pair<false>(x);
+    second = decode_pair<false>(x >> 4);
+  }
+}
+
+// Not volatile: the compiler moves it past the loads.
 template <bool kHalf>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {

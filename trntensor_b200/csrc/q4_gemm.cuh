@@ -240,11 +240,14 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     for (int d = 0; d < S::kDepth; ++d) fetch(ring[d]);
     int pass = 0, step = s0, term = p.scale_term[0];
     uint32_t it = sub;  // stage number
-    for (int i0 = 0; i0 < count && ok; i0 += S::kDepth) {
+    // No way out of the loop but its head, and every turn fetches: the ring
+    // then stays in its registers. (Leaving from the middle made copies of it,
+    // which waited for the newest loads.)
+    for (int i0 = 0; i0 < count; i0 += S::kDepth) {
 #pragma unroll
       for (int d = 0; d < S::kDepth; ++d) {
-        if (i0 + d >= count || !ok) break;
         Piece& x = ring[d];
+        const bool now = i0 + d < count && ok;
         if constexpr (kTrans) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
@@ -272,19 +275,21 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
               const __half2 sh = kScales == 1 ? sc[0] : (e == odd ? sc[0] : sc[kScales - 1]);
               uint32_t y[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t c = decode_pair<true>(wd >> (4 * j));
-                const __half2 z = __hmul2(reinterpret_cast<const __half2&>(c), sh);
-                y[j] = reinterpret_cast<const uint32_t&>(z);
+              for (int j = 0; j < 4; j += 2) {
+                uint32_t lo, hi;
+                decode_two_pairs(wd >> (4 * j), lo, hi);
+                const __half2 a = __hmul2(reinterpret_cast<const __half2&>(lo), sh);
+                const __half2 b = __hmul2(reinterpret_cast<const __half2&>(hi), sh);
+                y[j] = reinterpret_cast<const uint32_t&>(a);
+                y[j + 1] = reinterpret_cast<const uint32_t&>(b);
               }
               v[r][h][e] = make_uint4(y[0], y[1], y[2], y[3]);
             }
           }
         fetch(x);
+        if (now) {
         const int s = it % S::kStages;
-        ok = mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
         const uint32_t base = smem_u32(smem + s * S::kStageBytes);
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -302,6 +307,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full_a[s]);
+        }
         it += 2;
         if (++step == s1) {
           step = s0;
