@@ -4,11 +4,13 @@ the same fp32 operations, and attention against it in 64 bits.
 Tolerances of attention. The scores' fp32 sums are chains of at most
 dim / 16 + 16 additions, each off by at most 2^-23 of sum |q k|; two more
 roundings bring a score's error to d = (dim / 16 + 20) 2^-23 max_t sum |q k|
-scale, and ex2.approx adds 2^-21 of a weight. Weights are rounded to fp16
-(2^-12; two terms for fp32 operands: 2^-22) and q of fp32 likewise (2^-22 of
-its row's largest value). Numerator and denominator take the score's error
-once each. The sums over tokens add at most L / 16 + 64 roundings of 2^-23.
-Everything is relative to a = sum p |v|; the result is rounded once.
+scale, and ex2.approx adds 2^-21 of a weight. Weights are rounded to fp16,
+whose 11 significant bits leave half a step of 2^-11 (two terms for fp32
+operands: 2^-22), and q of fp32 likewise (2^-22 of its row's largest value).
+Below fp16's normal range a weight is off by half of 2^-24, in units of which
+the largest weight is at least 2^6. Numerator and denominator take the score's
+error once each. The sums over tokens add at most L / 16 + 64 roundings of
+2^-23. Everything is relative to a = sum p |v|; the result is rounded once.
 """
 
 from __future__ import annotations
@@ -258,8 +260,8 @@ def reference(q, parts, table, lengths, counts, causal, scale):
                 d = (dim / 16 + 20) * 2.0**-23 * float((kh.abs() @ x.abs()).max()) * abs(scale)
                 if two:
                     d += 2.0**-22 * float(x.abs().max() * kh.abs().sum(1).max()) * abs(scale)
-                e = (2.0**-22 if two else 2.0**-12) + 2 * d + 2.0**-20 + (n / 16 + 64) * 2.0**-22
-                loss[b, i, h] = e * mass + n * 2.0**-38 * float(vh.abs().max())
+                e = (2.0**-22 if two else 2.0**-11) + 2 * d + 2.0**-20 + (n / 16 + 64) * 2.0**-22
+                loss[b, i, h] = e * mass + n * 2.0**-31 * float(p.max() * vh.abs().max())
     return o, loss
 
 
@@ -301,7 +303,9 @@ def test_single_tokens(cuda_ok, dim, page, heads, kv, name):
 @pytest.mark.parametrize("dim,page,heads,kv,new,lengths,counts", [
     (64, 16, 4, 2, 5, [5, 40, 130], None), (128, 64, 8, 2, 9, [9, 64, 200], [9, 1, 0]),
     (32, 32, 3, 1, 33, [33, 90, 20], [33, 7, 33]), (128, 16, 6, 6, 70, [70, 300, 129], [70, 64, 65]),
-    (256, 64, 2, 1, 20, [100, 20, 64], None), (80, 128, 4, 1, 130, [130, 257, 260], [130, 1, 129])])
+    (256, 64, 2, 1, 20, [100, 20, 64], None), (80, 128, 4, 1, 130, [130, 257, 260], [130, 1, 129]),
+    (128, 64, 12, 6, 150, [700, 150, 20], [150, 149, 150]), (64, 32, 16, 16, 60, [60, 128, 513], [60, 1, 59]),
+    (96, 16, 24, 3, 40, [300, 40, 41], None), (16, 16, 8, 8, 300, [300, 1, 129], [300, 1, 128])])
 def test_several_tokens(cuda_ok, dim, page, heads, kv, new, lengths, counts, causal, name):
     """Tokens that enter with a prompt or a draft; more queries than tokens leave rows that see nothing."""
     attend_case(name, 3, new, heads, kv, dim, page, lengths, counts, causal)
@@ -323,6 +327,20 @@ def test_extremes(cuda_ok, name):
     attend_case(name, 2, 3, 4, 2, 64, 16, [500, 60], spread=6.0)        # scales decades apart
 
 
+def test_negative_scales(cuda_ok):
+    """A sign in a scale means the same as in its codes."""
+    kc, ks, vc, vs = filled(8, 2, 16, 32)
+    ks[::2], vs[1::3] = -ks[::2], -vs[1::3]
+    cache = tt.KVCache8.from_codes(kc.cuda(), ks.cuda(), vc.cuda(), vs.cuda())
+    k, v = cache.dequantize()
+    assert torch.equal(k.cpu(), kc.float() * ks[..., None, None])
+    assert torch.equal(v.cpu(), vc.float() * vs[..., None, None])
+    q = torch.randn(1, 3, 4, 32)
+    got = tt.kv_attention(q.cuda(), cache, int32([list(range(8))]), int32([125]))
+    want, loss = reference(q, (kc, ks, vc, vs), [list(range(8))], [125], [3], True, 32**-0.5)
+    assert ((got.cpu().double() - want).abs() <= 2.0**-24 * want.abs() + loss).all()
+
+
 def test_zero_pages_and_rows(cuda_ok):
     kc, ks, vc, vs = filled(8, 1, 16, 32)
     vs[::2] = 0
@@ -338,7 +356,7 @@ def test_zero_pages_and_rows(cuda_ok):
     assert tt.kv_attention(q.cuda()[:0], cache, int32([[0]])[:0], int32([4])[:0]).shape == (0, 1, 2, 32)
 
 
-@pytest.mark.parametrize("new", [1, 40, 140])
+@pytest.mark.parametrize("new", [1, 40, 140, 900])
 def test_not_finite_stays_where_it_belongs(cuda_ok, new):
     """A NaN scale, or an infinite query, reaches the rows that see it and no others."""
     kc, ks, vc, vs = filled(24, 2, 16, 64)

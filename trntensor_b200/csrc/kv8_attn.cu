@@ -1,6 +1,7 @@
 // Attention over a paged 8-bit cache: launches (csrc/kv8_attn.cuh).
 #include "common.cuh"
 #include "kv8_attn.cuh"
+#include "kv8_prefill.cuh"
 
 namespace tt {
 namespace kv8 {
@@ -18,9 +19,20 @@ int set_attr() {
              ? TT_OK
              : TT_ERR_CUDA;
 }
+template <typename T, int DP>
+int set_prefill() {
+  return cudaFuncSetAttribute(prefill_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              PreShape<DP>::kSmem) == cudaSuccess
+             ? TT_OK
+             : TT_ERR_CUDA;
+}
 template <typename T>
 int set_attrs() {
   int st = set_attr<T, 64>();
+  if constexpr (sizeof(T) == 2) {
+    if (st == TT_OK) st = set_prefill<T, 64>();
+    if (st == TT_OK) st = set_prefill<T, 128>();
+  }
   if (st == TT_OK) st = set_attr<T, 128>();
   if (st == TT_OK) st = set_attr<T, 192>();
   if (st == TT_OK) st = set_attr<T, 256>();
@@ -61,8 +73,28 @@ int launch(const Attend& p, int sms, cudaStream_t s) {
   cfg.numAttrs = 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, join_kernel<T>, p));
 }
+// 16-bit types with up to 128 values a head go to the tensor cores' tiles of
+// 256 rows where that is faster. There a block of 128 tokens takes about 2700
+// clocks of a CTA, however few of its rows are used, and the other kernel
+// about 1250 of an SM for each 64 tokens and 16 rows, spread over all SMs: the
+// first wins from rows x heads x sequences = 2560 for each wave of CTAs.
+bool many_rows(const Attend& p, int sms) {
+  const long long tiles = ((long long)p.rows + 255) / 256 * p.heads * p.batch;
+  return p.rows > 16 && (long long)p.rows * p.heads * p.batch > 2560 * ((tiles + sms - 1) / sms);
+}
+
+template <typename T, int DP>
+int launch_prefill(const Attend& p, cudaStream_t s) {
+  const long long tiles = ((long long)p.rows + 255) / 256;
+  prefill_kernel<T, DP><<<dim3((unsigned)tiles, p.heads, p.batch), kPreThreads, PreShape<DP>::kSmem, s>>>(p);
+  return cuda_status(cudaGetLastError());
+}
 template <typename T>
 int launch_dim(const Attend& p, int sms, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (many_rows(p, sms) && p.dim <= 128 && p.heads <= 65535 && p.batch <= 65535)
+      return p.dim <= 64 ? launch_prefill<T, 64>(p, s) : launch_prefill<T, 128>(p, s);
+  }
   if (p.dim <= 64) return launch<T, 64>(p, sms, s);
   if (p.dim <= 128) return launch<T, 128>(p, sms, s);
   if (p.dim <= 192) return launch<T, 192>(p, sms, s);

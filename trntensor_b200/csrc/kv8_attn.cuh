@@ -17,8 +17,9 @@
 // the codes are exact in fp16; a row of q is scaled by a power of two to below
 // 2^14 and rounded to fp16 (exact for 16-bit types down to 2^-27 of the row's
 // largest value, 2^-39 of that below) or, for fp32, kept as two fp16 terms.
-// The softmax weights are fp16 (2^-12, below the rounding of a bf16 result and
-// at that of an fp16 one; again held up by 2^14), two terms for fp32. Page
+// The softmax weights are fp16 (2^-11 of each, a quarter of a bf16 result's
+// rounding and as much as an fp16 one's; again held up by 2^14), two terms for
+// fp32. Page
 // scales multiply scores and weights in fp32; weights are held relative to the
 // largest value scale seen.
 //

@@ -1,0 +1,479 @@
+// Attention of many query rows over a paged 8-bit cache (csrc/kv8.cuh), on the
+// fifth-generation tensor cores. 16-bit operands, head dimensions up to 128.
+//
+// A CTA takes 256 query rows (tokens x heads of a kv head's group) of one
+// sequence and kv head, as two tiles of 128, and goes over the tokens in
+// blocks of 128:
+//   S_i = Q_i K^T (tcgen05, fp32 in TMEM)  ->  softmax warps of tile i
+//   P_i = 2^(S f - m) as fp16, in TMEM over S_i  ->  O_i += P_i V (A from TMEM)
+// While the tensor cores work for one tile, the softmax of the other runs.
+// Keys and values come as raw codes by bulk copies and are decoded once for
+// all 256 rows into swizzled fp16 operands (exact). Rows of q are scaled to
+// 2^13..2^14 by a power of two (exact for 16-bit types down to 2^-27 of the
+// row's largest value). Page scales: f = sk x the row's power x scale goes into
+// the exponent; values' scales relative to the sequence's largest one (found
+// first) go into the weights. The maximum m moves only when it would rise by
+// more than 2^8, and O is rescaled in TMEM only then: weights stay below 2^14,
+// fp16 rounds them by 2^-11, sums are fp32.
+//
+// What bounds it: tensor cores and the exponentials' unit need about the same
+// time (2048 clocks a block for 256 rows); decoding is a fifth of that.
+// Roles: warps 0-3 and 4-7 softmax of tiles 0 and 1 (a thread a row), 8-11
+// decode, 12 copies, 13 issues the MMAs.
+#pragma once
+#include "kv8_attn.cuh"
+#include "q4_gemm.cuh"
+
+namespace tt {
+namespace kv8 {
+
+constexpr int kPreThreads = 14 * 32;
+constexpr int kPreKeys = 128;        // tokens of a block
+constexpr int kScaleSlots = 8;
+constexpr float kPreUp = 64.f;       // a weight of 1, before m moves, in P
+
+template <int DP>
+struct PreShape {
+  static constexpr int kQ = 128 * DP * 2;             // bytes of a tile of Q
+  static constexpr int kKV = kPreKeys * DP * 2;       // of K or V as fp16
+  static constexpr int kRaw = kPreKeys * DP;          // and as codes
+  static constexpr int kSmem = 2 * kQ + 4 * kKV + 2 * kRaw + 1024;
+  static constexpr int kO = 256;                      // first column of O_0 (S_0 0, S_1 128)
+  static_assert(kSmem + 1536 <= 227 * 1024, "shared memory of an SM");
+};
+
+// D[tmem] (+)= A[tmem] B[smem]^T, fp16 operands.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p) {
+  using S = PreShape<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* sm_q = smem;
+  uint8_t* sm_k = sm_q + 2 * S::kQ;
+  uint8_t* sm_v = sm_k + 2 * S::kKV;
+  uint8_t* sm_raw = sm_v + 2 * S::kKV;
+  __shared__ uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2],
+      pv_done[2], q_ready, last;
+  __shared__ float sc_k[kScaleSlots][8], sc_v[kScaleSlots][8];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int dead, top_lim;
+  __shared__ unsigned int top_scale;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int dim = p.dim, group = p.heads_q / p.heads;
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int tile = gridDim.x - 1 - blockIdx.x;  // the longest first
+  const int length = (int)clamp_length(p, b, threadIdx.x == 0 && h == 0 && blockIdx.x == 0);
+  const int count = clamp_count(p, b, threadIdx.x == 0 && h == 0 && blockIdx.x == 0);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(&q_ready, 256);
+    mbar_init(&last, 1);
+    fence_mbar_init();
+    dead = 0;
+    top_lim = 0;
+    top_scale = 0;
+  }
+  if (warp == 13) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  // rows of this thread (softmax warps), and what they see
+  int lim = 0, row = -1;
+  const T* from = nullptr;
+  if (warp < 8) {
+    const int r = tile * 256 + threadIdx.x;
+    if (r < p.rows) {
+      row = r;
+      const int tok = r / group, head = h * group + r % group;
+      if (tok < count) {
+        lim = max(p.causal ? length - count + tok + 1 : length, 0);
+        from = static_cast<const T*>(p.q) + b * p.q_b + tok * p.q_s + head * p.q_h;
+      }
+    }
+    const int most = __reduce_max_sync(0xffffffffu, lim);
+    if (lane == 0) atomicMax(&top_lim, most);
+  }
+  __syncthreads();
+  const int blocks = (top_lim + kPreKeys - 1) / kPreKeys;
+  const int tiles = p.rows - tile * 256 > 128 ? 2 : 1;
+  {  // the largest value scale in sight
+    unsigned int top = 0;
+    const int pages = (top_lim + p.page - 1) >> p.page_log;
+    for (int i = threadIdx.x; i < pages; i += kPreThreads) {
+      const int page = p.table[b * p.table_b + i];
+      if (page < 0 || page >= p.pages) {
+        raise(p.status, kBadPage);
+        continue;
+      }
+      const float s = p.vs[(long long)page * p.heads + h];
+      if (s > 0.f) top = max(top, __float_as_uint(s));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) atomicMax(&top_scale, top);
+  }
+  if (dim < DP) {  // columns of K and Q behind the head dimension are zeros, for good
+    for (int i = threadIdx.x; i < (2 * S::kQ + 2 * S::kKV) / 16; i += kPreThreads)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const float ref = fmaxf(__uint_as_float(top_scale), 1e-30f);
+  int* err = &dead;
+
+  if (warp == 12) {
+    // ---- copies: a lane a unit of 16 tokens
+    for (int j = 0; j < blocks; ++j) {
+      const int tok = j * kPreKeys + 16 * lane;
+      int page = -1;
+      if (lane < 8 && tok < length) page = p.table[b * p.table_b + (tok >> p.page_log)];
+      if (page >= p.pages) page = -1;
+      const long long head = (long long)max(page, 0) * p.heads + h;
+      if (lane < 8) {
+        sc_k[j % kScaleSlots][lane] = page >= 0 ? p.ks[head] : 0.f;
+        sc_v[j % kScaleSlots][lane] = page >= 0 ? p.vs[head] : 0.f;
+      }
+      __syncwarp();  // before lane 0's arrival below, which the softmax warps wait behind
+      const unsigned has = __ballot_sync(0xffffffffu, page >= 0);
+      const long long at = (head * p.page + (tok & (p.page - 1))) * dim;
+      bool ok = true;
+      for (int v = 0; v < 2 && ok; ++v) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[v], (j & 1) ^ 1, err, kTimeout));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[v], __popc(has) * 16 * dim);
+        __syncwarp();
+        if (page >= 0)
+          bulk_load(smem_u32(sm_raw + v * S::kRaw + lane * 16 * dim), (v ? p.vc : p.kc) + at, 16 * dim,
+                    smem_u32(&raw_full[v]));
+      }
+      if (!ok) break;
+    }
+    // what is in flight arrives, or the wait for it is over
+    if (lane == 0 && blocks > 0 && dead != 0)
+      for (int v = 0; v < 2; ++v) mbar_wait_drain(&raw_full[v], (blocks - 1) & 1);
+    __syncwarp();
+  } else if (warp == 13) {
+    // ---- MMAs
+    if (lane == 0 && blocks > 0) {
+      constexpr uint32_t id_s = q4::idesc_f16(128, kPreKeys, 0), id_o = q4::idesc_f16(128, DP, 0);
+      auto scores = [&](int i, int j) {  // S_i of block j
+        const uint32_t q = smem_u32(sm_q + i * S::kQ), k = smem_u32(sm_k + (j & 1) * S::kKV);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+          const uint32_t off = (s / 4) * 128 * 128 + (s % 4) * 32;
+          q4::mma_f16(tmem + i * 128, smem_desc(q + off, 16, 1024, 2), smem_desc(k + off, 16, 1024, 2), id_s, s != 0);
+        }
+        mma_commit(&s_full[i]);
+      };
+      auto values = [&](int i, int j) {  // O_i += P_i V of block j
+        const uint32_t v = smem_u32(sm_v + (j & 1) * S::kKV);
+#pragma unroll
+        for (int s = 0; s < kPreKeys / 16; ++s) {
+          const uint32_t off = (s / 4) * DP * 128 + (s % 4) * 32;
+          mma_f16_ts(tmem + S::kO + i * DP, tmem + i * 128 + s * 8, smem_desc(v + off, 16, 1024, 2), id_o,
+                     (j | s) != 0);
+        }
+        mma_commit(&pv_done[i]);
+      };
+      bool ok = mbar_wait(&q_ready, 0, err, kTimeout) && mbar_wait(&k_full[0], 0, err, kTimeout);
+      if (ok) {
+        tc_fence_after();
+        scores(0, 0);
+        if (tiles == 2) scores(1, 0);
+        mma_commit(&k_empty[0]);
+      }
+      for (int j = 0; j < blocks && ok; ++j) {
+        for (int i = 0; i < tiles && ok; ++i) {
+          ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1, err, kTimeout) && mbar_wait(&p_full[i], j & 1, err, kTimeout);
+          if (!ok) break;
+          tc_fence_after();
+          values(i, j);
+          if (i + 1 == tiles) mma_commit(&v_empty[j & 1]);
+          if (j + 1 < blocks) {
+            ok = mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, err, kTimeout);
+            if (!ok) break;
+            tc_fence_after();
+            scores(i, j + 1);
+            if (i + 1 == tiles) mma_commit(&k_empty[(j + 1) & 1]);
+          }
+        }
+      }
+      // nothing may be in flight when the CTA gives its TMEM back
+      mma_commit(&last);
+      mbar_wait_drain(&last, 0);
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // ---- decoding
+    const int id = threadIdx.x - 256;
+    bool ok = true;
+    for (int j = 0; j < blocks && ok; ++j) {
+      const int buf = j & 1, phase = (j >> 1) & 1;
+      for (int v = 0; v < 2; ++v) {
+        ok = mbar_wait(&raw_full[v], j & 1, err, kTimeout) &&
+             mbar_wait(v ? &v_empty[buf] : &k_empty[buf], phase ^ 1, err, kTimeout);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t raw = smem_u32(sm_raw + v * S::kRaw);
+        const uint32_t to = smem_u32((v ? sm_v : sm_k) + buf * S::kKV);
+        const int per = dim / 16, all = kPreKeys * per;  // pieces of 16 codes
+#pragma unroll 4
+        for (int i = id; i < all; i += 128) {
+          const uint4 q = lds128(raw + i * 16);
+          uint32_t w[8];
+          decode4(q.x, w[0], w[1]);
+          decode4(q.y, w[2], w[3]);
+          decode4(q.z, w[4], w[5]);
+          decode4(q.w, w[6], w[7]);
+          uint32_t r, atom, c;
+          bool swap;  // which half first: eight lanes then meet all banks
+          if (v) {
+            // unit u, d: sixteen tokens of it, line d of the operand
+            const int u = i / dim;
+            r = i % dim;
+            atom = u / 4 * (DP * 128);
+            c = u % 4 * 2;
+            swap = false;
+          } else {
+            // token, sixteen d of it
+            r = i / per;
+            const int x = i % per;
+            atom = x / 4 * (kPreKeys * 128);
+            c = x % 4 * 2;
+            swap = x >= 4;
+          }
+          const uint32_t line = to + atom + r * 128;
+          const uint32_t a0 = line + ((c ^ (r & 7)) << 4), a1 = line + (((c + 1) ^ (r & 7)) << 4);
+          const uint32_t f = swap ? a1 : a0, g = swap ? a0 : a1;
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(f), "r"(swap ? w[4] : w[0]),
+                       "r"(swap ? w[5] : w[1]), "r"(swap ? w[6] : w[2]), "r"(swap ? w[7] : w[3])
+                       : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(g), "r"(swap ? w[0] : w[4]),
+                       "r"(swap ? w[1] : w[5]), "r"(swap ? w[2] : w[6]), "r"(swap ? w[3] : w[7])
+                       : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&raw_empty[v]);
+          mbar_arrive(v ? &v_full[buf] : &k_full[buf]);
+        }
+      }
+    }
+  } else {
+    // ---- softmax: a thread a row
+    const int i = warp >> 2;
+    float qs;
+    {  // this row of Q
+      float top = 0.f;
+      if (from != nullptr)
+        for (int d = 0; d < dim; d += 16) {
+          float x[16];
+          load16(from + d, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
+      int ex = (int)((__float_as_uint(top) >> 23) & 255);
+      ex = ex < 14 ? 14 : ex;
+      const float up = __uint_as_float((uint32_t)(267 - ex) << 23) * (p.scale < 0.f ? -1.f : 1.f);
+      qs = __uint_as_float((uint32_t)(ex - 13) << 23) * fabsf(p.scale);
+      const uint32_t r = threadIdx.x & 127;
+      for (int d = 0; d < dim; d += 16) {
+        float x[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.f;
+        if (from != nullptr) load16(from + d, x);
+        const uint32_t line = smem_u32(sm_q + i * S::kQ) + d / 64 * 16384 + r * 128;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float* y = x + 8 * c;
+          const uint32_t at = line + (((d % 64 / 8 + c) ^ (r & 7)) << 4);
+          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(q4::pack_f16(y[0] * up, y[1] * up)),
+                       "r"(q4::pack_f16(y[2] * up, y[3] * up)), "r"(q4::pack_f16(y[4] * up, y[5] * up)),
+                       "r"(q4::pack_f16(y[6] * up, y[7] * up))
+                       : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&q_ready);
+    }
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = lane_base + i * 128, to = lane_base + S::kO + i * DP;
+    // the least that a row of this warp which sees anything sees
+    int least = lim > 0 ? lim : 0x7fffffff;
+    least = __reduce_min_sync(0xffffffffu, least);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    if (i < tiles) {
+      for (int j = 0; j < blocks; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], j & 1, err, kTimeout));
+        if (!ok) break;
+        tc_fence_after();
+        const float* fk = sc_k[j % kScaleSlots];
+        const float* fv = sc_v[j % kScaleSlots];
+        const int tok0 = j * kPreKeys;
+        const bool mask = tok0 + kPreKeys > least;
+        // the block's maximum
+        float n = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          tmem_ld32(ts + 32 * c, s);
+          tmem_ld_wait();
+          if (mask) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (tok0 + 32 * c + e >= lim) s[e] = -INFINITY;
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float t = fmaxf(s[16 * u], s[16 * u + 1]);
+#pragma unroll
+            for (int e = 2; e < 16; ++e) t = fmaxf(t, s[16 * u + e]);
+            n = fmaxf(n, t * (qs * fk[2 * c + u]));  // a masked unit of scale 0 is not a number, and drops out
+          }
+        }
+        const bool rise = n > m + 8.f;  // from -inf: always, where anything is seen
+        if (__any_sync(0xffffffffu, rise)) {
+          const float now = rise ? n : m;
+          const float z = now == -INFINITY ? 0.f : now;
+          const float a = m == -INFINITY ? 0.f : exp2_approx(m - z);
+          l *= a;
+          m = now;
+          if (j > 0) {
+            // O of the blocks before must be there to be rescaled
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (j - 1) & 1, err, kTimeout));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 16) {
+              float o[16];
+              tmem_ld16(to + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] *= rise ? a : 1.f;
+              tmem_st16(to + c, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float z = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          tmem_ld32(ts + 32 * c, s);
+          tmem_ld_wait();
+          uint32_t w[16];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float* x = s + 16 * u;
+            const float f = qs * fk[2 * c + u], rel = __fdividef(fv[2 * c + u], ref) * kPreUp;
+            if (!mask && rel > 1e-30f) {
+              float lg;
+              asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
+              float sum = 0.f;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                x[e] = exp2_approx(fmaf(x[e], f, lg - z));
+                sum += x[e];
+              }
+              l = fmaf(sum, __fdividef(1.f, rel), l);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const bool hidden = mask && tok0 + 32 * c + 16 * u + e >= lim;
+                const float y = hidden ? 0.f : exp2_approx(fmaf(x[e], f, -z));
+                l += y;
+                x[e] = hidden ? 0.f : y * rel;
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
+          }
+          tmem_st16u(ts + 16 * c, w);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[i]);
+      }
+      if (ok && blocks > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (blocks - 1) & 1, err, kTimeout));
+        tc_fence_after();
+      }
+    }
+    const bool some = lim > 0 && blocks > 0;
+    const float inv = some && (l > 0.f || l != l) ? ref / (l * kPreUp) : 0.f;
+    for (int c = 0; c < dim; c += 16) {
+      float o[16];
+      if (blocks > 0 && i < tiles) {
+        tmem_ld16(to + c, o);
+        tmem_ld_wait();
+      }
+      if (row >= 0) {
+        T* at = static_cast<T*>(p.o) + row_offset(p, b, h, row) + c;
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = some ? o[2 * e] * inv : 0.f, y = some ? o[2 * e + 1] * inv : 0.f;
+          if constexpr (std::is_same<T, __half>::value) w[e] = q4::pack_f16(x, y);
+          else w[e] = q4::pack_bf16(x, y);
+        }
+        reinterpret_cast<uint4*>(at)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(at)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && dead != 0) raise(p.status, kTimeout);
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace kv8
+}  // namespace tt

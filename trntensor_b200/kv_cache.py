@@ -78,7 +78,8 @@ class KVCache8:
                    v_scales: torch.Tensor) -> "KVCache8":
         """A cache from int8 codes (pages, kv_heads, page_size, head_dim) in
         -127..127 and scales (pages, kv_heads), as :meth:`codes` and the scales
-        of another cache give them."""
+        of another cache give them (a negative scale is kept as its magnitude,
+        and its codes turn their signs)."""
         if k_codes.dim() != 4 or k_codes.dtype != torch.int8 or v_codes.dtype != torch.int8 \
                 or k_codes.shape != v_codes.shape:
             raise ValueError("from_codes: codes must be int8 (pages, kv_heads, page_size, head_dim)")
@@ -90,12 +91,18 @@ class KVCache8:
         dev = k_codes.device if k_codes.device.type == "cuda" else _device()
         self = cls.__new__(cls)
         self.num_pages, self.kv_heads, self.head_dim, self.page_size = n, h, d, p
+        # a negative scale's sign goes to its codes: the kernels compare scaled scores
+        k_scales = k_scales.to(dev, torch.float32)
+        v_scales = v_scales.to(dev, torch.float32)
+        k_codes, v_codes = k_codes.to(dev), v_codes.to(dev)
+        k_codes = torch.where((k_scales < 0)[..., None, None], -k_codes, k_codes)
+        v_codes = torch.where((v_scales < 0)[..., None, None], -v_codes, v_codes)
+        k_scales, v_scales = k_scales.abs(), v_scales.abs()
         # biased by 128: the sign bit turned over
-        self._k = k_codes.to(dev).contiguous().view(torch.uint8) ^ 128
-        v = v_codes.to(dev).view(n, h, p // 16, 16, d).transpose(-1, -2).contiguous()
+        self._k = k_codes.contiguous().view(torch.uint8) ^ 128
+        v = v_codes.reshape(n, h, p // 16, 16, d).transpose(-1, -2).contiguous()
         self._v = v.view(torch.uint8).bitwise_xor_(128)
-        self.k_scales = k_scales.to(dev, torch.float32, copy=True).contiguous()
-        self.v_scales = v_scales.to(dev, torch.float32, copy=True).contiguous()
+        self.k_scales, self.v_scales = k_scales.contiguous(), v_scales.contiguous()
         self.status = torch.zeros((), dtype=torch.int32, device=dev)
         return self
 
