@@ -21,8 +21,9 @@ int set_attr() {
 }
 template <typename T, int DP>
 int set_prefill() {
-  return cudaFuncSetAttribute(prefill_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              PreShape<DP>::kSmem) == cudaSuccess
+  const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  return cudaFuncSetAttribute(prefill_kernel<T, DP, true>, at, PreShape<DP>::kSmem) == cudaSuccess &&
+                 cudaFuncSetAttribute(prefill_kernel<T, DP, false>, at, PreShape<DP>::kSmem) == cudaSuccess
              ? TT_OK
              : TT_ERR_CUDA;
 }
@@ -86,7 +87,9 @@ bool many_rows(const Attend& p, int sms) {
 template <typename T, int DP>
 int launch_prefill(const Attend& p, cudaStream_t s) {
   const long long tiles = ((long long)p.rows + 255) / 256;
-  prefill_kernel<T, DP><<<dim3((unsigned)tiles, p.heads, p.batch), kPreThreads, PreShape<DP>::kSmem, s>>>(p);
+  const dim3 grid((unsigned)tiles, p.heads, p.batch);
+  if (p.dim == DP) prefill_kernel<T, DP, true><<<grid, kPreThreads, PreShape<DP>::kSmem, s>>>(p);
+  else prefill_kernel<T, DP, false><<<grid, kPreThreads, PreShape<DP>::kSmem, s>>>(p);
   return cuda_status(cudaGetLastError());
 }
 template <typename T>

@@ -29,7 +29,7 @@ namespace kv8 {
 
 constexpr int kPreThreads = 14 * 32;
 constexpr int kPreKeys = 128;        // tokens of a block
-constexpr int kScaleSlots = 8;
+constexpr int kScaleSlots = 6;       // the copies are at most three blocks ahead of the softmax
 constexpr float kPreUp = 64.f;       // a weight of 1, before m moves, in P
 
 template <int DP>
@@ -39,7 +39,7 @@ struct PreShape {
   static constexpr int kRaw = kPreKeys * DP;          // and as codes
   static constexpr int kSmem = 2 * kQ + 4 * kKV + 2 * kRaw + 1024;
   static constexpr int kO = 256;                      // first column of O_0 (S_0 0, S_1 128)
-  static_assert(kSmem + 1536 <= 227 * 1024, "shared memory of an SM");
+  static_assert(kSmem + 1280 + 512 <= 227 * 1024, "shared memory of an SM");
 };
 
 // D[tmem] (+)= A[tmem] B[smem]^T, fp16 operands.
@@ -72,7 +72,12 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[1
       : "memory");
 }
 
-template <typename T, int DP>
+__device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// kFull: the head dimension is DP.
+template <typename T, int DP, bool kFull>
 __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p) {
   using S = PreShape<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -83,12 +88,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   uint8_t* sm_raw = sm_v + 2 * S::kKV;
   __shared__ uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2],
       pv_done[2], q_ready, last;
-  __shared__ float sc_k[kScaleSlots][8], sc_v[kScaleSlots][8];
+  __shared__ float sc_k[kScaleSlots][8], sc_rel[kScaleSlots][8], sc_log[kScaleSlots][8], sc_inv[kScaleSlots][8];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead, top_lim;
   __shared__ unsigned int top_scale;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int dim = p.dim, group = p.heads_q / p.heads;
+  const int dim = kFull ? DP : p.dim, group = p.heads_q / p.heads;
   const int b = blockIdx.z, h = blockIdx.y;
   const int tile = gridDim.x - 1 - blockIdx.x;  // the longest first
   const int length = (int)clamp_length(p, b, threadIdx.x == 0 && h == 0 && blockIdx.x == 0);
@@ -174,7 +179,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       const long long head = (long long)max(page, 0) * p.heads + h;
       if (lane < 8) {
         sc_k[j % kScaleSlots][lane] = page >= 0 ? p.ks[head] : 0.f;
-        sc_v[j % kScaleSlots][lane] = page >= 0 ? p.vs[head] : 0.f;
+        const float rel = page >= 0 ? __fdividef(p.vs[head], ref) * kPreUp : 0.f;
+        float lg;
+        asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
+        sc_rel[j % kScaleSlots][lane] = rel;
+        sc_log[j % kScaleSlots][lane] = lg;
+        sc_inv[j % kScaleSlots][lane] = __fdividef(1.f, rel);
       }
       __syncwarp();  // before lane 0's arrival below, which the softmax warps wait behind
       const unsigned has = __ballot_sync(0xffffffffu, page >= 0);
@@ -252,6 +262,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     bool ok = true;
     for (int j = 0; j < blocks && ok; ++j) {
       const int buf = j & 1, phase = (j >> 1) & 1;
+#pragma unroll
       for (int v = 0; v < 2; ++v) {
         ok = mbar_wait(&raw_full[v], j & 1, err, kTimeout) &&
              mbar_wait(v ? &v_empty[buf] : &k_empty[buf], phase ^ 1, err, kTimeout);
@@ -259,8 +270,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         if (!ok) break;
         const uint32_t raw = smem_u32(sm_raw + v * S::kRaw);
         const uint32_t to = smem_u32((v ? sm_v : sm_k) + buf * S::kKV);
-        const int per = dim / 16, all = kPreKeys * per;  // pieces of 16 codes
-#pragma unroll 4
+        const int wide = kFull ? DP : dim;  // kFull: all divisions below are shifts
+        const int per = wide / 16, all = kPreKeys * per;  // pieces of 16 codes
+#pragma unroll 8
         for (int i = id; i < all; i += 128) {
           const uint4 q = lds128(raw + i * 16);
           uint32_t w[8];
@@ -268,32 +280,22 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           decode4(q.y, w[2], w[3]);
           decode4(q.z, w[4], w[5]);
           decode4(q.w, w[6], w[7]);
-          uint32_t r, atom, c;
-          bool swap;  // which half first: eight lanes then meet all banks
           if (v) {
-            // unit u, d: sixteen tokens of it, line d of the operand
-            const int u = i / dim;
-            r = i % dim;
-            atom = u / 4 * (DP * 128);
-            c = u % 4 * 2;
-            swap = false;
+            // unit u, d: sixteen tokens of it, in line d of the operand
+            const uint32_t u = i / wide, r = i % wide;
+            const uint32_t line = to + u / 4 * (DP * 128) + r * 128, c = u % 4 * 2;
+            sts128(line + ((c ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+            sts128(line + (((c + 1) ^ (r & 7)) << 4), w[4], w[5], w[6], w[7]);
           } else {
-            // token, sixteen d of it
-            r = i / per;
-            const int x = i % per;
-            atom = x / 4 * (kPreKeys * 128);
-            c = x % 4 * 2;
-            swap = x >= 4;
+            // a token, sixteen d of it; from 64 on the second half first:
+            // eight lanes then meet all banks
+            const uint32_t r = i / per, x = i % per;
+            const uint32_t line = to + x / 4 * (kPreKeys * 128) + r * 128, c = x % 4 * 2, swap = x / 4 & 1;
+            sts128(line + (((c + swap) ^ (r & 7)) << 4), swap ? w[4] : w[0], swap ? w[5] : w[1], swap ? w[6] : w[2],
+                   swap ? w[7] : w[3]);
+            sts128(line + (((c + 1 - swap) ^ (r & 7)) << 4), swap ? w[0] : w[4], swap ? w[1] : w[5],
+                   swap ? w[2] : w[6], swap ? w[3] : w[7]);
           }
-          const uint32_t line = to + atom + r * 128;
-          const uint32_t a0 = line + ((c ^ (r & 7)) << 4), a1 = line + (((c + 1) ^ (r & 7)) << 4);
-          const uint32_t f = swap ? a1 : a0, g = swap ? a0 : a1;
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(f), "r"(swap ? w[4] : w[0]),
-                       "r"(swap ? w[5] : w[1]), "r"(swap ? w[6] : w[2]), "r"(swap ? w[7] : w[3])
-                       : "memory");
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(g), "r"(swap ? w[0] : w[4]),
-                       "r"(swap ? w[1] : w[5]), "r"(swap ? w[2] : w[6]), "r"(swap ? w[3] : w[7])
-                       : "memory");
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -331,10 +333,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         for (int c = 0; c < 2; ++c) {
           const float* y = x + 8 * c;
           const uint32_t at = line + (((d % 64 / 8 + c) ^ (r & 7)) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(q4::pack_f16(y[0] * up, y[1] * up)),
-                       "r"(q4::pack_f16(y[2] * up, y[3] * up)), "r"(q4::pack_f16(y[4] * up, y[5] * up)),
-                       "r"(q4::pack_f16(y[6] * up, y[7] * up))
-                       : "memory");
+          sts128(at, q4::pack_f16(y[0] * up, y[1] * up), q4::pack_f16(y[2] * up, y[3] * up),
+                 q4::pack_f16(y[4] * up, y[5] * up), q4::pack_f16(y[6] * up, y[7] * up));
         }
       }
       fence_proxy_async_smem();
@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     // the least that a row of this warp which sees anything sees
     int least = lim > 0 ? lim : 0x7fffffff;
     least = __reduce_min_sync(0xffffffffu, least);
-    float m = -INFINITY, l = 0.f;
+    // a row that sees nothing stays out of the maxima's way
+    float m = lim > 0 ? -INFINITY : 0.f, l = 0.f;
     bool ok = true;
     if (i < tiles) {
       for (int j = 0; j < blocks; ++j) {
@@ -353,27 +354,66 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         if (!ok) break;
         tc_fence_after();
         const float* fk = sc_k[j % kScaleSlots];
-        const float* fv = sc_v[j % kScaleSlots];
+        // values' scales relative to the largest, their logarithms and inverses
+        const float* fr = sc_rel[j % kScaleSlots];
+        const float* fl = sc_log[j % kScaleSlots];
+        const float* fi = sc_inv[j % kScaleSlots];
         const int tok0 = j * kPreKeys;
         const bool mask = tok0 + kPreKeys > least;
-        // the block's maximum
-        float n = -INFINITY;
+        // Weights by the maximum so far, and the block's own maximum, in one
+        // pass; they are kept back until it is sure that m stands.
+        uint32_t w[4][16];
+        float n = -INFINITY, sum = 0.f;
+        if (!mask && __all_sync(0xffffffffu, m != -INFINITY)) {  // the warp goes together
+          bool plain = true;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float s[32];
+            tmem_ld32(ts + 32 * c, s);
+            tmem_ld_wait();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              float* x = s + 16 * u;
+              const float f = qs * fk[2 * c + u], rel = fr[2 * c + u], y = fl[2 * c + u] - m;
+              plain = plain && rel > 1e-30f;
+              float t[4], q[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(x[e], x[e + 4]), fmaxf(x[e + 8], x[e + 12]));
+              n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], f, y));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
+              sum = fmaf((q[0] + q[1]) + (q[2] + q[3]), fi[2 * c + u], sum);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[c][8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
+            }
+          }
+          // weights of units without a logarithm of their scale come below
+          if (__all_sync(0xffffffffu, lim == 0 || (n <= m + 8.f && plain))) {
+            l += sum;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_st16u(ts + 16 * c, w[c]);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[i]);
+            continue;
+          }
+        }
+        // First blocks, hidden tokens, a maximum that rises, odd scales.
+        n = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float s[32];
           tmem_ld32(ts + 32 * c, s);
           tmem_ld_wait();
-          if (mask) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (tok0 + 32 * c + e >= lim) s[e] = -INFINITY;
-          }
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            float t = fmaxf(s[16 * u], s[16 * u + 1]);
+            float t = -INFINITY;
 #pragma unroll
-            for (int e = 2; e < 16; ++e) t = fmaxf(t, s[16 * u + e]);
-            n = fmaxf(n, t * (qs * fk[2 * c + u]));  // a masked unit of scale 0 is not a number, and drops out
+            for (int e = 0; e < 16; ++e)
+              if (tok0 + 32 * c + 16 * u + e < lim) t = fmaxf(t, s[16 * u + e]);
+            n = fmaxf(n, t * (qs * fk[2 * c + u]));  // a hidden unit of scale 0 is not a number, and drops out
           }
         }
         const bool rise = n > m + 8.f;  // from -inf: always, where anything is seen
@@ -401,39 +441,27 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           }
         }
         const float z = m == -INFINITY ? 0.f : m;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float s[32];
           tmem_ld32(ts + 32 * c, s);
           tmem_ld_wait();
-          uint32_t w[16];
+          uint32_t v[16];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             float* x = s + 16 * u;
-            const float f = qs * fk[2 * c + u], rel = __fdividef(fv[2 * c + u], ref) * kPreUp;
-            if (!mask && rel > 1e-30f) {
-              float lg;
-              asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
-              float sum = 0.f;
+            const float f = qs * fk[2 * c + u], rel = fr[2 * c + u];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                x[e] = exp2_approx(fmaf(x[e], f, lg - z));
-                sum += x[e];
-              }
-              l = fmaf(sum, __fdividef(1.f, rel), l);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const bool hidden = mask && tok0 + 32 * c + 16 * u + e >= lim;
-                const float y = hidden ? 0.f : exp2_approx(fmaf(x[e], f, -z));
-                l += y;
-                x[e] = hidden ? 0.f : y * rel;
-              }
+            for (int e = 0; e < 16; ++e) {
+              const bool hidden = tok0 + 32 * c + 16 * u + e >= lim;
+              const float y = hidden ? 0.f : exp2_approx(fmaf(x[e], f, -z));
+              l += y;
+              x[e] = hidden ? 0.f : y * rel;
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
+            for (int e = 0; e < 8; ++e) v[8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
           }
-          tmem_st16u(ts + 16 * c, w);
+          tmem_st16u(ts + 16 * c, v);
         }
         tmem_st_wait();
         tc_fence_before();
