@@ -8,7 +8,7 @@ scale, and ex2.approx adds 2^-21 of a weight. Weights are rounded to fp16,
 whose 11 significant bits leave half a step of 2^-11 (two terms for fp32
 operands: 2^-22), and q of fp32 likewise (2^-22 of its row's largest value).
 Below fp16's normal range a weight is off by half of 2^-24, in units of which
-the largest weight is at least 2^6. Numerator and denominator take the score's
+the largest weight is at least 2^3. Numerator and denominator take the score's
 error once each. The sums over tokens add at most L / 16 + 64 roundings of
 2^-23. Everything is relative to a = sum p |v|; the result is rounded once.
 """
@@ -261,7 +261,7 @@ def reference(q, parts, table, lengths, counts, causal, scale):
                 if two:
                     d += 2.0**-22 * float(x.abs().max() * kh.abs().sum(1).max()) * abs(scale)
                 e = (2.0**-22 if two else 2.0**-11) + 2 * d + 2.0**-20 + (n / 16 + 64) * 2.0**-22
-                loss[b, i, h] = e * mass + n * 2.0**-31 * float(p.max() * vh.abs().max())
+                loss[b, i, h] = e * mass + n * 2.0**-28 * float(p.max() * vh.abs().max())
     return o, loss
 
 

@@ -3,21 +3,23 @@
 //
 // A CTA takes 256 query rows (tokens x heads of a kv head's group) of one
 // sequence and kv head, as two tiles of 128, and goes over the tokens in
-// blocks of 128:
+// blocks of 64:
 //   S_i = Q_i K^T (tcgen05, fp32 in TMEM)  ->  softmax warps of tile i
 //   P_i = 2^(S f - m) as fp16, in TMEM over S_i  ->  O_i += P_i V (A from TMEM)
-// While the tensor cores work for one tile, the softmax of the other runs.
+// A tile has two S in TMEM: the scores of the next block are there when the
+// softmax of one ends, so that its warps never wait for the way through the
+// tensor cores and back (with one S of 128 tokens that way was half the time).
 // Keys and values come as raw codes by bulk copies and are decoded once for
 // all 256 rows into swizzled fp16 operands (exact). Rows of q are scaled to
 // 2^13..2^14 by a power of two (exact for 16-bit types down to 2^-27 of the
 // row's largest value). Page scales: f = sk x the row's power x scale goes into
 // the exponent; values' scales relative to the sequence's largest one (found
-// first) go into the weights. The maximum m moves only when it would rise by
-// more than 2^8, and O is rescaled in TMEM only then: weights stay below 2^14,
-// fp16 rounds them by 2^-11, sums are fp32.
+// first) go into the weights. The maximum m is taken 2^3 above the block's when
+// it is set, moves only when a weight would pass 2^8, and O is rescaled in TMEM
+// only then: weights stay below 2^15, fp16 rounds them by 2^-11, sums are fp32.
 //
 // What bounds it: tensor cores and the exponentials' unit need about the same
-// time (2048 clocks a block for 256 rows); decoding is a fifth of that.
+// time (2048 to 2560 clocks for 128 tokens and 256 rows).
 // Roles: warps 0-3 and 4-7 softmax of tiles 0 and 1 (a thread a row), 8-11
 // decode, 12 copies, 13 issues the MMAs.
 #pragma once
@@ -28,17 +30,19 @@ namespace tt {
 namespace kv8 {
 
 constexpr int kPreThreads = 14 * 32;
-constexpr int kPreKeys = 128;        // tokens of a block
-constexpr int kScaleSlots = 6;       // the copies are at most three blocks ahead of the softmax
-constexpr float kPreUp = 64.f;       // a weight of 1, before m moves, in P
+constexpr int kPreKeys = 64;         // tokens of a block
+constexpr int kScaleSlots = 8;       // the copies are at most five blocks ahead of the softmax
+constexpr float kPreUp = 128.f;      // a weight of 1 in P
+constexpr float kPreRoom = 3.f;      // m above the largest score when it is set, and
+constexpr float kPreRise = 8.f;      // a score above m that it bears; both as powers of two
 
 template <int DP>
 struct PreShape {
   static constexpr int kQ = 128 * DP * 2;             // bytes of a tile of Q
   static constexpr int kKV = kPreKeys * DP * 2;       // of K or V as fp16
   static constexpr int kRaw = kPreKeys * DP;          // and as codes
-  static constexpr int kSmem = 2 * kQ + 4 * kKV + 2 * kRaw + 1024;
-  static constexpr int kO = 256;                      // first column of O_0 (S_0 0, S_1 128)
+  static constexpr int kSmem = 2 * kQ + 4 * kKV + 4 * kRaw + 1024;
+  static constexpr int kO = 256;                      // first column of O_0; S_i of block j at (2 i + j % 2) 64
   static_assert(kSmem + 1280 + 512 <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -86,9 +90,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   uint8_t* sm_k = sm_q + 2 * S::kQ;
   uint8_t* sm_v = sm_k + 2 * S::kKV;
   uint8_t* sm_raw = sm_v + 2 * S::kKV;
-  __shared__ uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2],
-      pv_done[2], q_ready, last;
-  __shared__ float sc_k[kScaleSlots][8], sc_rel[kScaleSlots][8], sc_log[kScaleSlots][8], sc_inv[kScaleSlots][8];
+  constexpr int kUnits = kPreKeys / 16;
+  // of block j: [..][j % 2], in its phase j / 2 % 2
+  __shared__ uint64_t raw_full[2][2], raw_empty[2][2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2],
+      p_full[2][2], pv_done[2], q_ready, last;
+  __shared__ float sc_k[kScaleSlots][kUnits], sc_rel[kScaleSlots][kUnits], sc_log[kScaleSlots][kUnits],
+      sc_inv[kScaleSlots][kUnits];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead, top_lim;
   __shared__ unsigned int top_scale;
@@ -101,14 +108,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 4);
+      for (int k = 0; k < 2; ++k) {
+        mbar_init(&raw_full[i][k], 1);
+        mbar_init(&raw_empty[i][k], 4);
+        mbar_init(&s_full[i][k], 1);
+        mbar_init(&p_full[i][k], 128);
+      }
       mbar_init(&k_full[i], 4);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 4);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(&q_ready, 256);
@@ -172,12 +181,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   if (warp == 12) {
     // ---- copies: a lane a unit of 16 tokens
     for (int j = 0; j < blocks; ++j) {
-      const int tok = j * kPreKeys + 16 * lane;
+      const int tok = j * kPreKeys + 16 * lane, buf = j & 1, phase = (j >> 1) & 1;
       int page = -1;
-      if (lane < 8 && tok < length) page = p.table[b * p.table_b + (tok >> p.page_log)];
+      if (lane < kUnits && tok < length) page = p.table[b * p.table_b + (tok >> p.page_log)];
       if (page >= p.pages) page = -1;
       const long long head = (long long)max(page, 0) * p.heads + h;
-      if (lane < 8) {
+      if (lane < kUnits) {
         sc_k[j % kScaleSlots][lane] = page >= 0 ? p.ks[head] : 0.f;
         const float rel = page >= 0 ? __fdividef(p.vs[head], ref) * kPreUp : 0.f;
         float lg;
@@ -191,19 +200,20 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       const long long at = (head * p.page + (tok & (p.page - 1))) * dim;
       bool ok = true;
       for (int v = 0; v < 2 && ok; ++v) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[v], (j & 1) ^ 1, err, kTimeout));
+        ok = __all_sync(0xffffffffu, mbar_wait(&raw_empty[v][buf], phase ^ 1, err, kTimeout));
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(&raw_full[v], __popc(has) * 16 * dim);
+        if (lane == 0) mbar_arrive_expect_tx(&raw_full[v][buf], __popc(has) * 16 * dim);
         __syncwarp();
         if (page >= 0)
-          bulk_load(smem_u32(sm_raw + v * S::kRaw + lane * 16 * dim), (v ? p.vc : p.kc) + at, 16 * dim,
-                    smem_u32(&raw_full[v]));
+          bulk_load(smem_u32(sm_raw + (2 * v + buf) * S::kRaw + lane * 16 * dim), (v ? p.vc : p.kc) + at, 16 * dim,
+                    smem_u32(&raw_full[v][buf]));
       }
       if (!ok) break;
     }
     // what is in flight arrives, or the wait for it is over
-    if (lane == 0 && blocks > 0 && dead != 0)
-      for (int v = 0; v < 2; ++v) mbar_wait_drain(&raw_full[v], (blocks - 1) & 1);
+    if (lane == 0 && dead != 0)
+      for (int j = max(blocks - 2, 0); j < blocks; ++j)
+        for (int v = 0; v < 2; ++v) mbar_wait_drain(&raw_full[v][j & 1], (j >> 1) & 1);
     __syncwarp();
   } else if (warp == 13) {
     // ---- MMAs
@@ -212,42 +222,41 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       auto scores = [&](int i, int j) {  // S_i of block j
         const uint32_t q = smem_u32(sm_q + i * S::kQ), k = smem_u32(sm_k + (j & 1) * S::kKV);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-          const uint32_t off = (s / 4) * 128 * 128 + (s % 4) * 32;
-          q4::mma_f16(tmem + i * 128, smem_desc(q + off, 16, 1024, 2), smem_desc(k + off, 16, 1024, 2), id_s, s != 0);
-        }
-        mma_commit(&s_full[i]);
+        for (int s = 0; s < DP / 16; ++s)
+          q4::mma_f16(tmem + (2 * i + (j & 1)) * kPreKeys, smem_desc(q + s / 4 * 16384 + s % 4 * 32, 16, 1024, 2),
+                      smem_desc(k + s / 4 * kPreKeys * 128 + s % 4 * 32, 16, 1024, 2), id_s, s != 0);
+        mma_commit(&s_full[i][j & 1]);
       };
       auto values = [&](int i, int j) {  // O_i += P_i V of block j
         const uint32_t v = smem_u32(sm_v + (j & 1) * S::kKV);
 #pragma unroll
-        for (int s = 0; s < kPreKeys / 16; ++s) {
-          const uint32_t off = (s / 4) * DP * 128 + (s % 4) * 32;
-          mma_f16_ts(tmem + S::kO + i * DP, tmem + i * 128 + s * 8, smem_desc(v + off, 16, 1024, 2), id_o,
-                     (j | s) != 0);
-        }
+        for (int s = 0; s < kPreKeys / 16; ++s)
+          mma_f16_ts(tmem + S::kO + i * DP, tmem + (2 * i + (j & 1)) * kPreKeys + s * 8,
+                     smem_desc(v + s * 32, 16, 1024, 2), id_o, (j | s) != 0);
         mma_commit(&pv_done[i]);
       };
-      bool ok = mbar_wait(&q_ready, 0, err, kTimeout) && mbar_wait(&k_full[0], 0, err, kTimeout);
-      if (ok) {
+      bool ok = mbar_wait(&q_ready, 0, err, kTimeout);
+      for (int j = 0; j < min(blocks, 2) && ok; ++j) {
+        ok = mbar_wait(&k_full[j], 0, err, kTimeout);
+        if (!ok) break;
         tc_fence_after();
-        scores(0, 0);
-        if (tiles == 2) scores(1, 0);
-        mma_commit(&k_empty[0]);
+        for (int i = 0; i < tiles; ++i) scores(i, j);
+        mma_commit(&k_empty[j]);
       }
       for (int j = 0; j < blocks && ok; ++j) {
+        const int buf = j & 1, phase = (j >> 1) & 1;
         for (int i = 0; i < tiles && ok; ++i) {
-          ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1, err, kTimeout) && mbar_wait(&p_full[i], j & 1, err, kTimeout);
+          ok = mbar_wait(&v_full[buf], phase, err, kTimeout) && mbar_wait(&p_full[i][buf], phase, err, kTimeout);
           if (!ok) break;
           tc_fence_after();
           values(i, j);
-          if (i + 1 == tiles) mma_commit(&v_empty[j & 1]);
-          if (j + 1 < blocks) {
-            ok = mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, err, kTimeout);
+          if (i + 1 == tiles) mma_commit(&v_empty[buf]);
+          if (j + 2 < blocks) {  // over P_i of this block, which goes first
+            ok = mbar_wait(&k_full[buf], phase ^ 1, err, kTimeout);
             if (!ok) break;
             tc_fence_after();
-            scores(i, j + 1);
-            if (i + 1 == tiles) mma_commit(&k_empty[(j + 1) & 1]);
+            scores(i, j + 2);
+            if (i + 1 == tiles) mma_commit(&k_empty[buf]);
           }
         }
       }
@@ -264,11 +273,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       const int buf = j & 1, phase = (j >> 1) & 1;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        ok = mbar_wait(&raw_full[v], j & 1, err, kTimeout) &&
+        ok = mbar_wait(&raw_full[v][buf], phase, err, kTimeout) &&
              mbar_wait(v ? &v_empty[buf] : &k_empty[buf], phase ^ 1, err, kTimeout);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t raw = smem_u32(sm_raw + v * S::kRaw);
+        const uint32_t raw = smem_u32(sm_raw + (2 * v + buf) * S::kRaw);
         const uint32_t to = smem_u32((v ? sm_v : sm_k) + buf * S::kKV);
         const int wide = kFull ? DP : dim;  // kFull: all divisions below are shifts
         const int per = wide / 16, all = kPreKeys * per;  // pieces of 16 codes
@@ -283,7 +292,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           if (v) {
             // unit u, d: sixteen tokens of it, in line d of the operand
             const uint32_t u = i / wide, r = i % wide;
-            const uint32_t line = to + u / 4 * (DP * 128) + r * 128, c = u % 4 * 2;
+            const uint32_t line = to + r * 128, c = u * 2;
             sts128(line + ((c ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
             sts128(line + (((c + 1) ^ (r & 7)) << 4), w[4], w[5], w[6], w[7]);
           } else {
@@ -300,7 +309,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&raw_empty[v]);
+          mbar_arrive(&raw_empty[v][buf]);
           mbar_arrive(v ? &v_full[buf] : &k_full[buf]);
         }
       }
@@ -341,7 +350,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       mbar_arrive(&q_ready);
     }
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t ts = lane_base + i * 128, to = lane_base + S::kO + i * DP;
+    const uint32_t to = lane_base + S::kO + i * DP;
     // the least that a row of this warp which sees anything sees
     int least = lim > 0 ? lim : 0x7fffffff;
     least = __reduce_min_sync(0xffffffffu, least);
@@ -350,9 +359,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     bool ok = true;
     if (i < tiles) {
       for (int j = 0; j < blocks; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], j & 1, err, kTimeout));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i][j & 1], (j >> 1) & 1, err, kTimeout));
         if (!ok) break;
         tc_fence_after();
+        const uint32_t ts = lane_base + (2 * i + (j & 1)) * kPreKeys;
         const float* fk = sc_k[j % kScaleSlots];
         // values' scales relative to the largest, their logarithms and inverses
         const float* fr = sc_rel[j % kScaleSlots];
@@ -360,50 +370,49 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         const float* fi = sc_inv[j % kScaleSlots];
         const int tok0 = j * kPreKeys;
         const bool mask = tok0 + kPreKeys > least;
+        uint32_t w[2][16];
+        float n = -INFINITY;
         // Weights by the maximum so far, and the block's own maximum, in one
         // pass; they are kept back until it is sure that m stands.
-        uint32_t w[4][16];
-        float n = -INFINITY, sum = 0.f;
         if (!mask && __all_sync(0xffffffffu, m != -INFINITY)) {  // the warp goes together
           bool plain = true;
+          float sum = 0.f;
+          float s[2][32];
+          tmem_ld32(ts, s[0]);
+          tmem_ld32(ts + 32, s[1]);
+          tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float s[32];
-            tmem_ld32(ts + 32 * c, s);
-            tmem_ld_wait();
+          for (int u = 0; u < kUnits; ++u) {
+            float* x = s[u / 2] + 16 * (u & 1);
+            const float f = qs * fk[u], y = fl[u] - m;
+            plain = plain && fr[u] > 1e-30f;
+            float t[4], q[4];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float* x = s + 16 * u;
-              const float f = qs * fk[2 * c + u], rel = fr[2 * c + u], y = fl[2 * c + u] - m;
-              plain = plain && rel > 1e-30f;
-              float t[4], q[4];
+            for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(x[e], x[e + 4]), fmaxf(x[e + 8], x[e + 12]));
+            n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(x[e], x[e + 4]), fmaxf(x[e + 8], x[e + 12]));
-              n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f);
+            for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], f, y));
 #pragma unroll
-              for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], f, y));
+            for (int e = 0; e < 4; ++e) q[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
+            sum = fmaf((q[0] + q[1]) + (q[2] + q[3]), fi[u], sum);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) q[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
-              sum = fmaf((q[0] + q[1]) + (q[2] + q[3]), fi[2 * c + u], sum);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) w[c][8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
-            }
+            for (int e = 0; e < 8; ++e) w[u / 2][8 * (u & 1) + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
           }
           // weights of units without a logarithm of their scale come below
-          if (__all_sync(0xffffffffu, lim == 0 || (n <= m + 8.f && plain))) {
+          if (__all_sync(0xffffffffu, lim == 0 || (n <= m + kPreRise && plain))) {
             l += sum;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_st16u(ts + 16 * c, w[c]);
+            tmem_st16u(ts, w[0]);
+            tmem_st16u(ts + 16, w[1]);
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&p_full[i]);
+            mbar_arrive(&p_full[i][j & 1]);
             continue;
           }
         }
         // First blocks, hidden tokens, a maximum that rises, odd scales.
         n = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           float s[32];
           tmem_ld32(ts + 32 * c, s);
           tmem_ld_wait();
@@ -416,9 +425,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
             n = fmaxf(n, t * (qs * fk[2 * c + u]));  // a hidden unit of scale 0 is not a number, and drops out
           }
         }
-        const bool rise = n > m + 8.f;  // from -inf: always, where anything is seen
+        const bool rise = n > m + kPreRise;  // from -inf: always, where anything is seen
         if (__any_sync(0xffffffffu, rise)) {
-          const float now = rise ? n : m;
+          const float now = rise ? n + kPreRoom : m;
           const float z = now == -INFINITY ? 0.f : now;
           const float a = m == -INFINITY ? 0.f : exp2_approx(m - z);
           l *= a;
@@ -441,12 +450,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           }
         }
         const float z = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
           float s[32];
           tmem_ld32(ts + 32 * c, s);
           tmem_ld_wait();
-          uint32_t v[16];
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             float* x = s + 16 * u;
@@ -459,18 +467,20 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
               x[e] = hidden ? 0.f : y * rel;
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
+            for (int e = 0; e < 8; ++e) w[c][8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
           }
-          tmem_st16u(ts + 16 * c, v);
+          tmem_st16u(ts + 16 * c, w[c]);
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[i]);
+        mbar_arrive(&p_full[i][j & 1]);
       }
-      if (ok && blocks > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (blocks - 1) & 1, err, kTimeout));
-        tc_fence_after();
-      }
+      // The last two products, one after the other: a barrier tells a phase
+      // from the one before only, and that the scores of the last block were
+      // there says that all before these two are done.
+      for (int j = max(blocks - 2, 0); j < blocks && ok; ++j)
+        ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], j & 1, err, kTimeout));
+      tc_fence_after();
     }
     const bool some = lim > 0 && blocks > 0;
     const float inv = some && (l > 0.f || l != l) ? ref / (l * kPreUp) : 0.f;
