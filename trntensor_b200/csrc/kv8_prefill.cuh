@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   constexpr int kUnits = kPreKeys / 16;
   // of block j: [..][j % 2], in its phase j / 2 % 2
   __shared__ uint64_t raw_full[2][2], raw_empty[2][2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2],
-      p_full[2][2], pv_done[2], q_ready, last;
+      p_full[2][2], pv_done[2][2], q_ready, last;
   __shared__ float sc_k[kScaleSlots][kUnits], sc_rel[kScaleSlots][kUnits], sc_log[kScaleSlots][kUnits],
       sc_inv[kScaleSlots][kUnits];
   __shared__ uint32_t tmem_slot;
@@ -113,12 +113,13 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         mbar_init(&raw_empty[i][k], 4);
         mbar_init(&s_full[i][k], 1);
         mbar_init(&p_full[i][k], 128);
+        mbar_init(&pv_done[i][k], 1);
       }
       mbar_init(&k_full[i], 4);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 4);
       mbar_init(&v_empty[i], 1);
-      mbar_init(&pv_done[i], 1);
+
     }
     mbar_init(&q_ready, 256);
     mbar_init(&last, 1);
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         for (int s = 0; s < kPreKeys / 16; ++s)
           mma_f16_ts(tmem + S::kO + i * DP, tmem + (2 * i + (j & 1)) * kPreKeys + s * 8,
                      smem_desc(v + s * 32, 16, 1024, 2), id_o, (j | s) != 0);
-        mma_commit(&pv_done[i]);
+        mma_commit(&pv_done[i][j & 1]);
       };
       bool ok = mbar_wait(&q_ready, 0, err, kTimeout);
       for (int j = 0; j < min(blocks, 2) && ok; ++j) {
@@ -434,7 +435,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           m = now;
           if (j > 0) {
             // O of the blocks before must be there to be rescaled
-            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (j - 1) & 1, err, kTimeout));
+            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i][(j - 1) & 1], ((j - 1) >> 1) & 1, err, kTimeout));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -475,11 +476,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         tc_fence_before();
         mbar_arrive(&p_full[i][j & 1]);
       }
-      // The last two products, one after the other: a barrier tells a phase
-      // from the one before only, and that the scores of the last block were
-      // there says that all before these two are done.
-      for (int j = max(blocks - 2, 0); j < blocks && ok; ++j)
-        ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], j & 1, err, kTimeout));
+      // `last` has one phase only. (pv_done could go on to the next phase, and
+      // look unfinished, before a slow warp asks for the one before.)
+      if (ok && blocks > 0) ok = __all_sync(0xffffffffu, mbar_wait(&last, 0, err, kTimeout));
       tc_fence_after();
     }
     const bool some = lim > 0 && blocks > 0;
