@@ -2,7 +2,7 @@
 
 Tolerances. A result is rounded once (half a step: eps / 2 of the value). The
 fp32 sum is a chain of at most 16 products, one addition for each 16 terms (8 a
-group and one a 128-wide block, or 8 a block, up to 16 rows, or 64 of 16-bit
+group and one a 128-wide block, or 8 a block, up to 16 rows, or 32 of 16-bit
 types over k), 8 warps and 8 CTAs; each of these loses at most a unit in the last place (2^-23, the tensor
 cores truncate) of a partial sum that sum |x W| bounds. Up to 16 rows the sum
 over n keeps 2^-16 of each product of 16-bit types. Above, fp16 terms: a 16-bit
@@ -42,7 +42,7 @@ def check(got, x, wide, over_n=False):
     """wide is (cols of x, cols of the result)."""
     ref = x.double() @ wide
     mass = x.double().abs() @ wide.abs()
-    if x.shape[0] <= 16 or (x.shape[0] <= 64 and not over_n and x.dtype != torch.float32):
+    if x.shape[0] <= 16 or (x.shape[0] <= 32 and not over_n and x.dtype != torch.float32):
         links = 48 + x.shape[1] / (16 if over_n else 128)
         loss = links * 2.0**-23 + (2.0**-16 if over_n and x.dtype != torch.float32 else 0)
     else:  # fp32: two or four passes over the sum

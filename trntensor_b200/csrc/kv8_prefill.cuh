@@ -47,12 +47,12 @@ struct PreShape {
 };
 
 // D[tmem] (+)= A[tmem] B[smem]^T, fp16 operands.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tmov.b64 y, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(q4::kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         mbar_init(&raw_full[i][k], 1);
         mbar_init(&raw_empty[i][k], 4);
         mbar_init(&s_full[i][k], 1);
-        mbar_init(&p_full[i][k], 128);
+        mbar_init(&p_full[i][k], 4);
         mbar_init(&pv_done[i][k], 1);
       }
       mbar_init(&k_full[i], 4);
@@ -217,53 +217,62 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         for (int v = 0; v < 2; ++v) mbar_wait_drain(&raw_full[v][j & 1], (j >> 1) & 1);
     __syncwarp();
   } else if (warp == 13) {
-    // ---- MMAs
-    if (lane == 0 && blocks > 0) {
+    // ---- MMAs: the warp goes together, one lane issues
+    if (blocks > 0) {
       constexpr uint32_t id_s = q4::idesc_f16(128, kPreKeys, 0), id_o = q4::idesc_f16(128, DP, 0);
-      auto scores = [&](int i, int j) {  // S_i of block j
-        const uint32_t q = smem_u32(sm_q + i * S::kQ), k = smem_u32(sm_k + (j & 1) * S::kKV);
+      const uint32_t q0 = q4::desc_low(smem_u32(sm_q)), k0 = q4::desc_low(smem_u32(sm_k)),
+                     v0 = q4::desc_low(smem_u32(sm_v)), d0 = __shfl_sync(0xffffffffu, tmem, 0);
+      auto scores = [&](int i, int buf, bool free_k) {  // S_i of the block in `buf`; the keys' last use?
+        const uint32_t q = q0 + i * (S::kQ >> 4), k = k0 + buf * (S::kKV >> 4), d = d0 + (2 * i + buf) * kPreKeys;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s)
-          q4::mma_f16(tmem + (2 * i + (j & 1)) * kPreKeys, smem_desc(q + s / 4 * 16384 + s % 4 * 32, 16, 1024, 2),
-                      smem_desc(k + s / 4 * kPreKeys * 128 + s % 4 * 32, 16, 1024, 2), id_s, s != 0);
-        mma_commit(&s_full[i][j & 1]);
+          for (int s = 0; s < DP / 16; ++s)
+            q4::mma_f16(d, q + s / 4 * (16384 >> 4) + s % 4 * 2, k + s / 4 * (kPreKeys * 128 >> 4) + s % 4 * 2, id_s,
+                        s != 0);
+          mma_commit(&s_full[i][buf]);
+          if (free_k) mma_commit(&k_empty[buf]);
+        }
+        __syncwarp();
       };
-      auto values = [&](int i, int j) {  // O_i += P_i V of block j
-        const uint32_t v = smem_u32(sm_v + (j & 1) * S::kKV);
+      auto values = [&](int i, int buf, bool first, bool free_v) {  // O_i += P_i V
+        const uint32_t v = v0 + buf * (S::kKV >> 4), d = d0 + S::kO + i * DP, a = d0 + (2 * i + buf) * kPreKeys;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < kPreKeys / 16; ++s)
-          mma_f16_ts(tmem + S::kO + i * DP, tmem + (2 * i + (j & 1)) * kPreKeys + s * 8,
-                     smem_desc(v + s * 32, 16, 1024, 2), id_o, (j | s) != 0);
-        mma_commit(&pv_done[i][j & 1]);
+          for (int s = 0; s < kPreKeys / 16; ++s) mma_f16_ts(d, a + s * 8, v + s * 2, id_o, !first || s != 0);
+          mma_commit(&pv_done[i][buf]);
+          if (free_v) mma_commit(&v_empty[buf]);
+        }
+        __syncwarp();
       };
-      bool ok = mbar_wait(&q_ready, 0, err, kTimeout);
-      for (int j = 0; j < min(blocks, 2) && ok; ++j) {
-        ok = mbar_wait(&k_full[j], 0, err, kTimeout);
-        if (!ok) break;
+      auto ready = [&](uint64_t* bar, int phase) {
+        const bool here = __all_sync(0xffffffffu, mbar_wait(bar, phase, err, kTimeout));
         tc_fence_after();
-        for (int i = 0; i < tiles; ++i) scores(i, j);
-        mma_commit(&k_empty[j]);
+        return here;
+      };
+      bool ok = ready(&q_ready, 0);
+      for (int j = 0; j < min(blocks, 2) && ok; ++j) {
+        ok = ready(&k_full[j], 0);
+        if (!ok) break;
+        for (int i = 0; i < tiles; ++i) scores(i, j, i + 1 == tiles);
       }
       for (int j = 0; j < blocks && ok; ++j) {
         const int buf = j & 1, phase = (j >> 1) & 1;
         for (int i = 0; i < tiles && ok; ++i) {
-          ok = mbar_wait(&v_full[buf], phase, err, kTimeout) && mbar_wait(&p_full[i][buf], phase, err, kTimeout);
+          ok = ready(&v_full[buf], phase) && ready(&p_full[i][buf], phase);
           if (!ok) break;
-          tc_fence_after();
-          values(i, j);
-          if (i + 1 == tiles) mma_commit(&v_empty[buf]);
+          values(i, buf, j == 0, i + 1 == tiles);
           if (j + 2 < blocks) {  // over P_i of this block, which goes first
-            ok = mbar_wait(&k_full[buf], phase ^ 1, err, kTimeout);
+            ok = ready(&k_full[buf], phase ^ 1);
             if (!ok) break;
-            tc_fence_after();
-            scores(i, j + 2);
-            if (i + 1 == tiles) mma_commit(&k_empty[buf]);
+            scores(i, buf, i + 1 == tiles);
           }
         }
       }
       // nothing may be in flight when the CTA gives its TMEM back
-      mma_commit(&last);
-      mbar_wait_drain(&last, 0);
+      if (elect_one()) {
+        mma_commit(&last);
+        mbar_wait_drain(&last, 0);
+      }
     }
     __syncwarp();
   } else if (warp >= 8) {
@@ -406,7 +415,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
             tmem_st16u(ts + 16, w[1]);
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&p_full[i][j & 1]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[i][j & 1]);
             continue;
           }
         }
@@ -474,7 +484,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_full[i][j & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i][j & 1]);
       }
       // `last` has one phase only. (pv_done could go on to the next phase, and
       // look unfinished, before a slow warp asks for the one before.)

@@ -24,7 +24,7 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;
 // Up to so many rows the products run here, above in csrc/q4_gemm.cuh.
-int few_rows(int type, bool transposed) { return !transposed && type != kF32 ? 64 : 16; }
+int few_rows(int type, bool transposed) { return !transposed && type != kF32 ? 32 : 16; }
 
 // ------------------------------------------------------- packing and decoding
 
@@ -514,9 +514,9 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
   }
 }
 
-// ------------------------------------------------- y = x W^T, up to 64 rows
+// ------------------------------------------------- y = x W^T, up to 32 rows
 
-// As the first product, for 16-bit types and 9 to 64 tokens. There the tokens'
+// As the first product, for 16-bit types and 9 to 32 tokens. There the tokens'
 // values are what a warp reads most of, so a CTA takes 128 rows of W, one row
 // tile a warp, and all its warps share the tokens' values from shared memory:
 // four blocks of k a stage, filled by cp.async one stage ahead, rows 64 bytes
@@ -532,7 +532,7 @@ template <int kTiles>
 constexpr int mid_smem() { return kMidStages * 8 * kTiles * kMidRow; }
 
 template <typename XT, typename ST, int kTiles, int kGroups>
-__global__ void __launch_bounds__(kWarps * 32, kTiles <= 4 ? 2 : 1)
+__global__ void __launch_bounds__(kWarps * 32, 2)
 mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ packed, const ST* __restrict__ scales,
            int M, int N, int K, int kblocks, int wide, XT* __restrict__ y, long long ldy) {
   constexpr bool kHalf = !std::is_same<XT, __nv_bfloat16>::value;
@@ -578,7 +578,7 @@ mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ pa
     uint4 qa, qb;
     uint32_t s[kGroups][2];
   };
-  constexpr int kDepth = kTiles <= 4 ? kMidBlocks : 2;
+  constexpr int kDepth = kMidBlocks;
   Piece ring[kDepth];
   int next = b0;
   const uint4* at_q = packed + (long long)rt * kblocks * 64 + lane;
@@ -773,8 +773,7 @@ bool set_group() {
             set_smem(matvec_t_kernel<XT, ST, 2, kGroups>, t_smem<2>());
   if constexpr (sizeof(XT) == 2)
     ok = ok && set_smem(mid_kernel<XT, ST, 2, kGroups>, mid_smem<2>()) &&
-         set_smem(mid_kernel<XT, ST, 4, kGroups>, mid_smem<4>()) &&
-         set_smem(mid_kernel<XT, ST, 8, kGroups>, mid_smem<8>());
+         set_smem(mid_kernel<XT, ST, 4, kGroups>, mid_smem<4>());
   return ok;
 }
 template <typename XT, typename ST>
@@ -818,8 +817,7 @@ int matmul_typed(bool transposed, const void* x, long long ldx, const void* pack
   }
   if constexpr (sizeof(XT) == 2) {
     if (M <= 16) return run_mid_group<XT, ST, 2>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
-    if (M <= 32) return run_mid_group<XT, ST, 4>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
-    return run_mid_group<XT, ST, 8>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
+    return run_mid_group<XT, ST, 4>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
   } else {
     if (gpb == 1) return run_matvec<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
     if (gpb == 2) return run_matvec<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);

@@ -66,12 +66,23 @@ struct GemmShape {
   static_assert(R == 2 || 128 * MT * 4 <= kStages * kStageBytes, "D fits where the stages were");
 };
 
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Descriptors of operands in 128-byte swizzle are two words: the upper is the
+// same for all (lines of eight rows 1 KB apart), the lower the address and, for
+// row-major operands, the distance of their 64-row columns. The MMAs are issued
+// by one lane of a warp that computes these words together, so that they stay
+// in uniform registers: worked out by the lane alone they cost about 100 clocks
+// an MMA, as much as a narrow one takes.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo = 16) {
+  return ((saddr >> 4) & 0x3FFFu) | (lbo >> 4) << 16;
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh)
       : "memory");
 }
 // fp16 operands, fp32 accumulator.
@@ -156,31 +167,31 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     }
     __syncwarp();
   } else if (warp == 17) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_f16(128, MT, kTrans ? 1 : 0);
-      uint32_t it = 0;
-      for (; it < 2u * count; ++it) {
-        const int s = it % S::kStages;
-        const uint32_t ph = (it / S::kStages) & 1u;
-        if (!mbar_wait(&full_b[s], ph, p.err, kDevTimeoutFull) ||
-            !mbar_wait(&full_a[s], ph, p.err, kDevTimeoutFull))
-          break;
-        tc_fence_after();
-        const uint32_t sa = smem_u32(smem + s * S::kStageBytes), sb = sa + S::kA;
+    constexpr uint32_t idesc = idesc_f16(128, MT, kTrans ? 1 : 0);
+    const uint32_t base = desc_low(smem_u32(smem), kTrans ? 8192 : 16), d0 = __shfl_sync(0xffffffffu, tmem, 0);
+    uint32_t it = 0;
+    for (; it < 2u * count; ++it) {
+      const int s = it % S::kStages;
+      const uint32_t ph = (it / S::kStages) & 1u;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full_b[s], ph, p.err, kDevTimeoutFull) &&
+                                       mbar_wait(&full_a[s], ph, p.err, kDevTimeoutFull)))
+        break;
+      tc_fence_after();
+      // sum-major A: 128-byte rows of 64 terms; row-major (kTrans): two columns
+      // of 64 rows, 8 KB apart, one term to a 128-byte line
+      const uint32_t a = base + s * (S::kStageBytes >> 4), b = a + (S::kA >> 4) - (kTrans ? (8192 - 16) << 12 : 0);
+      if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < kStageK / 16; ++ks) {
-          const uint64_t b = smem_desc(sb + ks * 32, 16, 1024, 2);
+        for (int ks = 0; ks < kStageK / 16; ++ks)
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            // sum-major: 128-byte rows of 64 terms; row-major (kTrans): two
-            // columns of 64 rows, 8 KB apart, one term to a 128-byte line
-            const uint64_t a = kTrans ? smem_desc(sa + r * 16384 + ks * 2048, 8192, 1024, 2)
-                                      : smem_desc(sa + r * 16384 + ks * 32, 16, 1024, 2);
-            mma_f16(tmem + r * MT, a, b, idesc, (it | ks) != 0);
-          }
-        }
+          for (int r = 0; r < R; ++r)
+            mma_f16(d0 + r * MT, a + r * (16384 >> 4) + ks * ((kTrans ? 2048 : 32) >> 4), b + ks * (32 >> 4), idesc,
+                    it != 0 || ks != 0);
         mma_commit(&empty[s]);
       }
+      __syncwarp();
+    }
+    if (elect_one()) {
       mma_commit(&done);
       mbar_wait_drain(&done, 0);
     }

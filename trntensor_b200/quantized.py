@@ -242,7 +242,7 @@ def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> tor
     """``x @ W^T``: (..., K) -> (..., N); with ``over_n`` ``x @ W``: (..., N) -> (..., K).
 
     x is fp32, bf16 or fp16; sums are fp32 and the result is rounded once to
-    x's type. Up to 16 rows (64 of 16-bit types over k) products over k are
+    x's type. Up to 16 rows (32 of 16-bit types over k) products over k are
     exact, and over n they keep 2^-16 (fp32: all bits). With more both operands are brought to fp16's
     range by powers of two a row: products are exact where scales are bf16 and
     x is of 16 bits and no smaller than 2^-27 of its row's largest value, else
