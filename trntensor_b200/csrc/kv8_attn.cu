@@ -14,10 +14,11 @@ int g_sms[kMaxDevices];
 template <typename T, int DP>
 int set_attr() {
   constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
-  return cudaFuncSetAttribute(attend_kernel<T, DP, kTerms>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              Shape<DP, kTerms>::kSmem) == cudaSuccess
-             ? TT_OK
-             : TT_ERR_CUDA;
+  const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  if (cudaFuncSetAttribute(attend_kernel<T, DP, kTerms, 1>, at, Shape<DP>::kSmem) != cudaSuccess) return TT_ERR_CUDA;
+  if constexpr (DP <= 128)
+    if (cudaFuncSetAttribute(attend_kernel<T, DP, kTerms, 2>, at, Shape<DP>::kSmem) != cudaSuccess) return TT_ERR_CUDA;
+  return TT_OK;
 }
 template <typename T, int DP>
 int set_prefill() {
@@ -57,14 +58,22 @@ size_t piece_bytes(int dim) { return (size_t)2 * 16 * (dim + 2) * 4; }
 size_t workspace_bytes(int dim, int sms) { return sms * (16 + (warps_of(dim) + 1) * piece_bytes(dim)); }
 
 template <typename T, int DP>
-int launch(const Attend& p, int sms, cudaStream_t s) {
+int launch(Attend p, int sms, cudaStream_t s) {
   constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
-  using S = Shape<DP, kTerms>;
-  attend_kernel<T, DP, kTerms><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+  using S = Shape<DP>;
+  // More than eight rows go sixteen at a time, which decodes the cache once for
+  // both halves, where the registers hold them.
+  p.tile_rows = p.rows <= 8 || DP > 128 ? 8 : 16;
+  p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
+  if (p.tile_rows == 8) {
+    attend_kernel<T, DP, kTerms, 1><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+  } else {
+    if constexpr (DP <= 128) attend_kernel<T, DP, kTerms, 2><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+  }
   int st = cuda_status(cudaGetLastError());
   if (st != TT_OK) return st;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sms, p.rows < 16 ? p.rows : 16);
+  cfg.gridDim = dim3(sms, p.rows < p.tile_rows ? p.rows : p.tile_rows);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -158,7 +167,6 @@ int tt_kv8_attention(const void* q, int type, long long q_stride_b, long long q_
   p.page_log = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   p.cols = columns;
   p.rows = (int)rows;
-  p.tiles = (int)((rows + 15) / 16);
   cudaStream_t s = (cudaStream_t)stream;
   if (type == q4::kF32) return kv8::launch_dim<float>(p, sms, s);
   if (type == q4::kBF16) return kv8::launch_dim<__nv_bfloat16>(p, sms, s);

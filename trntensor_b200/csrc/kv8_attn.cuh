@@ -3,29 +3,33 @@
 //   o = sum_t softmax_t(scale q.K^[t]) V^[t],  K^[t] = sk[page,h] ck[t]
 //
 // Two contractions with a softmax between; the scores stay in registers. A
-// kv head's query rows (tokens x heads of its group) make tiles of 16, and the
-// work is cut into chunks of 64 tokens of one tile. The chunks of all
+// kv head's query rows (tokens x heads of its group) make tiles of 8 or 16, and
+// the work is cut into chunks of 64 tokens of one tile. The chunks of all
 // sequences, heads and tiles form one line, of which every warp takes an equal
 // piece, so that ragged lengths and a lone long sequence both fill the GPU. A
 // tile whose chunks lie with several warps is joined in shared memory when
 // they are of one CTA, and by a second small kernel when they are not, always
 // in the same order.
 //
-// What bounds it: the cache's bytes. Each warp keeps its own ring of shared
-// memory slots (one unit quartet of keys or of values each) filled by bulk
-// copies two to three slots ahead, across tile borders. Tensor-core operands:
-// the codes are exact in fp16; a row of q is scaled by a power of two to below
-// 2^14 and rounded to fp16 (exact for 16-bit types down to 2^-27 of the row's
-// largest value, 2^-39 of that below) or, for fp32, kept as two fp16 terms.
-// The softmax weights are fp16 (2^-11 of each, a quarter of a bf16 result's
-// rounding and as much as an fp16 one's; again held up by 2^14), two terms for
-// fp32. Page
-// scales multiply scores and weights in fp32; weights are held relative to the
-// largest value scale seen.
+// What bounds it: the cache's bytes, and close behind them the instructions
+// that decode and multiply (with rows on the 16-wide side of the fragments,
+// half of it empty, they took a third more time). Each warp keeps its own ring
+// of shared memory slots (one unit quartet of keys or of values each) filled by
+// bulk copies two slots ahead or more, across tile borders. Tensor-core
+// operands: the codes are exact in fp16; a row of q is scaled by a power of two
+// to below 2^14 and rounded to fp16 (exact for 16-bit types down to 2^-27 of the
+// row's largest value, 2^-39 of that below) or, for fp32, kept as two fp16
+// terms. The softmax weights are fp16 (2^-11 of each, a quarter of a bf16
+// result's rounding and as much as an fp16 one's; again held up by 2^14), two
+// terms for fp32. Page scales multiply scores and weights in fp32; weights are
+// held relative to the largest value scale seen.
 //
-// Order of tokens in a chunk: lane 4 g + t of a fragment owns unit t's sixteen
-// tokens as score columns (tile j, column 2 t + e: token 16 t + 2 j + e), which
-// is also how a lane reads sixteen tokens of a value row at once.
+// Fragments: tokens are the 16-wide side of both products, query rows the
+// 8-wide one. Fragment s of a chunk has the tokens 4 s .. 4 s + 3 of its four
+// units: its row 2 u + e is token 4 s + e of unit u, row 8 + 2 u + e token 4 s +
+// 2 + e. So a lane's scores are all of one unit; eight by eight transposed
+// (movmatrix) they are the second product's operand; and a lane reads sixteen
+// neighbouring bytes of a key row, and all sixteen tokens of a value row.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -59,18 +63,16 @@ struct Attend {
   int* status;
   float scale;  // times log2(e)
   int causal;
-  int batch, S, heads_q, heads, dim, page, page_log, pages, cols, rows, tiles;
+  int batch, S, heads_q, heads, dim, page, page_log, pages, cols, rows, tiles, tile_rows;
 };
 
-template <int DP, int kTerms>
+template <int DP>
 struct Shape {
-  static constexpr bool kQRegs = DP <= 128 && kTerms == 1;
   static constexpr int kWarps = DP <= 128 ? 8 : 4;
   static constexpr int kUnit = 16 * DP;
   static constexpr int kSlot = 4 * (kUnit + 32) + 16;  // four units, and their scales
-  static constexpr int kSlots = DP == 64 ? 5 : DP == 192 ? 3 : kTerms == 1 ? 3 : 2;
-  static constexpr int kQBytes = kQRegs ? 0 : kTerms * 16 * DP * 2;
-  static constexpr int kSmem = kWarps * (kSlots * kSlot + kQBytes);
+  static constexpr int kSlots = DP == 64 ? 6 : DP == 192 ? 4 : 3;
+  static constexpr int kSmem = kWarps * kSlots * kSlot;
   static_assert(kSmem + 1024 <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -108,16 +110,6 @@ __device__ __forceinline__ void load16(const T* at, float (&x)[16]) {
     for (int j = 0; j < kPer; ++j) x[i * kPer + j] = q4::to_f(e[j]);
   }
 }
-template <typename T>
-__device__ __forceinline__ void store2(T* at, float a, float b) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float2*>(at) = make_float2(a, b);
-  } else if constexpr (std::is_same<T, __half>::value) {
-    *reinterpret_cast<uint32_t*>(at) = q4::pack_f16(a, b);
-  } else {
-    *reinterpret_cast<uint32_t*>(at) = q4::pack_bf16(a, b);
-  }
-}
 __device__ __forceinline__ float exp2_approx(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -136,6 +128,12 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   const __half2 rb = __hsub2(reinterpret_cast<const __half2&>(b), bias);
   lo = reinterpret_cast<const uint32_t&>(ra);
   hi = reinterpret_cast<const uint32_t&>(rb);
+}
+// An 8 x 8 matrix of 16-bit values in fragment order, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 // Two floats (below 65504) as kTerms fp16 pairs.
 template <int kTerms>
@@ -255,9 +253,11 @@ __device__ __forceinline__ long long row_offset(const Attend& p, int b, int h, i
   return (((long long)b * p.S + r / group) * p.heads_q + h * group + r % group) * p.dim;
 }
 
-template <typename T, int DP, int kTerms>
-__global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kernel(const Attend p) {
-  using S = Shape<DP, kTerms>;
+// NT: tiles of 8 rows that a warp has at a time.
+template <typename T, int DP, int kTerms, int NT>
+__global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const Attend p) {
+  using S = Shape<DP>;
+  constexpr int kTile = 8 * NT;
   using q4::from_f;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t bars[S::kWarps * S::kSlots];
@@ -406,11 +406,13 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     if (slot == 0) parity ^= 1;
   };
 
-  float acc[DP / 8][4];
-  uint32_t qf[S::kQRegs ? DP / 16 : 1][4];
-  unsigned char* qs = smem + S::kWarps * S::kSlots * S::kSlot + warp * S::kQBytes;  // [step][term][lane][4]
-  float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f, top_v = 0.f, qs0 = 0.f, qs1 = 0.f;
-  int lim0 = 0, lim1 = 0, lim_min = 0;
+  // Of rows 8 i + 2 t + e of the tile: maximum, sum, scale of the scores, tokens
+  // that it sees. Sums of values: acc[i][n][e + 2 f] is d 16 n + 8 f + g.
+  float acc[NT][DP / 16][4], m[NT][2], l[NT][2], qs[NT][2];
+  int lim[NT][2];
+  uint32_t qf[NT][DP / 16][kTerms][2];
+  float top_v = 0.f;
+  int lim_min = 0;
   bool fresh = true, whole = true;
 
   for (long long i = begin; i < end; ++i) {
@@ -418,237 +420,233 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
       fresh = false;
       whole = at.chunk == 0;
       const int count = clamp_count(p, at.b, false);
-      float top[2], x[2][DP / 64][16];
-      int lim[2];
-      bool has[2];
+      lim_min = (int)at.length;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = at.tile * 16 + g + 8 * h;
-        const int tok = r / group, head = at.h * group + r % group;
-        has[h] = r < p.rows && tok < count;
-        const T* row = static_cast<const T*>(p.q) + at.b * p.q_b + (has[h] ? tok * p.q_s + head * p.q_h : 0);
-        lim[h] = !has[h] ? 0 : p.causal ? (int)at.length - count + tok + 1 : (int)at.length;
-        if (lim[h] < 0) lim[h] = 0;
-        float m = 0.f;
+      for (int a = 0; a < NT; ++a) {
+        // what rows 2 t, 2 t + 1 see; a row that is not there sees nothing
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = at.tile * kTile + 8 * a + 2 * t + e, tok = r / group;
+          const bool has = r < p.rows && tok < count;
+          const int see = !has ? 0 : max(p.causal ? (int)at.length - count + tok + 1 : (int)at.length, 0);
+          lim[a][e] = see;
+          if (has) lim_min = min(lim_min, see);
+        }
+        // the operand: row g
+        const int r = at.tile * kTile + 8 * a + g, tok = r / group, head = at.h * group + r % group;
+        const bool has = r < p.rows && tok < count;
+        const T* row = static_cast<const T*>(p.q) + at.b * p.q_b + (has ? tok * p.q_s + head * p.q_h : 0);
+        float x[DP / 64][16], top = 0.f;
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c) {
           const int d = 16 * (t + 4 * c);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[h][c][e] = 0.f;
-          if (has[h] && d < dim) load16(row + d, x[h][c]);
+          for (int e = 0; e < 16; ++e) x[c][e] = 0.f;
+          if (has && d < dim) load16(row + d, x[c]);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) m = fmaxf(m, fabsf(x[h][c][e]));
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[c][e]));
         }
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        top[h] = m;
-      }
-      // a row's power of two: its largest value comes to 2^13 .. 2^14
-      float up[2], down[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        int ex = (int)((__float_as_uint(top[h]) >> 23) & 255);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // a row's power of two: its largest value comes to 2^13 .. 2^14
+        int ex = (int)((__float_as_uint(top) >> 23) & 255);
         ex = ex < 14 ? 14 : ex;  // up = 2^(140 - ex), down = 1 / up
-        up[h] = __uint_as_float((uint32_t)(267 - ex) << 23) * (p.scale < 0.f ? -1.f : 1.f);
-        down[h] = __uint_as_float((uint32_t)(ex - 13) << 23);
-      }
+        const float up = __uint_as_float((uint32_t)(267 - ex) << 23) * (p.scale < 0.f ? -1.f : 1.f);
+        const float down = __uint_as_float((uint32_t)(ex - 13) << 23) * fabsf(p.scale);
+        qs[a][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+        qs[a][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c)
+        for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t f[4][kTerms];
+          for (int w = 0; w < 4; ++w) {
+            const float* y = x[c] + 4 * w;
+            uint32_t lo[kTerms], hi[kTerms];
+            split_f16<kTerms>(y[0] * up, y[1] * up, lo);
+            split_f16<kTerms>(y[2] * up, y[3] * up, hi);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float* y = x[h][c] + 4 * w;
-            split_f16<kTerms>(y[0] * up[h], y[1] * up[h], f[h]);
-            split_f16<kTerms>(y[2] * up[h], y[3] * up[h], f[2 + h]);
+            for (int k = 0; k < kTerms; ++k) {
+              qf[a][c * 4 + w][k][0] = lo[k];
+              qf[a][c * 4 + w][k][1] = hi[k];
+            }
           }
-          const int step = c * 4 + w;
-          if constexpr (S::kQRegs) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) qf[step][r] = f[r][0];
-          } else {
-#pragma unroll
-            for (int k = 0; k < kTerms; ++k)
-              *reinterpret_cast<uint4*>(qs + ((step * kTerms + k) * 32 + lane) * 16) =
-                  make_uint4(f[0][k], f[1][k], f[2][k], f[3][k]);
-          }
+        for (int e = 0; e < 2; ++e) {
+          m[a][e] = -INFINITY;
+          l[a][e] = 0.f;
         }
-      qs0 = down[0] * fabsf(p.scale);
-      qs1 = down[1] * fabsf(p.scale);
-      lim0 = lim[0];
-      lim1 = lim[1];
-      lim_min = min(has[0] ? lim0 : (int)at.length, has[1] ? lim1 : (int)at.length);
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, o));
-      m0 = m1 = -INFINITY;
-      l0 = l1 = top_v = 0.f;
+        for (int n = 0; n < DP / 16; ++n)
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+          for (int e = 0; e < 4; ++e) acc[a][n][e] = 0.f;
+      }
+      lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+      top_v = 0.f;
     }
 
-    // scores: 16 rows x 64 tokens
-    float s[8][4];
+    // scores: sc[a][s][e + 2 f] is token 16 u + 4 s + 2 f + g % 2, u = g / 2, row 8 a + 2 t + e
+    float sc[NT][4][4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int a = 0; a < NT; ++a)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[a][j][e] = 0.f;
     arrive();
     if (!alive) break;
     {
       const uint32_t keys = smem_u32(mine + slot * S::kSlot) + (g >> 1) * (S::kUnit + 32) + (g & 1) * dim + t * 16;
 #pragma unroll
-      for (int c = 0; c < DP / 64; ++c) {
-        uint32_t qa[4][kTerms][4];
+      for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
-        for (int w = 0; w < 4; ++w)
+        for (int j0 = 0; j0 < 4; j0 += 2) {
+          uint4 va[2], vb[2];
 #pragma unroll
-          for (int k = 0; k < kTerms; ++k) {
-            if constexpr (S::kQRegs) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) qa[w][k][r] = qf[c * 4 + w][r];
-            } else {
-              const uint4 v = *reinterpret_cast<const uint4*>(qs + (((c * 4 + w) * kTerms + k) * 32 + lane) * 16);
-              qa[w][k][0] = v.x; qa[w][k][1] = v.y; qa[w][k][2] = v.z; qa[w][k][3] = v.w;
-            }
+          for (int j = 0; j < 2; ++j) {
+            va[j] = lds128(keys + 4 * (j0 + j) * dim + c * 64);
+            vb[j] = lds128(keys + (4 * (j0 + j) + 2) * dim + c * 64);
           }
-        // four tiles at a time, so that neighbouring products are of different sums
-#pragma unroll
-        for (int j0 = 0; j0 < 8; j0 += 4) {
-          uint4 v[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = lds128(keys + 2 * (j0 + j) * dim + c * 64);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t lo, hi;
-              decode4(w == 0 ? v[j].x : w == 1 ? v[j].y : w == 2 ? v[j].z : v[j].w, lo, hi);
+            for (int j = 0; j < 2; ++j) {
+              uint32_t a0, a1, a2, a3;
+              decode4(w == 0 ? va[j].x : w == 1 ? va[j].y : w == 2 ? va[j].z : va[j].w, a0, a2);
+              decode4(w == 0 ? vb[j].x : w == 1 ? vb[j].y : w == 2 ? vb[j].z : vb[j].w, a1, a3);
 #pragma unroll
-              for (int k = 0; k < kTerms; ++k)
-                q4::mma16816<true>(s[j0 + j], qa[w][k][0], qa[w][k][1], qa[w][k][2], qa[w][k][3], lo, hi);
+              for (int a = 0; a < NT; ++a)
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k)
+                  q4::mma16816<true>(sc[a][j0 + j], a0, a1, a2, a3, qf[a][c * 4 + w][k][0], qf[a][c * 4 + w][k][1]);
             }
         }
-      }
     }
-    const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * t);
+    const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
     release();
 
     // The scores are used as they are: scaled by f (at least 0, the same for a
     // lane's whole unit) only inside the exponent.
-    const float f0 = qs0 * sk, f1 = qs1 * sk;
-    const int tok0 = at.chunk * kChunk + 16 * t;
+    const int tok0 = at.chunk * kChunk + 16 * (g >> 1) + (g & 1);
     const bool mask = (at.chunk + 1) * kChunk > lim_min;
     if (mask) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int a = 0; a < NT; ++a)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (tok0 + 2 * j + e >= lim0) s[j][e] = -INFINITY;
-          if (tok0 + 2 * j + e >= lim1) s[j][2 + e] = -INFINITY;
-        }
-    }
-    float n0 = -INFINITY, n1 = -INFINITY;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      n0 = fmaxf(n0, fmaxf(s[j][0], s[j][1]));
-      n1 = fmaxf(n1, fmaxf(s[j][2], s[j][3]));
+          for (int e = 0; e < 4; ++e)
+            if (tok0 + 4 * j + (e & 2) >= lim[a][e & 1]) sc[a][j][e] = -INFINITY;
     }
-    n0 = fmaxf(m0, n0 * f0);  // a product that is not a number (a masked unit of scale 0) drops out
-    n1 = fmaxf(m1, n1 * f1);
-    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-    n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-    n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+    float f[NT][2], z[NT][2], old[NT][2];
+#pragma unroll
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        f[a][e] = qs[a][e] * sk;
+        float n = fmaxf(sc[a][0][e], sc[a][0][e + 2]);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) n = fmaxf(n, fmaxf(sc[a][j][e], sc[a][j][e + 2]));
+        n = fmaxf(m[a][e], n * f[a][e]);  // a product that is not a number (a hidden unit of scale 0) drops out
+        n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
+        n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
+        n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
+        z[a][e] = n == -INFINITY ? 0.f : n;
+        old[a][e] = exp2_approx(m[a][e] - z[a][e]);
+        m[a][e] = n;
+      }
     arrive();
     if (!alive) break;
-    const float sv = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * t);
+    const float sv = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
     // largest value scale so far; a NaN stays in its own page's weights
     float nv = fmaxf(top_v, sv);
-    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 1));
-    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 2));
+    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 8));
+    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 16));
     nv = fmaxf(nv, 1e-30f);
-    const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
-    const float old0 = exp2_approx(m0 - z0), old1 = exp2_approx(m1 - z1);
     const float shrink = __fdividef(top_v, nv), rel = __fdividef(sv, nv) * kUp;
-    const float a0 = old0 * shrink, a1 = old1 * shrink;
-    if (__any_sync(0xffffffffu, a0 != 1.f || a1 != 1.f)) {
+    top_v = nv;
+    bool same = shrink == 1.f;
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        acc[n][0] *= a0;
-        acc[n][1] *= a0;
-        acc[n][2] *= a1;
-        acc[n][3] *= a1;
+    for (int a = 0; a < NT; ++a) same = same && old[a][0] == 1.f && old[a][1] == 1.f;
+    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+      for (int a = 0; a < NT; ++a) {
+        const float b0 = old[a][0] * shrink, b1 = old[a][1] * shrink;
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+          acc[a][n][0] *= b0;
+          acc[a][n][1] *= b1;
+          acc[a][n][2] *= b0;
+          acc[a][n][3] *= b1;
+        }
       }
     }
-    m0 = n0;
-    m1 = n1;
-    top_v = nv;
     // Weights times the unit's value scale, 2^(s f - z + log2 rel). Where that
     // has no logarithm (a unit of scale 0, NaN), or tokens are hidden, the
     // weight is made first and multiplied after.
-    uint32_t w[4][4][kTerms];
-    float sum0 = 0.f, sum1 = 0.f;
-    if (!mask && !__any_sync(0xffffffffu, !(rel > 1e-30f))) {
-      float lg;
-      asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
-      const float y0 = lg - z0, y1 = lg - z1, back = __fdividef(1.f, rel);
+    uint32_t w[NT][4][kTerms][2];
+    const bool plain = !mask && __all_sync(0xffffffffu, rel > 1e-30f);
+    float lg, back = 1.f;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
+    if (plain) back = __fdividef(1.f, rel);
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+    for (int a = 0; a < NT; ++a) {
+      float sum[2] = {0.f, 0.f};
+      if (plain) {
+        const float y0 = lg - z[a][0], y1 = lg - z[a][1];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float* x = s[2 * kk + half];
-          x[0] = exp2_approx(fmaf(x[0], f0, y0));
-          x[1] = exp2_approx(fmaf(x[1], f0, y0));
-          x[2] = exp2_approx(fmaf(x[2], f1, y1));
-          x[3] = exp2_approx(fmaf(x[3], f1, y1));
-          sum0 += x[0] + x[1];
-          sum1 += x[2] + x[3];
-          split_f16<kTerms>(x[0], x[1], w[kk][2 * half]);
-          split_f16<kTerms>(x[2], x[3], w[kk][2 * half + 1]);
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sc[a][j][e] = exp2_approx(fmaf(sc[a][j][e], f[a][e & 1], e & 1 ? y1 : y0));
+          sum[0] += sc[a][j][0] + sc[a][j][2];
+          sum[1] += sc[a][j][1] + sc[a][j][3];
         }
-      sum0 *= back;
-      sum1 *= back;
-    } else {
+      } else {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float* x = s[2 * kk + half];
-          float y[4];
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const bool hidden = tok0 + 4 * kk + 2 * half + (e & 1) >= (e < 2 ? lim0 : lim1);
-            const float v = exp2_approx(fmaf(x[e], e < 2 ? f0 : f1, e < 2 ? -z0 : -z1));
-            x[e] = mask && hidden ? 0.f : v;
-            y[e] = mask && hidden ? 0.f : v * rel;
+            const bool hidden = mask && tok0 + 4 * j + (e & 2) >= lim[a][e & 1];
+            const float v = hidden ? 0.f : exp2_approx(fmaf(sc[a][j][e], f[a][e & 1], -z[a][e & 1]));
+            sum[e & 1] += v;
+            sc[a][j][e] = hidden ? 0.f : v * rel;
           }
-          sum0 += x[0] + x[1];
-          sum1 += x[2] + x[3];
-          split_f16<kTerms>(y[0], y[1], w[kk][2 * half]);
-          split_f16<kTerms>(y[2], y[3], w[kk][2 * half + 1]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t lo[kTerms], hi[kTerms];
+        split_f16<kTerms>(sc[a][j][0], sc[a][j][1], lo);
+        split_f16<kTerms>(sc[a][j][2], sc[a][j][3], hi);
+#pragma unroll
+        for (int k = 0; k < kTerms; ++k) {
+          w[a][j][k][0] = transpose8(lo[k]);
+          w[a][j][k][1] = transpose8(hi[k]);
         }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) l[a][e] = l[a][e] * old[a][e] + sum[e] * back;
     }
-    l0 = l0 * old0 + sum0;
-    l1 = l1 * old1 + sum1;
     {
       const uint32_t vals = smem_u32(mine + slot * S::kSlot) + t * (S::kUnit + 32) + g * 16;
 #pragma unroll
-      for (int n0 = 0; n0 < DP / 8; n0 += 4) {
-        uint4 v[4];
+      for (int n0 = 0; n0 < DP / 16; n0 += 2) {
+        uint4 va[2], vb[2];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) v[n] = lds128(vals + (n0 + n) * 128);
+        for (int n = 0; n < 2; ++n) {
+          va[n] = lds128(vals + (n0 + n) * 256);
+          vb[n] = lds128(vals + (n0 + n) * 256 + 128);
+        }
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            uint32_t lo, hi;
-            decode4(kk == 0 ? v[n].x : kk == 1 ? v[n].y : kk == 2 ? v[n].z : v[n].w, lo, hi);
+          for (int n = 0; n < 2; ++n) {
+            uint32_t a0, a1, a2, a3;
+            decode4(j == 0 ? va[n].x : j == 1 ? va[n].y : j == 2 ? va[n].z : va[n].w, a0, a2);
+            decode4(j == 0 ? vb[n].x : j == 1 ? vb[n].y : j == 2 ? vb[n].z : vb[n].w, a1, a3);
 #pragma unroll
-            for (int k = 0; k < kTerms; ++k)
-              q4::mma16816<true>(acc[n0 + n], w[kk][0][k], w[kk][1][k], w[kk][2][k], w[kk][3][k], lo, hi);
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int k = 0; k < kTerms; ++k)
+                q4::mma16816<true>(acc[a][n0 + n], a0, a1, a2, a3, w[a][j][k][0], w[a][j][k][1]);
           }
       }
     }
@@ -656,40 +654,42 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
 
     const bool last = at.chunk + 1 == at.chunks;
     if (last || i + 1 == end) {  // the tile's sums leave the warp
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = at.tile * 16 + g + 8 * h;
-        const bool none = (h ? lim1 : lim0) == 0;  // a row that sees nothing
-        const float l = none ? 0.f : h ? l1 : l0;
-        if (r < p.rows) {
-          if (whole && last) {
-            const float inv = l > 0.f || l != l ? top_v / (l * kUp) : 0.f;
-            T* o = static_cast<T*>(p.o) + row_offset(p, at.b, at.h, r);
+      for (int a = 0; a < NT; ++a)
 #pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-              const int d = n * 8 + 2 * t;
-              if (d < dim) store2(o + d, none ? 0.f : acc[n][2 * h] * inv, none ? 0.f : acc[n][2 * h + 1] * inv);
+        for (int e = 0; e < 2; ++e) {
+          float den = l[a][e];
+          den += __shfl_xor_sync(0xffffffffu, den, 4);
+          den += __shfl_xor_sync(0xffffffffu, den, 8);
+          den += __shfl_xor_sync(0xffffffffu, den, 16);
+          const int in_tile = 8 * a + 2 * t + e, r = at.tile * kTile + in_tile;
+          const bool none = lim[a][e] == 0;  // a row that sees nothing
+          if (none) den = 0.f;
+          if (r < p.rows) {
+            if (whole && last) {
+              const float inv = den > 0.f || den != den ? top_v / (den * kUp) : 0.f;
+              T* o = static_cast<T*>(p.o) + row_offset(p, at.b, at.h, r);
+#pragma unroll
+              for (int n = 0; n < DP / 16; ++n)
+                if (16 * n < dim) {
+                  o[16 * n + g] = from_f<T>(none ? 0.f : acc[a][n][e] * inv);
+                  o[16 * n + 8 + g] = from_f<T>(none ? 0.f : acc[a][n][e + 2] * inv);
+                }
+            } else {
+              // a piece for the joining: slot 0 of a tile that began before, 1 of one that goes on
+              const float back_v = none ? 0.f : top_v / kUp;
+              float* out = p.part + (((long long)blockIdx.x * S::kWarps + warp) * 2 + (whole ? 1 : 0)) * 16 * rows_of +
+                           in_tile * rows_of;
+#pragma unroll
+              for (int n = 0; n < DP / 16; ++n)
+                if (16 * n < dim) {
+                  out[2 + 16 * n + g] = none ? 0.f : acc[a][n][e] * back_v;
+                  out[2 + 16 * n + 8 + g] = none ? 0.f : acc[a][n][e + 2] * back_v;
+                }
+              if (g == 0) *reinterpret_cast<float2*>(out) = make_float2(none ? -INFINITY : m[a][e], den);
             }
-          } else {
-            // a piece for the joining: slot 0 of a tile that began before, 1 of one that goes on
-            const float back = none ? 0.f : top_v / kUp;
-            float* out = p.part + (((long long)blockIdx.x * S::kWarps + warp) * 2 + (whole ? 1 : 0)) * 16 * rows_of +
-                         (g + 8 * h) * rows_of;
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-              const int d = n * 8 + 2 * t;
-              if (d < dim)
-                *reinterpret_cast<float2*>(out + 2 + d) =
-                    make_float2(none ? 0.f : acc[n][2 * h] * back, none ? 0.f : acc[n][2 * h + 1] * back);
-            }
-            if (t == 0) *reinterpret_cast<float2*>(out) = make_float2(none ? -INFINITY : h ? m1 : m0, l);
           }
         }
-      }
       if (!(whole && last) && lane == 0) {
         const long long c1 = i + (at.chunks - 1 - at.chunk);  // the tile's last chunk, and who has it
         const int who = (int)((((c1 + 1) * workers - 1) / total) / per_cta);
@@ -719,12 +719,12 @@ __global__ void __launch_bounds__(Shape<DP, kTerms>::kWarps * 32, 1) attend_kern
     }
     const int h = own.y / p.tiles, tile = own.y % p.tiles;
     const bool begins = flags & 1, ends = flags & 2;
-    for (int r = warp; r < 16 && tile * 16 + r < p.rows; r += S::kWarps) {
+    for (int r = warp; r < kTile && tile * kTile + r < p.rows; r += S::kWarps) {
       const float* in = p.part + ((long long)blockIdx.x * S::kWarps * 2 * 16 + r) * rows_of;
       Joined<DP> x;
       x.join(in, 16 * rows_of, i, j, 1, dim, lane, left_at);
       if (begins && ends) {
-        x.finish(static_cast<T*>(p.o) + row_offset(p, own.x, h, tile * 16 + r), dim, lane);
+        x.finish(static_cast<T*>(p.o) + row_offset(p, own.x, h, tile * kTile + r), dim, lane);
       } else {
         float* out = p.joint + (((long long)blockIdx.x * 2 + (begins ? 1 : 0)) * 16 + r) * rows_of;
         x.keep(out, dim, lane);
@@ -744,8 +744,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Attend p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early, runs after attend_kernel
   const int c0 = blockIdx.x;
   const int4 meta = p.meta[c0];
-  const int tile = meta.y % p.tiles, r = blockIdx.y;
-  if (meta.w == 0 || tile * 16 + r >= p.rows) return;
+  const int row = meta.y % p.tiles * p.tile_rows + blockIdx.y, r = blockIdx.y;
+  if (meta.w == 0 || row >= p.rows) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int rows_of = p.dim + 2;
   // slot 1 of the first CTA, slot 0 of those after it
@@ -756,7 +756,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Attend p) {
   __syncthreads();
   if (warp != 0) return;
   x.join(sums[0], 258, 0, kW - 1, 1, p.dim, lane, nullptr);
-  x.finish(static_cast<T*>(p.o) + row_offset(p, meta.x, meta.y / p.tiles, tile * 16 + r), p.dim, lane);
+  x.finish(static_cast<T*>(p.o) + row_offset(p, meta.x, meta.y / p.tiles, row), p.dim, lane);
 }
 
 }  // namespace kv8
