@@ -37,192 +37,175 @@ struct Append {
   float* vs;
   int* status;
   int batch, S, heads, dim, page, pages, cols;
-  int wide;  // four neighbouring values can be read at once
+  int wide;  // rows can be read 16 bytes at a time
 };
-
-template <typename T>
-__device__ __forceinline__ void load4(const T* at, bool wide, float (&v)[4]) {
-  if (wide) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(at));
-      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else {
-      const uint2 u = __ldg(reinterpret_cast<const uint2*>(at));
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = q4::to_f(e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = q4::to_f(__ldg(at + i));
-  }
-}
-
-// Values d .. d + 3 of a token, turned: kTurn 0 as they stand, 1 pairs (j, j +
-// half), 2 pairs (2 j, 2 j + 1). cs: the token's (cos, sin) by pair.
-template <int kTurn, typename T>
-__device__ __forceinline__ void load_turned(const Append& p, const T* row, int d, const float2* cs, float (&v)[4]) {
-  load4(row + d, p.wide, v);
-  if (kTurn == 0 || d >= 2 * p.half) return;
-  if (kTurn == 2) {
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      if (d + i >= 2 * p.half) break;
-      const float2 a = cs[(d + i) / 2];
-      const float u = v[i], w = v[i + 1];
-      v[i] = u * a.x - w * a.y;
-      v[i + 1] = w * a.x + u * a.y;
-    }
-  } else if (p.half % 4 == 0) {  // the four partners lie together
-    const bool lead = d < p.half;
-    float o[4];
-    load4(row + (lead ? d + p.half : d - p.half), p.wide, o);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 a = cs[lead ? d + i : d + i - p.half];
-      v[i] = lead ? v[i] * a.x - o[i] * a.y : v[i] * a.x + o[i] * a.y;
-    }
-  } else {
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-      if (d + i >= 2 * p.half) break;
-      const bool lead = d + i < p.half;
-      const float2 a = cs[lead ? d + i : d + i - p.half];
-      const float w = q4::to_f(row[lead ? d + i + p.half : d + i - p.half]), u = q4::to_f(row[d + i]);
-      const float r = lead ? u * a.x - w * a.y : u * a.x + w * a.y;
-      if (i == 0) v[0] = r;
-      else if (i == 1) v[1] = r;
-      else if (i == 2) v[2] = r;
-      else v[3] = r;
-    }
-  }
-}
 
 // Four codes rint(x / s) + 128 as bytes, as the division rounds them: x times
 // the reciprocal is off by 127 2^-22 at most, so it decides unless it comes
 // that near to a half; then, and for scales with no finite reciprocal, the
-// division itself is made.
+// division itself is made. |x| <= 127 s, so that codes need no clamping.
+// Adding 1.5 2^23 rounds to an integer, which then is the low byte.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float s, float inv, bool tiny) {
-  float q[4];
+  constexpr float kRound = 12582912.f;
+  uint32_t q[4];
   bool near = tiny;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float y = x[e] * inv;
-    q[e] = rintf(y);
-    near |= fabsf(y - q[e]) > 0.49996f;
+    const float y = x[e] * inv, r = y + kRound;
+    q[e] = __float_as_uint(r);
+    near |= fabsf(y - (r - kRound)) > 0.49996f;
   }
   if (near) {
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      const float r = rintf(__fdiv_rn(e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3], s));
+      const uint32_t r = __float_as_uint(__fdiv_rn(e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3], s) + kRound);
       if (e == 0) q[0] = r;
       else if (e == 1) q[1] = r;
       else if (e == 2) q[2] = r;
       else q[3] = r;
     }
   }
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w |= (uint32_t)((int)fminf(fmaxf(q[e], -127.f), 127.f) + 128) << (8 * e);
-  return w;
+  return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410) ^ 0x80808080u;
 }
 
-// Largest magnitude, by its bits, of a warp's tokens; and their codes.
-template <int kTurn, typename T>
-__device__ __forceinline__ uint32_t top_of(const Append& p, const T* x, long long xs, int n, const float2* cs, int lane) {
-  uint32_t top = 0;
-  for (int d = 4 * lane; d < p.dim; d += 128)
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      float v[4];
-      load_turned<kTurn>(p, x + i * xs, d, cs + i * p.half, v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[e])));
-    }
-  return __reduce_max_sync(0xffffffffu, top);
-}
-template <int kTurn, typename T>
-__device__ __forceinline__ void put_keys(const Append& p, const T* x, long long xs, int n, const float2* cs, int lane,
-                                         unsigned char* to, float s, float inv, bool none, bool tiny) {
-  for (int d = 4 * lane; d < p.dim; d += 128)
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      float v[4];
-      load_turned<kTurn>(p, x + i * xs, d, cs + i * p.half, v);
-      *reinterpret_cast<uint32_t*>(to + (long long)i * p.dim + d) = none ? 0x80808080u : codes_of(v, s, inv, tiny);
-    }
-}
-
-// A warp takes a page of a sequence, a head, and keys or values: once over the
-// new tokens for their largest value, once for the codes (from L1 or L2). The
-// CTA's warps are neighbouring heads, which share the table of cosines.
-// Bound by bytes: k and v read once from HBM, codes written once.
+// Four neighbouring values.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) append_kernel(const Append p) {
-  extern __shared__ float2 table[];  // [token][pair]
-  const int b = blockIdx.z, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const bool first = blockIdx.y == 0;
-  const long long start = p.lengths[b];
-  long long count = p.n_new ? p.n_new[b] : p.S;
-  if (start < 0 || count < 0 || count > p.S || start + count > (long long)p.cols * p.page) {
-    if (first && blockIdx.x == 0 && threadIdx.x == 0) raise(p.status, kBadLength);
-    if (start < 0) return;
-    count = count < 0 ? 0 : count > p.S ? p.S : count;
+__device__ __forceinline__ void four(const T* at, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(at);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(at);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q4::to_f(e[i]);
   }
-  const long long col = start / p.page + blockIdx.x;
-  const long long t0 = max(start, col * p.page), t1 = min(start + count, (col + 1) * p.page);
-  if (t0 >= t1 || col >= p.cols) return;
-  const int page = p.table[b * p.table_b + col];
-  if (page < 0 || page >= p.pages) {
-    if (first && threadIdx.x == 0) raise(p.status, kBadPage);
+}
+
+// A warp's new tokens of a page and head. kTurn: 0 as they stand, 1 turned in
+// pairs (j, j + half), 2 in pairs (2 j, 2 j + 1). Sixteen tokens by 128 values
+// at a time stand in the warp's part of shared memory (in registers they cost
+// code for each of the sixteen, which the instruction caches did not hold).
+constexpr int kRowTokens = 16, kRowValues = 128;
+template <int kTurn, typename T>
+struct Tokens {
+  const T* x;           // the first
+  long long stride;     // to the next
+  const float2* cs;     // (cos, sin) by token and pair
+  T* tile;              // [token][kRowValues]
+  int n, half, dim;
+  bool wide;            // 16-byte loads
+
+  // Asks for tokens i0 .. at values d0 ..
+  __device__ __forceinline__ void stage(int i0, int d0, int lane) const {
+    constexpr int kPer = 16 / sizeof(T), kPieces = kRowValues / kPer;
+    const int have = min(kRowTokens, n - i0) * kPieces;
+#pragma unroll 4
+    for (int i = lane; i < have; i += 32) {
+      const int tok = i / kPieces, d = i % kPieces * kPer;
+      if (d0 + d >= dim) continue;
+      const T* from = x + (i0 + tok) * stride + d0 + d;
+      T* to = tile + tok * kRowValues + d;
+      if (wide) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                     : "memory");
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) to[e] = from[e];
+      }
+    }
+  }
+  __device__ __forceinline__ void arrive() const {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+  }
+  // Values d .. d + 3 of token i0 + i, of which the tile has those from d0 on.
+  __device__ __forceinline__ void turned(int i0, int i, int d0, int d, float (&v)[4]) const {
+    const T* at = tile + i * kRowValues + (d - d0);
+    four(at, v);
+    if (kTurn == 0 || d >= 2 * half) return;
+    const float2* c = cs + (i0 + i) * half;
+    if (kTurn == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        if (d + e >= 2 * half) break;
+        const float2 k = c[(d + e) / 2];
+        const float u = v[e], w = v[e + 1];
+        v[e] = u * k.x - w * k.y;
+        v[e + 1] = w * k.x + u * k.y;
+      }
+    } else if (half % 4 == 0 && 2 * half <= kRowValues) {  // the four partners lie together, in the tile too
+      const bool lead = d < half;
+      float o[4];
+      four(lead ? at + half : at - half, o);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 k = c[lead ? d + e : d + e - half];
+        v[e] = lead ? v[e] * k.x - o[e] * k.y : v[e] * k.x + o[e] * k.y;
+      }
+    } else {
+      const T* row = x + (i0 + i) * stride;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (d + e >= 2 * half) break;
+        const bool lead = d + e < half;
+        const float2 k = c[lead ? d + e : d + e - half];
+        const float w = q4::to_f(row[lead ? d + e + half : d + e - half]);
+        v[e] = lead ? v[e] * k.x - w * k.y : v[e] * k.x + w * k.y;
+      }
+    }
+  }
+};
+
+// The new tokens' codes and their page's scale. kValues: values' storage order,
+// else keys'. A lane has four neighbouring values of a token. The first tokens
+// are asked for before the page is known (`ready` waits for the table), and a
+// page's that all fit the tile are loaded once.
+template <bool kValues, int kTurn, typename T, typename F>
+__device__ __forceinline__ void put(const Append& p, const Tokens<kTurn, T>& in, int slot0, int h, int lane, F ready) {
+  const int dim = p.dim, n = in.n;
+  const bool once = n <= kRowTokens && dim <= kRowValues;
+  in.stage(0, 0, lane);
+  const int page = ready();
+  if (page < 0) {
+    in.arrive();
     return;
   }
-  if (first) {  // is the page written for another place too?
-    const long long all = (long long)p.batch * gridDim.x;
-    for (long long i = threadIdx.x; i < all; i += kThreads) {
-      const int o = (int)(i / gridDim.x);
-      const long long so = p.lengths[o], no = min((long long)(p.n_new ? p.n_new[o] : p.S), (long long)p.S);
-      const long long c = so / p.page + i % gridDim.x;
-      if (so >= 0 && c * p.page < so + no && c < p.cols && !(o == b && c == col) &&
-          p.table[o * p.table_b + c] == page)
-        raise(p.status, kSharedPage);
-    }
-  }
-  const int slot0 = (int)(t0 - col * p.page), n = (int)(t1 - t0), dim = p.dim;
-  const bool keys_here = blockIdx.y * kWarps < p.heads;
-  if (keys_here && p.half > 0) {
-    for (int i = threadIdx.x; i < n * p.half; i += kThreads) {
-      float c, sn;
-      turn(t0 + i / p.half, p.inv_freq[i % p.half], &c, &sn);
-      table[i] = make_float2(c, sn);
-    }
-    __syncthreads();
-  }
-  const int task = blockIdx.y * kWarps + warp;
-  if (task >= 2 * p.heads) return;
-  const bool values = task >= p.heads;
-  const int h = values ? task - p.heads : task;
-  const T* x = static_cast<const T*>(values ? p.v : p.k);
-  const long long xs = values ? p.v_s : p.k_s;
-  x += b * (values ? p.v_b : p.k_b) + (t0 - start) * xs + h * (values ? p.v_h : p.k_h);
-  const int mode = values || p.half == 0 ? 0 : p.interleaved ? 2 : 1;
-  const uint32_t top = mode == 0 ? top_of<0>(p, x, xs, n, table, lane)
-                       : mode == 1 ? top_of<1>(p, x, xs, n, table, lane) : top_of<2>(p, x, xs, n, table, lane);
-  float* scale = (values ? p.vs : p.ks) + (long long)page * p.heads + h;
-  const float nan = __int_as_float(0x7fffffff);
+  unsigned char* base = (kValues ? p.vc : p.kc) + ((long long)page * p.heads + h) * p.page * dim;
+  float* scale = (kValues ? p.vs : p.ks) + (long long)page * p.heads + h;
   const float old = slot0 == 0 ? 0.f : *scale;
+  in.arrive();
+  uint32_t top = 0;  // largest magnitude by its bits, whose order puts infinities and NaN on top
+  for (int i0 = 0; i0 < n; i0 += kRowTokens)
+    for (int d0 = 0; d0 < dim; d0 += kRowValues) {
+      if (i0 + d0 > 0) {
+        __syncwarp();
+        in.stage(i0, d0, lane);
+        in.arrive();
+      }
+      const int d = d0 + 4 * lane;
+      if (d < dim)
+#pragma unroll 4
+        for (int i = 0; i < min(kRowTokens, n - i0); ++i) {
+          float v[4];
+          in.turned(i0, i, d0, d, v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[e])));
+        }
+    }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float nan = __int_as_float(0x7fffffff);
   const float need = top >= 0x7f800000u ? nan : __fdiv_rn(__uint_as_float(top), 127.f);
   const float now = old != old || need != need ? nan : fmaxf(old, need);
   __syncwarp();
   if (lane == 0) *scale = now;
-  unsigned char* base = (values ? p.vc : p.kc) + ((long long)page * p.heads + h) * p.page * dim;
   if (slot0 > 0 && now > old) {  // earlier tokens onto the larger scale
     const float ratio = __fdiv_rn(old, now);
     // keys: whole rows; values: a unit's 16 tokens of a d, of which the last unit keeps those behind slot0
-    const int pieces = values ? (slot0 + 15) / 16 * dim : slot0 * dim / 16;
+    const int pieces = kValues ? (slot0 + 15) / 16 * dim : slot0 * dim / 16;
     for (int i = lane; i < pieces; i += 32) {
       uint4* at = reinterpret_cast<uint4*>(base) + i;
-      const int have = values ? min(16, slot0 - i / dim * 16) : 16;
+      const int have = kValues ? min(16, slot0 - i / dim * 16) : 16;
       uint4 q = *at;
       uint32_t* w = reinterpret_cast<uint32_t*>(&q);
 #pragma unroll
@@ -237,45 +220,118 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const Append p) {
   }
   const float inv = now > 0.f ? __fdiv_rn(1.f, now) : 0.f;
   const bool none = !(now > 0.f), tiny = now < 1e-36f;  // the reciprocal of a tiny scale is not finite
-  if (!values) {
-    unsigned char* to = base + (long long)slot0 * dim;
-    if (mode == 0) put_keys<0>(p, x, xs, n, table, lane, to, now, inv, none, tiny);
-    else if (mode == 1) put_keys<1>(p, x, xs, n, table, lane, to, now, inv, none, tiny);
-    else put_keys<2>(p, x, xs, n, table, lane, to, now, inv, none, tiny);
-    return;
-  }
-  for (int unit = slot0 / 16; unit * 16 < slot0 + n; ++unit) {
-    const int lo = max(slot0 - unit * 16, 0), hi = min(slot0 + n - unit * 16, 16);
-    for (int d = 4 * lane; d < dim; d += 128) {
-      uint32_t row[16];  // four codes of a token
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        row[i] = 0x80808080u;
-        if (i >= lo && i < hi && !none) {
-          float v[4];
-          load4(x + (unit * 16 + i - slot0) * xs + d, p.wide, v);
-          row[i] = codes_of(v, now, inv, tiny);
-        }
+  for (int i0 = 0; i0 < n; i0 += kRowTokens)
+    for (int d0 = 0; d0 < dim; d0 += kRowValues) {
+      if (!once) {
+        __syncwarp();
+        in.stage(i0, d0, lane);
+        in.arrive();
       }
+      const int d = d0 + 4 * lane, have = min(kRowTokens, n - i0), slot = slot0 + i0;
+      if (d >= dim) continue;
+      if (!kValues || have < 16 || slot % 16 != 0) {
+#pragma unroll 4
+        for (int i = 0; i < have; ++i) {
+          float v[4];
+          in.turned(i0, i, d0, d, v);
+          const uint32_t q = none ? 0x80808080u : codes_of(v, now, inv, tiny);
+          if constexpr (!kValues) {
+            *reinterpret_cast<uint32_t*>(base + (long long)(slot + i) * dim + d) = q;
+          } else {
+            unsigned char* at = base + ((long long)((slot + i) / 16) * dim + d) * 16 + (slot + i) % 16;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        unsigned char* at = base + ((long long)unit * dim + d + e) * 16;
-        if (hi - lo == 16) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t a = __byte_perm(row[4 * j], row[4 * j + 1], 0x0040 + 0x11 * e);
-            const uint32_t c = __byte_perm(row[4 * j + 2], row[4 * j + 3], 0x0040 + 0x11 * e);
-            w[j] = __byte_perm(a, c, 0x5410);
+            for (int e = 0; e < 4; ++e) at[16 * e] = (unsigned char)(q >> (8 * e));
           }
-          *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (i >= lo && i < hi) at[i] = (unsigned char)(row[i] >> (8 * e));
         }
+      } else {  // a whole unit of values
+        uint32_t w[4][4];  // [d][four tokens]
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t row[4];  // four codes of a token
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float v[4];
+            in.turned(i0, 4 * j + i, d0, d, v);
+            row[i] = none ? 0x80808080u : codes_of(v, now, inv, tiny);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e][j] = __byte_perm(__byte_perm(row[0], row[1], 0x0040 + 0x11 * e),
+                                  __byte_perm(row[2], row[3], 0x0040 + 0x11 * e), 0x5410);
+        }
+        uint4* at = reinterpret_cast<uint4*>(base + ((long long)(slot / 16) * dim + d) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at[e] = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
       }
     }
+}
+
+// A warp takes a page of a sequence, a head, and keys or values. The CTA's
+// warps are neighbouring heads, which share the table of cosines; the CTAs of
+// the last y look for pages that the call writes for two places.
+// Bound by bytes: k and v read once from HBM, codes written once.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) append_kernel(const Append p) {
+  extern __shared__ __align__(16) unsigned char append_smem[];
+  float2* table = reinterpret_cast<float2*>(append_smem + kWarps * kRowTokens * kRowValues * sizeof(T));  // [token][pair]
+  const int b = blockIdx.z, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const bool look = blockIdx.y + 1 == gridDim.y;
+  const long long start = p.lengths[b];
+  long long count = p.n_new ? p.n_new[b] : p.S;
+  if (start < 0 || count < 0 || count > p.S || start + count > (long long)p.cols * p.page) {
+    if (look && blockIdx.x == 0 && threadIdx.x == 0) raise(p.status, kBadLength);
+    if (start < 0) return;
+    count = count < 0 ? 0 : count > p.S ? p.S : count;
+  }
+  const long long col = start / p.page + blockIdx.x;
+  const long long t0 = max(start, col * p.page), t1 = min(start + count, (col + 1) * p.page);
+  if (t0 >= t1 || col >= p.cols) return;
+  const int page = p.table[b * p.table_b + col];
+  if (look) {
+    if (page < 0 || page >= p.pages) {
+      if (threadIdx.x == 0) raise(p.status, kBadPage);
+      return;
+    }
+    const long long all = (long long)p.batch * gridDim.x;
+    for (long long i = threadIdx.x; i < all; i += kThreads) {
+      const int o = (int)(i / gridDim.x);
+      const long long so = p.lengths[o], no = min((long long)(p.n_new ? p.n_new[o] : p.S), (long long)p.S);
+      const long long c = so / p.page + i % gridDim.x;
+      if (so >= 0 && c * p.page < so + no && c < p.cols && !(o == b && c == col) &&
+          p.table[o * p.table_b + c] == page)
+        raise(p.status, kSharedPage);
+    }
+    return;
+  }
+  const int slot0 = (int)(t0 - col * p.page), n = (int)(t1 - t0);
+  const bool turns = blockIdx.y * kWarps < p.heads && p.half > 0;  // keys are among this CTA's
+  const int task = blockIdx.y * kWarps + warp;
+  const bool values = task >= p.heads;
+  const int h = min(values ? task - p.heads : task, p.heads - 1);  // behind the last: for the barrier alone
+  T* tile = reinterpret_cast<T*>(append_smem) + warp * kRowTokens * kRowValues;
+  // between a warp's loads and their use: the table of cosines, and the page
+  auto ready = [&]() -> int {
+    if (turns) {
+      for (int i = threadIdx.x; i < n * p.half; i += kThreads) {
+        float c, sn;
+        turn(t0 + i / p.half, p.inv_freq[i % p.half], &c, &sn);
+        table[i] = make_float2(c, sn);
+      }
+      __syncthreads();
+    }
+    return task >= 2 * p.heads || page < 0 || page >= p.pages ? -1 : page;
+  };
+  if (values) {
+    const T* x = static_cast<const T*>(p.v) + b * p.v_b + (t0 - start) * p.v_s + h * p.v_h;
+    put<true, 0, T>(p, {x, p.v_s, table, tile, n, p.half, p.dim, p.wide != 0}, slot0, h, lane, ready);
+  } else {
+    const T* x = static_cast<const T*>(p.k) + b * p.k_b + (t0 - start) * p.k_s + h * p.k_h;
+    if (p.half == 0)
+      put<false, 0, T>(p, {x, p.k_s, table, tile, n, p.half, p.dim, p.wide != 0}, slot0, h, lane, ready);
+    else if (!p.interleaved)
+      put<false, 1, T>(p, {x, p.k_s, table, tile, n, p.half, p.dim, p.wide != 0}, slot0, h, lane, ready);
+    else
+      put<false, 2, T>(p, {x, p.k_s, table, tile, n, p.half, p.dim, p.wide != 0}, slot0, h, lane, ready);
   }
 }
 
@@ -393,7 +449,7 @@ int g_ok[kMaxDevices];
 
 int setup(int dev) {
   return once_per_device(g_flags, g_ok, dev, []() -> int {
-    const int bytes = kTableBytes;
+    const int bytes = kTableBytes + kWarps * kRowTokens * kRowValues * 4;
     const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
     if (cudaFuncSetAttribute(append_kernel<float>, at, bytes) != cudaSuccess ||
         cudaFuncSetAttribute(append_kernel<__nv_bfloat16>, at, bytes) != cudaSuccess ||
@@ -438,11 +494,12 @@ int tt_kv8_append(const void* k, const void* v, int type, long long k_stride_b, 
   p.batch = batch; p.S = S; p.heads = heads; p.dim = dim; p.page = page; p.pages = pages; p.cols = columns;
   // S tokens lie in at most this many pages, wherever they start
   const unsigned most = (unsigned)(((long long)S + page - 2) / page + 1);
-  const dim3 grid(most, (2u * heads + kv8::kWarps - 1) / kv8::kWarps, batch);
-  const int smem = (S < page ? S : page) * pairs * 8;
+  const dim3 grid(most, (2u * heads + kv8::kWarps - 1) / kv8::kWarps + 1, batch);
   const int size = type == q4::kF32 ? 4 : 2;
-  p.wide = ((uintptr_t)k | (uintptr_t)v) % (4 * size) == 0 && k_stride_b % 4 == 0 && k_stride_s % 4 == 0 &&
-           k_stride_h % 4 == 0 && v_stride_b % 4 == 0 && v_stride_s % 4 == 0 && v_stride_h % 4 == 0;
+  const int smem = (S < page ? S : page) * pairs * 8 + kv8::kWarps * kv8::kRowTokens * kv8::kRowValues * size;
+  const int per = 16 / size;
+  p.wide = aligned16(k) && aligned16(v) && k_stride_b % per == 0 && k_stride_s % per == 0 && k_stride_h % per == 0 &&
+           v_stride_b % per == 0 && v_stride_s % per == 0 && v_stride_h % per == 0;
   cudaStream_t s = (cudaStream_t)stream;
   if (type == q4::kF32) kv8::append_kernel<float><<<grid, kv8::kThreads, smem, s>>>(p);
   else if (type == q4::kBF16) kv8::append_kernel<__nv_bfloat16><<<grid, kv8::kThreads, smem, s>>>(p);

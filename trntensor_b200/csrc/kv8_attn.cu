@@ -53,7 +53,7 @@ int setup(int dev) {
 }
 
 // One CTA an SM; for each a word of meta, two pieces a warp, and two joined.
-int warps_of(int dim) { return dim <= 128 ? 8 : 4; }
+int warps_of(int dim) { return dim <= 128 ? Shape<128>::kWarps : dim <= 192 ? Shape<192>::kWarps : Shape<256>::kWarps; }
 size_t piece_bytes(int dim) { return (size_t)2 * 16 * (dim + 2) * 4; }
 size_t workspace_bytes(int dim, int sms) { return sms * (16 + (warps_of(dim) + 1) * piece_bytes(dim)); }
 

@@ -15,7 +15,7 @@
 // that decode and multiply (with rows on the 16-wide side of the fragments,
 // half of it empty, they took a third more time). Each warp keeps its own ring
 // of shared memory slots (one unit quartet of keys or of values each) filled by
-// bulk copies two slots ahead or more, across tile borders. Tensor-core
+// bulk copies two or three slots ahead, across tile borders. Tensor-core
 // operands: the codes are exact in fp16; a row of q is scaled by a power of two
 // to below 2^14 and rounded to fp16 (exact for 16-bit types down to 2^-27 of the
 // row's largest value, 2^-39 of that below) or, for fp32, kept as two fp16
@@ -68,10 +68,13 @@ struct Attend {
 
 template <int DP>
 struct Shape {
-  static constexpr int kWarps = DP <= 128 ? 8 : 4;
+  // Measured for 32 x 1 over 8192 with 8 kv heads (us): 128 wide 8 x 2 83, 8 x 3
+  // 86, 12 x 2 110; 192 wide 6 x 2 124, 4 x 2 141, 4 x 3 133; 256 wide 4 x 3 170,
+  // 4 x 2 189, 6 x 2 190.
+  static constexpr int kWarps = DP <= 128 ? 8 : DP == 192 ? 6 : 4;
   static constexpr int kUnit = 16 * DP;
   static constexpr int kSlot = 4 * (kUnit + 32) + 16;  // four units, and their scales
-  static constexpr int kSlots = DP == 64 ? 6 : DP == 192 ? 4 : 3;
+  static constexpr int kSlots = DP == 256 ? 3 : 2;
   static constexpr int kSmem = kWarps * kSlots * kSlot;
   static_assert(kSmem + 1024 <= 227 * 1024, "shared memory of an SM");
 };
