@@ -55,7 +55,7 @@ def einsum(
     target = _resolve_dtype(dtype)
     if target is not None:
         operands = tuple(op if isinstance(op, Q4Matrix) else op.to(target) for op in operands)
-    if any(isinstance(op, Q4Matrix) for op in operands):
+    if Q4Matrix in map(type, operands):
         result = einsum_q4(subscripts, operands, precision)
     else:
         plan = plan_contraction(subscripts, *operands, precision=precision)

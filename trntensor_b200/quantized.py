@@ -18,6 +18,7 @@ import torch
 
 from . import _lib
 from .dispatch import _device, _ptr
+from .plan import _check_precision, _parse_subscripts, _validate_subscripts
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GROUPS = (32, 64, 128)
@@ -29,7 +30,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(dev: torch.device):
     """Context in which ``dev`` is the current CUDA device."""
-    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    return _HERE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _stream_of(dev: torch.device) -> int:
@@ -190,6 +191,10 @@ def pack_q4(codes: torch.Tensor, scales: torch.Tensor, *, group: int = 128) -> Q
 
 def _product(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
     """(M, K) -> (M, N) or, over_n, (M, N) -> (M, K) on the matrix's device."""
+    dev = x.device
+    if torch._C._cuda_getDevice() != dev.index:
+        with torch.cuda.device(dev):
+            return _product(x, w, over_n)
     n, k = w.shape
     m, have = x.shape
     cols = k if over_n else n
@@ -205,17 +210,16 @@ def _product(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
         ldx = have
     lib = _lib.load()
     fn = lib.tt_q4_matmul_t if over_n else lib.tt_q4_matmul
-    dev, kind = x.device, _TYPES[x.dtype]
+    kind = _TYPES[x.dtype]
     ws, ws_bytes = None, 0
     if m > _FEW_ROWS:
         ws_bytes = lib.tt_q4_matmul_workspace_bytes(kind, _TYPES[w.scales.dtype], over_n, m, n, k)
         if ws_bytes:
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        st = fn(x.data_ptr(), kind, ldx, w.packed.data_ptr(), w.scales.data_ptr(),
-                _TYPES[w.scales.dtype], w.row_scale.data_ptr(), m, n, k, w.group, out.data_ptr(),
-                cols, None if ws is None else ws.data_ptr(), ws_bytes, w.status.data_ptr(),
-                _stream_of(dev))
+    st = fn(x.data_ptr(), kind, ldx, w.packed.data_ptr(), w.scales.data_ptr(),
+            _TYPES[w.scales.dtype], w.row_scale.data_ptr(), m, n, k, w.group, out.data_ptr(),
+            cols, None if ws is None else ws.data_ptr(), ws_bytes, w.status.data_ptr(),
+            _stream_of(dev))
     if st:
         _lib.check(st, "tt_q4_matmul_t" if over_n else "tt_q4_matmul")
     return out
@@ -229,7 +233,7 @@ class _Q4Product(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _Q4Product.apply(dy, ctx.w, not ctx.over_n), None, None
+        return _dispatch(dy, ctx.w, not ctx.over_n), None, None
 
 
 def _dispatch(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
@@ -276,8 +280,6 @@ _FORMS: dict[tuple, tuple] = {}
 def _form(subscripts: str, operands: tuple, held: int) -> tuple:
     """(axis of x that is contracted, its permutation or None, over_n, the
     result's permutation or None) of a contraction with one Q4Matrix."""
-    from .plan import _parse_subscripts, _validate_subscripts
-
     _validate_subscripts(subscripts, operands)
     lhs, out = _parse_subscripts(subscripts)
     terms = lhs.split(",")
@@ -303,8 +305,6 @@ def _form(subscripts: str, operands: tuple, held: int) -> tuple:
 def einsum_q4(subscripts: str, operands: tuple, precision: str) -> torch.Tensor:
     """Two-operand einsum with one :class:`Q4Matrix`: a product over k or over n
     with the dense operand's other indices kept."""
-    from .plan import _check_precision, _validate_subscripts
-
     if len(operands) != 2 or isinstance(operands[0], Q4Matrix) == isinstance(operands[1], Q4Matrix):
         _validate_subscripts(subscripts, operands)
         raise ValueError(
