@@ -5,10 +5,12 @@
 // sequence and kv head, as two tiles of 128, and goes over the tokens in
 // blocks of 64:
 //   S_i = Q_i K^T (tcgen05, fp32 in TMEM)  ->  softmax warps of tile i
-//   P_i = 2^(S f - m) as fp16, in TMEM over S_i  ->  O_i += P_i V (A from TMEM)
-// A tile has two S in TMEM: the scores of the next block are there when the
-// softmax of one ends, so that its warps never wait for the way through the
-// tensor cores and back (with one S of 128 tokens that way was half the time).
+//   P_i = 2^(S f - m) as fp16, in TMEM  ->  O_i += P_i V (A from TMEM)
+// S is free for the next block's scores as soon as its warps have it in
+// registers, so that they never wait for the way through the tensor cores and
+// back. An MMA with both operands in shared memory is bound by reading them
+// (97 clocks for 128 x 64 x 16 against 32 of arithmetic): the first 64 elements
+// of the rows of Q lie in TMEM, which is then full.
 // Keys and values come as raw codes by bulk copies and are decoded once for
 // all 256 rows into swizzled fp16 operands (exact). Rows of q are scaled to
 // 2^13..2^14 by a power of two (exact for 16-bit types down to 2^-27 of the
@@ -21,7 +23,7 @@
 // What bounds it: tensor cores and the exponentials' unit need about the same
 // time (2048 to 2560 clocks for 128 tokens and 256 rows).
 // Roles: warps 0-3 and 4-7 softmax of tiles 0 and 1 (a thread a row), 8-11
-// decode, 12 copies, 13 issues the MMAs.
+// decode, 12 copies, 13 and 14 issue the MMAs of tiles 0 and 1.
 #pragma once
 #include "kv8_attn.cuh"
 #include "q4_gemm.cuh"
@@ -29,20 +31,22 @@
 namespace tt {
 namespace kv8 {
 
-constexpr int kPreThreads = 14 * 32;
+constexpr int kPreThreads = 15 * 32;
 constexpr int kPreKeys = 64;         // tokens of a block
-constexpr int kScaleSlots = 8;       // the copies are at most five blocks ahead of the softmax
+constexpr int kPreBufs = 4;          // decoded blocks of K and of V
+constexpr int kScaleSlots = 8;       // the copies are at most six blocks ahead of the softmax
 constexpr float kPreUp = 128.f;      // a weight of 1 in P
 constexpr float kPreRoom = 3.f;      // m above the largest score when it is set, and
 constexpr float kPreRise = 8.f;      // a score above m that it bears; both as powers of two
 
 template <int DP>
 struct PreShape {
-  static constexpr int kQ = 128 * DP * 2;             // bytes of a tile of Q
+  static constexpr int kQ = 128 * (DP - 64) * 2;      // bytes of a tile of Q behind element 64
   static constexpr int kKV = kPreKeys * DP * 2;       // of K or V as fp16
   static constexpr int kRaw = kPreKeys * DP;          // and as codes
-  static constexpr int kSmem = 2 * kQ + 4 * kKV + 4 * kRaw + 1024;
-  static constexpr int kO = 256;                      // first column of O_0; S_i of block j at (2 i + j % 2) 64
+  static constexpr int kSmem = 2 * kQ + 2 * kPreBufs * kKV + 4 * kRaw + 1024;
+  // first columns of tile 0; tile 1 is as many behind as one takes
+  static constexpr int kS = 0, kP = 128, kQt = 192, kO = 256;
   static_assert(kSmem + 1280 + 512 <= 227 * 1024, "shared memory of an SM");
 };
 
@@ -75,6 +79,11 @@ __device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[1
       "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -88,12 +97,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sm_q = smem;
   uint8_t* sm_k = sm_q + 2 * S::kQ;
-  uint8_t* sm_v = sm_k + 2 * S::kKV;
-  uint8_t* sm_raw = sm_v + 2 * S::kKV;
+  uint8_t* sm_v = sm_k + kPreBufs * S::kKV;
+  uint8_t* sm_raw = sm_v + kPreBufs * S::kKV;
   constexpr int kUnits = kPreKeys / 16;
-  // of block j: [..][j % 2], in its phase j / 2 % 2
-  __shared__ uint64_t raw_full[2][2], raw_empty[2][2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2],
-      p_full[2][2], pv_done[2][2], q_ready, last;
+  // of block j: [..][j % 2], in its phase j / 2 % 2, or with kPreBufs for 2
+  __shared__ uint64_t raw_full[2][2], raw_empty[2][2], k_full[kPreBufs], k_empty[kPreBufs], v_full[kPreBufs],
+      v_empty[kPreBufs], q_ready, last;
+  // of tile i, in the phase j % 2 of block j
+  __shared__ uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
   __shared__ float sc_k[kScaleSlots][kUnits], sc_rel[kScaleSlots][kUnits], sc_log[kScaleSlots][kUnits],
       sc_inv[kScaleSlots][kUnits];
   __shared__ uint32_t tmem_slot;
@@ -103,6 +114,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   const int dim = kFull ? DP : p.dim, group = p.heads_q / p.heads;
   const int b = blockIdx.z, h = blockIdx.y;
   const int tile = gridDim.x - 1 - blockIdx.x;  // the longest first
+  const int tiles = p.rows - tile * 256 > 128 ? 2 : 1;
   const int length = (int)clamp_length(p, b, threadIdx.x == 0 && h == 0 && blockIdx.x == 0);
   const int count = clamp_count(p, b, threadIdx.x == 0 && h == 0 && blockIdx.x == 0);
 
@@ -111,18 +123,20 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       for (int k = 0; k < 2; ++k) {
         mbar_init(&raw_full[i][k], 1);
         mbar_init(&raw_empty[i][k], 4);
-        mbar_init(&s_full[i][k], 1);
-        mbar_init(&p_full[i][k], 4);
-        mbar_init(&pv_done[i][k], 1);
       }
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < kPreBufs; ++i) {
       mbar_init(&k_full[i], 4);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], tiles);
       mbar_init(&v_full[i], 4);
-      mbar_init(&v_empty[i], 1);
-
+      mbar_init(&v_empty[i], tiles);
     }
     mbar_init(&q_ready, 256);
-    mbar_init(&last, 1);
+    mbar_init(&last, tiles);
     fence_mbar_init();
     dead = 0;
     top_lim = 0;
@@ -151,7 +165,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   }
   __syncthreads();
   const int blocks = (top_lim + kPreKeys - 1) / kPreKeys;
-  const int tiles = p.rows - tile * 256 > 128 ? 2 : 1;
   {  // the largest value scale in sight
     unsigned int top = 0;
     const int pages = (top_lim + p.page - 1) >> p.page_log;
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     if (lane == 0) atomicMax(&top_scale, top);
   }
   if (dim < DP) {  // columns of K and Q behind the head dimension are zeros, for good
-    for (int i = threadIdx.x; i < (2 * S::kQ + 2 * S::kKV) / 16; i += kPreThreads)
+    for (int i = threadIdx.x; i < (2 * S::kQ + kPreBufs * S::kKV) / 16; i += kPreThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
   }
@@ -216,31 +229,35 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       for (int j = max(blocks - 2, 0); j < blocks; ++j)
         for (int v = 0; v < 2; ++v) mbar_wait_drain(&raw_full[v][j & 1], (j >> 1) & 1);
     __syncwarp();
-  } else if (warp == 13) {
-    // ---- MMAs: the warp goes together, one lane issues
-    if (blocks > 0) {
+  } else if (warp >= 13) {
+    // ---- MMAs, a warp a tile: it goes together, one lane issues
+    const int i = warp - 13;
+    if (blocks > 0 && i < tiles) {
       constexpr uint32_t id_s = q4::idesc_f16(128, kPreKeys, 0), id_o = q4::idesc_f16(128, DP, 0);
-      const uint32_t q0 = q4::desc_low(smem_u32(sm_q)), k0 = q4::desc_low(smem_u32(sm_k)),
+      const uint32_t q = q4::desc_low(smem_u32(sm_q + i * S::kQ)), k0 = q4::desc_low(smem_u32(sm_k)),
                      v0 = q4::desc_low(smem_u32(sm_v)), d0 = __shfl_sync(0xffffffffu, tmem, 0);
-      auto scores = [&](int i, int buf, bool free_k) {  // S_i of the block in `buf`; the keys' last use?
-        const uint32_t q = q0 + i * (S::kQ >> 4), k = k0 + buf * (S::kKV >> 4), d = d0 + (2 * i + buf) * kPreKeys;
+      const uint32_t ds = d0 + S::kS + i * kPreKeys, dq = d0 + S::kQt + i * 32, dp = d0 + S::kP + i * 32,
+                     o = d0 + S::kO + i * DP;
+      auto scores = [&](int buf) {  // S of the block in `buf`
+        const uint32_t k = k0 + buf * (S::kKV >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < DP / 16; ++s)
-            q4::mma_f16(d, q + s / 4 * (16384 >> 4) + s % 4 * 2, k + s / 4 * (kPreKeys * 128 >> 4) + s % 4 * 2, id_s,
-                        s != 0);
-          mma_commit(&s_full[i][buf]);
-          if (free_k) mma_commit(&k_empty[buf]);
+          for (int s = 0; s < 4; ++s) mma_f16_ts(ds, dq + s * 8, k + s * 2, id_s, s != 0);
+#pragma unroll
+          for (int s = 4; s < DP / 16; ++s)
+            q4::mma_f16(ds, q + (s - 4) * 2, k + (kPreKeys * 128 >> 4) + (s - 4) * 2, id_s, 1);
+          mma_commit(&s_full[i]);
+          mma_commit(&k_empty[buf]);
         }
         __syncwarp();
       };
-      auto values = [&](int i, int buf, bool first, bool free_v) {  // O_i += P_i V
-        const uint32_t v = v0 + buf * (S::kKV >> 4), d = d0 + S::kO + i * DP, a = d0 + (2 * i + buf) * kPreKeys;
+      auto values = [&](int buf, bool first) {  // O += P V
+        const uint32_t v = v0 + buf * (S::kKV >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < kPreKeys / 16; ++s) mma_f16_ts(d, a + s * 8, v + s * 2, id_o, !first || s != 0);
-          mma_commit(&pv_done[i][buf]);
-          if (free_v) mma_commit(&v_empty[buf]);
+          for (int s = 0; s < kPreKeys / 16; ++s) mma_f16_ts(o, dp + s * 8, v + s * 2, id_o, !first || s != 0);
+          mma_commit(&pv_done[i]);
+          mma_commit(&v_empty[buf]);
         }
         __syncwarp();
       };
@@ -249,24 +266,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         tc_fence_after();
         return here;
       };
-      bool ok = ready(&q_ready, 0);
-      for (int j = 0; j < min(blocks, 2) && ok; ++j) {
-        ok = ready(&k_full[j], 0);
-        if (!ok) break;
-        for (int i = 0; i < tiles; ++i) scores(i, j, i + 1 == tiles);
-      }
+      bool ok = ready(&q_ready, 0) && ready(&k_full[0], 0);
+      if (ok) scores(0);
       for (int j = 0; j < blocks && ok; ++j) {
-        const int buf = j & 1, phase = (j >> 1) & 1;
-        for (int i = 0; i < tiles && ok; ++i) {
-          ok = ready(&v_full[buf], phase) && ready(&p_full[i][buf], phase);
+        if (j + 1 < blocks) {  // the next block's scores, before the softmax of this one ends
+          const int n = (j + 1) % kPreBufs, phase = (j + 1) / kPreBufs & 1;
+          ok = ready(&k_full[n], phase) && ready(&s_free[i], j & 1);
           if (!ok) break;
-          values(i, buf, j == 0, i + 1 == tiles);
-          if (j + 2 < blocks) {  // over P_i of this block, which goes first
-            ok = ready(&k_full[buf], phase ^ 1);
-            if (!ok) break;
-            scores(i, buf, i + 1 == tiles);
-          }
+          scores(n);
         }
+        ok = ready(&v_full[j % kPreBufs], j / kPreBufs & 1) && ready(&p_full[i], j & 1);
+        if (ok) values(j % kPreBufs, j == 0);
       }
       // nothing may be in flight when the CTA gives its TMEM back
       if (elect_one()) {
@@ -280,14 +290,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     const int id = threadIdx.x - 256;
     bool ok = true;
     for (int j = 0; j < blocks && ok; ++j) {
-      const int buf = j & 1, phase = (j >> 1) & 1;
+      const int from_buf = j & 1, buf = j % kPreBufs;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        ok = mbar_wait(&raw_full[v][buf], phase, err, kTimeout) &&
-             mbar_wait(v ? &v_empty[buf] : &k_empty[buf], phase ^ 1, err, kTimeout);
+        ok = mbar_wait(&raw_full[v][from_buf], (j >> 1) & 1, err, kTimeout) &&
+             mbar_wait(v ? &v_empty[buf] : &k_empty[buf], (j / kPreBufs & 1) ^ 1, err, kTimeout);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t raw = smem_u32(sm_raw + (2 * v + buf) * S::kRaw);
+        const uint32_t raw = smem_u32(sm_raw + (2 * v + from_buf) * S::kRaw);
         const uint32_t to = smem_u32((v ? sm_v : sm_k) + buf * S::kKV);
         const int wide = kFull ? DP : dim;  // kFull: all divisions below are shifts
         const int per = wide / 16, all = kPreKeys * per;  // pieces of 16 codes
@@ -319,7 +329,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&raw_empty[v][buf]);
+          mbar_arrive(&raw_empty[v][from_buf]);
           mbar_arrive(v ? &v_full[buf] : &k_full[buf]);
         }
       }
@@ -327,6 +337,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   } else {
     // ---- softmax: a thread a row
     const int i = warp >> 2;
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float qs;
     {  // this row of Q
       float top = 0.f;
@@ -342,25 +353,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       const float up = __uint_as_float((uint32_t)(267 - ex) << 23) * (p.scale < 0.f ? -1.f : 1.f);
       qs = __uint_as_float((uint32_t)(ex - 13) << 23) * fabsf(p.scale);
       const uint32_t r = threadIdx.x & 127;
-      for (int d = 0; d < dim; d += 16) {
+      for (int d = 0; d < (dim > 64 ? dim : 64); d += 16) {
         float x[16];
+        uint32_t w[8];
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        if (from != nullptr) load16(from + d, x);
-        const uint32_t line = smem_u32(sm_q + i * S::kQ) + d / 64 * 16384 + r * 128;
+        if (from != nullptr && d < dim) load16(from + d, x);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float* y = x + 8 * c;
-          const uint32_t at = line + (((d % 64 / 8 + c) ^ (r & 7)) << 4);
-          sts128(at, q4::pack_f16(y[0] * up, y[1] * up), q4::pack_f16(y[2] * up, y[3] * up),
-                 q4::pack_f16(y[4] * up, y[5] * up), q4::pack_f16(y[6] * up, y[7] * up));
+        for (int e = 0; e < 8; ++e) w[e] = q4::pack_f16(x[2 * e] * up, x[2 * e + 1] * up);
+        __syncwarp();
+        if (d < 64) {
+          tmem_st8u(lane_base + S::kQt + i * 32 + d / 2, w);
+        } else {
+          const uint32_t line = smem_u32(sm_q + i * S::kQ) + r * 128, c = d % 64 / 8;
+          sts128(line + ((c ^ (r & 7)) << 4), w[0], w[1], w[2], w[3]);
+          sts128(line + (((c + 1) ^ (r & 7)) << 4), w[4], w[5], w[6], w[7]);
         }
       }
+      tmem_st_wait();
+      tc_fence_before();
       fence_proxy_async_smem();
       mbar_arrive(&q_ready);
     }
-    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const uint32_t to = lane_base + S::kO + i * DP;
+    const uint32_t to = lane_base + S::kO + i * DP, ts = lane_base + S::kS + i * kPreKeys, tp = lane_base + S::kP + i * 32;
     // the least that a row of this warp which sees anything sees
     int least = lim > 0 ? lim : 0x7fffffff;
     least = __reduce_min_sync(0xffffffffu, least);
@@ -369,10 +384,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     bool ok = true;
     if (i < tiles) {
       for (int j = 0; j < blocks; ++j) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i][j & 1], (j >> 1) & 1, err, kTimeout));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], j & 1, err, kTimeout));
         if (!ok) break;
         tc_fence_after();
-        const uint32_t ts = lane_base + (2 * i + (j & 1)) * kPreKeys;
         const float* fk = sc_k[j % kScaleSlots];
         // values' scales relative to the largest, their logarithms and inverses
         const float* fr = sc_rel[j % kScaleSlots];
@@ -382,8 +396,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         const bool mask = tok0 + kPreKeys > least;
         uint32_t w[2][16];
         float n = -INFINITY;
-        // Weights by the maximum so far, and the block's own maximum, in one
-        // pass; they are kept back until it is sure that m stands.
+        // Nothing hidden, and a maximum to go by: it stays unless the block's
+        // own is too far above it.
         if (!mask && __all_sync(0xffffffffu, m != -INFINITY)) {  // the warp goes together
           bool plain = true;
           float sum = 0.f;
@@ -393,30 +407,43 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           tmem_ld_wait();
 #pragma unroll
           for (int u = 0; u < kUnits; ++u) {
-            float* x = s[u / 2] + 16 * (u & 1);
-            const float f = qs * fk[u], y = fl[u] - m;
+            const float* x = s[u / 2] + 16 * (u & 1);
+            float t[4];
             plain = plain && fr[u] > 1e-30f;
-            float t[4], q[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(x[e], x[e + 4]), fmaxf(x[e + 8], x[e + 12]));
-            n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * f);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], f, y));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
-            sum = fmaf((q[0] + q[1]) + (q[2] + q[3]), fi[u], sum);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[u / 2][8 * (u & 1) + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
+            n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * (qs * fk[u]));
           }
           // weights of units without a logarithm of their scale come below
           if (__all_sync(0xffffffffu, lim == 0 || (n <= m + kPreRise && plain))) {
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&s_free[i]);
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+              float* x = s[u / 2] + 16 * (u & 1);
+              const float f = qs * fk[u], y = fl[u] - m;
+              float q[4];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], f, y));
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[e] = (x[e] + x[e + 4]) + (x[e + 8] + x[e + 12]);
+              sum = fmaf((q[0] + q[1]) + (q[2] + q[3]), fi[u], sum);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[u / 2][8 * (u & 1) + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
+            }
             l += sum;
-            tmem_st16u(ts, w[0]);
-            tmem_st16u(ts + 16, w[1]);
+            if (j > 0) {  // P of the block before has been read
+              ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (j - 1) & 1, err, kTimeout));
+              if (!ok) break;
+              tc_fence_after();
+            }
+            tmem_st16u(tp, w[0]);
+            tmem_st16u(tp + 16, w[1]);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[i][j & 1]);
+            if (lane == 0) mbar_arrive(&p_full[i]);
             continue;
           }
         }
@@ -436,6 +463,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
             n = fmaxf(n, t * (qs * fk[2 * c + u]));  // a hidden unit of scale 0 is not a number, and drops out
           }
         }
+        if (j > 0) {  // P of the block before has been read, and O is there to be rescaled
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (j - 1) & 1, err, kTimeout));
+          if (!ok) break;
+          tc_fence_after();
+        }
         const bool rise = n > m + kPreRise;  // from -inf: always, where anything is seen
         if (__any_sync(0xffffffffu, rise)) {
           const float now = rise ? n + kPreRoom : m;
@@ -444,18 +476,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           l *= a;
           m = now;
           if (j > 0) {
-            // O of the blocks before must be there to be rescaled
-            ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i][(j - 1) & 1], ((j - 1) >> 1) & 1, err, kTimeout));
-            if (!ok) break;
-            tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < DP; c += 16) {
-              float o[16];
-              tmem_ld16(to + c, o);
+            for (int c = 0; c < DP; c += 32) {
+              float o[2][16];
+              tmem_ld16(to + c, o[0]);
+              tmem_ld16(to + c + 16, o[1]);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= rise ? a : 1.f;
-              tmem_st16(to + c, o);
+              for (int e = 0; e < 32; ++e) o[e / 16][e % 16] *= rise ? a : 1.f;
+              tmem_st16(to + c, o[0]);
+              tmem_st16(to + c + 16, o[1]);
             }
             tmem_st_wait();
           }
@@ -480,12 +510,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[c][8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
           }
-          tmem_st16u(ts + 16 * c, w[c]);
+          tmem_st16u(tp + 16 * c, w[c]);
         }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i][j & 1]);
+        if (lane == 0) {
+          mbar_arrive(&s_free[i]);
+          mbar_arrive(&p_full[i]);
+        }
       }
       // `last` has one phase only. (pv_done could go on to the next phase, and
       // look unfinished, before a slow warp asks for the one before.)
