@@ -341,26 +341,29 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     float qs;
     {  // this row of Q
       float top = 0.f;
-      if (from != nullptr)
-        for (int d = 0; d < dim; d += 16) {
-          float x[16];
-          load16(from + d, x);
+      uint4 raw[DP / 8];  // all loads go out together
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(x[e]));
-        }
+      for (int c = 0; c < DP / 8; ++c)
+        raw[c] = from != nullptr && 8 * c < dim ? __ldg(reinterpret_cast<const uint4*>(from) + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < DP / 8; ++c) {
+        const T* x = reinterpret_cast<const T*>(&raw[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(q4::to_f(x[e])));
+      }
       int ex = (int)((__float_as_uint(top) >> 23) & 255);
       ex = ex < 14 ? 14 : ex;
       const float up = __uint_as_float((uint32_t)(267 - ex) << 23) * (p.scale < 0.f ? -1.f : 1.f);
       qs = __uint_as_float((uint32_t)(ex - 13) << 23) * fabsf(p.scale);
       const uint32_t r = threadIdx.x & 127;
-      for (int d = 0; d < (dim > 64 ? dim : 64); d += 16) {
-        float x[16];
+#pragma unroll
+      for (int d = 0; d < DP; d += 16) {
         uint32_t w[8];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-        if (from != nullptr && d < dim) load16(from + d, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = q4::pack_f16(x[2 * e] * up, x[2 * e + 1] * up);
+        for (int e = 0; e < 8; ++e) {
+          const T* x = reinterpret_cast<const T*>(&raw[d / 8]) + 2 * e;
+          w[e] = q4::pack_f16(q4::to_f(x[0]) * up, q4::to_f(x[1]) * up);
+        }
         __syncwarp();
         if (d < 64) {
           tmem_st8u(lane_base + S::kQt + i * 32 + d / 2, w);
@@ -382,6 +385,27 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     // a row that sees nothing stays out of the maxima's way
     float m = lim > 0 ? -INFINITY : 0.f, l = 0.f;
     bool ok = true;
+    // rows whose maximum rises, to a new one above n: l and O follow
+    auto lift = [&](bool rise, float n, bool first) {
+      const float now = rise ? n + kPreRoom : m;
+      const float z = now == -INFINITY ? 0.f : now;
+      const float a = m == -INFINITY ? 0.f : exp2_approx(m - z);
+      l *= a;
+      m = now;
+      if (first) return;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[2][16];
+        tmem_ld16(to + c, o[0]);
+        tmem_ld16(to + c + 16, o[1]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e / 16][e % 16] *= rise ? a : 1.f;
+        tmem_st16(to + c, o[0]);
+        tmem_st16(to + c + 16, o[1]);
+      }
+      tmem_st_wait();
+    };
     if (i < tiles) {
       for (int j = 0; j < blocks; ++j) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], j & 1, err, kTimeout));
@@ -396,8 +420,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         const bool mask = tok0 + kPreKeys > least;
         uint32_t w[2][16];
         float n = -INFINITY;
-        // Nothing hidden, and a maximum to go by: it stays unless the block's
-        // own is too far above it.
+        // Nothing hidden, and a maximum to go by.
         if (!mask && __all_sync(0xffffffffu, m != -INFINITY)) {  // the warp goes together
           bool plain = true;
           float sum = 0.f;
@@ -415,10 +438,19 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
             n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * (qs * fk[u]));
           }
           // weights of units without a logarithm of their scale come below
-          if (__all_sync(0xffffffffu, lim == 0 || (n <= m + kPreRise && plain))) {
+          if (__all_sync(0xffffffffu, plain)) {
             tc_fence_before();
             if (lane == 0) mbar_arrive(&s_free[i]);
             __syncwarp();
+            const bool rise = lim > 0 && n > m + kPreRise;
+            if (__any_sync(0xffffffffu, rise)) {
+              if (j > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (j - 1) & 1, err, kTimeout));
+                if (!ok) break;
+                tc_fence_after();
+              }
+              lift(rise, n, j == 0);
+            }
 #pragma unroll
             for (int u = 0; u < kUnits; ++u) {
               float* x = s[u / 2] + 16 * (u & 1);
@@ -447,7 +479,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
             continue;
           }
         }
-        // First blocks, hidden tokens, a maximum that rises, odd scales.
+        // First blocks, hidden tokens, odd scales.
         n = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -469,27 +501,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           tc_fence_after();
         }
         const bool rise = n > m + kPreRise;  // from -inf: always, where anything is seen
-        if (__any_sync(0xffffffffu, rise)) {
-          const float now = rise ? n + kPreRoom : m;
-          const float z = now == -INFINITY ? 0.f : now;
-          const float a = m == -INFINITY ? 0.f : exp2_approx(m - z);
-          l *= a;
-          m = now;
-          if (j > 0) {
-#pragma unroll 1
-            for (int c = 0; c < DP; c += 32) {
-              float o[2][16];
-              tmem_ld16(to + c, o[0]);
-              tmem_ld16(to + c + 16, o[1]);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e / 16][e % 16] *= rise ? a : 1.f;
-              tmem_st16(to + c, o[0]);
-              tmem_st16(to + c + 16, o[1]);
-            }
-            tmem_st_wait();
-          }
-        }
+        if (__any_sync(0xffffffffu, rise)) lift(rise, n, j == 0);
         const float z = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
