@@ -110,7 +110,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
   constexpr int kArrive = 8;  // decoding warps that fill a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full_a[S::kStages], full_b[S::kStages], empty[S::kStages], done;
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], done;
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = gridDim.x, rank = blockIdx.x;
@@ -125,8 +125,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(&full_a[s], kArrive);
-      mbar_init(&full_b[s], 1);
+      mbar_init(&full[s], kArrive + 1);  // and the copies' arrival
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, 1);
@@ -153,8 +152,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(&full_b[s], S::kB);
-          tma_load_3d(smem + s * S::kStageBytes + S::kA, &mapB, &full_b[s], step * 128 + sub * 64, m0,
+          mbar_arrive_expect_tx(&full[s], S::kB);
+          tma_load_3d(smem + s * S::kStageBytes + S::kA, &mapB, &full[s], step * 128 + sub * 64, m0,
                       p.x_term[pass]);
         }
         if (++step == s1) {
@@ -163,7 +162,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
         }
       }
       for (uint32_t k = it > S::kStages ? it - S::kStages : 0; k < it; ++k)
-        mbar_wait_drain(&full_b[k % S::kStages], (k / S::kStages) & 1u);
+        mbar_wait_drain(&full[k % S::kStages], (k / S::kStages) & 1u);
     }
     __syncwarp();
   } else if (warp == 17) {
@@ -173,9 +172,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     for (; it < 2u * count; ++it) {
       const int s = it % S::kStages;
       const uint32_t ph = (it / S::kStages) & 1u;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full_b[s], ph, p.err, kDevTimeoutFull) &&
-                                       mbar_wait(&full_a[s], ph, p.err, kDevTimeoutFull)))
-        break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, p.err, kDevTimeoutFull))) break;
       tc_fence_after();
       // sum-major A: 128-byte rows of 64 terms; row-major (kTrans): two columns
       // of 64 rows, 8 KB apart, one term to a 128-byte line
@@ -224,20 +221,30 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     }
     int next = s0;  // step to fetch
     // Everything is fetched from somewhere: what lies behind the last row tile
-    // or block is dropped below, or never leaves the tile.
+    // or block is dropped below, or never leaves the tile. One multiplication
+    // an address: row tile (over n) or block (over k) times its bytes.
+    const int size = p.scales_f32 ? 4 : 2;
+    const char* at_q[R];
+    const char* at_s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long blk = kTrans ? min(row0 / 128 + r, (long long)p.kblocks - 1)
+                                   : min(row0 / 16 + r * 8 + w8, rtiles - 1) * p.kblocks;
+      at_q[r] = reinterpret_cast<const char*>(p.packed) + blk * kBlockBytes + lane * 16 + pair * 8;
+      at_s[r] = static_cast<const char*>(p.scales) + (blk * kGroups + pair * kGroups / 2) * kRows * size +
+                (size == 4 ? g * 4 : (g & ~1) * 2);
+    }
     auto fetch = [&](Piece& x) {
+      const long long i = kTrans ? min(next * 8LL + w8, rtiles - 1) * p.kblocks : (long long)next;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const long long rt = min(kTrans ? next * 8LL + w8 : row0 / 16 + r * 8 + w8, rtiles - 1);
-        const long long kb = min(kTrans ? row0 / 128 + r : (long long)next, (long long)p.kblocks - 1);
-        const long long blk = rt * p.kblocks + kb;
+        const char* q = at_q[r] + i * kBlockBytes;
+        const char* sc = at_s[r] + i * (kGroups * kRows * size);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          x.q[r][h] = ldg64(reinterpret_cast<const uint2*>(p.packed + blk * 64 + h * 32 + lane) + pair);
+          x.q[r][h] = ldg64(q + h * 512);
 #pragma unroll
-          for (int k = 0; k < kScales; ++k)
-            x.s[r][h][k] =
-                scale_word(p.scales, p.scales_f32, (blk * kGroups + pair * kGroups / 2 + k) * kRows + g + 8 * h);
+          for (int k = 0; k < kScales; ++k) x.s[r][h][k] = ldg32(sc + (k * kRows + 8 * h) * size);
         }
       }
       if constexpr (kTrans) {
@@ -317,7 +324,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
             }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full_a[s]);
+        if (lane == 0) mbar_arrive(&full[s]);
         }
         it += 2;
         if (++step == s1) {
