@@ -659,17 +659,25 @@ mid_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ pa
   __syncthreads();
   if (splits > 1) cluster.sync();
   if (active) {
-    for (int o = threadIdx.x + blockIdx.x * kWarps * 32; o < kTok * kWarps * kRows; o += splits * kWarps * 32) {
-      const int m = o / (kWarps * kRows), r = o % (kWarps * kRows);
-      const long long n = group_of * kWarps * kRows + r;
-      if (m >= M || n >= N) continue;
-      float v = 0.f;
-      if (splits > 1) {
-        for (int k = 0; k < splits; ++k) v += cluster.map_shared_rank(sums, k)[m * kLine + r];
-      } else {
-        v = sums[m * kLine + r];
+    // A thread has a row and every 2 splits-th token of it. Four of those at a
+    // time: what another CTA holds is far away.
+    static_assert(kWarps * 32 == 2 * kWarps * kRows, "two tokens at a time");
+    const int r = threadIdx.x % (kWarps * kRows);
+    const long long n = group_of * kWarps * kRows + r;
+    const int step = 2 * splits;
+    for (int m0 = 2 * blockIdx.x + threadIdx.x / (kWarps * kRows); m0 < kTok; m0 += 4 * step) {
+      float v[4] = {};
+      for (int k = 0; k < splits; ++k) {
+        const float* from = splits > 1 ? cluster.map_shared_rank(sums, k) : sums;
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = from[min(m0 + i * step, kTok - 1) * kLine + r];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += w[i];
       }
-      y[m * ldy + n] = from_f<XT>(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (m0 + i * step < M && n < N) y[(m0 + i * step) * ldy + n] = from_f<XT>(v[i]);
     }
   }
   if (splits > 1) cluster.sync();
