@@ -3,8 +3,9 @@
 Tolerances. A result is rounded once (half a step: eps / 2 of the value). The
 fp32 sum is a chain of at most 16 products, one addition for each 16 terms (8 a
 group and one a 128-wide block, or 8 a block, up to 16 rows, or 32 of 16-bit
-types over k), 8 warps and 8 CTAs; each of these loses at most a unit in the last place (2^-23, the tensor
-cores truncate) of a partial sum that sum |x W| bounds. Up to 16 rows the sum
+types over k), 8 warps and 8 CTAs; each of these loses at most a unit in the
+last place (2^-23, the tensor cores truncate) of a partial sum that sum |x W|
+bounds. fp32 rows above 16 are summed 256 terms at a time. Up to 16 rows the sum
 over n keeps 2^-16 of each product of 16-bit types. Above, fp16 terms: a 16-bit
 operand with bf16 scales loses only what lies below 2^-39 of its row's largest
 value; two 8-bit terms of an fp32 scale leave 2^-18; fp32 rows in two terms
@@ -45,13 +46,32 @@ def check(got, x, wide, over_n=False):
     if x.shape[0] <= 16 or (x.shape[0] <= 32 and not over_n and x.dtype != torch.float32):
         links = 48 + x.shape[1] / (16 if over_n else 128)
         loss = links * 2.0**-23 + (2.0**-16 if over_n and x.dtype != torch.float32 else 0)
-    else:  # fp32: two or four passes over the sum
-        links = 48 + x.shape[1] / 16 * (4 if x.dtype == torch.float32 else 2)
-        loss = links * 2.0**-23 + (2.0**-22 + 2.0**-20 if x.dtype == torch.float32 else 2.0**-18)
+    elif x.dtype == torch.float32:
+        # 16 in the tensor cores, 8 CTAs, and an addition (rounded: half of
+        # 2^-23) for each 256 terms of up to four passes
+        links = 24 + x.shape[1] / 128
+        loss = links * 2.0**-23 + 2.0**-22 + 2.0**-20
+    else:  # one or two passes over the sum
+        links = 48 + x.shape[1] / 16 * 2
+        loss = links * 2.0**-23 + 2.0**-18
     tol = torch.finfo(x.dtype).eps / 2 * ref.abs() + 1.01 * loss * mass + torch.finfo(x.dtype).tiny
     assert got.dtype == x.dtype and got.shape == ref.shape
     worst = ((got.double().cpu() - ref).abs() / tol).max().item()
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("m,n,k", [(20, 9600, 2000), (70, 300, 6000), (300, 500, 4100)])
+@pytest.mark.parametrize("scale_dtype", [torch.bfloat16, torch.float32])
+def test_fp32_sums_of_one_sign(cuda_ok, m, n, k, scale_dtype):
+    # what an accumulator loses at each addition then adds up
+    codes, scales, _ = make(n, k, 64, scale_dtype)
+    codes = codes.abs().clamp(1, 7)
+    wide = codes.double() * scales.double().repeat_interleave(64, 1)[:, :k]
+    w = tt.pack_q4(codes.cuda(), scales.cuda(), group=64)
+    x = rows(m, k, torch.float32).abs()
+    check(tt.q4_matmul(x.cuda(), w), x, wide.T)
+    dy = rows(m, n, torch.float32).abs()
+    check(tt.q4_matmul(dy.cuda(), w, over_n=True), dy, wide, over_n=True)
 
 
 SHAPES = [(1, 1, 1), (1, 16, 128), (1, 4096, 1024), (2, 17, 129), (3, 1001, 777), (7, 40, 4100),

@@ -11,32 +11,35 @@ std::once_flag g_flags[kMaxDevices];
 int g_ok[kMaxDevices];
 int g_sms[kMaxDevices];
 
-template <int R, int MT, int kGroups, bool kTrans>
+template <int R, int MT, int kGroups, bool kTrans, bool kSums>
 int set_attr() {
-  return cudaFuncSetAttribute(gemm_kernel<R, MT, kGroups, kTrans>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              GemmShape<R, MT>::kSmem) == cudaSuccess
+  return cudaFuncSetAttribute(gemm_kernel<R, MT, kGroups, kTrans, kSums>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              GemmShape<R, MT, kSums>::kSmem) == cudaSuccess
              ? TT_OK
              : TT_ERR_CUDA;
 }
-template <int R, int MT>
+template <int R, int MT, bool kSums>
 int set_attrs() {
-  int st = set_attr<R, MT, 1, false>();
-  if (st == TT_OK) st = set_attr<R, MT, 2, false>();
-  if (st == TT_OK) st = set_attr<R, MT, 4, false>();
-  if (st == TT_OK) st = set_attr<R, MT, 1, true>();
-  if (st == TT_OK) st = set_attr<R, MT, 2, true>();
-  if (st == TT_OK) st = set_attr<R, MT, 4, true>();
+  int st = set_attr<R, MT, 1, false, kSums>();
+  if (st == TT_OK) st = set_attr<R, MT, 2, false, kSums>();
+  if (st == TT_OK) st = set_attr<R, MT, 4, false, kSums>();
+  if (st == TT_OK) st = set_attr<R, MT, 1, true, kSums>();
+  if (st == TT_OK) st = set_attr<R, MT, 2, true, kSums>();
+  if (st == TT_OK) st = set_attr<R, MT, 4, true, kSums>();
   return st;
 }
 int setup(int dev) {
   return once_per_device(g_flags, g_ok, dev, [dev]() -> int {
     if (cudaDeviceGetAttribute(&g_sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
       return TT_ERR_CUDA;
-    int st = set_attrs<1, 32>();
-    if (st == TT_OK) st = set_attrs<1, 64>();
-    if (st == TT_OK) st = set_attrs<1, 128>();
-    if (st == TT_OK) st = set_attrs<1, 256>();
-    if (st == TT_OK) st = set_attrs<2, 256>();
+    int st = set_attrs<1, 32, false>();
+    if (st == TT_OK) st = set_attrs<1, 64, false>();
+    if (st == TT_OK) st = set_attrs<1, 128, false>();
+    if (st == TT_OK) st = set_attrs<1, 256, false>();
+    if (st == TT_OK) st = set_attrs<2, 256, false>();
+    if (st == TT_OK) st = set_attrs<1, 32, true>();
+    if (st == TT_OK) st = set_attrs<1, 64, true>();
+    if (st == TT_OK) st = set_attrs<1, 128, true>();
     return st;
   });
 }
@@ -44,7 +47,7 @@ int setup(int dev) {
 inline size_t al256(size_t x) { return (x + 255) / 256 * 256; }
 inline long long pad64(long long x) { return (x + 63) / 64 * 64; }
 
-template <int R, int MT, int kGroups, bool kTrans>
+template <int R, int MT, int kGroups, bool kTrans, bool kSums>
 int launch(const CUtensorMap& map, Gemm p, int splits, cudaStream_t s) {
   const long long rows = kTrans ? p.K : p.N;
   p.tiles_m = (p.M + MT - 1) / MT;
@@ -52,7 +55,7 @@ int launch(const CUtensorMap& map, Gemm p, int splits, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   if (!grid_of(tiles, splits, &cfg.gridDim)) return TT_ERR_SHAPE;
   cfg.blockDim = dim3(kGemmThreads);
-  cfg.dynamicSmemBytes = GemmShape<R, MT>::kSmem;
+  cfg.dynamicSmemBytes = GemmShape<R, MT, kSums>::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -61,21 +64,26 @@ int launch(const CUtensorMap& map, Gemm p, int splits, cudaStream_t s) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, gemm_kernel<R, MT, kGroups, kTrans>, map, p));
+  return cuda_status(cudaLaunchKernelEx(&cfg, gemm_kernel<R, MT, kGroups, kTrans, kSums>, map, p));
 }
-template <int R, int MT, bool kTrans>
+template <int R, int MT, bool kTrans, bool kSums>
 int launch_groups(const CUtensorMap& map, const Gemm& p, int group, int splits, cudaStream_t s) {
-  if (group == 128) return launch<R, MT, 1, kTrans>(map, p, splits, s);
-  if (group == 64) return launch<R, MT, 2, kTrans>(map, p, splits, s);
-  return launch<R, MT, 4, kTrans>(map, p, splits, s);
+  if (group == 128) return launch<R, MT, 1, kTrans, kSums>(map, p, splits, s);
+  if (group == 64) return launch<R, MT, 2, kTrans, kSums>(map, p, splits, s);
+  return launch<R, MT, 4, kTrans, kSums>(map, p, splits, s);
 }
 template <bool kTrans>
 int launch_tile(const CUtensorMap& map, const Gemm& p, int group, int R, int MT, int splits, cudaStream_t s) {
-  if (R == 2) return launch_groups<2, 256, kTrans>(map, p, group, splits, s);
-  if (MT == 32) return launch_groups<1, 32, kTrans>(map, p, group, splits, s);
-  if (MT == 64) return launch_groups<1, 64, kTrans>(map, p, group, splits, s);
-  if (MT == 128) return launch_groups<1, 128, kTrans>(map, p, group, splits, s);
-  return launch_groups<1, 256, kTrans>(map, p, group, splits, s);
+  if (p.type == kF32) {
+    if (MT == 32) return launch_groups<1, 32, kTrans, true>(map, p, group, splits, s);
+    if (MT == 64) return launch_groups<1, 64, kTrans, true>(map, p, group, splits, s);
+    return launch_groups<1, 128, kTrans, true>(map, p, group, splits, s);
+  }
+  if (R == 2) return launch_groups<2, 256, kTrans, false>(map, p, group, splits, s);
+  if (MT == 32) return launch_groups<1, 32, kTrans, false>(map, p, group, splits, s);
+  if (MT == 64) return launch_groups<1, 64, kTrans, false>(map, p, group, splits, s);
+  if (MT == 128) return launch_groups<1, 128, kTrans, false>(map, p, group, splits, s);
+  return launch_groups<1, 256, kTrans, false>(map, p, group, splits, s);
 }
 
 template <typename XT>
@@ -148,7 +156,8 @@ int run_gemm(bool transposed, const void* x, int type, long long ldx, const void
   }
   // Tile: all tokens up to 256 at a time; 256 rows of the matrix where that
   // makes the last wave of CTAs no emptier (time goes by waves times rows).
-  const int MT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  // fp32 sums take registers: 128 tokens at most.
+  const int MT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 || type == kF32 ? 128 : 256;
   const long long tiles_m = ((long long)M + MT - 1) / MT;
   const long long one = (rows + 127) / 128 * tiles_m, two = (rows + 255) / 256 * tiles_m;
   const int R = MT == 256 && (two + sms - 1) / sms * 2 <= (one + sms - 1) / sms ? 2 : 1;

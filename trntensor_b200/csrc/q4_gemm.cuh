@@ -50,14 +50,15 @@ struct Gemm {
   int* err;
 };
 
-template <int R, int MT>
+// kSums: sums leave TMEM in between (below).
+template <int R, int MT, bool kSums>
 struct GemmShape {
   static constexpr int kA = R * 128 * 128;  // bytes of operand A in a stage
   static constexpr int kB = MT * 128;
   static constexpr int kStageBytes = kA + kB;
   static constexpr int kStages = R == 2 ? 3 : MT == 256 ? 4 : MT == 128 ? 6 : 8;
   static constexpr int kSmem = kStages * kStageBytes + 1024;
-  static constexpr int kColumns = R * MT;
+  static constexpr int kColumns = R * MT * (kSums ? 2 : 1);
   // half blocks that a decoding warp keeps in flight, for each of its R
   static constexpr int kDepth = R == 2 ? 2 : 4;
   // TMEM columns that a warp brings out at the end
@@ -103,14 +104,24 @@ __device__ __forceinline__ float scale_term(float s, int i) {
   return i == 1 ? b : r - b;
 }
 
-template <int R, int MT, int kGroups, bool kTrans>
+// The tensor cores cut an accumulator off to 24 bits at every addition: each of
+// the K / 16 takes up to 2^-23 of the sum so far, to one side (measured 2.7e-8
+// of the result a step; 1.2e-5 for fp32 rows, whose four passes make 470 of
+// them of K = 1900). Results of 16 bits do not show it. For fp32 ones (kSums) D
+// starts anew every kSumSteps steps of the sum, in the other half of TMEM,
+// and the decoding warps add the finished half to fp32 registers: 16 cut
+// additions at most, then rounded ones.
+constexpr int kSumSteps = 2;
+
+template <int R, int MT, int kGroups, bool kTrans, bool kSums>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
-  using S = GemmShape<R, MT>;
+  using S = GemmShape<R, MT, kSums>;
+  static_assert(!kSums || R == 1, "D twice in TMEM");
   constexpr int kArrive = 8;  // decoding warps that fill a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[S::kStages], empty[S::kStages], done;
+  __shared__ uint64_t full[S::kStages], empty[S::kStages], done, d_full[2], d_free[2];
   __shared__ uint32_t tmem_slot;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = gridDim.x, rank = blockIdx.x;
@@ -129,6 +140,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
       mbar_init(&empty[s], 1);
     }
     mbar_init(&done, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_free[i], kDecodeWarps);
+    }
     fence_mbar_init();
     tma_prefetch_desc(&mapB);
   }
@@ -172,6 +187,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     for (; it < 2u * count; ++it) {
       const int s = it % S::kStages;
       const uint32_t ph = (it / S::kStages) & 1u;
+      const uint32_t part = it / (2 * kSumSteps), of_part = it % (2 * kSumSteps);  // kSums
+      if (kSums && of_part == 0 &&
+          !__all_sync(0xffffffffu, mbar_wait(&d_free[part & 1], (part >> 1 & 1) ^ 1, p.err, kDevTimeoutAcc)))
+        break;
       if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, p.err, kDevTimeoutFull))) break;
       tc_fence_after();
       // sum-major A: 128-byte rows of 64 terms; row-major (kTrans): two columns
@@ -182,9 +201,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
         for (int ks = 0; ks < kStageK / 16; ++ks)
 #pragma unroll
           for (int r = 0; r < R; ++r)
-            mma_f16(d0 + r * MT, a + r * (16384 >> 4) + ks * ((kTrans ? 2048 : 32) >> 4), b + ks * (32 >> 4), idesc,
-                    it != 0 || ks != 0);
+            mma_f16(d0 + (kSums ? (part & 1) * MT : r * MT), a + r * (16384 >> 4) + ks * ((kTrans ? 2048 : 32) >> 4), b + ks * (32 >> 4), idesc,
+                    (kSums ? of_part : it) != 0 || ks != 0);
         mma_commit(&empty[s]);
+        if (kSums && (of_part == 2 * kSumSteps - 1 || it + 1 == 2u * count)) mma_commit(&d_full[part & 1]);
       }
       __syncwarp();
     }
@@ -256,6 +276,31 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     };
 #pragma unroll
     for (int d = 0; d < S::kDepth; ++d) fetch(ring[d]);
+    // Of D, a warp has lanes (its quarter of the rows) and a quarter of the
+    // columns: of all 2 MT, rows 128 and up behind MT.
+    const int quad = warp & 3, first = (warp >> 2) * S::kOut;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    float sum[kSums ? S::kOut : 1];
+    int summed = 0;
+    auto take = [&]() {  // the next part of the sum
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&d_full[summed & 1], summed >> 1 & 1, p.err, kDevTimeoutAcc));
+      if (!ok) return;
+      tc_fence_after();
+      if (first < MT) {
+#pragma unroll
+        for (int c = 0; c < (kSums ? S::kOut : 0); c += 16) {
+          float v[16];
+          tmem_ld16(lanes + (summed & 1) * MT + first + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) sum[c + k] = summed == 0 ? v[k] : sum[c + k] + v[k];
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&d_free[summed & 1]);
+      ++summed;
+    };
     int pass = 0, step = s0, term = p.scale_term[0];
     uint32_t it = sub;  // stage number
     // No way out of the loop but its head, and every turn fetches: the ring
@@ -326,6 +371,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[s]);
         }
+        if constexpr (kSums)  // one part behind
+          if (now && (i0 + d) % kSumSteps == kSumSteps - 1 && i0 + d >= 2 * kSumSteps - 1) take();
         it += 2;
         if (++step == s1) {
           step = s0;
@@ -334,24 +381,19 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
         }
       }
     }
+    if constexpr (kSums)
+      while (ok && summed * kSumSteps < count) take();
     // D: lanes are rows of the tile, columns are tokens
     ok = mbar_wait(&done, 0, p.err, kDevTimeoutAcc) && ok;
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     if (ok && active) {
-      // a quarter of the columns each: of all 2 MT, rows 128 and up behind MT
-      const int quad = warp & 3, first = (warp >> 2) * S::kOut;
       const int half = R == 2 ? first / MT : 0;
       const long long row = row0 + half * 128 + quad * 32 + lane;
-      const int c0 = first - half * MT, c1 = first < S::kColumns ? c0 + S::kOut : c0;
-      const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16) + half * MT;
+      const int c0 = first - half * MT;
       const float up = !kTrans && row < rows ? __ldg(p.row_scale + row) : 1.f;
       float* dsm = reinterpret_cast<float*>(smem);
-      for (int c = c0; c < c1; c += 16) {
-        if (m0 + c >= p.M) break;
-        float v[16];
-        tmem_ld16(from + c, v);
-        tmem_ld_wait();
+      auto bring = [&](int c, const float (&v)[16]) {
         if (splits > 1) {
 #pragma unroll
           for (int k = 0; k < 16; ++k) dsm[(c + k) * 128 + quad * 32 + lane] = v[k];
@@ -362,6 +404,22 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
             if (m < p.M)
               store_out(p, m * p.ldo + row, v[k] * up * (p.f ? __ldg(p.f + m) : 1.f));
           }
+        }
+      };
+      const int c1 = first < R * MT ? c0 + S::kOut : c0;
+      float v[16];
+      if constexpr (kSums) {
+#pragma unroll
+        for (int j = 0; j < S::kOut; j += 16) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = sum[j + k];
+          if (c0 < c1 && m0 + c0 + j < p.M) bring(c0 + j, v);
+        }
+      } else {
+        for (int c = c0; c < c1 && m0 + c < p.M; c += 16) {
+          tmem_ld16(lanes + half * MT + c, v);
+          tmem_ld_wait();
+          bring(c, v);
         }
       }
     }
