@@ -318,6 +318,29 @@ def test_long_and_ragged(cuda_ok, length):
     got, _ = attend_case("fp16", 7, 1, 4, 4, 128, 128, [length // (b + 1) for b in range(7)])
 
 
+def test_long_sums_of_fp32(cuda_ok):
+    """So many sequences that a warp has a hundred blocks of 64 tokens of each:
+    what the tensor cores cut off may add up inside a block (8 additions, and the
+    score's own), then rounded ones follow (half of 2^-23 a block, and a rounding
+    of each block's own sum of weights). All sequences read the same pages; all
+    values are positive, so that every cut goes the same way."""
+    pages, dim, batch = 128, 64, 1000
+    kc, ks, vc, vs = filled(pages, 1, 64, dim, seed=9, spread=0.1)
+    vc = vc.abs().clamp(min=1)
+    cache = tt.KVCache8.from_codes(kc.cuda(), ks.cuda(), vc.cuda(), vs.cuda())
+    q = torch.randn(batch, 1, 1, dim, generator=torch.Generator().manual_seed(3)) * 0.1
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, -1)
+    got = tt.kv_attention(q.cuda(), cache, table, int32([64 * pages] * batch)).double().cpu()
+    k = (kc.double() * ks.double()[..., None, None]).reshape(-1, dim)
+    v = (vc.double() * vs.double()[..., None, None]).reshape(-1, dim)
+    s = q[:, 0, 0].double() @ k.T * dim ** -0.5
+    want = torch.softmax(s, -1) @ v
+    d = (dim / 16 * 2 + 20) * 2.0**-23 * (q[:, 0, 0].double().abs() @ k.abs().T).max().item() * dim ** -0.5
+    tol = 2 * d + 2 * 2.0**-22 + 2.0**-21 + (8 + pages / 2 + 8) * 2.0**-23
+    worst = ((got[:, 0, 0] - want).abs() / want).max().item()
+    assert worst <= tol, (worst, tol)
+
+
 @pytest.mark.parametrize("name", list(TYPES))
 def test_extremes(cuda_ok, name):
     attend_case(name, 2, 1, 4, 2, 64, 16, [100, 50], q_scale=0.0)       # all scores alike

@@ -638,6 +638,17 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
           va[n] = lds128(vals + (n0 + n) * 256);
           vb[n] = lds128(vals + (n0 + n) * 256 + 128);
         }
+        // fp32: an accumulator of the chunk's own, since the tensor cores cut
+        // off at every addition (4e-6 of the result after 90 chunks)
+        float own[kTerms == 2 ? NT : 1][2][4];
+        if constexpr (kTerms == 2) {
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) own[a][n][e] = 0.f;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -649,8 +660,17 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
             for (int a = 0; a < NT; ++a)
 #pragma unroll
               for (int k = 0; k < kTerms; ++k)
-                q4::mma16816<true>(acc[a][n0 + n], a0, a1, a2, a3, w[a][j][k][0], w[a][j][k][1]);
+                q4::mma16816<true>(kTerms == 2 ? own[a % (kTerms == 2 ? NT : 1)][n] : acc[a][n0 + n], a0, a1, a2, a3,
+                                   w[a][j][k][0], w[a][j][k][1]);
           }
+        if constexpr (kTerms == 2) {
+#pragma unroll
+          for (int a = 0; a < NT; ++a)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[a][n0 + n][e] += own[a][n][e];
+        }
       }
     }
     release();
