@@ -311,6 +311,17 @@ def test_several_tokens(cuda_ok, dim, page, heads, kv, new, lengths, counts, cau
     attend_case(name, 3, new, heads, kv, dim, page, lengths, counts, causal)
 
 
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim,page,heads,kv,new,lengths,counts", [
+    (64, 32, 16, 16, 210, [210, 128, 513], [210, 1, 209]), (96, 16, 24, 3, 140, [300, 40, 41], None),
+    (16, 16, 8, 8, 400, [400, 1, 129], [400, 1, 128]), (80, 128, 4, 1, 800, [830, 257, 260], [800, 1, 129]),
+    (128, 64, 12, 6, 270, [700, 150, 20], [270, 149, 270]), (128, 16, 40, 40, 64, [64, 65, 1000], [64, 63, 64])])
+def test_tiles_of_many_rows(cuda_ok, dim, page, heads, kv, new, lengths, counts, causal, name):
+    """Enough rows for the tensor cores' tiles on any GPU of up to 148 SMs."""
+    attend_case(name, 3, new, heads, kv, dim, page, lengths, counts, causal)
+
+
 @pytest.mark.parametrize("length", [1000, 20011])
 def test_long_and_ragged(cuda_ok, length):
     attend_case("bf16", 1, 1, 8, 2, 128, 64, [length])
@@ -350,6 +361,13 @@ def test_extremes(cuda_ok, name):
     attend_case(name, 2, 3, 4, 2, 64, 16, [500, 60], spread=6.0)        # scales decades apart
 
 
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("more", [
+    {"q_scale": 0.0}, {"q_scale": 60.0}, {"scale": -0.3}, {"scale": 0.0}, {"spread": 6.0}])
+def test_extremes_of_many_rows(cuda_ok, name, more):
+    attend_case(name, 3, 800, 4, 1, 64, 16, [830, 257, 900], **more)
+
+
 def test_negative_scales(cuda_ok):
     """A sign in a scale means the same as in its codes."""
     kc, ks, vc, vs = filled(8, 2, 16, 32)
@@ -379,7 +397,7 @@ def test_zero_pages_and_rows(cuda_ok):
     assert tt.kv_attention(q.cuda()[:0], cache, int32([[0]])[:0], int32([4])[:0]).shape == (0, 1, 2, 32)
 
 
-@pytest.mark.parametrize("new", [1, 40, 140, 900])
+@pytest.mark.parametrize("new", [1, 40, 140, 900, 1300])
 def test_not_finite_stays_where_it_belongs(cuda_ok, new):
     """A NaN scale, or an infinite query, reaches the rows that see it and no others."""
     kc, ks, vc, vs = filled(24, 2, 16, 64)
@@ -448,7 +466,7 @@ def test_query_strides(cuda_ok):
             assert torch.equal(tt.kv_attention(q, cache, table, lengths), want)
 
 
-@pytest.mark.parametrize("new,heads", [(1, 8), (6, 4), (200, 4)])
+@pytest.mark.parametrize("new,heads", [(1, 8), (6, 4), (200, 4), (1200, 8)])
 def test_same_bits_graphs_and_streams(cuda_ok, new, heads):
     """Eager calls, two graphs and two streams at a time give the same bits."""
     parts = filled(64, 2, 32, 128)

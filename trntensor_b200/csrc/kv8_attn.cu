@@ -84,13 +84,18 @@ int launch(Attend p, int sms, cudaStream_t s) {
   return cuda_status(cudaLaunchKernelEx(&cfg, join_kernel<T>, p));
 }
 // 16-bit types with up to 128 values a head go to the tensor cores' tiles of
-// 256 rows where that is faster. There a block of 128 tokens takes about 2700
-// clocks of a CTA, however few of its rows are used, and the other kernel
-// about 1250 of an SM for each 64 tokens and 16 rows, spread over all SMs: the
-// first wins from rows x heads x sequences = 2560 for each wave of CTAs.
-bool many_rows(const Attend& p, int sms) {
-  const long long tiles = ((long long)p.rows + 255) / 256 * p.heads * p.batch;
-  return p.rows > 16 && (long long)p.rows * p.heads * p.batch > 2560 * ((tiles + sms - 1) / sms);
+// 256 rows where that is faster. There 64 tokens take about 2850 clocks of a
+// CTA (2250 if no more than 128 rows are used), however few of the SMs have
+// one, and the other kernel about 620 of an SM for each 16 rows, spread over
+// all SMs: the first wins from rows x heads x sequences = 64 (48) an SM for each
+// wave of CTAs. (8192 tokens, 128 a head: 16 x 8 x 40 rows 153 against 149 us,
+// 16 x 8 x 80 rows 152 against 238, 1 x 8 x 400 rows 190 against 110.)
+// It adds up a row's values in the tensor cores, which cut off 2^-25 or so at
+// each 16 tokens: not where a table can hold so many that a result shows it.
+bool many_rows(const Attend& p, int sms, bool fp16) {
+  const long long tiles = ((long long)p.rows + 255) / 256 * p.heads * p.batch, waves = (tiles + sms - 1) / sms;
+  return p.rows > 16 && (long long)p.rows * p.heads * p.batch > (p.rows > 128 ? 64 : 48) * waves * sms &&
+         (long long)p.cols * p.page <= (fp16 ? 1 << 17 : 1 << 20);
 }
 
 template <typename T, int DP>
@@ -104,7 +109,7 @@ int launch_prefill(const Attend& p, cudaStream_t s) {
 template <typename T>
 int launch_dim(const Attend& p, int sms, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (many_rows(p, sms) && p.dim <= 128 && p.heads <= 65535 && p.batch <= 65535)
+    if (many_rows(p, sms, std::is_same<T, __half>::value) && p.dim <= 128 && p.heads <= 65535 && p.batch <= 65535)
       return p.dim <= 64 ? launch_prefill<T, 64>(p, s) : launch_prefill<T, 128>(p, s);
   }
   if (p.dim <= 64) return launch<T, 64>(p, sms, s);
