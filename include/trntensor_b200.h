@@ -330,8 +330,8 @@ int tt_q4_dequantize(const void* packed, const void* packed_scales, int scale_ty
  * into fp16's range in products of many rows. */
 int tt_q4_row_scale(const void* packed_scales, int scale_type, int N, int K, int group,
                     float* row_scale, void* stream);
-/* Bytes of workspace for a product (0 up to 16 rows, and up to 32 of 16-bit
- * types over k, where it may be NULL). */
+/* Bytes of workspace for a product (0 up to 8 rows, up to 32 of 16-bit types
+ * over k and up to 16 of fp32 over n, where it may be NULL). */
 size_t tt_q4_matmul_workspace_bytes(int type, int scale_type, int transposed, int M, int N, int K);
 /* y (M, N; row stride ldy) = x (M, K; row stride ldx) W^T: fp32 sums, rounded
  * once to x's type. dev_status as in the file's head; unlike other calls these

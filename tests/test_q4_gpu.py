@@ -2,10 +2,10 @@
 
 Tolerances. A result is rounded once (half a step: eps / 2 of the value). The
 fp32 sum is a chain of at most 16 products, one addition for each 16 terms (8 a
-group and one a 128-wide block, or 8 a block, up to 16 rows, or 32 of 16-bit
-types over k), 8 warps and 8 CTAs; each of these loses at most a unit in the
+group and one a 128-wide block, or 8 a block, up to 8 rows, 32 of 16-bit types
+over k, 16 of fp32 over n), 8 warps and 8 CTAs; each of these loses at most a unit in the
 last place (2^-23, the tensor cores truncate) of a partial sum that sum |x W|
-bounds. fp32 rows above 16 are summed 256 terms at a time. Up to 16 rows the sum
+bounds. More rows of fp32 are summed 256 terms at a time. Up to 8 rows the sum
 over n keeps 2^-16 of each product of 16-bit types. Above, fp16 terms: a 16-bit
 operand with bf16 scales loses only what lies below 2^-39 of its row's largest
 value; two 8-bit terms of an fp32 scale leave 2^-18; fp32 rows in two terms
@@ -43,7 +43,8 @@ def check(got, x, wide, over_n=False):
     """wide is (cols of x, cols of the result)."""
     ref = x.double() @ wide
     mass = x.double().abs() @ wide.abs()
-    if x.shape[0] <= 16 or (x.shape[0] <= 32 and not over_n and x.dtype != torch.float32):
+    wide_type = x.dtype == torch.float32
+    if x.shape[0] <= ((16 if wide_type else 8) if over_n else (8 if wide_type else 32)):
         links = 48 + x.shape[1] / (16 if over_n else 128)
         loss = links * 2.0**-23 + (2.0**-16 if over_n and x.dtype != torch.float32 else 0)
     elif x.dtype == torch.float32:

@@ -23,8 +23,12 @@ namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8;
 constexpr int kMaxCluster = 8;
-// Up to so many rows the products run here, above in csrc/q4_gemm.cuh.
-int few_rows(int type, bool transposed) { return !transposed && type != kF32 ? 32 : 16; }
+// Up to so many rows the products run here, above in csrc/q4_gemm.cuh. Measured
+// on both sides with 16384 x 8192 and 4096 x 4096, in us: over k, 32 rows of
+// bf16 40 here and 44 there, 16 rows of fp32 190 and 28 here, 101 and 20 there;
+// over n, 16 rows of bf16 63 and 30 here, 60 and 16 there, of fp32 76 and 32
+// here, 122 and 23 there.
+int few_rows(int type, bool transposed) { return transposed ? (type == kF32 ? 16 : 8) : type == kF32 ? 8 : 32; }
 
 // ------------------------------------------------------- packing and decoding
 
@@ -195,20 +199,20 @@ __device__ __forceinline__ void load_eight(const XT* __restrict__ at, int left, 
 
 // ------------------------------------------------------------ y = x W^T, few rows
 
-// A CTA owns 16 rows of W and 8 kTiles tokens; its warps take the row tile's
+// Up to eight tokens. A CTA owns 16 rows of W; its warps take the row tile's
 // blocks in turn, and the CTAs of a cluster (blockIdx.x is the rank) share
 // them, so that a short matrix still fills the GPU. Each group of k gets a
 // fragment of its own, which is scaled in fp32 when the group ends. The parts
 // are added in a fixed order: warps through shared memory, CTAs through the
 // cluster's.
-template <typename XT, typename ST, int kTiles, int kGroups>
-__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 && sizeof(XT) == 2 ? 3 : 1)
+template <typename XT, typename ST, int kGroups>
+__global__ void __launch_bounds__(kWarps * 32, sizeof(XT) == 2 ? 3 : 1)
 matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ packed,
               const ST* __restrict__ scales, int M, int N, int K, int kblocks, int wide,
               XT* __restrict__ y, long long ldy) {
   constexpr bool kHalf = sizeof(XT) == 2 && !std::is_same<XT, __nv_bfloat16>::value;
   constexpr int kTerms = sizeof(XT) == 2 ? 1 : 3;
-  constexpr int kOut = kRows * 8 * kTiles;
+  constexpr int kOut = kRows * 8;
   __shared__ float part[kWarps * kOut];
   cg::cluster_group cluster = cg::this_cluster();
   const int warp = threadIdx.x / 32, warps = blockDim.x / 32, lane = threadIdx.x & 31;
@@ -216,22 +220,13 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
   const int splits = gridDim.x;
   const long long rt = blockIdx.y + (long long)blockIdx.z * gridDim.y;
   const long long rtiles = ((long long)N + kRows - 1) / kRows;
-  const long long mtiles = ((long long)M + 8 * kTiles - 1) / (8 * kTiles);
-  const long long tile = rt;  // row tile fastest: neighbours share x in L2
-  const bool active = tile < rtiles * mtiles;
-  const long long row_tile = active ? tile % rtiles : 0;
-  const long long m0 = active ? tile / rtiles * (8 * kTiles) : 0;
+  const bool active = rt < rtiles;
 
-  float acc[kTiles][4];
-#pragma unroll
-  for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
 
   if (active) {
-    const XT* xr[kTiles];  // a token that is not there reads another's values: its column is dropped
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j) xr[j] = x + min(m0 + 8 * j + g, (long long)M - 1) * ldx + 8 * t;
+    // a token that is not there reads another's values: its column is dropped
+    const XT* xr = x + (long long)min(g, M - 1) * ldx + 8 * t;
     const int whole = wide ? K / kCols : 0;  // blocks whose 128 columns can be read as they stand
     // A ring of blocks in registers: codes, scales and the tokens' values are
     // asked for kDepth blocks ahead.
@@ -245,7 +240,7 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
     const int stride = splits * warps;
     int next = blockIdx.x * warps + warp;
     auto fetch = [&](Piece& f) {  // behind the last block: the last again, for nothing
-      const long long blk = row_tile * kblocks + min(next, kblocks - 1);
+      const long long blk = rt * kblocks + min(next, kblocks - 1);
       f.qa = ldg128(packed + blk * 64 + lane);
       f.qb = ldg128(packed + blk * 64 + 32 + lane);
 #pragma unroll
@@ -263,23 +258,17 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
         // past the end the last block is fetched again, and counts for nothing
         const int kb = min(kb0 + d * stride, kblocks - 1);
         const bool on = kb0 + d * stride < kblocks;
-        uint32_t xp[kTiles][4][kTerms][4];
+        uint32_t xp[4][kTerms][4];
 #pragma unroll
-        for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            load_eight<XT, kTerms>(xr[j] + (long long)kb * kCols + 32 * w, K - kb * kCols - 32 * w - 8 * t, kb < whole,
-                                   xp[j][w]);
+        for (int w = 0; w < 4; ++w)
+          load_eight<XT, kTerms>(xr + (long long)kb * kCols + 32 * w, K - kb * kCols - 32 * w - 8 * t, kb < whole,
+                                 xp[w]);
         const Piece f = ring[d];
         fetch(ring[d]);
         const uint32_t wa[4] = {f.qa.x, f.qa.y, f.qa.z, f.qa.w}, wb[4] = {f.qb.x, f.qb.y, f.qb.z, f.qb.w};
 #pragma unroll
         for (int gi = 0; gi < kGroups; ++gi) {
-          float c[kTiles][4];
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int w = gi * 4 / kGroups; w < (gi + 1) * 4 / kGroups; ++w)
 #pragma unroll
@@ -288,33 +277,26 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
               decode_four<kHalf>(wa[w] >> (8 * half), a0, a2);
               decode_four<kHalf>(wb[w] >> (8 * half), a1, a3);
 #pragma unroll
-              for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-                for (int i = 0; i < kTerms; ++i)
-                  mma16816<kHalf>(c[j], a0, a1, a2, a3, xp[j][w][i][2 * half], xp[j][w][i][2 * half + 1]);
+              for (int i = 0; i < kTerms; ++i)
+                mma16816<kHalf>(c, a0, a1, a2, a3, xp[w][i][2 * half], xp[w][i][2 * half + 1]);
             }
           const float s0 = scale_value(f.s[gi][0], kF32Scale, g & 1), s1 = scale_value(f.s[gi][1], kF32Scale, g & 1);
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j)
-            if (on) {
-              acc[j][0] += s0 * c[j][0];
-              acc[j][1] += s0 * c[j][1];
-              acc[j][2] += s1 * c[j][2];
-              acc[j][3] += s1 * c[j][3];
-            }
+          if (on) {
+            acc[0] += s0 * c[0];
+            acc[1] += s0 * c[1];
+            acc[2] += s1 * c[2];
+            acc[3] += s1 * c[3];
+          }
         }
       }
     }
   }
   // part[warp][token][row]
   float* mine = part + warp * kOut;
-#pragma unroll
-  for (int j = 0; j < kTiles; ++j) {
-    mine[(8 * j + 2 * t) * kRows + g] = acc[j][0];
-    mine[(8 * j + 2 * t + 1) * kRows + g] = acc[j][1];
-    mine[(8 * j + 2 * t) * kRows + g + 8] = acc[j][2];
-    mine[(8 * j + 2 * t + 1) * kRows + g + 8] = acc[j][3];
-  }
+  mine[2 * t * kRows + g] = acc[0];
+  mine[(2 * t + 1) * kRows + g] = acc[1];
+  mine[2 * t * kRows + g + 8] = acc[2];
+  mine[(2 * t + 1) * kRows + g + 8] = acc[3];
   __syncthreads();
   for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
     float v = part[o];
@@ -336,7 +318,7 @@ matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__
   }
   if (blockIdx.x == 0 && active) {
     for (int o = threadIdx.x; o < kOut; o += blockDim.x) {
-      const long long m = m0 + o / kRows, n = row_tile * kRows + o % kRows;
+      const long long m = o / kRows, n = rt * kRows + o % kRows;
       if (m < M && n < N) y[m * ldy + n] = from_f<XT>(part[o]);
     }
   }
@@ -718,19 +700,18 @@ int pick_splits(long long tiles, long long steps, int sms) {
   return s;
 }
 
-template <typename XT, typename ST, int kTiles, int kGroups>
+template <typename XT, typename ST, int kGroups>
 int run_matvec(const void* x, long long ldx, const void* packed, const void* scales, int M, int N,
                int K, void* y, long long ldy, int sms, cudaStream_t s) {
   const int kblocks = (int)(((long long)K + kCols - 1) / kCols);
   const long long rtiles = ((long long)N + kRows - 1) / kRows;
-  const long long mtiles = ((long long)M + 8 * kTiles - 1) / (8 * kTiles);
-  const int splits = pick_splits(rtiles * mtiles, kblocks, sms);
+  const int splits = pick_splits(rtiles, kblocks, sms);
   dim3 grid;
-  if (!grid_of(rtiles * mtiles, splits, &grid)) return TT_ERR_SHAPE;
+  if (!grid_of(rtiles, splits, &grid)) return TT_ERR_SHAPE;
   int wide = K % 8 == 0 && ldx % (16 / (int)sizeof(XT)) == 0 && aligned16(x);
   int kb = kblocks;
   void* args[] = {&x, &ldx, &packed, &scales, &M, &N, &K, &kb, &wide, &y, &ldy};
-  return launch_cluster(matvec_kernel<XT, ST, kTiles, kGroups>, grid, kWarps * 32, 0, splits, s, args);
+  return launch_cluster(matvec_kernel<XT, ST, kGroups>, grid, kWarps * 32, 0, splits, s, args);
 }
 
 template <typename XT, typename ST, int kTiles, int kGroups>
@@ -777,8 +758,8 @@ bool set_smem(F kernel, int bytes) {
 }
 template <typename XT, typename ST, int kGroups>
 bool set_group() {
-  bool ok = set_smem(matvec_t_kernel<XT, ST, 1, kGroups>, t_smem<1>()) &&
-            set_smem(matvec_t_kernel<XT, ST, 2, kGroups>, t_smem<2>());
+  bool ok = set_smem(matvec_t_kernel<XT, ST, 1, kGroups>, t_smem<1>());
+  if constexpr (sizeof(XT) == 4) ok = ok && set_smem(matvec_t_kernel<XT, ST, 2, kGroups>, t_smem<2>());
   if constexpr (sizeof(XT) == 2)
     ok = ok && set_smem(mid_kernel<XT, ST, 2, kGroups>, mid_smem<2>()) &&
          set_smem(mid_kernel<XT, ST, 4, kGroups>, mid_smem<4>());
@@ -809,28 +790,24 @@ int matmul_typed(bool transposed, const void* x, long long ldx, const void* pack
                  int sms, cudaStream_t s) {
   const int gpb = kCols / group;
   if (transposed) {
-    if (M <= 8) {
-      if (gpb == 1) return run_matvec_t<XT, ST, 1, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-      if (gpb == 2) return run_matvec_t<XT, ST, 1, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-      return run_matvec_t<XT, ST, 1, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if constexpr (sizeof(XT) == 4) {
+      if (M > 8) {
+        if (gpb == 1) return run_matvec_t<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+        if (gpb == 2) return run_matvec_t<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+        return run_matvec_t<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+      }
     }
-    if (gpb == 1) return run_matvec_t<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    if (gpb == 2) return run_matvec_t<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    return run_matvec_t<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-  }
-  if (M <= 8) {
-    if (gpb == 1) return run_matvec<XT, ST, 1, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    if (gpb == 2) return run_matvec<XT, ST, 1, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    return run_matvec<XT, ST, 1, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (gpb == 1) return run_matvec_t<XT, ST, 1, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (gpb == 2) return run_matvec_t<XT, ST, 1, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    return run_matvec_t<XT, ST, 1, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
   }
   if constexpr (sizeof(XT) == 2) {
-    if (M <= 16) return run_mid_group<XT, ST, 2>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
-    return run_mid_group<XT, ST, 4>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
-  } else {
-    if (gpb == 1) return run_matvec<XT, ST, 2, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    if (gpb == 2) return run_matvec<XT, ST, 2, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
-    return run_matvec<XT, ST, 2, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+    if (M > 16) return run_mid_group<XT, ST, 4>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
+    if (M > 8) return run_mid_group<XT, ST, 2>(x, ldx, packed, scales, M, N, K, group, y, ldy, sms, s);
   }
+  if (gpb == 1) return run_matvec<XT, ST, 1>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  if (gpb == 2) return run_matvec<XT, ST, 2>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
+  return run_matvec<XT, ST, 4>(x, ldx, packed, scales, M, N, K, y, ldy, sms, s);
 }
 
 template <typename XT>

@@ -22,7 +22,7 @@ from .plan import _check_precision, _parse_subscripts, _validate_subscripts
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GROUPS = (32, 64, 128)
-_FEW_ROWS = 16  # up to here no product needs a workspace
+_FEW_ROWS = 8  # up to here no product needs a workspace
 
 
 _HERE = contextlib.nullcontext()
@@ -246,8 +246,9 @@ def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> tor
     """``x @ W^T``: (..., K) -> (..., N); with ``over_n`` ``x @ W``: (..., N) -> (..., K).
 
     x is fp32, bf16 or fp16; sums are fp32 and the result is rounded once to
-    x's type. Up to 16 rows (32 of 16-bit types over k) products over k are
-    exact, and over n they keep 2^-16 (fp32: all bits). With more both operands are brought to fp16's
+    x's type. Up to 8 rows (32 of 16-bit types over k, 16 of fp32 over n)
+    products over k are exact, and over n they keep 2^-16 (fp32: all bits).
+    With more both operands are brought to fp16's
     range by powers of two a row: products are exact where scales are bf16 and
     x is of 16 bits and no smaller than 2^-27 of its row's largest value, else
     they keep 2^-18 (fp32: 2^-20) of themselves and 2^-38 of the largest.
