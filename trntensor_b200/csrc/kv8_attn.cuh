@@ -13,7 +13,9 @@
 //
 // What bounds it: the cache's bytes, and close behind them the instructions
 // that decode and multiply (with rows on the 16-wide side of the fragments,
-// half of it empty, they took a third more time). Each warp keeps its own ring
+// half of it empty, they took a third more time). bf16, 128 a head: 64
+// sequences x 8192 tokens x 8 kv heads 144 us (5.7 TB/s of cache), one of 131000
+// tokens 56 us (4.8 TB/s); three of 100 tokens 13 us, launches and waits. Each warp keeps its own ring
 // of shared memory slots (one unit quartet of keys or of values each) filled by
 // bulk copies two or three slots ahead, across tile borders. Tensor-core
 // operands: the codes are exact in fp16; a row of q is scaled by a power of two

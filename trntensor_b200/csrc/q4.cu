@@ -4,8 +4,9 @@
 //   y[m,n]  = sum_k x[m,k] s[n,g(k)] c[n,k]
 //   dx[m,k] = sum_n dy[m,n] s[n,g(k)] c[n,k]
 //
-// Both products with few rows read the matrix once (4.1 bits a weight) and
-// are bound by that. The codes are exact in bf16 and fp16, so the products
+// Both products with few rows read the matrix once (4.1 bits a weight). What
+// bounds them is not that yet but the instructions that decode it and the wait
+// for the first bytes. The codes are exact in bf16 and fp16, so the products
 // run on mma.sync tensor-core fragments decoded in registers and accumulate
 // in fp32; tcgen05 would want the decoded matrix in shared memory first,
 // which costs more than it saves while the rows fit one fragment.
@@ -204,7 +205,9 @@ __device__ __forceinline__ void load_eight(const XT* __restrict__ at, int left, 
 // them, so that a short matrix still fills the GPU. Each group of k gets a
 // fragment of its own, which is scaled in fp32 when the group ends. The parts
 // are added in a fixed order: warps through shared memory, CTAs through the
-// cluster's.
+// cluster's. bf16, one row: 4096 x 4096 5 us (1.6 TB/s of matrix, mostly the
+// launch and the first wait), 16384 x 8192 25 us (2.8 TB/s: 256 instructions a
+// block of 1 KB fill half of the issue slots, and waits for memory the rest).
 template <typename XT, typename ST, int kGroups>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(XT) == 2 ? 3 : 1)
 matvec_kernel(const XT* __restrict__ x, long long ldx, const uint4* __restrict__ packed,
@@ -340,7 +343,8 @@ __device__ __forceinline__ float value_of(uint32_t bits) {
 // for 16-bit types: 2^-16 of each product, against 2^-9 or 2^-12 for the
 // result's own rounding; three for fp32). A fragment of W takes the columns
 // k = 32 w + 8 (c / 2) + 2 j + c % 2 of a block, c = 0 .. 7, for two j, so that
-// all its columns share a group.
+// all its columns share a group. bf16, one row: 4096 x 4096 10.5 us, 16384 x
+// 8192 36 us (1.9 TB/s): decoding and the doubled products bound it.
 template <typename XT, typename ST, int kTiles, int kGroups>
 __global__ void __launch_bounds__(kWarps * 32)
 matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restrict__ packed,
@@ -503,9 +507,11 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
 // tile a warp, and all its warps share the tokens' values from shared memory:
 // four blocks of k a stage, filled by cp.async one stage ahead, rows 64 bytes
 // off each other's banks. The CTAs of a cluster share the sum over k.
-// The alternative, tcgen05 with the matrix decoded into shared memory, took 64
-// us for 32 x 16384 x 8192: decoding with the scale and storing 16 bits a
-// weight is more than the SM can issue at the rate of the loads.
+// 32 x 16384 x 8192 in bf16 takes 40 us (1.7 TB/s of matrix): about 270
+// instructions a block and row tile, 41% of the time on the products alone (17
+// us at the least). tcgen05 with the matrix decoded into shared memory takes 44
+// (csrc/q4_gemm.cuh); CTAs of seven warps, which would fill the SMs evenly,
+// took 43.
 constexpr int kMidBlocks = 4;                                // of k in a stage
 constexpr int kMidRow = kMidBlocks * kCols * 2 + 64;         // bytes of a token's row there
 constexpr int kMidStages = 2;

@@ -15,10 +15,12 @@
 // into dy. fp32 scales are taken as 8-bit terms and fp32 rows as two fp16
 // terms, one pass over the sum for each pair of terms that matters.
 //
-// What bounds it: the tensor cores for many tokens (256 x 256 tiles, so that
-// the L2 has to deliver only 40 bytes a clock and SM), the matrix's bytes for
-// few (the decoding warps then keep four blocks in flight each, and CTAs of a
-// cluster share the sum when there are too few tiles for all SMs).
+// What bounds it: shared memory and the tensor cores for many tokens (256 x 256
+// tiles, so that the L2 has to deliver only 40 bytes a clock and SM), the
+// decoding for few (its warps then keep four blocks in flight each, and CTAs of
+// a cluster share the sum when there are too few tiles for all SMs). bf16, 2048
+// x 8192 x 8192: 217 us, 1.27 PFLOP/s, with 1.73 tiles an SM in two rounds;
+// forward and backward of 2000 x 8192 x 4096 in fp16 260 us, 1.03 PFLOP/s.
 // Roles: warps 0-15 decode (registers to swizzled shared memory, then, at the
 // end, D to global memory), warp 16 issues the TMA loads, warp 17 the MMAs.
 #pragma once
