@@ -206,7 +206,7 @@ __device__ __forceinline__ void load_eight(const XT* __restrict__ at, int left, 
 // fragment of its own, which is scaled in fp32 when the group ends. The parts
 // are added in a fixed order: warps through shared memory, CTAs through the
 // cluster's. bf16, one row: 4096 x 4096 5 us (1.6 TB/s of matrix, mostly the
-// launch and the first wait), 16384 x 8192 25 us (2.8 TB/s: 256 instructions a
+// launch and the first wait), 16384 x 8192 25 us (2.8 TB/s: 187 instructions a
 // block of 1 KB fill half of the issue slots, and waits for memory the rest).
 template <typename XT, typename ST, int kGroups>
 __global__ void __launch_bounds__(kWarps * 32, sizeof(XT) == 2 ? 3 : 1)
