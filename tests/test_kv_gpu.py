@@ -95,6 +95,10 @@ def test_codes_round_trip(cuda_ok):
         assert torch.equal(k[0].cpu(), kc[1].float() * ks[1][..., None, None]) and not k[1:].any()
         with pytest.raises(ValueError, match="page id"):
             c.check()
+        k, _ = c.dequantize(torch.tensor([1, 2**32, -2**32], device="cuda"))  # 64 bits
+        assert torch.equal(k[0].cpu(), kc[1].float() * ks[1][..., None, None]) and not k[1:].any()
+        with pytest.raises(ValueError, match="page id"):
+            c.check()
 
 
 @pytest.mark.parametrize("name", list(TYPES))
@@ -366,6 +370,7 @@ def test_extremes(cuda_ok, name):
     {"q_scale": 0.0}, {"q_scale": 60.0}, {"scale": -0.3}, {"scale": 0.0}, {"spread": 6.0}])
 def test_extremes_of_many_rows(cuda_ok, name, more):
     attend_case(name, 3, 800, 4, 1, 64, 16, [830, 257, 900], **more)
+    attend_case(name, 3, 800, 4, 1, 64, 16, [0, 1, 900], counts=[800, 0, 800], **more)
 
 
 def test_negative_scales(cuda_ok):
@@ -421,6 +426,27 @@ def test_not_finite_stays_where_it_belongs(cuda_ok, new):
     got = tt.kv_attention(q.cuda(), cache, int32([table[1], table[1]]), int32([40, 40]), n_query=int32([1, 1]))
     bad = got.isnan().any(-1).nonzero().tolist()
     assert bad == [[0, 0, 0], [1, 0, 1]]
+
+
+@pytest.mark.parametrize("new", [1, 40, 1300])
+def test_infinite_scales_stay_where_they_belong(cuda_ok, new):
+    """Rows that do not see a page are as they were; those that do are not finite."""
+    kc, ks, vc, vs = filled(12, 2, 16, 64, seed=4)
+    q = torch.randn(2, new, 8, 64, device="cuda")
+    table, lengths = int32([list(range(12)), list(range(12))]), int32([192, 150])
+    for dtype in TYPES.values():
+        want = tt.kv_attention(q.to(dtype), tt.KVCache8.from_codes(kc.cuda(), ks.cuda(), vc.cuda(), vs.cuda()),
+                               table, lengths)
+        wild = vs.clone()
+        wild[11] = float("inf")  # tokens 176 .. 191: rows from position 176 of sequence 0
+        got = tt.kv_attention(q.to(dtype), tt.KVCache8.from_codes(kc.cuda(), ks.cuda(), vc.cuda(), wild.cuda()),
+                              table, lengths)
+        first = max(0, 176 - (192 - new))
+        assert not got[0, first:].isfinite().any()
+        # (weights are relative to the largest scale in sight, and round by it)
+        tol = {torch.float32: 1e-5, torch.float16: 2.0**-9, torch.bfloat16: 2.0**-7}[dtype]
+        assert ((got - want)[0, :first].abs() <= tol * want[0, :first].abs().amax(-1, keepdim=True)).all()
+        assert ((got - want)[1].abs() <= tol * want[1].abs().amax(-1, keepdim=True)).all()
 
 
 def test_stale_slots_do_not_matter(cuda_ok):

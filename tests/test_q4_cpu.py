@@ -127,3 +127,11 @@ def test_library_refuses_bad_arguments():
     assert lib.tt_q4_pack(p, p, 2, 8, 8, 32, p, p, None) == _lib.TT_ERR_SHAPE
     assert lib.tt_q4_dequantize(p, p, 0, 8, 8, 33, p, 0, None) == _lib.TT_ERR_SHAPE
     assert lib.tt_q4_packed_bytes(0, 5) == 0 and lib.tt_q4_scale_count(5, 5, 31) == 0
+
+
+def test_sizes_past_32_bits_are_refused():
+    from trntensor_b200 import quantized
+
+    for n, k in ((2**31, 1), (1, 2**31)):
+        with pytest.raises(ValueError, match="at most"):
+            quantized._empty_q4(n, k, 32, torch.float32, torch.device("cpu"))

@@ -561,8 +561,8 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
     arrive();
     if (!alive) break;
     const float sv = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
-    // largest value scale so far; a NaN stays in its own page's weights
-    float nv = fmaxf(top_v, sv);
+    // largest finite value scale so far; others stay in their own page's weights
+    float nv = fmaxf(top_v, sv < INFINITY ? sv : 0.f);
     nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 8));
     nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 16));
     nv = fmaxf(nv, 1e-30f);

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   }
   __syncthreads();
   const int blocks = (top_lim + kPreKeys - 1) / kPreKeys;
-  {  // the largest value scale in sight
+  {  // the largest finite value scale in sight
     unsigned int top = 0;
     const int pages = (top_lim + p.page - 1) >> p.page_log;
     for (int i = threadIdx.x; i < pages; i += kPreThreads) {
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         continue;
       }
       const float s = p.vs[(long long)page * p.heads + h];
-      if (s > 0.f) top = max(top, __float_as_uint(s));
+      if (s > 0.f && s < INFINITY) top = max(top, __float_as_uint(s));
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if (lane == 0) atomicMax(&top_scale, top);

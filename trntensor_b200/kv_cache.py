@@ -113,13 +113,15 @@ class KVCache8:
 
     def dequantize(self, pages: torch.Tensor | None = None, *,
                    dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
-        """Keys and values of the given pages (int32 ids; default all) as floats,
+        """Keys and values of the given pages (int32 or int64 ids; default all) as floats,
         each (n, kv_heads, page_size, head_dim)."""
         if dtype not in _TYPES:
             raise ValueError(f"dequantize: dtype must be fp32, bf16 or fp16, got {dtype}")
         if pages is not None:
             if pages.dim() != 1 or pages.dtype not in (torch.int32, torch.int64):
-                raise ValueError("dequantize: pages must be a 1D tensor of int32 ids")
+                raise ValueError("dequantize: pages must be a 1D tensor of int32 or int64 ids")
+            if pages.dtype == torch.int64:  # what int32 cannot hold stays out of range
+                pages = pages.clamp(-1, 2**31 - 1)
             pages = pages.to(self.device, torch.int32).contiguous()
         n = self.num_pages if pages is None else int(pages.shape[0])
         k = torch.empty((n, self.kv_heads, self.page_size, self.head_dim), dtype=dtype,

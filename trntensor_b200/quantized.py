@@ -23,7 +23,7 @@ from .plan import _check_precision, _parse_subscripts, _validate_subscripts
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GROUPS = (32, 64, 128)
 _FEW_ROWS = 8  # up to here no product needs a workspace
-
+_MOST = 2**31 - 1024  # rows or columns: sizes are 32-bit in the library
 
 _HERE = contextlib.nullcontext()
 
@@ -131,6 +131,8 @@ def _on_device(t: torch.Tensor) -> torch.Tensor:
 
 
 def _empty_q4(n: int, k: int, group: int, scale_dtype: torch.dtype, dev: torch.device):
+    if max(n, k) > _MOST:
+        raise ValueError(f"a 4-bit matrix has at most {_MOST} rows and columns, got {(n, k)}")
     lib = _lib.load()
     packed = torch.empty(int(lib.tt_q4_packed_bytes(n, k)), dtype=torch.uint8, device=dev)
     scales = torch.empty(int(lib.tt_q4_scale_count(n, k, group)), dtype=scale_dtype, device=dev)
@@ -198,6 +200,8 @@ def _product(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
     n, k = w.shape
     m, have = x.shape
     cols = k if over_n else n
+    if m > _MOST:
+        raise ValueError(f"q4_matmul: at most {_MOST} rows, got {m}")
     out = x.new_empty((m, cols))
     if m == 0 or cols == 0:
         return out
