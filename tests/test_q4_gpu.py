@@ -269,3 +269,37 @@ def test_same_bits_and_graphs(cuda_ok, m):
         torch.cuda.synchronize()
         for out in (eager, graphs[0][1], graphs[1][1]):
             assert torch.equal(out[0], want) and torch.equal(out[1], back)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp32"])
+@pytest.mark.parametrize("m", [7, 100])
+def test_forward_and_backward_in_a_graph(cuda_ok, m, name):
+    """A captured step replays with new inputs, and with another one in flight between."""
+    codes, scales, _ = make(300, 2000, 64)
+    w = tt.pack_q4(codes.cuda(), scales.cuda(), group=64)
+
+    def step(x, dy):
+        leaf = x.detach().requires_grad_()
+        y = tt.einsum("mk,nk->mn", leaf, w)
+        (dx,) = torch.autograd.grad(y, leaf, dy)
+        return y.detach(), dx
+
+    x, dy = rows(m, 2000, TYPES[name]).cuda(), rows(m, 300, TYPES[name]).cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, dy)
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        got = step(x, dy)
+    for seed in (3, 4):
+        x.copy_(rows(m, 2000, TYPES[name], seed=seed))
+        dy.copy_(rows(m, 300, TYPES[name], seed=seed + 9))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            gr.replay()
+        want = step(x, dy)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    w.check()
