@@ -510,6 +510,16 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
             va[j] = lds128(keys + 4 * (j0 + j) * dim + c * 64);
             vb[j] = lds128(keys + (4 * (j0 + j) + 2) * dim + c * 64);
           }
+          // fp32: an accumulator of these 64 d's own, as for the values below
+          float own[kTerms == 2 ? NT : 1][2][4];
+          if constexpr (kTerms == 2) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) own[a][j][e] = 0.f;
+          }
 #pragma unroll
           for (int w = 0; w < 4; ++w)
 #pragma unroll
@@ -521,8 +531,17 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
               for (int a = 0; a < NT; ++a)
 #pragma unroll
                 for (int k = 0; k < kTerms; ++k)
-                  q4::mma16816<true>(sc[a][j0 + j], a0, a1, a2, a3, qf[a][c * 4 + w][k][0], qf[a][c * 4 + w][k][1]);
+                  q4::mma16816<true>(kTerms == 2 ? own[a % (kTerms == 2 ? NT : 1)][j] : sc[a][j0 + j], a0, a1, a2, a3,
+                                     qf[a][c * 4 + w][k][0], qf[a][c * 4 + w][k][1]);
             }
+          if constexpr (kTerms == 2) {
+#pragma unroll
+            for (int a = 0; a < NT; ++a)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[a][j0 + j][e] += own[a][j][e];
+          }
         }
     }
     const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
