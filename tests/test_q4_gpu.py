@@ -46,6 +46,10 @@ def check(got, x, wide, over_n=False):
     wide_type = x.dtype == torch.float32
     if x.shape[0] <= ((16 if wide_type else 8) if over_n else (8 if wide_type else 32)):
         links = 48 + x.shape[1] / (16 if over_n else 128)
+        if over_n and wide_type:
+            # 12 in the tensor cores, 8 warps, 8 CTAs, and for every 64 of a
+            # warp's rows (an eighth of all) an addition that rounds (half)
+            links = 28 + x.shape[1] / 1024
         loss = links * 2.0**-23 + (2.0**-16 if over_n and x.dtype != torch.float32 else 0)
     elif x.dtype == torch.float32:
         # 16 in the tensor cores, 8 CTAs, and an addition (rounded: half of
@@ -61,7 +65,7 @@ def check(got, x, wide, over_n=False):
     assert worst <= 1.0, worst
 
 
-@pytest.mark.parametrize("m,n,k", [(20, 9600, 2000), (70, 300, 6000), (300, 500, 4100)])
+@pytest.mark.parametrize("m,n,k", [(20, 9600, 2000), (70, 300, 6000), (300, 500, 4100), (2, 14272, 2000), (16, 9600, 300)])
 @pytest.mark.parametrize("scale_dtype", [torch.bfloat16, torch.float32])
 def test_fp32_sums_of_one_sign(cuda_ok, m, n, k, scale_dtype):
     # what an accumulator loses at each addition then adds up

@@ -27,7 +27,7 @@ constexpr int kMaxCluster = 8;
 // Up to so many rows the products run here, above in csrc/q4_gemm.cuh. Measured
 // on both sides with 16384 x 8192 and 4096 x 4096, in us: over k, 32 rows of
 // bf16 40 here and 44 there, 16 rows of fp32 190 and 28 here, 101 and 20 there;
-// over n, 16 rows of bf16 63 and 30 here, 60 and 16 there, of fp32 76 and 32
+// over n, 16 rows of bf16 63 and 30 here, 60 and 16 there, of fp32 68 and 30
 // here, 122 and 23 there.
 int few_rows(int type, bool transposed) { return transposed ? (type == kF32 ? 16 : 8) : type == kF32 ? 8 : 32; }
 
@@ -343,10 +343,12 @@ __device__ __forceinline__ float value_of(uint32_t bits) {
 // for 16-bit types: 2^-16 of each product, against 2^-9 or 2^-12 for the
 // result's own rounding; three for fp32). A fragment of W takes the columns
 // k = 32 w + 8 (c / 2) + 2 j + c % 2 of a block, c = 0 .. 7, for two j, so that
-// all its columns share a group. bf16, one row: 4096 x 4096 10.5 us, 16384 x
-// 8192 36 us (1.9 TB/s): decoding and the doubled products bound it.
+// all its columns share a group. The tensor cores cut off at every addition,
+// which a long sum in fp32 shows (2.4e-6 of the result for 14000 rows): there
+// the fragments are emptied into rounded sums every four row tiles. bf16, one row: 4096 x 4096 9.6 us, 16384 x
+// 8192 35 us (2.0 TB/s): decoding and the doubled products bound it.
 template <typename XT, typename ST, int kTiles, int kGroups>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, kTiles == 1 ? 2 : 1)
 matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restrict__ packed,
                 const ST* __restrict__ scales, int M, int N, int K, int kblocks,
                 XT* __restrict__ dx, long long lddx) {
@@ -413,7 +415,22 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
     };
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) fetch(ring[d]);
+    float whole[kTerms == 3 ? kTiles : 1][8][4] = {};
+    int turn = 0;
     for (int rt0 = blockIdx.x * warps + warp; rt0 < rtiles; rt0 += stride * kDepth) {
+      if constexpr (kTerms == 3) {
+        if (turn++ & 1) {
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                whole[j][i][e] += acc[j][i][e];
+                acc[j][i][e] = 0.f;
+              }
+        }
+      }
 #pragma unroll
       for (int dd = 0; dd < kDepth; ++dd) {
         const int rt = rt0 + dd * stride;  // behind the last: dy counts as zero, and the scale too
@@ -456,6 +473,14 @@ matvec_t_kernel(const XT* __restrict__ dy, long long lddy, const uint4* __restri
           }
         }
       }
+    }
+    if constexpr (kTerms == 3) {
+#pragma unroll
+      for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][i][e] += whole[j][i][e];
     }
   }
   // acc[j][2 w + i]: columns 32 w + 8 (g / 2) + 4 i + g % 2, and 2 on, tokens 8 j + 2 t, 2 t + 1
