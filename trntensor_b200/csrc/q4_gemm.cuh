@@ -456,7 +456,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
 }
 
 // 2^e_n of each row: the exponent that brings its largest finite |s| to
-// 2^11 .. 2^12 when divided by. A row of zeros gets 1.
+// 2^11 .. 2^12 when divided by. A row of zeros gets the smallest: over n the
+// power goes into dy, whose largest product sets the range for all others, and
+// dy of such a row (but for an infinity or NaN) counts for nothing.
 template <typename ST>
 __global__ void row_scale_kernel(const ST* __restrict__ scales, int N, int kblocks, int gpb,
                                  float* __restrict__ out) {
@@ -474,7 +476,7 @@ __global__ void row_scale_kernel(const ST* __restrict__ scales, int N, int kbloc
   }
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
   int e = (int)(top >> 23) - 11;  // biased exponent of 2^e
-  e = top == 0 ? 127 : e < 1 ? 1 : e > 253 ? 253 : e;
+  e = e < 1 ? 1 : e > 253 ? 253 : e;
   const long long n = rt * kRows + (lane & 15);
   if (lane < 16 && n < N) out[n] = __uint_as_float((uint32_t)e << 23);
 }
