@@ -1,4 +1,4 @@
-"""4-bit matrices on the GPU: rows without a scale.
+"""4-bit matrices on the GPU: rows without a scale, forward-mode derivatives.
 
 Tolerances are those of test_q4_gpu.check."""
 
@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 from test_q4_gpu import TYPES, check, make, rows
 
 import trntensor_b200 as tt
@@ -46,3 +47,41 @@ def test_zero_matrix_and_infinities(cuda_ok, m):
         dy[1, 7], dy[2, 39] = float("inf"), float("nan")
         got = tt.q4_matmul(dy, w, over_n=True)
         assert got[1:3].isnan().all() and not got[0].any() and not got[3:].any()
+
+
+@pytest.mark.parametrize("over_n", [False, True])
+@pytest.mark.parametrize("m", [4, 200])
+def test_forward_mode(cuda_ok, m, over_n):
+    """The map is linear: its derivative along t is the product of t."""
+    codes, scales, _ = make(60, 100, 32)
+    w = tt.pack_q4(codes.cuda(), scales.cuda(), group=32)
+    x, t = (rows(m, 60 if over_n else 100, torch.float32, seed=s).cuda() for s in (1, 2))
+    sub = "mn,nk->mk" if over_n else "mk,nk->mn"
+    want, slope = tt.q4_matmul(x, w, over_n=over_n), tt.q4_matmul(t, w, over_n=over_n)
+    for leaf in (x, x.clone().requires_grad_()):
+        with fwd.dual_level():
+            dual = fwd.make_dual(leaf, t)
+            for y in (tt.q4_matmul(dual, w, over_n=over_n), tt.einsum(sub, dual, w),
+                      tt.q4_matmul(dual.view(2, m // 2, -1), w, over_n=over_n).flatten(0, 1)):
+                primal, tangent = fwd.unpack_dual(y)
+                assert tangent is not None and torch.equal(tangent, slope)
+                assert torch.equal(primal, want)
+            with torch.no_grad():
+                assert torch.equal(fwd.unpack_dual(tt.q4_matmul(dual, w, over_n=over_n)).tangent, slope)
+    # forward over backward: the gradient along a moving dy
+    leaf = x.clone().requires_grad_()
+    dy, dt = (rows(m, 100 if over_n else 60, torch.float32, seed=s).cuda() for s in (3, 4))
+    with fwd.dual_level():
+        (dx,) = torch.autograd.grad(tt.q4_matmul(leaf, w, over_n=over_n), leaf, fwd.make_dual(dy, dt))
+        primal, tangent = fwd.unpack_dual(dx)
+    assert torch.equal(primal, tt.q4_matmul(dy, w, over_n=not over_n))
+    assert torch.equal(tangent, tt.q4_matmul(dt, w, over_n=not over_n))
+    # a plain operand inside the level has no tangent
+    with fwd.dual_level():
+        assert fwd.unpack_dual(tt.q4_matmul(x, w, over_n=over_n)).tangent is None
+    # functional transforms are refused, not answered wrongly
+    for call in (lambda: torch.func.jvp(lambda a: tt.q4_matmul(a, w, over_n=over_n), (x,), (t,)),
+                 lambda: torch.func.vmap(lambda a: tt.q4_matmul(a, w, over_n=over_n))(x.view(2, m // 2, -1)),
+                 lambda: torch.func.grad(lambda a: tt.q4_matmul(a, w, over_n=over_n).sum())(x)):
+        with pytest.raises(RuntimeError):
+            call()

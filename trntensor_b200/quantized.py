@@ -15,6 +15,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dispatch import _device, _ptr
@@ -239,9 +240,15 @@ class _Q4Product(torch.autograd.Function):
     def backward(ctx, dy):
         return _dispatch(dy, ctx.w, not ctx.over_n), None, None
 
+    @staticmethod
+    def jvp(ctx, t, *_):  # the map is linear
+        return _dispatch(t, ctx.w, ctx.over_n)
+
 
 def _dispatch(x: torch.Tensor, w: Q4Matrix, over_n: bool) -> torch.Tensor:
-    if x.requires_grad and torch.is_grad_enabled():
+    # a tangent asks for no gradient, and stands without grad mode too
+    if (x.requires_grad and torch.is_grad_enabled()) or (
+            forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None):
         return _Q4Product.apply(x, w, over_n)
     return _product(x.detach() if x.requires_grad else x, w, over_n)
 
@@ -256,7 +263,7 @@ def q4_matmul(x: torch.Tensor, weight: Q4Matrix, *, over_n: bool = False) -> tor
     range by powers of two a row: products are exact where scales are bf16 and
     x is of 16 bits and no smaller than 2^-27 of its row's largest value, else
     they keep 2^-18 (fp32: 2^-20) of themselves and 2^-38 of the largest.
-    Differentiable in x, any number of times. A host x is copied to the
+    Differentiable in x, any number of times and in forward mode. A host x is copied to the
     matrix's device and the result comes back.
     """
     if not isinstance(weight, Q4Matrix):
