@@ -1,0 +1,23 @@
+"""The 8-bit cache without a GPU: what is refused rather than answered in part."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+from test_kv_cpu import append, attend, parts
+
+
+def test_gradients_are_refused():
+    """Nothing here is differentiable: an operand that asks for a gradient is not detached in silence."""
+    p = parts()
+    freq = torch.ones(4, requires_grad=True)
+    for name, call in (("q", attend), ("k", append), ("v", append)):
+        with pytest.raises(ValueError, match=f"^{name} requires grad.*detach"):
+            call(p | {name: p[name].clone().requires_grad_()})
+        with fwd.dual_level():
+            dual = fwd.make_dual(p[name], torch.ones_like(p[name]))
+            with pytest.raises(ValueError, match=f"^{name} has a tangent.*detach"):
+                call(p | {name: dual})
+    with pytest.raises(ValueError, match="inv_freq requires grad"):
+        append(p, inv_freq=freq)

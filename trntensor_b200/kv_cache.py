@@ -21,6 +21,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dispatch import _device
@@ -164,14 +165,21 @@ def _check_table(table: torch.Tensor, batch: int, dev: torch.device) -> torch.Te
     return table if table.stride(1) == 1 else table.contiguous()
 
 
+def _check_underived(x: torch.Tensor, name: str) -> None:
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad, but no gradient is computed here: detach it, or call "
+                         "under torch.no_grad()")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError(f"{name} has a tangent, but no derivative is computed here: detach it")
+
+
 def _check_tokens(x: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
     if x.dim() != 4 or x.dtype not in _TYPES:
         raise ValueError(f"{name} must be fp32, bf16 or fp16 (batch, tokens, heads, head_dim), "
                          f"got {x.dtype} {tuple(x.shape)}")
     if x.device != dev:
         raise ValueError(f"{name} must be on {dev}, got {x.device}")
-    if x.requires_grad:
-        x = x.detach()
+    _check_underived(x, name)
     return x if x.stride(3) == 1 else x.contiguous()
 
 
@@ -180,6 +188,7 @@ def _check_freq(inv_freq: torch.Tensor, dim: int, dev: torch.device) -> torch.Te
             or not 1 <= inv_freq.shape[0] <= dim // 2:
         raise ValueError(f"inv_freq must be fp32 of 1 to {dim // 2} values on {dev}, got "
                          f"{inv_freq.dtype} {tuple(inv_freq.shape)} on {inv_freq.device}")
+    _check_underived(inv_freq, "inv_freq")
     return inv_freq.contiguous()
 
 
@@ -195,7 +204,9 @@ def kv_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
     it grows as tokens come in, and the earlier tokens' codes are then rounded
     onto it. A call that writes a page's first token starts that page anew.
     Rows of the same call may share a page for reading, but a page that is
-    written belongs to one sequence. ``lengths`` is left as it is.
+    written belongs to one sequence. ``lengths`` is left as it is. Codes are
+    integers and have no gradient: a k or v that requires grad is refused where
+    gradients are on.
     """
     dev = cache.device
     k, v = _check_tokens(k, "k", dev), _check_tokens(v, "v", dev)
@@ -224,7 +235,8 @@ def kv_append(cache: KVCache8, k: torch.Tensor, v: torch.Tensor, block_table: to
 def kv_rotate(x: torch.Tensor, lengths: torch.Tensor, inv_freq: torch.Tensor, *,
               interleaved: bool = False) -> torch.Tensor:
     """x (batch, S, heads, head_dim) turned to the positions ``lengths[b] + i``,
-    as :func:`kv_append` turns keys; a new tensor."""
+    as :func:`kv_append` turns keys; a new tensor. Not differentiated: an x that
+    requires grad is refused where gradients are on."""
     dev = x.device
     if dev.type != "cuda":
         raise ValueError(f"kv_rotate: x must be on a CUDA device, got {dev}")
@@ -253,7 +265,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, le
     and sees the tokens up to its own. ``scale`` defaults to
     ``head_dim ** -0.5``. Rows that see no token, and padding rows, are zero.
     Scores, softmax sums and outputs are held in fp32; the result has q's type.
-    There is no gradient: the cache's codes are integers.
+    Nothing here is differentiated: a q that requires grad (or has a tangent) is
+    refused where gradients are on.
     """
     dev = cache.device
     q = _check_tokens(q, "q", dev)
