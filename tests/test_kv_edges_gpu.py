@@ -7,11 +7,104 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_kv_gpu import filled, int32
+from test_kv_gpu import TYPES, attend_case, filled, int32, reference
 
 import trntensor_b200 as tt
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("new", [1, 20, 1300])
+@pytest.mark.parametrize("factor", [1e6, 1e10])
+def test_large_scales_out_of_sight(cuda_ok, factor, new, name):
+    """A page with finite value scales far above the others', which most rows do not see:
+    those rows come out as the definition has them."""
+    kc, ks, vc, vs = filled(12, 2, 16, 64, seed=4)
+    vs[11] *= factor  # tokens 176 .. 191
+    parts = (kc, ks, vc, vs)
+    q = torch.randn(2, new, 8, 64, generator=torch.Generator().manual_seed(new)).to(TYPES[name])
+    table, lengths = [list(range(12))] * 2, [192, 150]
+    cache = tt.KVCache8.from_codes(*(x.cuda() for x in parts))
+    got = tt.kv_attention(q.cuda(), cache, int32(table), int32(lengths)).cpu()
+    cache.check()
+    want, loss = reference(q, parts, table, lengths, [new] * 2, True, 64**-0.5)
+    tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 1.01 * loss + torch.finfo(q.dtype).tiny
+    first = max(0, 176 - (192 - new))  # the first row of sequence 0 that sees it
+    for g, w, t in ((got[0, :first], want[0, :first], tol[0, :first]), (got[1], want[1], tol[1])):
+        assert not ((g.double() - w).abs() > t).any() and g.isfinite().all()
+    if name != "fp16":  # whose range the others leave
+        # a scale's logarithm is up to 2^5 and off by 2^-22 of itself; the exponent it
+        # enters is up to 2^6 and rounded to 2^-18: 2^-16 of a weight in all
+        off = (got.double() - want).abs()
+        assert not (off > tol + 2.0**-16 * want.abs().amax(-1, keepdim=True)).any()
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("new", [1, 6, 1300])
+@pytest.mark.parametrize("ratio", [-24, -34, -44, -70])
+def test_small_scales_with_all_the_weight(cuda_ok, ratio, new, name):
+    """Pages whose value scales are 2^ratio of the largest in sight, and which the
+    attention goes to all the same: what counts is weight times scale."""
+    dim, kv = 64, 1
+    kc, ks, vc, vs = filled(12, kv, 16, dim, seed=6, spread=0.1)
+    small = torch.arange(12) % 2 == 0
+    vs[small] *= 2.0**ratio
+    # scores of the small pages: q.k = 16 x 8 x 127 x ks; of the others 0
+    kc[:, :, :, :16], ks[:] = 127, 0.02
+    kc[:, :, :, 16:] = 0
+    ks[~small] = 0
+    scale = 1.0
+    # e^(-gap) x 2^-ratio is below 2^-24 of the small pages' own sum
+    gap = (30 - ratio) * 0.6931
+    q = torch.zeros(1, new, 4, dim)
+    q[..., :16] = gap / (16 * 127 * 0.02)
+    q = q.to(TYPES[name])
+    parts, table, lengths = (kc, ks, vc, vs), [list(range(12))], [192]
+    cache = tt.KVCache8.from_codes(*(x.cuda() for x in parts))
+    got = tt.kv_attention(q.cuda(), cache, int32(table), int32(lengths), scale=scale, causal=False).cpu().double()
+    s = q[0, 0, 0].double() @ (kc[:, 0].double() * ks[:, 0].double()[:, None, None]).flatten(0, 1).T
+    p = torch.softmax(s, 0)
+    v = (vc[:, 0].double() * vs[:, 0].double()[:, None, None]).flatten(0, 1)
+    want, mass = p @ v, p @ v.abs()
+    # test_kv_gpu's terms; the slack of small weights goes by weight times scale
+    two = name == "fp32"
+    d = (dim / 16 + 20) * 2.0**-23 * float(s.abs().max()) + (2.0**-22 * float(s.abs().max()) if two else 0)
+    loss = ((2.0**-22 if two else 2.0**-11) + 2 * d + 2.0**-20 + (192 / 16 + 64) * 2.0**-22 + 2.0**-16) * mass
+    loss = loss + 192 * 2.0**-28 * float((p[:, None] * v.abs()).max())
+    tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 1.01 * loss + torch.finfo(q.dtype).tiny
+    assert not ((got[0] - want).abs() > tol).any(), ((got[0] - want).abs() / tol).max()
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("dim,page,heads,kv,new,lengths", [
+    (64, 16, 12, 12, 1, [1, 16, 65, 300, 3]), (128, 64, 8, 1, 1, [1000, 64, 9]), (192, 32, 4, 2, 1, [300, 5]),
+    (256, 32, 4, 2, 3, [200, 64]), (80, 32, 6, 2, 5, [40, 5, 130])])
+def test_few_rows_closely(cuda_ok, dim, page, heads, kv, new, lengths, name):
+    """Few rows have their weights held up by 2^14: what is lost of small ones is half of
+    2^-24 of that, 2^-39 of the largest."""
+    got, want = attend_case(name, len(lengths), new, heads, kv, dim, page, lengths, seed=2)
+    g = torch.Generator().manual_seed(2 + dim + page)  # attend_case's inputs
+    pages = len(lengths) * max(1, -(-max(lengths) // page))
+    parts = filled(pages, kv, page, dim, 2)
+    table = torch.randperm(pages, generator=g).view(len(lengths), -1).tolist()
+    q = (torch.randn(len(lengths), new, heads, dim, generator=g) * 2.0).to(TYPES[name])
+    kk, vv = parts[0].double() * parts[1].double()[..., None, None], parts[2].double() * parts[3].double()[..., None, None]
+    two = name == "fp32"
+    for b, n in enumerate(lengths):
+        k, v = (x[table[b]].transpose(0, 1).flatten(1, 2) for x in (kk, vv))
+        for i in range(new):
+            see = n - new + i + 1
+            for h in range(heads if see > 0 else 0):
+                kh, vh, x = k[h // (heads // kv), :see], v[h // (heads // kv), :see], q[b, i, h].double()
+                p = torch.softmax(kh @ x * dim**-0.5, 0)
+                d = (dim / 16 + 20) * 2.0**-23 * float((kh.abs() @ x.abs()).max()) * dim**-0.5
+                if two:
+                    d += 2.0**-22 * float(x.abs().max() * kh.abs().sum(1).max()) * dim**-0.5
+                e = (2.0**-22 if two else 2.0**-11) + 2 * d + 2.0**-20 + (n / 16 + 64) * 2.0**-22
+                tol = (torch.finfo(q.dtype).eps / 2 * want[b, i, h].abs() + 1.01 * e * (p @ vh.abs())
+                       + n * 2.0**-38 * float(p.max() * vh.abs().max()))
+                assert ((got[b, i, h].cpu().double() - want[b, i, h]).abs() <= tol).all()
 
 
 def test_gradients_are_refused(cuda_ok):

@@ -23,8 +23,10 @@
 // row's largest value, 2^-39 of that below) or, for fp32, kept as two fp16
 // terms. The softmax weights are fp16 (2^-11 of each, a quarter of a bf16
 // result's rounding and as much as an fp16 one's; again held up by 2^14), two
-// terms for fp32. Page scales multiply scores and weights in fp32; weights are
-// held relative to the largest value scale seen.
+// terms for fp32. Page scales enter in fp32: keys' into the exponent, and
+// values' too, so that a weight times its value scale is what a row's maximum is
+// of and what is rounded: scales of pages that a row does not see, or gives no
+// weight to, take no bits from the others.
 //
 // Fragments: tokens are the 16-wide side of both products, query rows the
 // 8-wide one. Fragment s of a chunk has the tokens 4 s .. 4 s + 3 of its four
@@ -45,7 +47,7 @@ namespace tt {
 namespace kv8 {
 
 constexpr int kChunk = 64;
-constexpr float kUp = 16384.f;  // the largest fp16 weight of a chunk
+constexpr float kUp = 16384.f, kUpLog = 14.f;  // the largest fp16 weight of a chunk
 
 struct Attend {
   const void* q;
@@ -75,7 +77,7 @@ struct Shape {
   // 4 x 2 189, 6 x 2 190.
   static constexpr int kWarps = DP <= 128 ? 8 : DP == 192 ? 6 : 4;
   static constexpr int kUnit = 16 * DP;
-  static constexpr int kSlot = 4 * (kUnit + 32) + 16;  // four units, and their scales
+  static constexpr int kSlot = 4 * (kUnit + 32) + 32;  // four units; with keys their scales, and the values'
   static constexpr int kSlots = DP == 256 ? 3 : 2;
   static constexpr int kSmem = kWarps * kSlots * kSlot;
   static_assert(kSmem + 1024 <= 227 * 1024, "shared memory of an SM");
@@ -87,10 +89,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
-// Four bytes into shared memory (zeros where not `on`), noted on the barrier
-// when they and all of this lane's earlier ones are there.
-__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool on, uint32_t bar) {
+// Four bytes into shared memory (zeros where not `on`).
+__device__ __forceinline__ void copy_scale(uint32_t dst, const float* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+// Notes on the barrier that all of this lane's earlier copies are there.
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ float lds32(uint32_t a) {
@@ -133,6 +137,31 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   const __half2 rb = __hsub2(reinterpret_cast<const __half2&>(b), bias);
   lo = reinterpret_cast<const uint32_t&>(ra);
   hi = reinterpret_cast<const uint32_t&>(rb);
+}
+// A value scale as 2^lg x odd, with lg in -80 .. 80, and back = 2^-lg / up. lg
+// goes into the exponent of the weights; odd is what is left: 1, or the scale's
+// mantissa where lg is to be exact, and for a scale outside of the range (0,
+// infinity, NaN and what is next to them) the rest of it.
+struct Level {
+  float lg, odd, back;
+};
+template <bool kExact>
+__device__ __forceinline__ Level level_of(float s, float up) {
+  Level v;
+  const float c = fminf(fmaxf(s, 0x1p-80f), 0x1p80f);  // NaN: the least
+  if constexpr (kExact) {
+    const uint32_t e = __float_as_uint(c) >> 23;
+    const float inv = __uint_as_float((254u - e) << 23);
+    v.lg = (float)((int)e - 127);
+    v.odd = s * inv;
+    v.back = inv * (1.f / up);
+  } else {
+    const float inv = __fdividef(1.f, c);
+    asm("lg2.approx.f32 %0, %1;" : "=f"(v.lg) : "f"(c));
+    v.odd = s == c ? 1.f : s * inv;
+    v.back = inv * (1.f / up);
+  }
+  return v;
 }
 // An 8 x 8 matrix of 16-bit values in fragment order, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
@@ -275,7 +304,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   const int dim = p.dim;
   const uint32_t unit_bytes = 16 * dim;
 
-  if (lane < S::kSlots) mbar_init(bar + lane, 1 + 4);  // the units' bytes, and a scale each
+  if (lane < S::kSlots) mbar_init(bar + lane, 1 + 4);  // the units' bytes, and their scales
   fence_mbar_init();
   __syncwarp();
 
@@ -347,7 +376,8 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
     return p.table[x.b * p.table_b + (tok >> p.page_log)];
   };
   uint32_t slot_in = 0;
-  auto ask = [&](const unsigned char* codes, const float* scales, int page, int h, int tok) {
+  // Keys bring both scales with them: the maxima are of scores with the values'.
+  auto ask = [&](const unsigned char* codes, bool keys, int page, int h, int tok) {
     const unsigned has = __ballot_sync(0xffffffffu, page >= 0) & 15u;
     uint64_t* b = bar + slot_in;
     unsigned char* to = mine + slot_in * S::kSlot;
@@ -358,7 +388,11 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
       if (page >= 0)
         bulk_load(smem_u32(to + t * (S::kUnit + 32)),
                   codes + (head * p.page + (tok & (p.page - 1))) * dim, unit_bytes, smem_u32(b));
-      copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 4 * t), scales + head, page >= 0, smem_u32(b));
+      if (keys) {
+        copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 4 * t), p.ks + head, page >= 0);
+        copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 16 + 4 * t), p.vs + head, page >= 0);
+      }
+      copies_arrive(smem_u32(b));
     }
     slot_in = slot_in + 1 == S::kSlots ? 0 : slot_in + 1;
   };
@@ -371,7 +405,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   bool want_values = false;  // the next copy is of values
   auto ask_next = [&]() {
     if (want_values) {
-      ask(p.vc, p.vs, page_v, head_v, tok_v);
+      ask(p.vc, false, page_v, head_v, tok_v);
       want_values = false;
       return;
     }
@@ -384,7 +418,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
     page_v = page_k;
     head_v = ahead.h;
     tok_v = ahead.chunk * kChunk + 16 * t;
-    ask(p.kc, p.ks, page_v, head_v, tok_v);
+    ask(p.kc, true, page_v, head_v, tok_v);
     want_values = true;
     if (left > 0) {
       advance(p, ahead);
@@ -413,10 +447,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
 
   // Of rows 8 i + 2 t + e of the tile: maximum, sum, scale of the scores, tokens
   // that it sees. Sums of values: acc[i][n][e + 2 f] is d 16 n + 8 f + g.
+  // Maxima are of a score in the exponent plus its unit's value scale there.
   float acc[NT][DP / 16][4], m[NT][2], l[NT][2], qs[NT][2];
   int lim[NT][2];
   uint32_t qf[NT][DP / 16][kTerms][2];
-  float top_v = 0.f;
   int lim_min = 0;
   bool fresh = true, whole = true;
 
@@ -485,7 +519,6 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
           for (int e = 0; e < 4; ++e) acc[a][n][e] = 0.f;
       }
       lim_min = __reduce_min_sync(0xffffffffu, lim_min);
-      top_v = 0.f;
     }
 
     // scores: sc[a][s][e + 2 f] is token 16 u + 4 s + 2 f + g % 2, u = g / 2, row 8 a + 2 t + e
@@ -545,6 +578,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
         }
     }
     const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
+    const Level sv = level_of<kTerms == 2>(lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 16 + 4 * (g >> 1)), kUp);
     release();
 
     // The scores are used as they are: scaled by f (at least 0, the same for a
@@ -561,6 +595,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
             if (tok0 + 4 * j + (e & 2) >= lim[a][e & 1]) sc[a][j][e] = -INFINITY;
     }
     float f[NT][2], z[NT][2], old[NT][2];
+    bool same = true;
 #pragma unroll
     for (int a = 0; a < NT; ++a)
 #pragma unroll
@@ -569,53 +604,35 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
         float n = fmaxf(sc[a][0][e], sc[a][0][e + 2]);
 #pragma unroll
         for (int j = 1; j < 4; ++j) n = fmaxf(n, fmaxf(sc[a][j][e], sc[a][j][e + 2]));
-        n = fmaxf(m[a][e], n * f[a][e]);  // a product that is not a number (a hidden unit of scale 0) drops out
+        n = fmaxf(m[a][e], fmaf(n, f[a][e], sv.lg));  // what is not a number (a hidden unit of scale 0) drops out
         n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 4));
         n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 8));
         n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, 16));
         z[a][e] = n == -INFINITY ? 0.f : n;
         old[a][e] = exp2_approx(m[a][e] - z[a][e]);
         m[a][e] = n;
+        same = same && old[a][e] == 1.f;
       }
-    arrive();
-    if (!alive) break;
-    const float sv = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
-    // largest finite value scale so far; others stay in their own page's weights
-    float nv = fmaxf(top_v, sv < INFINITY ? sv : 0.f);
-    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 8));
-    nv = fmaxf(nv, __shfl_xor_sync(0xffffffffu, nv, 16));
-    nv = fmaxf(nv, 1e-30f);
-    const float shrink = __fdividef(top_v, nv), rel = __fdividef(sv, nv) * kUp;
-    top_v = nv;
-    bool same = shrink == 1.f;
-#pragma unroll
-    for (int a = 0; a < NT; ++a) same = same && old[a][0] == 1.f && old[a][1] == 1.f;
     if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
-      for (int a = 0; a < NT; ++a) {
-        const float b0 = old[a][0] * shrink, b1 = old[a][1] * shrink;
+      for (int a = 0; a < NT; ++a)
 #pragma unroll
         for (int n = 0; n < DP / 16; ++n) {
-          acc[a][n][0] *= b0;
-          acc[a][n][1] *= b1;
-          acc[a][n][2] *= b0;
-          acc[a][n][3] *= b1;
+          acc[a][n][0] *= old[a][0];
+          acc[a][n][1] *= old[a][1];
+          acc[a][n][2] *= old[a][0];
+          acc[a][n][3] *= old[a][1];
         }
-      }
     }
-    // Weights times the unit's value scale, 2^(s f - z + log2 rel). Where that
-    // has no logarithm (a unit of scale 0, NaN), or tokens are hidden, the
-    // weight is made first and multiplied after.
+    // Weights times the unit's value scale, and times kUp. What is left of an odd
+    // scale, or an exact one's mantissa, is multiplied after.
     uint32_t w[NT][4][kTerms][2];
-    const bool plain = !mask && __all_sync(0xffffffffu, rel > 1e-30f);
-    float lg, back = 1.f;
-    asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
-    if (plain) back = __fdividef(1.f, rel);
+    const bool plain = !mask && (kTerms == 2 || __all_sync(0xffffffffu, sv.odd == 1.f));
 #pragma unroll
     for (int a = 0; a < NT; ++a) {
       float sum[2] = {0.f, 0.f};
+      const float y0 = (sv.lg + kUpLog) - z[a][0], y1 = (sv.lg + kUpLog) - z[a][1];
       if (plain) {
-        const float y0 = lg - z[a][0], y1 = lg - z[a][1];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -623,6 +640,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
             sc[a][j][e] = exp2_approx(fmaf(sc[a][j][e], f[a][e & 1], e & 1 ? y1 : y0));
           sum[0] += sc[a][j][0] + sc[a][j][2];
           sum[1] += sc[a][j][1] + sc[a][j][3];
+          if constexpr (kTerms == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[a][j][e] *= sv.odd;
+          }
         }
       } else {
 #pragma unroll
@@ -630,9 +651,9 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const bool hidden = mask && tok0 + 4 * j + (e & 2) >= lim[a][e & 1];
-            const float v = hidden ? 0.f : exp2_approx(fmaf(sc[a][j][e], f[a][e & 1], -z[a][e & 1]));
+            const float v = hidden ? 0.f : exp2_approx(fmaf(sc[a][j][e], f[a][e & 1], e & 1 ? y1 : y0));
             sum[e & 1] += v;
-            sc[a][j][e] = hidden ? 0.f : v * rel;
+            sc[a][j][e] = hidden ? 0.f : v * sv.odd;
           }
       }
 #pragma unroll
@@ -647,8 +668,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
         }
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) l[a][e] = l[a][e] * old[a][e] + sum[e] * back;
+      for (int e = 0; e < 2; ++e) l[a][e] = l[a][e] * old[a][e] + sum[e] * sv.back;
     }
+    arrive();
+    if (!alive) break;
     {
       const uint32_t vals = smem_u32(mine + slot * S::kSlot) + t * (S::kUnit + 32) + g * 16;
 #pragma unroll
@@ -711,7 +734,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
           if (none) den = 0.f;
           if (r < p.rows) {
             if (whole && last) {
-              const float inv = den > 0.f || den != den ? top_v / (den * kUp) : 0.f;
+              const float inv = den > 0.f || den != den ? 1.f / (den * kUp) : 0.f;
               T* o = static_cast<T*>(p.o) + row_offset(p, at.b, at.h, r);
 #pragma unroll
               for (int n = 0; n < DP / 16; ++n)
@@ -721,7 +744,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
                 }
             } else {
               // a piece for the joining: slot 0 of a tile that began before, 1 of one that goes on
-              const float back_v = none ? 0.f : top_v / kUp;
+              const float back_v = none ? 0.f : 1.f / kUp;
               float* out = p.part + (((long long)blockIdx.x * S::kWarps + warp) * 2 + (whole ? 1 : 0)) * 16 * rows_of +
                            in_tile * rows_of;
 #pragma unroll

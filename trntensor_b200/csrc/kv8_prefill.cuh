@@ -15,10 +15,13 @@
 // all 256 rows into swizzled fp16 operands (exact). Rows of q are scaled to
 // 2^13..2^14 by a power of two (exact for 16-bit types down to 2^-27 of the
 // row's largest value). Page scales: f = sk x the row's power x scale goes into
-// the exponent; values' scales relative to the sequence's largest one (found
-// first) go into the weights. The maximum m is taken 2^3 above the block's when
-// it is set, moves only when a weight would pass 2^8, and O is rescaled in TMEM
-// only then: weights stay below 2^15, fp16 rounds them by 2^-11, sums are fp32.
+// the exponent, and so do values' scales: a weight is 2^(S f + log2 sv - m), its
+// sum is taken back by 2^-log2 sv, and what a row does not see, or gives no
+// weight to, takes no bits from what it sees. The maximum m (of S f + log2 sv) is
+// taken 2^3 above the block's when it is set, and O is rescaled in TMEM only when
+// it moves: where a weight would pass 2^8, or, in blocks with hidden tokens or odd
+// scales, 1. Weights (times 2^7) stay below 2^15 + 2^3, fp16 rounds them by 2^-11,
+// sums are fp32.
 //
 // What bounds it: for 64 tokens and 256 rows the MMAs take about 1550 clocks
 // (the half of Q in shared memory most of it), the exponentials 1024; the way
@@ -39,7 +42,7 @@ constexpr int kPreThreads = 15 * 32;
 constexpr int kPreKeys = 64;         // tokens of a block
 constexpr int kPreBufs = 4;          // decoded blocks of K and of V
 constexpr int kScaleSlots = 8;       // the copies are at most six blocks ahead of the softmax
-constexpr float kPreUp = 128.f;      // a weight of 1 in P
+constexpr float kPreUp = 128.f, kPreUpLog = 7.f;  // a weight of 1 in P
 constexpr float kPreRoom = 3.f;      // m above the largest score when it is set, and
 constexpr float kPreRise = 8.f;      // a score above m that it bears; both as powers of two
 
@@ -109,11 +112,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       v_empty[kPreBufs], q_ready, last;
   // of tile i, in the phase j % 2 of block j
   __shared__ uint64_t s_full[2], s_free[2], p_full[2], pv_done[2];
-  __shared__ float sc_k[kScaleSlots][kUnits], sc_rel[kScaleSlots][kUnits], sc_log[kScaleSlots][kUnits],
+  // keys' scales, and values' (Level)
+  __shared__ float sc_k[kScaleSlots][kUnits], sc_odd[kScaleSlots][kUnits], sc_log[kScaleSlots][kUnits],
       sc_inv[kScaleSlots][kUnits];
   __shared__ uint32_t tmem_slot;
   __shared__ int dead, top_lim;
-  __shared__ unsigned int top_scale;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dim = kFull ? DP : p.dim, group = p.heads_q / p.heads;
   const int b = blockIdx.z, h = blockIdx.y;
@@ -144,7 +147,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     fence_mbar_init();
     dead = 0;
     top_lim = 0;
-    top_scale = 0;
   }
   if (warp == 13) {
     tmem_alloc(&tmem_slot, 512);
@@ -169,21 +171,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   }
   __syncthreads();
   const int blocks = (top_lim + kPreKeys - 1) / kPreKeys;
-  {  // the largest finite value scale in sight
-    unsigned int top = 0;
-    const int pages = (top_lim + p.page - 1) >> p.page_log;
-    for (int i = threadIdx.x; i < pages; i += kPreThreads) {
-      const int page = p.table[b * p.table_b + i];
-      if (page < 0 || page >= p.pages) {
-        raise(p.status, kBadPage);
-        continue;
-      }
-      const float s = p.vs[(long long)page * p.heads + h];
-      if (s > 0.f && s < INFINITY) top = max(top, __float_as_uint(s));
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) atomicMax(&top_scale, top);
-  }
   if (dim < DP) {  // columns of K and Q behind the head dimension are zeros, for good
     for (int i = threadIdx.x; i < (2 * S::kQ + kPreBufs * S::kKV) / 16; i += kPreThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
@@ -193,7 +180,6 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const float ref = fmaxf(__uint_as_float(top_scale), 1e-30f);
   int* err = &dead;
 
   if (warp == 12) {
@@ -202,16 +188,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       const int tok = j * kPreKeys + 16 * lane, buf = j & 1, phase = (j >> 1) & 1;
       int page = -1;
       if (lane < kUnits && tok < length) page = p.table[b * p.table_b + (tok >> p.page_log)];
-      if (page >= p.pages) page = -1;
+      if (lane < kUnits && tok < length && (page < 0 || page >= p.pages)) {
+        raise(p.status, kBadPage);
+        page = -1;
+      }
       const long long head = (long long)max(page, 0) * p.heads + h;
       if (lane < kUnits) {
         sc_k[j % kScaleSlots][lane] = page >= 0 ? p.ks[head] : 0.f;
-        const float rel = page >= 0 ? __fdividef(p.vs[head], ref) * kPreUp : 0.f;
-        float lg;
-        asm("lg2.approx.f32 %0, %1;" : "=f"(lg) : "f"(rel));
-        sc_rel[j % kScaleSlots][lane] = rel;
-        sc_log[j % kScaleSlots][lane] = lg;
-        sc_inv[j % kScaleSlots][lane] = __fdividef(1.f, rel);
+        const Level sv = level_of<false>(page >= 0 ? p.vs[head] : 0.f, kPreUp);
+        sc_odd[j % kScaleSlots][lane] = sv.odd;
+        sc_log[j % kScaleSlots][lane] = sv.lg;
+        sc_inv[j % kScaleSlots][lane] = sv.back;
       }
       __syncwarp();  // before lane 0's arrival below, which the softmax warps wait behind
       const unsigned has = __ballot_sync(0xffffffffu, page >= 0);
@@ -416,8 +403,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         if (!ok) break;
         tc_fence_after();
         const float* fk = sc_k[j % kScaleSlots];
-        // values' scales relative to the largest, their logarithms and inverses
-        const float* fr = sc_rel[j % kScaleSlots];
+        // values' scales: their logarithms, inverses, and what is left of odd ones
+        const float* fo = sc_odd[j % kScaleSlots];
         const float* fl = sc_log[j % kScaleSlots];
         const float* fi = sc_inv[j % kScaleSlots];
         const int tok0 = j * kPreKeys;
@@ -436,12 +423,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           for (int u = 0; u < kUnits; ++u) {
             const float* x = s[u / 2] + 16 * (u & 1);
             float t[4];
-            plain = plain && fr[u] > 1e-30f;
+            plain = plain && fo[u] == 1.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(x[e], x[e + 4]), fmaxf(x[e + 8], x[e + 12]));
-            n = fmaxf(n, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * (qs * fk[u]));
+            n = fmaxf(n, fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), qs * fk[u], fl[u]));
           }
-          // weights of units without a logarithm of their scale come below
+          // units of odd scales come below
           if (__all_sync(0xffffffffu, plain)) {
             tc_fence_before();
             if (lane == 0) mbar_arrive(&s_free[i]);
@@ -458,7 +445,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
 #pragma unroll
             for (int u = 0; u < kUnits; ++u) {
               float* x = s[u / 2] + 16 * (u & 1);
-              const float f = qs * fk[u], y = fl[u] - m;
+              const float f = qs * fk[u], y = fl[u] + (kPreUpLog - m);
               float q[4];
 #pragma unroll
               for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], f, y));
@@ -496,7 +483,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
               if (tok0 + 32 * c + 16 * u + e < lim) t = fmaxf(t, s[16 * u + e]);
-            n = fmaxf(n, t * (qs * fk[2 * c + u]));  // a hidden unit of scale 0 is not a number, and drops out
+            // a hidden unit of scale 0 is not a number, and drops out
+            n = fmaxf(n, fmaf(t, qs * fk[2 * c + u], fl[2 * c + u]));
           }
         }
         if (j > 0) {  // P of the block before has been read, and O is there to be rescaled
@@ -515,14 +503,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             float* x = s + 16 * u;
-            const float f = qs * fk[2 * c + u], rel = fr[2 * c + u];
+            const float f = qs * fk[2 * c + u], y = fl[2 * c + u] + (kPreUpLog - z), odd = fo[2 * c + u];
+            float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const bool hidden = tok0 + 32 * c + 16 * u + e >= lim;
-              const float y = hidden ? 0.f : exp2_approx(fmaf(x[e], f, -z));
-              l += y;
-              x[e] = hidden ? 0.f : y * rel;
+              const float v = hidden ? 0.f : exp2_approx(fmaf(x[e], f, y));
+              sum += v;
+              x[e] = hidden ? 0.f : v * odd;
             }
+            l = fmaf(sum, fi[2 * c + u], l);
 #pragma unroll
             for (int e = 0; e < 8; ++e) w[c][8 * u + e] = q4::pack_f16(x[2 * e], x[2 * e + 1]);
           }
@@ -542,7 +532,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       tc_fence_after();
     }
     const bool some = lim > 0 && blocks > 0;
-    const float inv = some && (l > 0.f || l != l) ? ref / (l * kPreUp) : 0.f;
+    const float inv = some && (l > 0.f || l != l) ? 1.f / (l * kPreUp) : 0.f;
     for (int c = 0; c < dim; c += 16) {
       float o[16];
       if (blocks > 0 && i < tiles) {
