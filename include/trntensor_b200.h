@@ -348,7 +348,7 @@ int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed,
 
 /*
  * Paged key-value cache held in 8 bits: x^ = s c, c in -127..127 stored biased
- * by 128, one fp32 scale for each page and head. A page holds `page` tokens
+ * by 128, one fp32 scale (not negative) for each page and head. A page holds `page` tokens
  * (16, 32, 64 or 128) of all `heads` heads of `dim` values (a multiple of 16,
  * at most 256):
  *   k_codes [pages][heads][page][dim]
@@ -357,9 +357,10 @@ int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed,
  * (16-byte aligned). block_table (batch rows of `columns` page ids, row stride
  * table_stride) gives the page of each sequence's tokens page by page.
  * Lengths, counts, tables and the status word live on the device; the kernels
- * leave out what points outside the cache and OR a bit into *status: 1 a page
- * id outside the cache, 2 a length or count out of range, 4 one append that
- * writes a page for two places, 8 a copy that never arrived. Activations are
+ * leave out what points outside the cache (attention: its tokens are not there)
+ * and OR a bit into *status: 1 a page id outside the cache, 2 a length or count
+ * out of range, 4 one append that writes a page for two places, 8 a copy that
+ * never arrived. Activations are
  * fp32, bf16 or fp16 (types as above) with strides in elements over (batch,
  * token, head) and neighbouring values in a head.
  */

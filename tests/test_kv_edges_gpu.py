@@ -77,6 +77,41 @@ def test_small_scales_with_all_the_weight(cuda_ok, ratio, new, name):
 
 
 @pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("new,causal", [(1, True), (20, True), (1300, True), (7, False), (1300, False)])
+def test_pages_outside_are_left_out(cuda_ok, new, causal, name):
+    """Tokens of a page that the cache does not have are not there: no weight, wherever
+    they stand, and a row that has no others is zero."""
+    pages, page, kv, dim = 12, 16, 2, 64
+    parts = filled(pages, kv, page, dim, seed=8)
+    parts[0].abs_()  # all scores are well below 0: a token of score 0 would have all the weight
+    q = -torch.rand(3, new, 8, dim, generator=torch.Generator().manual_seed(new)).to(TYPES[name]) - 0.5
+    wrong = {1: pages, 4: -1, 5: 2**31 - 1, 9: -2**31}
+    table = [[wrong.get(i, i) for i in range(12)], [wrong.get(i, i) for i in range(12)], [-1] * 12]
+    lengths = [12 * page - 3, 5 * page, 40]
+    cache = tt.KVCache8.from_codes(*(x.cuda() for x in parts))
+    got = tt.kv_attention(q.cuda(), cache, int32(table), int32(lengths), causal=causal)
+    with pytest.raises(ValueError, match="page id"):
+        cache.check()
+    # the definition over the tokens that are there: rows by the last of those that they see
+    there = [[t for t in range(n) if 0 <= table[b][t // page] < pages] for b, n in enumerate(lengths)]
+    ids = [i for i in range(12) if i not in wrong]
+    for b in range(3):
+        first = lengths[b] - new
+        by_seen = {}
+        for i in range(new):
+            by_seen.setdefault(sum(t <= first + i for t in there[b]) if causal else len(there[b]), []).append(i)
+        for seen, rows in by_seen.items():
+            if seen == 0:
+                assert not got[b, rows].any()
+                continue
+            # sequence b's own tokens stand side by side in the pages `ids`
+            want, loss = reference(q[b:b + 1, rows], parts, [ids], [seen], [len(rows)], False, dim**-0.5)
+            tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 1.01 * loss + torch.finfo(q.dtype).tiny
+            off = (got[b:b + 1, rows].cpu().double() - want).abs()
+            assert not (off > tol).any() and not off.isnan().any(), (b, seen, (off / tol).max())
+
+
+@pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("dim,page,heads,kv,new,lengths", [
     (64, 16, 12, 12, 1, [1, 16, 65, 300, 3]), (128, 64, 8, 1, 1, [1000, 64, 9]), (192, 32, 4, 2, 1, [300, 5]),
     (256, 32, 4, 2, 3, [200, 64]), (80, 32, 6, 2, 5, [40, 5, 130])])

@@ -47,6 +47,7 @@ namespace tt {
 namespace kv8 {
 
 constexpr int kChunk = 64;
+constexpr int kNever = 0x7fffff00;  // behind the last token that any row sees (lengths are at most this)
 constexpr float kUp = 16384.f, kUpLog = 14.f;  // the largest fp16 weight of a chunk
 
 struct Attend {
@@ -82,6 +83,9 @@ struct Shape {
   static constexpr int kSmem = kWarps * kSlots * kSlot;
   static_assert(kSmem + 1024 <= 227 * 1024, "shared memory of an SM");
 };
+
+// The key scale of a unit whose page is outside the cache: its tokens are hidden.
+__device__ const float kGone = -1.f;
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   };
   uint32_t slot_in = 0;
   // Keys bring both scales with them: the maxima are of scores with the values'.
-  auto ask = [&](const unsigned char* codes, bool keys, int page, int h, int tok) {
+  auto ask = [&](const unsigned char* codes, bool keys, bool gone, int page, int h, int tok) {
     const unsigned has = __ballot_sync(0xffffffffu, page >= 0) & 15u;
     uint64_t* b = bar + slot_in;
     unsigned char* to = mine + slot_in * S::kSlot;
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
         bulk_load(smem_u32(to + t * (S::kUnit + 32)),
                   codes + (head * p.page + (tok & (p.page - 1))) * dim, unit_bytes, smem_u32(b));
       if (keys) {
-        copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 4 * t), p.ks + head, page >= 0);
+        copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 4 * t), gone ? &kGone : p.ks + head, gone || page >= 0);
         copy_scale(smem_u32(to + 4 * (S::kUnit + 32) + 16 + 4 * t), p.vs + head, page >= 0);
       }
       copies_arrive(smem_u32(b));
@@ -403,22 +407,25 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   // asked for last.
   int page_k = page_at(ahead), page_v = -1, head_v = 0, tok_v = 0;
   bool want_values = false;  // the next copy is of values
+  bool lost = false;         // a page outside the cache has come by: from there on, tokens are looked at one by one
   auto ask_next = [&]() {
     if (want_values) {
-      ask(p.vc, false, page_v, head_v, tok_v);
+      ask(p.vc, false, false, page_v, head_v, tok_v);
       want_values = false;
       return;
     }
     if (left == 0) return;
     --left;
-    if (page_k >= p.pages || (page_k < 0 && ahead.chunk * kChunk + 16 * t < (int)ahead.length)) {
-      if (g == 0) raise(p.status, kBadPage);
-      page_k = -1;
+    const bool gone = page_k >= p.pages || (page_k < 0 && ahead.chunk * kChunk + 16 * t < (int)ahead.length);
+    if (__any_sync(0xffffffffu, gone)) {
+      lost = true;
+      if (gone && g == 0) raise(p.status, kBadPage);
+      if (gone) page_k = -1;
     }
     page_v = page_k;
     head_v = ahead.h;
     tok_v = ahead.chunk * kChunk + 16 * t;
-    ask(p.kc, true, page_v, head_v, tok_v);
+    ask(p.kc, true, gone, page_v, head_v, tok_v);
     want_values = true;
     if (left > 0) {
       advance(p, ahead);
@@ -577,14 +584,16 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
           }
         }
     }
-    const float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
+    float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
+    const bool gone = sk < 0.f;
+    if (gone) sk = 0.f;
     const Level sv = level_of<kTerms == 2>(lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 16 + 4 * (g >> 1)), kUp);
     release();
 
     // The scores are used as they are: scaled by f (at least 0, the same for a
     // lane's whole unit) only inside the exponent.
-    const int tok0 = at.chunk * kChunk + 16 * (g >> 1) + (g & 1);
-    const bool mask = (at.chunk + 1) * kChunk > lim_min;
+    const int tok0 = gone ? kNever : at.chunk * kChunk + 16 * (g >> 1) + (g & 1);
+    const bool mask = (at.chunk + 1) * kChunk > lim_min || lost;
     if (mask) {
 #pragma unroll
       for (int a = 0; a < NT; ++a)

@@ -188,13 +188,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
       const int tok = j * kPreKeys + 16 * lane, buf = j & 1, phase = (j >> 1) & 1;
       int page = -1;
       if (lane < kUnits && tok < length) page = p.table[b * p.table_b + (tok >> p.page_log)];
-      if (lane < kUnits && tok < length && (page < 0 || page >= p.pages)) {
+      const bool gone = lane < kUnits && tok < length && (page < 0 || page >= p.pages);
+      if (gone) {
         raise(p.status, kBadPage);
         page = -1;
       }
       const long long head = (long long)max(page, 0) * p.heads + h;
       if (lane < kUnits) {
-        sc_k[j % kScaleSlots][lane] = page >= 0 ? p.ks[head] : 0.f;
+        sc_k[j % kScaleSlots][lane] = page >= 0 ? p.ks[head] : gone ? kGone : 0.f;
         const Level sv = level_of<false>(page >= 0 ? p.vs[head] : 0.f, kPreUp);
         sc_odd[j % kScaleSlots][lane] = sv.odd;
         sc_log[j % kScaleSlots][lane] = sv.lg;
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
             for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(x[e], x[e + 4]), fmaxf(x[e + 8], x[e + 12]));
             n = fmaxf(n, fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), qs * fk[u], fl[u]));
           }
-          // units of odd scales come below
+          // units of odd scales, and those that are not there (their values' scale is 0), come below
           if (__all_sync(0xffffffffu, plain)) {
             tc_fence_before();
             if (lane == 0) mbar_arrive(&s_free[i]);
@@ -479,12 +480,14 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           tmem_ld_wait();
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
+            const float sk = fk[2 * c + u];
+            const int end = sk < 0.f ? 0 : lim;  // nothing is seen of a page that is not there
             float t = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              if (tok0 + 32 * c + 16 * u + e < lim) t = fmaxf(t, s[16 * u + e]);
+              if (tok0 + 32 * c + 16 * u + e < end) t = fmaxf(t, s[16 * u + e]);
             // a hidden unit of scale 0 is not a number, and drops out
-            n = fmaxf(n, fmaf(t, qs * fk[2 * c + u], fl[2 * c + u]));
+            n = fmaxf(n, fmaf(t, qs * (sk < 0.f ? 0.f : sk), fl[2 * c + u]));
           }
         }
         if (j > 0) {  // P of the block before has been read, and O is there to be rescaled
@@ -504,10 +507,11 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           for (int u = 0; u < 2; ++u) {
             float* x = s + 16 * u;
             const float f = qs * fk[2 * c + u], y = fl[2 * c + u] + (kPreUpLog - z), odd = fo[2 * c + u];
+            const int end = fk[2 * c + u] < 0.f ? 0 : lim;
             float sum = 0.f;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const bool hidden = tok0 + 32 * c + 16 * u + e >= lim;
+              const bool hidden = tok0 + 32 * c + 16 * u + e >= end;
               const float v = hidden ? 0.f : exp2_approx(fmaf(x[e], f, y));
               sum += v;
               x[e] = hidden ? 0.f : v * odd;
