@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_kv_gpu import TYPES, attend_case, filled, int32, reference
+from test_kv_gpu import TYPES, Ref, attend_case, filled, int32, reference
 
 import trntensor_b200 as tt
 
@@ -140,6 +140,26 @@ def test_few_rows_closely(cuda_ok, dim, page, heads, kv, new, lengths, name):
                 tol = (torch.finfo(q.dtype).eps / 2 * want[b, i, h].abs() + 1.01 * e * (p @ vh.abs())
                        + n * 2.0**-38 * float(p.max() * vh.abs().max()))
                 assert ((got[b, i, h].cpu().double() - want[b, i, h]).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("top", [1, 63, 64, 100, 190, 191, 500, 127 * 127])
+def test_append_of_subnormals(cuda_ok, top):
+    """Values of a few times 2^-149: the page's scale is so coarse that a value can be more
+    than 127 of it, and codes stop at 127."""
+    step = 2.0**-149
+    cache = tt.KVCache8(2, 1, 32, page_size=16)
+    ref = Ref(cache)
+    at = 0
+    for factor in (1, 2, 1):
+        x = torch.linspace(-top * factor, top * factor, 5 * 32).round().view(1, 5, 1, 32).double().mul(step).float()
+        assert float(x.abs().max()) > 0
+        tt.kv_append(cache, x.cuda(), -x.cuda(), int32([[1]]), int32([at]))
+        ref.append(x.numpy(), 0, [[1]], [at], [5])
+        ref.append(-x.numpy(), 1, [[1]], [at], [5])
+        ref.same(cache)
+        at += 5
+    assert min(c.min().item() for c in cache.codes()) >= -127
+    cache.check()
 
 
 def test_gradients_are_refused(cuda_ok):

@@ -47,8 +47,10 @@ struct Append {
 // Four codes rint(x / s) + 128 as bytes, as the division rounds them: x times
 // the reciprocal is off by 127 2^-22 at most, so it decides unless it comes
 // that near to a half; then, and for scales with no finite reciprocal, the
-// division itself is made. |x| <= 127 s, so that codes need no clamping.
-// Adding 1.5 2^23 rounds to an integer, which then is the low byte.
+// division itself is made. |x| <= 127 s up to a rounding of s, so that codes need
+// no clamping but where s is subnormal and that rounding large: a few units of
+// 2^-149 for values of up to 190 such units. Adding 1.5 2^23 rounds to an
+// integer, which then is the low byte.
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float s, float inv, bool tiny) {
   constexpr float kRound = 12582912.f;
   uint32_t q[4];
@@ -62,7 +64,8 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float s, float
   if (near) {
 #pragma unroll 1
     for (int e = 0; e < 4; ++e) {
-      const uint32_t r = __float_as_uint(__fdiv_rn(e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3], s) + kRound);
+      const float y = __fdiv_rn(e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3], s);
+      const uint32_t r = __float_as_uint(fminf(fmaxf(y, -127.f), 127.f) + kRound);
       if (e == 0) q[0] = r;
       else if (e == 1) q[1] = r;
       else if (e == 2) q[2] = r;
