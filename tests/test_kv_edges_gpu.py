@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_kv_gpu import TYPES, Ref, attend_case, filled, int32, reference
+from test_kv_gpu import TYPES, Ref, attend_case, filled, int32, reference, turned
 
 import trntensor_b200 as tt
 
@@ -160,6 +160,50 @@ def test_append_of_subnormals(cuda_ok, top):
         at += 5
     assert min(c.min().item() for c in cache.codes()) >= -127
     cache.check()
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("page,dim,half", [(32, 128, 64), (64, 192, 96), (128, 256, 128), (128, 256, 100),
+                                           (64, 192, 33), (128, 80, 18), (16, 256, 128)])
+def test_rotation_in_every_page(cuda_ok, page, dim, half, aligned, interleaved, name):
+    """Rotation beyond a page's first sixteen tokens and a head's first 128 values, with
+    tokens that cannot be read sixteen bytes at a time."""
+    g = torch.Generator().manual_seed(dim + page)
+    new, start, kv = 2 * page + 21, [page - 3, 5], 2
+    freq = (10000.0 ** (-torch.arange(half) / half)).float()
+    wide = torch.randn(2, new, kv, dim + 1, generator=g).to(TYPES[name]).cuda()
+    k = wide[..., 1:]
+    if aligned:
+        k = k.contiguous()
+    v = -k
+    cols = (page + new) // page + 1
+    cache = tt.KVCache8(2 * cols, kv, dim, page_size=page)
+    table = torch.randperm(2 * cols, generator=g).view(2, cols)
+    lengths = int32(start)
+    tt.kv_append(cache, k, v if aligned else (-wide)[..., 1:], table.int().cuda(), lengths, inv_freq=freq.cuda(),
+                 interleaved=interleaved)
+    cache.check()
+    pos = torch.tensor(start)[:, None] + torch.arange(new)
+    x = k.cpu().double()
+    want = turned(x, pos.double(), freq, interleaved)
+    got = tt.kv_rotate(k, lengths, freq.cuda(), interleaved=interleaved).cpu().double()
+    # the angle to 2^-23 turns of a half circle, the sine and the sum to a few units, a rounding
+    eps = 2.0**-20 * x.abs().max()
+    assert ((got - want).abs() <= eps + torch.finfo(TYPES[name]).eps / 2 * want.abs()).all()
+    keys, values = (y.cpu().double() for y in cache.dequantize())
+    ks, vs = cache.k_scales.cpu().double(), cache.v_scales.cpu().double()
+    for b in range(2):
+        home, slot = table[b][pos[b] // page], pos[b] % page
+        off = (keys[home, :, slot] - want[b]).abs()
+        assert (off <= 0.5001 * ks[home][..., None] + 2 * eps).all()
+        # a page's scale is its largest value / 127
+        for p in home.unique():
+            top = want[b][home == p].abs().amax((0, 2))
+            assert ((ks[p] * 127 - top).abs() <= 2 * eps).all()
+        off = (values[home, :, slot] + x[b]).abs()
+        assert (off <= 0.5001 * vs[home][..., None]).all()
 
 
 def test_gradients_are_refused(cuda_ok):
