@@ -162,6 +162,17 @@ def test_append_of_subnormals(cuda_ok, top):
     cache.check()
 
 
+def test_sequences_that_add_nothing_share_pages(cuda_ok):
+    """A sequence without new tokens writes nothing: the page of its last token may be
+    another's to write."""
+    k = torch.randn(3, 4, 1, 16, device="cuda")
+    for counts, wrong in (([4, 0, 0], False), ([4, 0, 4], True), ([0, 0, 0], False), ([4, -1, 0], False)):
+        cache = tt.KVCache8(4, 1, 16, page_size=16)
+        tt.kv_append(cache, k, k, int32([[2, 0], [2, 1], [2, 3]]), int32([5, 5, 5]), n_new=int32(counts))
+        code = int(cache.status.item())
+        assert bool(code & 4) == wrong and bool(code & 2) == (min(counts) < 0), (counts, code)
+
+
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("aligned", [True, False])

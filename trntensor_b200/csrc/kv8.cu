@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const Append p) {
       const int o = (int)(i / gridDim.x);
       const long long so = p.lengths[o], no = min((long long)(p.n_new ? p.n_new[o] : p.S), (long long)p.S);
       const long long c = so / p.page + i % gridDim.x;
-      if (so >= 0 && c * p.page < so + no && c < p.cols && !(o == b && c == col) &&
+      // a sequence that adds nothing writes no page
+      if (so >= 0 && no > 0 && c * p.page < so + no && c < p.cols && !(o == b && c == col) &&
           p.table[o * p.table_b + c] == page)
         raise(p.status, kSharedPage);
     }
