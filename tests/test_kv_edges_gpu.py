@@ -173,6 +173,36 @@ def test_sequences_that_add_nothing_share_pages(cuda_ok):
         assert bool(code & 4) == wrong and bool(code & 2) == (min(counts) < 0), (counts, code)
 
 
+@pytest.mark.parametrize("batch,new,page", [(3, 40, 16), (64, 600, 16), (5, 12000, 16), (2, 8191, 128)])
+def test_shared_pages_are_found(cuda_ok, batch, new, page):
+    """One page twice among few and among thousands, anywhere; and none where there is none."""
+    cols = -(-(new + 7) // page)
+    pages = batch * cols + 5
+    k = torch.zeros(batch, new, 1, 16, device="cuda", dtype=torch.bfloat16)
+    cache = tt.KVCache8(pages, 1, 16, page_size=page)
+    good = torch.randperm(pages, generator=torch.Generator().manual_seed(batch))[:batch * cols].view(batch, cols).int()
+    start = int32([7 * (b % 2) for b in range(batch)])
+    tt.kv_append(cache, k, k, good.cuda(), start)
+    cache.check()
+    last = (new - 1) // page
+    for (b, c), (o, d) in (((0, 0), (batch - 1, last)), ((1, last), (1, 0)), ((0, last // 2), (1, last // 2))):
+        table = good.clone()
+        table[b, c] = table[o, d]
+        tt.kv_append(cache, k, k, table.cuda(), start)
+        with pytest.raises(ValueError, match="two places"):
+            cache.check()
+    # a page that stands twice behind what is written, and ids that are not there, are no sharing
+    table = torch.cat((good, good[:1, :1].expand(batch, 2)), 1)
+    tt.kv_append(cache, k, k, table.cuda(), start)
+    cache.check()
+    table = good.clone()
+    table[:2, 0] = pages
+    tt.kv_append(cache, k, k, table.cuda(), start)
+    with pytest.raises(ValueError, match="page id") as wrong:
+        cache.check()
+    assert "two places" not in str(wrong.value)
+
+
 @pytest.mark.parametrize("name", list(TYPES))
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("aligned", [True, False])
@@ -237,3 +267,21 @@ def test_gradients_are_refused(cuda_ok):
     with torch.inference_mode():
         tt.kv_append(cache, k, k, table, lengths)
     cache.check()
+
+
+def test_shared_pages_of_a_large_cache(cuda_ok):
+    """More page ids than one search has bits for."""
+    pages, batch, new = 600_000, 2, 4096
+    cols = new // 16
+    cache = tt.KVCache8(pages, 1, 16, page_size=16)
+    k = torch.zeros(batch, new, 1, 16, device="cuda", dtype=torch.bfloat16)
+    good = torch.arange(batch * cols).mul(1171).view(batch, cols).int()  # 0 .. 598381, all parts
+    assert int(good.max()) < pages
+    tt.kv_append(cache, k, k, good.cuda(), int32([0, 0]))
+    cache.check()
+    for a, b in ((0, batch * cols - 1), (100, 101), (batch * cols - 1, batch * cols - 2), (230, 5)):
+        table = good.flatten().clone()
+        table[a] = table[b]
+        tt.kv_append(cache, k, k, table.view(batch, cols).cuda(), int32([0, 0]))
+        with pytest.raises(ValueError, match="two places"):
+            cache.check()

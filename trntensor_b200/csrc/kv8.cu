@@ -24,6 +24,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kTableBytes = 128 * 128 * 8;  // cos and sin of a page's tokens, at most
+// Page ids that a CTA's bits cover when it looks for pages written twice, and
+// pages of a call (counted by its grid) up to which they are compared in pairs
+// (one token for each of 64 sequences: 4.6 us, with bits 4.8; 272 pages 13.3 with
+// either; 512 sequences 12.3 and 11.3; 32832 pages 4116 and 390).
+constexpr int kBitsPages = 1 << 18;
+constexpr int kPairs = 256;
+static_assert(kBitsPages / 8 <= kWarps * 16 * 128 * 2, "the bits fit where the least staged tokens lie");
 
 struct Append {
   const void* k;
@@ -273,16 +280,67 @@ __device__ __forceinline__ void put(const Append& p, const Tokens<kTurn, T>& in,
     }
 }
 
+// Pages that the call writes for two places, where there are too many to compare
+// each with each: a bit for each page id of a part of them, which finds its
+// second setting. A thread asks for four pages of the call's grid at a time.
+__device__ __forceinline__ void find_shared(const Append& p, uint32_t* bits, int part) {
+  const int first = part * kBitsPages, ids = min(kBitsPages, p.pages - first), shift = 31 - __clz(p.page);
+  for (int i = threadIdx.x; i < (ids + 31) / 32; i += kThreads) bits[i] = 0;
+  __syncthreads();
+  const unsigned most = gridDim.x, step_b = kThreads / most, step_c = kThreads % most;
+  unsigned b = threadIdx.x / most, c = threadIdx.x % most;  // the sequence, and the column behind its first
+  bool twice = false;
+  while (b < (unsigned)p.batch) {
+    int start[4], count[4], id[4];
+    unsigned at_b[4], at_c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      at_b[i] = b;
+      at_c[i] = c;
+      const bool in = b < (unsigned)p.batch;
+      start[i] = in ? p.lengths[b] : -1;
+      count[i] = in && p.n_new ? p.n_new[b] : p.S;
+      b += step_b;
+      c += step_c;
+      if (c >= most) {
+        c -= most;
+        ++b;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long col = ((long long)start[i] >> shift) + at_c[i], end = (long long)start[i] + min(count[i], p.S);
+      // a sequence that adds nothing writes no page
+      const bool in = start[i] >= 0 && count[i] > 0 && col << shift < end && col < p.cols;
+      id[i] = in ? p.table[at_b[i] * p.table_b + col] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (id[i] < first || id[i] - first >= ids) continue;
+      const uint32_t at = id[i] - first, bit = 1u << (at & 31);
+      twice |= (atomicOr(bits + at / 32, bit) & bit) != 0;
+    }
+  }
+  if (twice) raise(p.status, kSharedPage);
+  __syncthreads();
+}
+
 // A warp takes a page of a sequence, a head, and keys or values. The CTA's
 // warps are neighbouring heads, which share the table of cosines; the CTAs of
-// the last y look for pages that the call writes for two places.
+// the last y look for pages that the call writes for two places: each compares
+// its own with all others or, where they are many (kMany), the first few go over
+// all with bits in shared memory.
 // Bound by bytes: k and v read once from HBM, codes written once.
-template <typename T>
+template <typename T, bool kMany>
 __global__ void __launch_bounds__(kThreads, 4) append_kernel(const Append p) {
   extern __shared__ __align__(16) unsigned char append_smem[];
   float2* table = reinterpret_cast<float2*>(append_smem + kWarps * kRowTokens * kRowValues * sizeof(T));  // [token][pair]
   const int b = blockIdx.z, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const bool look = blockIdx.y + 1 == gridDim.y;
+  const long long all = (long long)p.batch * gridDim.x;
+  if (kMany && look)
+    for (long long part = (long long)blockIdx.z * gridDim.x + blockIdx.x; part * kBitsPages < p.pages; part += all)
+      find_shared(p, reinterpret_cast<uint32_t*>(append_smem), (int)part);
   const long long start = p.lengths[b];
   long long count = p.n_new ? p.n_new[b] : p.S;
   if (start < 0 || count < 0 || count > p.S || start + count > (long long)p.cols * p.page) {
@@ -299,8 +357,7 @@ __global__ void __launch_bounds__(kThreads, 4) append_kernel(const Append p) {
       if (threadIdx.x == 0) raise(p.status, kBadPage);
       return;
     }
-    const long long all = (long long)p.batch * gridDim.x;
-    for (long long i = threadIdx.x; i < all; i += kThreads) {
+    for (long long i = threadIdx.x; !kMany && i < all; i += kThreads) {
       const int o = (int)(i / gridDim.x);
       const long long so = p.lengths[o], no = min((long long)(p.n_new ? p.n_new[o] : p.S), (long long)p.S);
       const long long c = so / p.page + i % gridDim.x;
@@ -452,16 +509,26 @@ bool good_shape(int pages, int heads, int page, int dim) {
          (page == 16 || page == 32 || page == 64 || page == 128) && dim >= 16 && dim <= 256 && dim % 16 == 0;
 }
 
+template <typename T>
+bool set_append(int bytes) {
+  const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  return cudaFuncSetAttribute(append_kernel<T, false>, at, bytes) == cudaSuccess &&
+         cudaFuncSetAttribute(append_kernel<T, true>, at, bytes) == cudaSuccess;
+}
+template <typename T>
+int run_append(const Append& p, dim3 grid, int smem, cudaStream_t s) {
+  if ((long long)p.batch * grid.x > kPairs) append_kernel<T, true><<<grid, kThreads, smem, s>>>(p);
+  else append_kernel<T, false><<<grid, kThreads, smem, s>>>(p);
+  return cuda_status(cudaGetLastError());
+}
+
 std::once_flag g_flags[kMaxDevices];
 int g_ok[kMaxDevices];
 
 int setup(int dev) {
   return once_per_device(g_flags, g_ok, dev, []() -> int {
     const int bytes = kTableBytes + kWarps * kRowTokens * kRowValues * 4;
-    const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if (cudaFuncSetAttribute(append_kernel<float>, at, bytes) != cudaSuccess ||
-        cudaFuncSetAttribute(append_kernel<__nv_bfloat16>, at, bytes) != cudaSuccess ||
-        cudaFuncSetAttribute(append_kernel<__half>, at, bytes) != cudaSuccess)
+    if (!set_append<float>(bytes) || !set_append<__nv_bfloat16>(bytes) || !set_append<__half>(bytes))
       return TT_ERR_CUDA;
     return TT_OK;
   });
@@ -509,10 +576,9 @@ int tt_kv8_append(const void* k, const void* v, int type, long long k_stride_b, 
   p.wide = aligned16(k) && aligned16(v) && k_stride_b % per == 0 && k_stride_s % per == 0 && k_stride_h % per == 0 &&
            v_stride_b % per == 0 && v_stride_s % per == 0 && v_stride_h % per == 0;
   cudaStream_t s = (cudaStream_t)stream;
-  if (type == q4::kF32) kv8::append_kernel<float><<<grid, kv8::kThreads, smem, s>>>(p);
-  else if (type == q4::kBF16) kv8::append_kernel<__nv_bfloat16><<<grid, kv8::kThreads, smem, s>>>(p);
-  else kv8::append_kernel<__half><<<grid, kv8::kThreads, smem, s>>>(p);
-  return cuda_status(cudaGetLastError());
+  if (type == q4::kF32) return kv8::run_append<float>(p, grid, smem, s);
+  if (type == q4::kBF16) return kv8::run_append<__nv_bfloat16>(p, grid, smem, s);
+  return kv8::run_append<__half>(p, grid, smem, s);
 }
 
 int tt_kv8_rotate(const void* x, int type, long long stride_b, long long stride_s, long long stride_h,
