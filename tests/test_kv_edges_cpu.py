@@ -7,6 +7,8 @@ import torch
 import torch.autograd.forward_ad as fwd
 from test_kv_cpu import append, attend, parts
 
+from trntensor_b200 import kv_cache
+
 
 def test_gradients_are_refused():
     """Nothing here is differentiable: an operand that asks for a gradient is not detached in silence."""
@@ -21,3 +23,22 @@ def test_gradients_are_refused():
                 call(p | {name: dual})
     with pytest.raises(ValueError, match="inv_freq requires grad"):
         append(p, inv_freq=freq)
+
+
+def test_a_failed_size_is_asked_for_again(monkeypatch):
+    """One failure to get the workspace's size is an error then, and not for good."""
+    class Lib:
+        sizes = [0, 4096]
+
+        def tt_kv8_attention_workspace_bytes(self, dim):
+            return self.sizes.pop(0)
+
+        def tt_last_cuda_error(self):
+            return b"device busy"
+
+    monkeypatch.setattr(kv_cache, "_WORKSPACE", {})
+    lib, dev = Lib(), torch.device("cuda", 3)
+    with pytest.raises(RuntimeError, match="device busy"):
+        kv_cache._workspace_bytes(lib, dev, 64)
+    assert kv_cache._workspace_bytes(lib, dev, 64) == 4096
+    assert kv_cache._workspace_bytes(lib, dev, 64) == 4096 and not lib.sizes

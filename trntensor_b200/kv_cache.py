@@ -254,6 +254,18 @@ def kv_rotate(x: torch.Tensor, lengths: torch.Tensor, inv_freq: torch.Tensor, *,
     return out
 
 
+def _workspace_bytes(lib, dev: torch.device, dim: int) -> int:
+    """Workspace of an attention on the current device ``dev``; a size is kept, a failure is not."""
+    n = _WORKSPACE.get((dev.index, dim))
+    if n is None:
+        n = int(lib.tt_kv8_attention_workspace_bytes(dim))
+        if n == 0:
+            raise RuntimeError(f"tt_kv8_attention_workspace_bytes: no size for head_dim {dim} on {dev} "
+                               f"({lib.tt_last_cuda_error().decode()})")
+        _WORKSPACE[dev.index, dim] = n
+    return n
+
+
 def kv_attention(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, lengths: torch.Tensor,
                  *, n_query: torch.Tensor | None = None, causal: bool = True,
                  scale: float | None = None) -> torch.Tensor:
@@ -290,10 +302,7 @@ def kv_attention(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, le
         sb, ss, sh, _ = q.stride()
     lib = _lib.load()
     with _on(dev):
-        ws_bytes = _WORKSPACE.get((dev.index, dim))
-        if ws_bytes is None:
-            ws_bytes = int(lib.tt_kv8_attention_workspace_bytes(dim))
-            _WORKSPACE[dev.index, dim] = ws_bytes
+        ws_bytes = _workspace_bytes(lib, dev, dim)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _lib.check(lib.tt_kv8_attention(
             _at(q), _TYPES[q.dtype], sb, ss, sh, _at(cache._k),
