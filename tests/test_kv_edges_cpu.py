@@ -42,3 +42,25 @@ def test_a_failed_size_is_asked_for_again(monkeypatch):
         kv_cache._workspace_bytes(lib, dev, 64)
     assert kv_cache._workspace_bytes(lib, dev, 64) == 4096
     assert kv_cache._workspace_bytes(lib, dev, 64) == 4096 and not lib.sizes
+
+
+def test_sizes_past_32_bits_are_refused():
+    """Expanded operands can have more tokens, sequences or heads than the library counts."""
+    p = parts(batch=1, new=1, heads=2, kv=2)
+    big = 2**32 + 1
+    far = p["k"].expand(1, big, 2, 32)
+    with pytest.raises(ValueError, match="at most"):
+        append(p, k=far, v=far)
+    with pytest.raises(ValueError, match="at most"):
+        attend(p, q=p["q"].expand(1, big, 2, 32))
+    with pytest.raises(ValueError, match="at most"):
+        attend(p, q=p["q"][:, :, :1].expand(1, 1, big + 1, 32))
+    wide = p["table"][:, :1].expand(1, big)
+    for call in (append, attend):
+        with pytest.raises(ValueError, match="at most"):
+            call(p, table=wide)
+    many = dict(table=p["table"].expand(big, 2), lengths=p["lengths"].expand(big))
+    with pytest.raises(ValueError, match="at most"):
+        append(p, k=p["k"].expand(big, 1, 2, 32), v=p["k"].expand(big, 1, 2, 32), **many)
+    with pytest.raises(ValueError, match="at most"):
+        attend(p, q=p["q"].expand(big, 1, 2, 32), **many)

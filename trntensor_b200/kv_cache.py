@@ -25,7 +25,7 @@ from torch.autograd import forward_ad
 
 from . import _lib
 from .dispatch import _device
-from .quantized import _TYPES, _on, _stream_of
+from .quantized import _MOST, _TYPES, _on, _stream_of
 
 _WORKSPACE: dict[tuple[int, int], int] = {}  # bytes by (device, head_dim)
 _PAGES = (16, 32, 64, 128)
@@ -162,6 +162,8 @@ def _check_table(table: torch.Tensor, batch: int, dev: torch.device) -> torch.Te
             or (batch and table.shape[1] < 1):
         raise ValueError(f"block_table must be int32 ({batch}, columns) on {dev}, got {table.dtype} "
                          f"{tuple(table.shape)} on {table.device}")
+    if table.shape[1] > _MOST:
+        raise ValueError(f"block_table may have at most {_MOST} columns, got {table.shape[1]}")
     return table if table.stride(1) == 1 else table.contiguous()
 
 
@@ -177,6 +179,8 @@ def _check_tokens(x: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor
     if x.dim() != 4 or x.dtype not in _TYPES:
         raise ValueError(f"{name} must be fp32, bf16 or fp16 (batch, tokens, heads, head_dim), "
                          f"got {x.dtype} {tuple(x.shape)}")
+    if max(x.shape) > _MOST:
+        raise ValueError(f"{name} may have at most {_MOST} of each, got {tuple(x.shape)}")
     if x.device != dev:
         raise ValueError(f"{name} must be on {dev}, got {x.device}")
     _check_underived(x, name)
