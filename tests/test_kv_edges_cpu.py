@@ -44,6 +44,13 @@ def test_a_failed_size_is_asked_for_again(monkeypatch):
     assert kv_cache._workspace_bytes(lib, dev, 64) == 4096 and not lib.sizes
 
 
+def test_scale_beyond_fp32():
+    """A scale that is finite in 64 bits alone would be infinite in the library."""
+    for scale in (1e300, -1e39, 2.0**127, float("inf")):
+        with pytest.raises(ValueError, match="scale must be finite"):
+            attend(parts(), scale=scale)
+
+
 def test_sizes_past_32_bits_are_refused():
     """Expanded operands can have more tokens, sequences or heads than the library counts."""
     p = parts(batch=1, new=1, heads=2, kv=2)

@@ -18,7 +18,6 @@ device: a page id, length or count out of range is left out and noted, and
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 from torch.autograd import forward_ad
@@ -294,8 +293,8 @@ def kv_attention(q: torch.Tensor, cache: KVCache8, block_table: torch.Tensor, le
     lengths = _int32(lengths, "lengths", (batch,), dev)
     n_query = _int32(n_query, "n_query", (batch,), dev)
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) < 2.0**127:  # the library takes it as fp32, times log2(e)
+        raise ValueError(f"scale must be finite, and below 2^127, got {scale}")
     out = torch.empty((batch, new, heads, dim), dtype=q.dtype, device=dev)
     if out.numel() == 0:
         return out
