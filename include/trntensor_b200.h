@@ -335,7 +335,8 @@ int tt_q4_row_scale(const void* packed_scales, int scale_type, int N, int K, int
 size_t tt_q4_matmul_workspace_bytes(int type, int scale_type, int transposed, int M, int N, int K);
 /* y (M, N; row stride ldy) = x (M, K; row stride ldx) W^T: fp32 sums, rounded
  * once to x's type. dev_status as in the file's head; unlike other calls these
- * do not clear it. */
+ * do not clear it. Where it is set, by a wait that ran out in this call or an
+ * earlier one, the results of a product with a workspace are NaN. */
 int tt_q4_matmul(const void* x, int type, long long ldx, const void* packed,
                  const void* packed_scales, int scale_type, const float* row_scale, int M, int N,
                  int K, int group, void* y, long long ldy, void* workspace, size_t workspace_bytes,
@@ -360,7 +361,8 @@ int tt_q4_matmul_t(const void* dy, int type, long long lddy, const void* packed,
  * leave out what points outside the cache (attention: its tokens are not there)
  * and OR a bit into *status: 1 a page id outside the cache, 2 a length or count
  * out of range, 4 one append that writes a page for two places, 8 a copy that
- * never arrived. Activations are
+ * never arrived. With that last one the attention's results are NaN, and so are
+ * those of later calls until the bit is cleared. Activations are
  * fp32, bf16 or fp16 (types as above) with strides in elements over (batch,
  * token, head) and neighbouring values in a head.
  */

@@ -10,6 +10,7 @@ import torch
 from test_kv_gpu import TYPES, Ref, attend_case, filled, int32, reference, turned
 
 import trntensor_b200 as tt
+from trntensor_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -285,3 +286,26 @@ def test_shared_pages_of_a_large_cache(cuda_ok):
         tt.kv_append(cache, k, k, table.view(batch, cols).cuda(), int32([0, 0]))
         with pytest.raises(ValueError, match="two places"):
             cache.check()
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("new", [1, 6, 1300])
+def test_a_copy_that_never_arrived_is_not_a_result(cuda_ok, new, name):
+    """With the timeout noted, what sees a token is NaN until the word has been read; other
+    notes leave results alone."""
+    cache = tt.KVCache8.from_codes(*(x.cuda() for x in filled(24, 2, 16, 64)))
+    table, lengths = int32([list(range(12)), list(range(12, 24))]), int32([180, 0])
+    q = torch.randn(2, new, 8, 64, device="cuda").to(TYPES[name])
+    want = tt.kv_attention(q, cache, table, lengths)
+    sees = max(0, new - 180)  # the first row that sees a token
+    cache.status.fill_(8)
+    for _ in range(2):
+        got = tt.kv_attention(q, cache, table, lengths)
+        assert got[0, sees:].isnan().all() and not got[0, :sees].any() and not got[1].any()
+    with pytest.raises(_lib.DeviceError, match="never arrived"):
+        cache.check()
+    assert torch.equal(tt.kv_attention(q, cache, table, lengths), want)
+    cache.status.fill_(7)
+    assert torch.equal(tt.kv_attention(q, cache, table, lengths), want)
+    with pytest.raises(ValueError, match="page id.*length.*two places"):
+        cache.check()

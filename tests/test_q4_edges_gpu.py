@@ -10,6 +10,7 @@ import torch.autograd.forward_ad as fwd
 from test_q4_gpu import TYPES, check, make, rows
 
 import trntensor_b200 as tt
+from trntensor_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +86,21 @@ def test_forward_mode(cuda_ok, m, over_n):
                  lambda: torch.func.grad(lambda a: tt.q4_matmul(a, w, over_n=over_n).sum())(x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("name", list(TYPES))
+@pytest.mark.parametrize("m", [40, 300, 700])
+def test_a_wait_that_ran_out_is_not_a_result(cuda_ok, m, name):
+    """With a timeout noted, products of many rows are NaN until the word has been read."""
+    codes, scales, _ = make(300, 2000, 64)
+    w = tt.pack_q4(codes.cuda(), scales.cuda(), group=64)
+    for over_n, cols in ((False, 2000), (True, 300)):
+        x = rows(m, cols, TYPES[name]).cuda()
+        want = tt.q4_matmul(x, w, over_n=over_n)
+        w.status.fill_(0x101)
+        for _ in range(2):
+            assert tt.q4_matmul(x, w, over_n=over_n).isnan().all()
+        with pytest.raises(_lib.DeviceError, match="0x101"):
+            w.check()
+        assert torch.equal(tt.q4_matmul(x, w, over_n=over_n), want)
+        w.check()

@@ -303,6 +303,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   // pieces of tiles that this CTA's warps leave: tile, whether it began and ended here
   __shared__ int4 left_at[S::kWarps * 2];
   if (threadIdx.x < S::kWarps * 2) left_at[threadIdx.x] = make_int4(-1, 0, 0, 0);
+  // a copy of an earlier call never arrived, and nobody has looked at that yet:
+  // what leaves here is NaN, as it is where a copy of this call does not arrive
+  __shared__ int before;
+  const int status = threadIdx.x == 0 ? *(volatile int*)p.status : 0;
   unsigned char* mine = smem + warp * S::kSlots * S::kSlot;
   uint64_t* bar = bars + warp * S::kSlots;
   const int dim = p.dim;
@@ -322,7 +326,10 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
         static_cast<T*>(p.o)[b * all + i] = from_f<T>(0.f);
     }
   }
-  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) {
+    before = status & kTimeout;
+    p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -432,8 +439,11 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
       page_k = page_at(ahead);
     }
   };
+  const long long stop = before == 0 ? end : begin;
+  if (stop == end) {
 #pragma unroll
-  for (int i = 0; i < S::kSlots; ++i) ask_next();
+    for (int i = 0; i < S::kSlots; ++i) ask_next();
+  }
 
   uint32_t slot = 0, parity = 0;
   bool alive = true;
@@ -461,7 +471,8 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   int lim_min = 0;
   bool fresh = true, whole = true;
 
-  for (long long i = begin; i < end; ++i) {
+  long long i = begin;
+  for (; i < stop; ++i) {
     if (fresh) {  // a tile begins: its queries
       fresh = false;
       whole = at.chunk == 0;
@@ -775,6 +786,34 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
       fresh = true;
     }
     if (i + 1 < end) advance(p, at);
+  }
+  // What this warp has left to do is lost: NaN for each row that sees a token.
+  for (; i < end; fresh = true) {
+    if (fresh) whole = at.chunk == 0;
+    const int rest = (int)min(end - i, (long long)(at.chunks - at.chunk)), count = clamp_count(p, at.b, false);
+    const bool last = rest == at.chunks - at.chunk;
+    for (int in_tile = 0; in_tile < kTile; ++in_tile) {
+      const int r = at.tile * kTile + in_tile, tok = r / group;
+      if (r >= p.rows) break;
+      const bool none = tok >= count || (p.causal && (int)at.length - count + tok + 1 <= 0);
+      const float lost = none ? 0.f : __int_as_float(0x7fffffff);
+      if (whole && last) {
+        T* o = static_cast<T*>(p.o) + row_offset(p, at.b, at.h, r);
+        for (int d = lane; d < dim; d += 32) o[d] = from_f<T>(lost);
+      } else {
+        float* out = p.part + (((long long)blockIdx.x * S::kWarps + warp) * 2 + (whole ? 1 : 0)) * 16 * rows_of +
+                     in_tile * rows_of;
+        for (int d = lane; d < rows_of; d += 32) out[d] = d == 0 ? (none ? -INFINITY : 0.f) : lost;
+      }
+    }
+    if (!(whole && last) && lane == 0) {
+      const long long c1 = i + (at.chunks - 1 - at.chunk);
+      left_at[warp * 2 + (whole ? 1 : 0)] = make_int4(at.b, at.h * p.tiles + at.tile, (whole ? 1 : 0) | (last ? 2 : 0),
+                                                      (int)((((c1 + 1) * workers - 1) / total) / per_cta));
+    }
+    i += rest;
+    at.chunk = at.chunks - 1;
+    if (i < end) advance(p, at);
   }
   }  // works
   __syncthreads();

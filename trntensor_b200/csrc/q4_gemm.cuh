@@ -125,6 +125,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ uint64_t full[S::kStages], empty[S::kStages], done, d_full[2], d_free[2];
   __shared__ uint32_t tmem_slot;
+  __shared__ int dead;  // a wait ran out
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = gridDim.x, rank = blockIdx.x;
   const long long tile = blockIdx.y + (long long)blockIdx.z * gridDim.y;
@@ -148,6 +149,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     }
     fence_mbar_init();
     tma_prefetch_desc(&mapB);
+    dead = 0;
   }
   if (warp == 17) {
     tmem_alloc(&tmem_slot, S::kColumns);
@@ -165,7 +167,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
       for (int i = 0, pass = 0, step = s0; i < count && ok; ++i) {
         for (int sub = 0; sub < 2; ++sub, ++it) {
           const int s = it % S::kStages;
-          if (!mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty)) {
+          if (!mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &dead, kDevTimeoutEmpty)) {
             ok = false;
             break;
           }
@@ -191,9 +193,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
       const uint32_t ph = (it / S::kStages) & 1u;
       const uint32_t part = it / (2 * kSumSteps), of_part = it % (2 * kSumSteps);  // kSums
       if (kSums && of_part == 0 &&
-          !__all_sync(0xffffffffu, mbar_wait(&d_free[part & 1], (part >> 1 & 1) ^ 1, p.err, kDevTimeoutAcc)))
+          !__all_sync(0xffffffffu, mbar_wait(&d_free[part & 1], (part >> 1 & 1) ^ 1, &dead, kDevTimeoutAcc)))
         break;
-      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, p.err, kDevTimeoutFull))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&full[s], ph, &dead, kDevTimeoutFull))) break;
       tc_fence_after();
       // sum-major A: 128-byte rows of 64 terms; row-major (kTrans): two columns
       // of 64 rows, 8 KB apart, one term to a 128-byte line
@@ -285,7 +287,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     float sum[kSums ? S::kOut : 1];
     int summed = 0;
     auto take = [&]() {  // the next part of the sum
-      ok = ok && __all_sync(0xffffffffu, mbar_wait(&d_full[summed & 1], summed >> 1 & 1, p.err, kDevTimeoutAcc));
+      ok = ok && __all_sync(0xffffffffu, mbar_wait(&d_full[summed & 1], summed >> 1 & 1, &dead, kDevTimeoutAcc));
       if (!ok) return;
       tc_fence_after();
       if (first < MT) {
@@ -354,7 +356,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
         fetch(x);
         if (now) {
         const int s = it % S::kStages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, p.err, kDevTimeoutEmpty));
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &dead, kDevTimeoutEmpty));
         const uint32_t base = smem_u32(smem + s * S::kStageBytes);
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -385,11 +387,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
     }
     if constexpr (kSums)
       while (ok && summed * kSumSteps < count) take();
-    // D: lanes are rows of the tile, columns are tokens
-    ok = mbar_wait(&done, 0, p.err, kDevTimeoutAcc) && ok;
-    ok = __all_sync(0xffffffffu, ok);
+    // D: lanes are rows of the tile, columns are tokens. Where a wait ran out,
+    // here or in an earlier call that nobody has looked at yet, it is NaN.
+    ok = *(volatile int*)p.err == 0 && ok;
+    ok = mbar_wait(&done, 0, &dead, kDevTimeoutAcc) && ok;
+    ok = __all_sync(0xffffffffu, ok && *(volatile int*)&dead == 0);
     tc_fence_after();
-    if (ok && active) {
+    if (active) {
       const int half = R == 2 ? first / MT : 0;
       const long long row = row0 + half * 128 + quad * 32 + lane;
       const int c0 = first - half * MT;
@@ -410,7 +414,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
       };
       const int c1 = first < R * MT ? c0 + S::kOut : c0;
       float v[16];
-      if constexpr (kSums) {
+      if (!ok) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __int_as_float(0x7fffffff);
+        for (int c = c0; c < c1 && m0 + c < p.M; c += 16) bring(c, v);
+      } else if constexpr (kSums) {
 #pragma unroll
         for (int j = 0; j < S::kOut; j += 16) {
 #pragma unroll
@@ -449,6 +457,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap mapB, const Gemm p) {
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && dead != 0) atomicCAS(p.err, 0, dead);
   if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kColumns);

@@ -50,7 +50,8 @@ class KVCache8:
     """Pages of keys and values as int8 codes with fp32 scales (page, head).
 
     All pages start as zeros. ``status`` is a device word that collects what the
-    calls found wrong; :meth:`check` reads it.
+    calls found wrong; :meth:`check` reads it. Where a device copy never arrived
+    attention gives NaN, until the word has been read.
     """
 
     def __init__(self, num_pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64,

@@ -46,7 +46,8 @@ class Q4Matrix:
     Made by :func:`quantize_q4` or :func:`pack_q4`; ``packed`` and ``scales``
     are the stored bytes and scales (bf16 or fp32), padded to 16 x 128 blocks,
     ``row_scale`` a power of two a row. ``status`` is a device word in which a
-    product notes a device wait that ran out; :meth:`check` reads it.
+    product notes a device wait that ran out; its result is NaN, and so are those
+    of later products of many rows until :meth:`check` has read the word.
     """
 
     ndim = 2
