@@ -104,3 +104,24 @@ def test_a_wait_that_ran_out_is_not_a_result(cuda_ok, m, name):
             w.check()
         assert torch.equal(tt.q4_matmul(x, w, over_n=over_n), want)
         w.check()
+
+
+@pytest.mark.parametrize("name,terms", [("fp16", 60_000), ("fp16", 300_000), ("bf16", 600_000)])
+@pytest.mark.parametrize("over_n", [False, True])
+def test_very_long_sums(cuda_ok, name, terms, over_n):
+    """Terms of one sign, in so many tiles that no CTAs share a sum: what is cut off at each
+    step of the tensor cores (up to 2^-23 of the sum) would come to as much as the result's
+    rounding. Here 16 such steps make a part, and the parts' additions round: half of 2^-23 for
+    each 256 terms."""
+    other, m = 9600, 40
+    n, k = (terms, other) if over_n else (other, terms)
+    codes = torch.full((n, k), 7, dtype=torch.int8, device="cuda")
+    w = tt.pack_q4(codes, torch.full((n, -(-k // 128)), 2.0**-6, dtype=torch.bfloat16, device="cuda"))
+    del codes
+    g = torch.Generator().manual_seed(3)
+    x = (0.75 + 0.25 * torch.rand(m, terms, generator=g)).mul(2.0**-4).to(TYPES[name])
+    got = tt.q4_matmul(x.cuda(), w, over_n=over_n).double().cpu()
+    want = x.double().sum(1, keepdim=True) * (7 * 2.0**-6)
+    bound = torch.finfo(x.dtype).eps / 2 + 1.01 * (16 * 2.0**-23 + (terms / 256 + 8) * 2.0**-24)
+    worst = ((got - want).abs() / want).max().item()
+    assert worst <= bound, (worst, bound)

@@ -73,8 +73,8 @@ int launch_groups(const CUtensorMap& map, const Gemm& p, int group, int splits, 
   return launch<R, MT, 4, kTrans, kSums>(map, p, splits, s);
 }
 template <bool kTrans>
-int launch_tile(const CUtensorMap& map, const Gemm& p, int group, int R, int MT, int splits, cudaStream_t s) {
-  if (p.type == kF32) {
+int launch_tile(const CUtensorMap& map, const Gemm& p, int group, int R, int MT, bool sums, int splits, cudaStream_t s) {
+  if (sums) {
     if (MT == 32) return launch_groups<1, 32, kTrans, true>(map, p, group, splits, s);
     if (MT == 64) return launch_groups<1, 64, kTrans, true>(map, p, group, splits, s);
     return launch_groups<1, 128, kTrans, true>(map, p, group, splits, s);
@@ -154,10 +154,14 @@ int run_gemm(bool transposed, const void* x, int type, long long ldx, const void
     strides[0] = (uint64_t)Cp * 2;
     strides[1] = (uint64_t)Cp * 2 * M;
   }
+  // Sums that leave the tensor cores in between: for fp32, and for sums so long
+  // that what is cut off may come to half of the result's rounding (fp16: 2048
+  // times 1.1e-7, of 4.9e-4; bf16 eight times as many).
+  const bool sums = type == kF32 || C > (type == kF16 ? 1 << 15 : 1 << 18);
   // Tile: all tokens up to 256 at a time; 256 rows of the matrix where that
   // makes the last wave of CTAs no emptier (time goes by waves times rows).
-  // fp32 sums take registers: 128 tokens at most.
-  const int MT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 || type == kF32 ? 128 : 256;
+  // Sums take registers: 128 tokens at most.
+  const int MT = M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 || sums ? 128 : 256;
   const long long tiles_m = ((long long)M + MT - 1) / MT;
   const long long one = (rows + 127) / 128 * tiles_m, two = (rows + 255) / 256 * tiles_m;
   const int R = MT == 256 && (two + sms - 1) / sms * 2 <= (one + sms - 1) / sms ? 2 : 1;
@@ -167,8 +171,8 @@ int run_gemm(bool transposed, const void* x, int type, long long ldx, const void
   CUtensorMap map;
   if (encode_tmap(&map, b, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT16))
     return TT_ERR_TMA;
-  return transposed ? launch_tile<true>(map, p, group, R, MT, splits, s)
-                    : launch_tile<false>(map, p, group, R, MT, splits, s);
+  return transposed ? launch_tile<true>(map, p, group, R, MT, sums, splits, s)
+                    : launch_tile<false>(map, p, group, R, MT, sums, splits, s);
 }
 
 int run_row_scale(const void* scales, int scale_type, int N, int K, int group, float* out, cudaStream_t s) {

@@ -107,11 +107,12 @@ __device__ __forceinline__ float scale_term(float s, int i) {
 }
 
 // The tensor cores cut an accumulator off to 24 bits at every addition: each of
-// the K / 16 takes up to 2^-23 of the sum so far, to one side (measured 2.7e-8
-// of the result a step; 1.2e-5 for fp32 rows, whose four passes make 470 of
-// them of K = 1900). Results of 16 bits do not show it. For fp32 ones (kSums) D
-// starts anew every kSumSteps steps of the sum, in the other half of TMEM,
-// and the decoding warps add the finished half to fp32 registers: 16 cut
+// the K / 16 takes up to 2^-23 of the sum so far, to one side (measured where all
+// terms have one sign: 1.1e-7 of the result a step for equal ones, 2.7e-8 for
+// others; 1.2e-5 for fp32 rows, whose four passes make 470 of them of K = 1900).
+// Results of 16 bits do not show it unless sums are very long. For those and for
+// fp32 (kSums) D starts anew every kSumSteps steps of the sum, in the other half
+// of TMEM, and the decoding warps add the finished half to fp32 registers: 16 cut
 // additions at most, then rounded ones.
 constexpr int kSumSteps = 2;
 
