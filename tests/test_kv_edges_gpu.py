@@ -309,3 +309,35 @@ def test_a_copy_that_never_arrived_is_not_a_result(cuda_ok, new, name):
     assert torch.equal(tt.kv_attention(q, cache, table, lengths), want)
     with pytest.raises(ValueError, match="page id.*length.*two places"):
         cache.check()
+
+
+@pytest.mark.parametrize("name", ["fp16", "bf16"])
+@pytest.mark.parametrize("heads,batch", [(1, 1200), (12, 1190)])
+def test_long_runs_of_one_warp(cuda_ok, heads, batch, name):
+    """So many long sequences that a warp has whole ones, of values of one sign. Tensor cores
+    cut off up to 2^-23 of a sum at every 16 tokens: 1024 times in a run of 256 blocks, where
+    262144 tokens in one would lose 1.6e-3. Then there are roundings, half of 2^-23 for each of
+    the 16 runs, and for each of the 4096 blocks in the sum of the weights. The weights' own
+    roundings (2^-11, of N weights of about 1 / N and of either sign) come to 6 of their standard
+    deviations; scores are below 1 and good to 2^-19."""
+    pages, dim, page = 2048, 16, 128
+    g = torch.Generator().manual_seed(1)
+    kc = torch.randint(-127, 128, (pages, 1, page, dim), generator=g, dtype=torch.int8)
+    vc = torch.randint(64, 128, (pages, 1, page, dim), generator=g, dtype=torch.int8)
+    ks, vs = torch.full((pages, 1), 1 / 500), (1 + 0.2 * torch.rand(pages, 1, generator=g)) / 128
+    cache = tt.KVCache8.from_codes(kc.cuda(), ks.cuda(), vc.cuda(), vs.cuda())
+    q = (torch.randn(1, 1, heads, dim, generator=g) * 0.3).to(TYPES[name])
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, -1)
+    n = pages * page
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    lengths[1::2] -= 1001
+    got = tt.kv_attention(q.cuda().expand(batch, -1, -1, -1), cache, table, lengths)[:, 0].double().cpu()
+    k = (kc.double() * ks.double()[..., None, None]).reshape(-1, dim)
+    v = (vc.double() * vs.double()[..., None, None]).reshape(-1, dim)
+    bound = (torch.finfo(TYPES[name]).eps / 2 + 1024 * 2.0**-23 + (16 + 4096) * 2.0**-24
+             + 6 * 2.0**-11 / (n / 2) ** 0.5 + 2 * 2.0**-19)
+    for b in (0, 1):
+        end = n - 1001 * b
+        want = torch.softmax(q[0, 0].double() @ k[:end].T * dim**-0.5, -1) @ v[:end]
+        worst = ((got[b::2] - want).abs() / want).max().item()
+        assert worst <= bound, (worst, bound)

@@ -11,14 +11,12 @@ std::once_flag g_flags[kMaxDevices];
 int g_ok[kMaxDevices];
 int g_sms[kMaxDevices];
 
-template <typename T, int DP>
+template <typename T, int DP, int NT, bool kLong>
 int set_attr() {
-  constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
-  const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  if (cudaFuncSetAttribute(attend_kernel<T, DP, kTerms, 1>, at, Shape<DP>::kSmem) != cudaSuccess) return TT_ERR_CUDA;
-  if constexpr (DP <= 128)
-    if (cudaFuncSetAttribute(attend_kernel<T, DP, kTerms, 2>, at, Shape<DP>::kSmem) != cudaSuccess) return TT_ERR_CUDA;
-  return TT_OK;
+  return cudaFuncSetAttribute(attend_kernel<T, DP, sizeof(T) == 4 ? 2 : 1, NT, kLong>,
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem) == cudaSuccess
+             ? TT_OK
+             : TT_ERR_CUDA;
 }
 template <typename T, int DP>
 int set_prefill() {
@@ -30,14 +28,21 @@ int set_prefill() {
 }
 template <typename T>
 int set_attrs() {
-  int st = set_attr<T, 64>();
+  constexpr bool k16 = sizeof(T) == 2;
+  int st = set_attr<T, 64, 1, k16>();
+  if (st == TT_OK) st = set_attr<T, 128, 1, k16>();
+  if (st == TT_OK) st = set_attr<T, 192, 1, k16>();
+  if (st == TT_OK) st = set_attr<T, 256, 1, k16>();
+  if (st == TT_OK) st = set_attr<T, 64, 2, false>();
+  if (st == TT_OK) st = set_attr<T, 128, 2, false>();
+  if constexpr (k16) {
+    if (st == TT_OK) st = set_attr<T, 64, 2, true>();
+    if (st == TT_OK) st = set_attr<T, 128, 2, true>();
+  }
   if constexpr (sizeof(T) == 2) {
     if (st == TT_OK) st = set_prefill<T, 64>();
     if (st == TT_OK) st = set_prefill<T, 128>();
   }
-  if (st == TT_OK) st = set_attr<T, 128>();
-  if (st == TT_OK) st = set_attr<T, 192>();
-  if (st == TT_OK) st = set_attr<T, 256>();
   return st;
 }
 
@@ -57,18 +62,34 @@ int warps_of(int dim) { return dim <= 128 ? Shape<128>::kWarps : dim <= 192 ? Sh
 size_t piece_bytes(int dim) { return (size_t)2 * 16 * (dim + 2) * 4; }
 size_t workspace_bytes(int dim, int sms) { return sms * (16 + (warps_of(dim) + 1) * piece_bytes(dim)); }
 
-template <typename T, int DP>
-int launch(Attend p, int sms, cudaStream_t s) {
+template <typename T, int DP, int NT>
+void launch_rows(const Attend& p, int sms, cudaStream_t s) {
   constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
   using S = Shape<DP>;
+  // Tiles of sixteen rows have no registers to spare: for them what long runs need
+  // is left out where no warp can have one, if all sequences fill the table (32 x
+  // 16 rows over 8192 tokens, 128 a head, 128 against 135 us).
+  const long long chunks = ((long long)p.cols * p.page + kChunk - 1) / kChunk;
+  const long long share = chunks * p.tiles * p.heads * p.batch / (sms * S::kWarps) + 1;
+  if constexpr (kTerms == 1) {
+    if (NT == 1 || (chunks > kLongRun && share > kLongRun)) {
+      attend_kernel<T, DP, kTerms, NT, true><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+      return;
+    }
+  }
+  if constexpr (kTerms == 2 || NT == 2)
+    attend_kernel<T, DP, kTerms, NT, false><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+}
+template <typename T, int DP>
+int launch(Attend p, int sms, cudaStream_t s) {
   // More than eight rows go sixteen at a time, which decodes the cache once for
   // both halves, where the registers hold them.
   p.tile_rows = p.rows <= 8 || DP > 128 ? 8 : 16;
   p.tiles = (p.rows + p.tile_rows - 1) / p.tile_rows;
   if (p.tile_rows == 8) {
-    attend_kernel<T, DP, kTerms, 1><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+    launch_rows<T, DP, 1>(p, sms, s);
   } else {
-    if constexpr (DP <= 128) attend_kernel<T, DP, kTerms, 2><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+    if constexpr (DP <= 128) launch_rows<T, DP, 2>(p, sms, s);
   }
   int st = cuda_status(cudaGetLastError());
   if (st != TT_OK) return st;

@@ -47,6 +47,10 @@ namespace tt {
 namespace kv8 {
 
 constexpr int kChunk = 64;
+// Chunks (a power of two) after which the sums of values of 16-bit types are put
+// aside and start anew: the tensor cores cut off up to 2^-23 of them at every 16
+// tokens, to one side, 1.1e-4 until then. (fp32 types empty theirs every chunk.)
+constexpr int kLongRun = 256;
 constexpr int kNever = 0x7fffff00;  // behind the last token that any row sees (lengths are at most this)
 constexpr float kUp = 16384.f, kUpLog = 14.f;  // the largest fp16 weight of a chunk
 
@@ -291,8 +295,9 @@ __device__ __forceinline__ long long row_offset(const Attend& p, int b, int h, i
   return (((long long)b * p.S + r / group) * p.heads_q + h * group + r % group) * p.dim;
 }
 
-// NT: tiles of 8 rows that a warp has at a time.
-template <typename T, int DP, int kTerms, int NT>
+// NT: tiles of 8 rows that a warp has at a time. kLong: a warp may have more
+// than kLongRun chunks of a tile.
+template <typename T, int DP, int kTerms, int NT, bool kLong>
 __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const Attend p) {
   using S = Shape<DP>;
   constexpr int kTile = 8 * NT;
@@ -469,7 +474,38 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
   int lim[NT][2];
   uint32_t qf[NT][DP / 16][kTerms][2];
   int lim_min = 0;
-  bool fresh = true, whole = true;
+  bool fresh = true, whole = true, aside = false;
+  // The sums of values join those put aside before, in this warp's place for the
+  // tile's piece: there, to start anew, or here, to leave (`back`).
+  auto join_aside = [&](bool back) {
+    float* base = p.part + (((long long)blockIdx.x * S::kWarps + warp) * 2 + (whole ? 1 : 0)) * 16 * rows_of;
+#pragma unroll
+    for (int a = 0; a < NT; ++a)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float* out = base + (8 * a + 2 * t + e) * rows_of;
+        const float top = m[a][e] == -INFINITY ? 0.f : m[a][e], keep = aside ? exp2_approx(out[0] - top) : 0.f;
+        __syncwarp();
+        if (g == 0) out[0] = m[a][e];
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n)
+          if (16 * n < dim) {
+            float x = acc[a][n][e], y = acc[a][n][e + 2];
+            if (aside) {
+              x += out[2 + 16 * n + g] * keep;
+              y += out[2 + 16 * n + 8 + g] * keep;
+            }
+            if (!back) {
+              out[2 + 16 * n + g] = x;
+              out[2 + 16 * n + 8 + g] = y;
+            }
+            acc[a][n][e] = back ? x : 0.f;
+            acc[a][n][e + 2] = back ? y : 0.f;
+          }
+      }
+    __syncwarp();
+    aside = !back;
+  };
 
   long long i = begin;
   for (; i < stop; ++i) {
@@ -739,8 +775,11 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
     }
     release();
 
-    const bool last = at.chunk + 1 == at.chunks;
-    if (last || i + 1 == end) {  // the tile's sums leave the warp
+    const bool last = at.chunk + 1 == at.chunks, leaves = last || i + 1 == end;
+    if constexpr (kLong) {
+      if (leaves ? aside : (at.chunk & (kLongRun - 1)) == kLongRun - 1) join_aside(leaves);
+    }
+    if (leaves) {  // the tile's sums leave the warp
 #pragma unroll
       for (int a = 0; a < NT; ++a)
 #pragma unroll
