@@ -341,3 +341,60 @@ def test_long_runs_of_one_warp(cuda_ok, heads, batch, name):
         want = torch.softmax(q[0, 0].double() @ k[:end].T * dim**-0.5, -1) @ v[:end]
         worst = ((got[b::2] - want).abs() / want).max().item()
         assert worst <= bound, (worst, bound)
+
+
+@pytest.mark.parametrize("name,most", [("fp16", 2**15), ("bf16", 2**18)])
+def test_prompts_in_a_wide_table(cuda_ok, name, most):
+    """Many rows of sequences on both sides of the length up to which the tensor cores keep a
+    row's sum: each as the definition has it, the short ones as with a narrow table."""
+    page, kv, dim, new, heads = 128, 2, 64, 900, 8
+    pages = most // page + 3
+    parts = filled(pages, kv, page, dim, seed=5)
+    cache = tt.KVCache8.from_codes(*(x.cuda() for x in parts))
+    g = torch.Generator().manual_seed(2)
+    table = torch.randperm(pages, generator=g)[None].repeat(4, 1)
+    lengths = [most + 300, most, 1000, 0]
+    q = torch.randn(4, new, heads, dim, generator=g).to(TYPES[name])
+    got = tt.kv_attention(q.cuda(), cache, table.int().cuda(), int32(lengths))
+    cache.check()
+    assert not got[3].any() and got.isfinite().all()
+    narrow = tt.kv_attention(q[1:3].cuda(), cache, table[1:3, :most // page].int().cuda().contiguous(), int32(lengths[1:3]))
+    assert torch.equal(got[1:3], narrow)
+    ks, vs = (parts[i].double() * parts[i + 1].double()[..., None, None] for i in (0, 2))
+    for b in range(3):
+        n = lengths[b]
+        k, v = (x[table[b]].transpose(0, 1).flatten(1, 2)[:, :n].cuda() for x in (ks, vs))
+        for i in (0, 1, 450, 899):
+            see = n - new + i + 1
+            for h in (0, 3, 4, 7):
+                kh, vh, x = k[h // 4, :see], v[h // 4, :see], q[b, i, h].double().cuda()
+                p = torch.softmax(kh @ x * dim**-0.5, 0)
+                want = p @ vh
+                d = (dim / 16 + 20) * 2.0**-23 * float((kh.abs() @ x.abs()).max()) * dim**-0.5
+                e = 2.0**-11 + 2 * d + 2.0**-20 + (n / 16 + 64) * 2.0**-23
+                tol = (torch.finfo(q.dtype).eps / 2 * want.abs() + 1.01 * e * (p @ vh.abs())
+                       + n * 2.0**-28 * float(p.max() * vh.abs().max()))
+                assert ((got[b, i, h].double() - want).abs() <= tol).all(), (b, i, h)
+
+
+@pytest.mark.parametrize("name,bits", [("fp16", 11), ("bf16", 8)])
+def test_prompts_over_long_runs(cuda_ok, name, bits):
+    """Values of one sign over more tokens than a tile's sums may stay in the tensor cores for.
+    The bound is test_long_runs_of_one_warp's."""
+    page, dim, new = 128, 16, 1000
+    n = 2**19 if name == "bf16" else 2**17
+    pages = n // page
+    g = torch.Generator().manual_seed(1)
+    kc = torch.randint(-127, 128, (pages, 1, page, dim), generator=g, dtype=torch.int8)
+    vc = torch.randint(64, 128, (pages, 1, page, dim), generator=g, dtype=torch.int8)
+    ks, vs = torch.full((pages, 1), 1 / 500), (1 + 0.2 * torch.rand(pages, 1, generator=g)) / 128
+    cache = tt.KVCache8.from_codes(kc.cuda(), ks.cuda(), vc.cuda(), vs.cuda())
+    q = (torch.randn(1, 1, 12, dim, generator=g) * 0.3).to(TYPES[name])
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    got = tt.kv_attention(q.cuda().expand(1, new, -1, -1), cache, table, int32([n]), causal=False)[0].double().cpu()
+    k = (kc.double() * ks.double()[..., None, None]).reshape(-1, dim)
+    v = (vc.double() * vs.double()[..., None, None]).reshape(-1, dim)
+    want = torch.softmax(q[0, 0].double() @ k.T * dim**-0.5, -1) @ v
+    bound = (2.0**-bits + 1024 * 2.0**-23 + n / 64 * 2.0**-24 + 6 * 2.0**-11 / (n / 2) ** 0.5 + 2 * 2.0**-19)
+    worst = ((got - want).abs() / want).max().item()
+    assert worst <= bound, (worst, bound)

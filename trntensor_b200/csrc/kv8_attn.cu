@@ -21,8 +21,10 @@ int set_attr() {
 template <typename T, int DP>
 int set_prefill() {
   const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  return cudaFuncSetAttribute(prefill_kernel<T, DP, true>, at, PreShape<DP>::kSmem) == cudaSuccess &&
-                 cudaFuncSetAttribute(prefill_kernel<T, DP, false>, at, PreShape<DP>::kSmem) == cudaSuccess
+  return cudaFuncSetAttribute(prefill_kernel<T, DP, true, false>, at, PreShape<DP>::kSmem) == cudaSuccess &&
+                 cudaFuncSetAttribute(prefill_kernel<T, DP, false, false>, at, PreShape<DP>::kSmem) == cudaSuccess &&
+                 cudaFuncSetAttribute(prefill_kernel<T, DP, true, true>, at, PreShape<DP>::kSmem) == cudaSuccess &&
+                 cudaFuncSetAttribute(prefill_kernel<T, DP, false, true>, at, PreShape<DP>::kSmem) == cudaSuccess
              ? TT_OK
              : TT_ERR_CUDA;
 }
@@ -111,26 +113,38 @@ int launch(Attend p, int sms, cudaStream_t s) {
 // all SMs: the first wins from rows x heads x sequences = 64 (48) an SM for each
 // wave of CTAs. (8192 tokens, 128 a head: 16 x 8 x 40 rows 153 against 149 us,
 // 16 x 8 x 80 rows 152 against 238, 1 x 8 x 400 rows 190 against 110.)
-// It adds up a row's values in the tensor cores, which cut off 2^-25 or so at
-// each 16 tokens: not where a table can hold so many that a result shows it.
-bool many_rows(const Attend& p, int sms, bool fp16) {
+bool many_rows(const Attend& p, int sms) {
   const long long tiles = ((long long)p.rows + 255) / 256 * p.heads * p.batch, waves = (tiles + sms - 1) / sms;
-  return p.rows > 16 && (long long)p.rows * p.heads * p.batch > (p.rows > 128 ? 64 : 48) * waves * sms &&
-         (long long)p.cols * p.page <= (fp16 ? 1 << 17 : 1 << 20);
+  return p.rows > 16 && (long long)p.rows * p.heads * p.batch > (p.rows > 128 ? 64 : 48) * waves * sms;
 }
 
-template <typename T, int DP>
-int launch_prefill(const Attend& p, cudaStream_t s) {
+template <typename T, int DP, bool kLong>
+int launch_tiles(const Attend& p, cudaStream_t s) {
   const long long tiles = ((long long)p.rows + 255) / 256;
   const dim3 grid((unsigned)tiles, p.heads, p.batch);
-  if (p.dim == DP) prefill_kernel<T, DP, true><<<grid, kPreThreads, PreShape<DP>::kSmem, s>>>(p);
-  else prefill_kernel<T, DP, false><<<grid, kPreThreads, PreShape<DP>::kSmem, s>>>(p);
+  if (p.dim == DP) prefill_kernel<T, DP, true, kLong><<<grid, kPreThreads, PreShape<DP>::kSmem, s>>>(p);
+  else prefill_kernel<T, DP, false, kLong><<<grid, kPreThreads, PreShape<DP>::kSmem, s>>>(p);
   return cuda_status(cudaGetLastError());
+}
+template <typename T, int DP>
+int launch_prefill(Attend p, cudaStream_t s) {
+  // What the tensor cores cut off may come to half of a result's rounding for so
+  // many tokens (fp16: 2048 times 1.1e-7, of 4.9e-4): above, sums are put aside in
+  // between. A place has 256 rows of dim, 1 KB dim, of an SM's share of the
+  // workspace: 16 + 9 x 128 (dim + 2) bytes.
+  p.most = std::is_same<T, __half>::value ? 1 << 15 : 1 << 18;
+  if ((long long)p.cols * p.page > p.most) {
+    p.places = (int*)p.meta;
+    p.aside = (float*)(p.meta + p.sms);
+    const int st = cuda_status(cudaMemsetAsync(p.places, 0, p.sms * sizeof(int), s));
+    return st == TT_OK ? launch_tiles<T, DP, true>(p, s) : st;
+  }
+  return launch_tiles<T, DP, false>(p, s);
 }
 template <typename T>
 int launch_dim(const Attend& p, int sms, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    if (many_rows(p, sms, std::is_same<T, __half>::value) && p.dim <= 128 && p.heads <= 65535 && p.batch <= 65535)
+    if (many_rows(p, sms) && p.dim <= 128 && p.heads <= 65535 && p.batch <= 65535)
       return p.dim <= 64 ? launch_prefill<T, 64>(p, s) : launch_prefill<T, 128>(p, s);
   }
   if (p.dim <= 64) return launch<T, 64>(p, sms, s);
@@ -192,6 +206,10 @@ int tt_kv8_attention(const void* q, int type, long long q_stride_b, long long q_
   p.batch = batch; p.S = S; p.heads_q = heads_q; p.heads = heads; p.dim = dim; p.page = page; p.pages = pages;
   p.page_log = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
   p.cols = columns;
+  p.sms = sms;
+  p.most = 0;
+  p.places = nullptr;
+  p.aside = nullptr;
   p.rows = (int)rows;
   cudaStream_t s = (cudaStream_t)stream;
   if (type == q4::kF32) return kv8::launch_dim<float>(p, sms, s);

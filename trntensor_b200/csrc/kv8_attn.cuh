@@ -69,10 +69,12 @@ struct Attend {
   float* part;         // pieces: [CTA][warp][2][16][2 + dim] (maximum, sum, values)
   float* joint;        // and joined: [CTA][2][16][2 + dim]
   int4* meta;          // [CTA]: (b, h * tiles + tile, last CTA, 1) of a tile that others finish
+  int* places;         // prefill_kernel, above `most` tokens: [SM] 1 where the place is taken, zeros at first
+  float* aside;        // and the places: [SM][dim][256 rows]
   int* status;
   float scale;  // times log2(e)
   int causal;
-  int batch, S, heads_q, heads, dim, page, page_log, pages, cols, rows, tiles, tile_rows;
+  int batch, S, heads_q, heads, dim, page, page_log, pages, cols, rows, tiles, tile_rows, sms, most;
 };
 
 template <int DP>

@@ -38,6 +38,10 @@
 namespace tt {
 namespace kv8 {
 
+// Sums of values stay in the tensor cores, which cut off up to 2^-23 of them at
+// every 16 tokens, to one side. Where a table can hold so many that a result
+// would show it, a tile's rows put O aside every kLongRun blocks, in a place of
+// the workspace that the CTA takes when it starts, and the next block starts anew.
 constexpr int kPreThreads = 15 * 32;
 constexpr int kPreKeys = 64;         // tokens of a block
 constexpr int kPreBufs = 4;          // decoded blocks of K and of V
@@ -96,8 +100,9 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// kFull: the head dimension is DP.
-template <typename T, int DP, bool kFull>
+// kFull: the head dimension is DP. kLong: O is put aside (its code costs the
+// others 3 to 13% of their time, by registers).
+template <typename T, int DP, bool kFull, bool kLong>
 __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p) {
   using S = PreShape<DP>;
   extern __shared__ uint8_t smem_raw[];
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   __shared__ float sc_k[kScaleSlots][kUnits], sc_odd[kScaleSlots][kUnits], sc_log[kScaleSlots][kUnits],
       sc_inv[kScaleSlots][kUnits];
   __shared__ uint32_t tmem_slot;
-  __shared__ int dead, top_lim, before;
+  __shared__ int dead, top_lim, before, place;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int dim = kFull ? DP : p.dim, group = p.heads_q / p.heads;
   const int b = blockIdx.z, h = blockIdx.y;
@@ -148,6 +153,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     dead = 0;
     top_lim = 0;
     before = 0;
+    place = -1;
   }
   if (warp == 13) {
     tmem_alloc(&tmem_slot, 512);
@@ -172,6 +178,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   }
   __syncthreads();
   const int blocks = (top_lim + kPreKeys - 1) / kPreKeys;
+  if (kLong && top_lim > p.most && threadIdx.x == 0) {
+    // no more CTAs than places run at a time; were there none free, O would stay
+    for (int i = 0; i < p.sms && place < 0; ++i)
+      if (atomicCAS(p.places + i, 0, 1) == 0) place = i;
+    __threadfence();
+  }
   if (dim < DP) {  // columns of K and Q behind the head dimension are zeros, for good
     for (int i = threadIdx.x; i < (2 * S::kQ + kPreBufs * S::kKV) / 16; i += kPreThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
@@ -271,7 +283,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
           scores(n);
         }
         ok = ready(&v_full[j % kPreBufs], j / kPreBufs & 1) && ready(&p_full[i], j & 1);
-        if (ok) values(j % kPreBufs, j == 0);
+        if (ok) values(j % kPreBufs, j == 0 || (kLong && place >= 0 && j % kLongRun == 0));
       }
       // nothing may be in flight when the CTA gives its TMEM back
       if (elect_one()) {
@@ -380,6 +392,24 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     // a row that sees nothing stays out of the maxima's way
     float m = lim > 0 ? -INFINITY : 0.f, l = 0.f;
     bool ok = true;
+    // O put aside, relative to the maximum at that time
+    float m_aside = -INFINITY;
+    float* aside = !kLong || place < 0 ? nullptr : p.aside + (long long)place * 256 * dim + threadIdx.x;
+    auto put_aside = [&]() {
+      const float z = m == -INFINITY ? 0.f : m, keep = exp2_approx(m_aside - z);
+#pragma unroll 1
+      for (int c = 0; c < dim; c += 16) {
+        float o[16];
+        tmem_ld16(to + c, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float* at = aside + (c + e) * 256;
+          *at = m_aside == -INFINITY ? o[e] : fmaf(*at, keep, o[e]);
+        }
+      }
+      m_aside = z;
+    };
     // rows whose maximum rises, to a new one above n: l and O follow
     auto lift = [&](bool rise, float n, bool first) {
       const float now = rise ? n + kPreRoom : m;
@@ -406,6 +436,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[i], j & 1, err, kTimeout));
         if (!ok) break;
         tc_fence_after();
+        if (kLong && aside != nullptr && j > 0 && j % kLongRun == 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&pv_done[i], (j - 1) & 1, err, kTimeout));
+          if (!ok) break;
+          tc_fence_after();
+          put_aside();
+        }
         const float* fk = sc_k[j % kScaleSlots];
         // values' scales: their logarithms, inverses, and what is left of odd ones
         const float* fo = sc_odd[j % kScaleSlots];
@@ -542,11 +578,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
     // then, or where a wait ran out here, the result is not a number
     const bool lost = !ok || *(volatile int*)&dead != 0 || *(volatile int*)&before != 0;
     const float inv = lost ? __int_as_float(0x7fffffff) : some && (l > 0.f || l != l) ? 1.f / (l * kPreUp) : 0.f;
+    const float keep = exp2_approx(m_aside - (m == -INFINITY ? 0.f : m));
     for (int c = 0; c < dim; c += 16) {
       float o[16];
       if (blocks > 0 && i < tiles) {
         tmem_ld16(to + c, o);
         tmem_ld_wait();
+        if (kLong && aside != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = fmaf(aside[(c + e) * 256], keep, o[e]);
+        }
       }
       if (row >= 0) {
         T* at = static_cast<T*>(p.o) + row_offset(p, b, h, row) + c;
@@ -565,6 +606,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && dead != 0) raise(p.status, kTimeout);
+  if (kLong && threadIdx.x == 0 && place >= 0) {  // all rows have theirs
+    __threadfence();
+    atomicExch(p.places + place, 0);
+  }
   if (warp == 13) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
