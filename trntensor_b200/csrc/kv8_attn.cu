@@ -11,12 +11,14 @@ std::once_flag g_flags[kMaxDevices];
 int g_ok[kMaxDevices];
 int g_sms[kMaxDevices];
 
-template <typename T, int DP, int NT, bool kLong>
+template <typename T, int DP, int NT>
 int set_attr() {
-  return cudaFuncSetAttribute(attend_kernel<T, DP, sizeof(T) == 4 ? 2 : 1, NT, kLong>,
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem) == cudaSuccess
-             ? TT_OK
-             : TT_ERR_CUDA;
+  constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+  const auto at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  if (cudaFuncSetAttribute(attend_kernel<T, DP, kTerms, NT, false>, at, Shape<DP>::kSmem) != cudaSuccess) return TT_ERR_CUDA;
+  if constexpr (kTerms == 1)
+    if (cudaFuncSetAttribute(attend_kernel<T, DP, kTerms, NT, true>, at, Shape<DP>::kSmem) != cudaSuccess) return TT_ERR_CUDA;
+  return TT_OK;
 }
 template <typename T, int DP>
 int set_prefill() {
@@ -30,17 +32,12 @@ int set_prefill() {
 }
 template <typename T>
 int set_attrs() {
-  constexpr bool k16 = sizeof(T) == 2;
-  int st = set_attr<T, 64, 1, k16>();
-  if (st == TT_OK) st = set_attr<T, 128, 1, k16>();
-  if (st == TT_OK) st = set_attr<T, 192, 1, k16>();
-  if (st == TT_OK) st = set_attr<T, 256, 1, k16>();
-  if (st == TT_OK) st = set_attr<T, 64, 2, false>();
-  if (st == TT_OK) st = set_attr<T, 128, 2, false>();
-  if constexpr (k16) {
-    if (st == TT_OK) st = set_attr<T, 64, 2, true>();
-    if (st == TT_OK) st = set_attr<T, 128, 2, true>();
-  }
+  int st = set_attr<T, 64, 1>();
+  if (st == TT_OK) st = set_attr<T, 64, 2>();
+  if (st == TT_OK) st = set_attr<T, 128, 1>();
+  if (st == TT_OK) st = set_attr<T, 128, 2>();
+  if (st == TT_OK) st = set_attr<T, 192, 1>();
+  if (st == TT_OK) st = set_attr<T, 256, 1>();
   if constexpr (sizeof(T) == 2) {
     if (st == TT_OK) st = set_prefill<T, 64>();
     if (st == TT_OK) st = set_prefill<T, 128>();
@@ -68,19 +65,18 @@ template <typename T, int DP, int NT>
 void launch_rows(const Attend& p, int sms, cudaStream_t s) {
   constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
   using S = Shape<DP>;
-  // Tiles of sixteen rows have no registers to spare: for them what long runs need
-  // is left out where no warp can have one, if all sequences fill the table (32 x
-  // 16 rows over 8192 tokens, 128 a head, 128 against 135 us).
+  // What long runs need is left out where no warp can have one, even if all
+  // sequences fill the table: it costs registers (32 x 16 rows over 8192 tokens, 128
+  // a head, 128 against 135 us, 8 rows over 131000 58 against 61).
   const long long chunks = ((long long)p.cols * p.page + kChunk - 1) / kChunk;
   const long long share = chunks * p.tiles * p.heads * p.batch / (sms * S::kWarps) + 1;
   if constexpr (kTerms == 1) {
-    if (NT == 1 || (chunks > kLongRun && share > kLongRun)) {
+    if (chunks > kLongRun && share > kLongRun) {
       attend_kernel<T, DP, kTerms, NT, true><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
       return;
     }
   }
-  if constexpr (kTerms == 2 || NT == 2)
-    attend_kernel<T, DP, kTerms, NT, false><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
+  attend_kernel<T, DP, kTerms, NT, false><<<sms, S::kWarps * 32, S::kSmem, s>>>(p);
 }
 template <typename T, int DP>
 int launch(Attend p, int sms, cudaStream_t s) {
