@@ -634,14 +634,18 @@ __global__ void __launch_bounds__(Shape<DP>::kWarps * 32, 1) attend_kernel(const
         }
     }
     float sk = lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 4 * (g >> 1));
-    const bool gone = sk < 0.f;
-    if (gone) sk = 0.f;
+    bool gone = false;
+    if (lost) {
+      gone = sk < 0.f;
+      if (gone) sk = 0.f;
+    }
     const Level sv = level_of<kTerms == 2>(lds32(smem_u32(mine + slot * S::kSlot) + 4 * (S::kUnit + 32) + 16 + 4 * (g >> 1)), kUp);
     release();
 
     // The scores are used as they are: scaled by f (at least 0, the same for a
     // lane's whole unit) only inside the exponent.
-    const int tok0 = gone ? kNever : at.chunk * kChunk + 16 * (g >> 1) + (g & 1);
+    int tok0 = at.chunk * kChunk + 16 * (g >> 1) + (g & 1);
+    if (lost && gone) tok0 = kNever;
     const bool mask = (at.chunk + 1) * kChunk > lim_min || lost;
     if (mask) {
 #pragma unroll
