@@ -396,7 +396,8 @@ int tt_kv8_read(const void* k_codes, const void* v_codes, const float* k_scales,
  * that see nothing, and those from n_query[b] on, are zero. What is rounded for
  * the second product is a weight times its page's value scale (fp16 for 16-bit
  * types: 2^-11 of itself, or 2^-29 of the row's largest where that is more; two
- * such terms for fp32; value scales outside of 2^-80 .. 2^80 keep fewer bits).
+ * such terms for fp32; value scales in a row's sight below 2^-80, or 2^-100 of the
+ * largest, keep fewer bits).
  * q and its strides
  * are 16-byte aligned; scale is one host float, read during the call. Workspace
  * for the current device: */

@@ -398,3 +398,24 @@ def test_prompts_over_long_runs(cuda_ok, name, bits):
     bound = (2.0**-bits + 1024 * 2.0**-23 + n / 64 * 2.0**-24 + 6 * 2.0**-11 / (n / 2) ** 0.5 + 2 * 2.0**-19)
     worst = ((got - want).abs() / want).max().item()
     assert worst <= bound, (worst, bound)
+
+
+@pytest.mark.parametrize("name", ["fp32", "bf16"])
+@pytest.mark.parametrize("new", [1, 6, 1300])
+@pytest.mark.parametrize("size", [2.0**81, 2.0**100, 2.0**120])
+def test_huge_scales(cuda_ok, size, new, name):
+    """Values near the end of fp32's range, in all pages or in one of them. (Scales in a row's
+    sight may be 2^100 apart: a weight is 2^14 times 2^-100 then, and as many scores' bits below
+    the largest as are left down to fp32's 2^-126. The others here are about 2^-6.)"""
+    for mixed in (False, True) if size <= 2.0**100 else (False,):
+        kc, ks, vc, vs = filled(12, 2, 16, 64, seed=11)
+        vs[3 if mixed else slice(None)] *= size * (1 / 8 if mixed else 15)
+        parts = (kc, ks, vc, vs)
+        q = torch.randn(1, new, 4, 64, generator=torch.Generator().manual_seed(new)).to(TYPES[name])
+        cache = tt.KVCache8.from_codes(*(x.cuda() for x in parts))
+        got = tt.kv_attention(q.cuda(), cache, int32([list(range(12))]), int32([190])).cpu().double()
+        want, loss = reference(q, parts, [list(range(12))], [190], [new], True, 64**-0.5)
+        # a scale's logarithm is up to 2^7 and off by 2^-22 of itself, and the exponent it enters
+        # is rounded to 2^-17: 2^-14 of a weight in all
+        tol = torch.finfo(q.dtype).eps / 2 * want.abs() + 1.01 * loss + 2.0**-14 * want.abs().amax(-1, keepdim=True)
+        assert not ((got - want).abs() > tol).any() and not got.isnan().any()

@@ -148,17 +148,19 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   lo = reinterpret_cast<const uint32_t&>(ra);
   hi = reinterpret_cast<const uint32_t&>(rb);
 }
-// A value scale as 2^lg x odd, with lg in -80 .. 80, and back = 2^-lg / up. lg
+// A value scale as 2^lg x odd, with lg in -80 .. 125, and back = 2^-lg / up. lg
 // goes into the exponent of the weights; odd is what is left: 1, or the scale's
 // mantissa where lg is to be exact, and for a scale outside of the range (0,
-// infinity, NaN and what is next to them) the rest of it.
+// infinity, NaN and what is next to them) the rest of it. (Sums of weights reach
+// 2^80 of the largest; the scale of a page of finite values is below 2^121. Scales
+// in a row's sight may be 2^100 apart, or weights of the smaller ones are lost.)
 struct Level {
   float lg, odd, back;
 };
 template <bool kExact>
 __device__ __forceinline__ Level level_of(float s, float up) {
   Level v;
-  const float c = fminf(fmaxf(s, 0x1p-80f), 0x1p80f);  // NaN: the least
+  const float c = fminf(fmaxf(s, 0x1p-80f), 0x1p125f);  // NaN: the least
   if constexpr (kExact) {
     const uint32_t e = __float_as_uint(c) >> 23;
     const float inv = __uint_as_float((254u - e) << 23);
