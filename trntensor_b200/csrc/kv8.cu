@@ -11,8 +11,8 @@
 // (j, j + R/2) or (2 j, 2 j + 1).
 // What bounds it: instructions (turning, maxima, rounding: 48 us of issue for
 // the prompt below), then bytes. 8 kv heads of 128: a prompt of 2 x 8191 tokens in
-// pages of 16, fp16, with its read back 62 us (2.7 TB/s), 64 sequences x 1 token
-// in pages of 64, bf16, with theirs 12 us.
+// pages of 16, fp16, with its read back 60 us (2.8 TB/s), 64 sequences x 1 token
+// in pages of 64, bf16, with theirs 16 us.
 #include "common.cuh"
 #include "kv8.cuh"
 #include "q4.cuh"

@@ -14,14 +14,14 @@
 // What bounds it: the cache's bytes, and close behind them the instructions
 // that decode and multiply (with rows on the 16-wide side of the fragments,
 // half of it empty, they took a third more time). bf16, 128 a head: 64
-// sequences x 8192 tokens x 8 kv heads 144 us (5.7 TB/s of cache), one of 131000
-// tokens 56 us (4.8 TB/s); three of 100 tokens 13 us, launches and waits. Each warp keeps its own ring
-// of shared memory slots (one unit quartet of keys or of values each) filled by
-// bulk copies two or three slots ahead, across tile borders. Tensor-core
-// operands: the codes are exact in fp16; a row of q is scaled by a power of two
+// sequences of 4400 to 8192 tokens x 8 kv heads 149 us (5.5 TB/s of cache), one of
+// 131000 tokens 57 us (4.7 TB/s); three of 100 tokens 13 us, launches and waits.
+// Each warp keeps its own ring of shared memory slots (one unit quartet of keys or
+// of values each) filled by bulk copies two or three slots ahead, across tile
+// borders. Tensor-core operands: the codes are exact in fp16; a row of q is scaled by a power of two
 // to below 2^14 and rounded to fp16 (exact for 16-bit types down to 2^-27 of the
 // row's largest value, 2^-39 of that below) or, for fp32, kept as two fp16
-// terms. The softmax weights are fp16 (2^-11 of each, a quarter of a bf16
+// terms. The softmax weights are fp16 (2^-11 of each, an eighth of a bf16
 // result's rounding and as much as an fp16 one's; again held up by 2^14), two
 // terms for fp32. Page scales enter in fp32: keys' into the exponent, and
 // values' too, so that a weight times its value scale is what a row's maximum is

@@ -20,13 +20,13 @@
 // weight to, takes no bits from what it sees. The maximum m (of S f + log2 sv) is
 // taken 2^3 above the block's when it is set, and O is rescaled in TMEM only when
 // it moves: where a weight would pass 2^8, or, in blocks with hidden tokens or odd
-// scales, 1. Weights (times 2^7) stay below 2^15 + 2^3, fp16 rounds them by 2^-11,
+// scales, 1. Weights (times 2^7) stay below 2^15, fp16 rounds them by 2^-11,
 // sums are fp32.
 //
 // What bounds it: for 64 tokens and 256 rows the MMAs take about 1550 clocks
 // (the half of Q in shared memory most of it), the exponentials 1024; the way
 // from scores through a tile's softmax to P and back is longer than both, so
-// that it takes 2400. bf16, 2 x 1000 over 8000, 32 heads: 302 us, 0.59 PFLOP/s of
+// that it takes 2400. bf16, 2 x 1000 over 8000, 32 heads: 297 us, 0.60 PFLOP/s of
 // the products it needs, with 1.73 CTAs an SM in two rounds. Blocks of 128
 // tokens with one S, both operands in shared memory, took 365.
 // Roles: warps 0-3 and 4-7 softmax of tiles 0 and 1 (a thread a row), 8-11

@@ -19,8 +19,8 @@
 // tiles, so that the L2 has to deliver only 40 bytes a clock and SM), the
 // decoding for few (its warps then keep four blocks in flight each, and CTAs of
 // a cluster share the sum when there are too few tiles for all SMs). bf16, 2048
-// x 8192 x 8192: 217 us, 1.27 PFLOP/s, with 1.73 tiles an SM in two rounds;
-// forward and backward of 2000 x 8192 x 4096 in fp16 260 us, 1.03 PFLOP/s.
+// x 8192 x 8192: 223 us, 1.23 PFLOP/s, with 1.73 tiles an SM in two rounds;
+// forward and backward of 2000 x 8192 x 4096 in fp16 271 us, 0.99 PFLOP/s.
 // Roles: warps 0-15 decode (registers to swizzled shared memory, then, at the
 // end, D to global memory), warp 16 issues the TMA loads, warp 17 the MMAs.
 #pragma once
