@@ -101,7 +101,8 @@ __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint
 }
 
 // kFull: the head dimension is DP. kLong: O is put aside (its code costs the
-// others 3 to 13% of their time, by registers).
+// others 3 to 13% of their time, by registers; 1000 rows over 60000 tokens in
+// fp16 1372 us, without it 1290).
 template <typename T, int DP, bool kFull, bool kLong>
 __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p) {
   using S = PreShape<DP>;
@@ -179,9 +180,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) prefill_kernel(const Attend p)
   __syncthreads();
   const int blocks = (top_lim + kPreKeys - 1) / kPreKeys;
   if (kLong && top_lim > p.most && threadIdx.x == 0) {
-    // no more CTAs than places run at a time; were there none free, O would stay
-    for (int i = 0; i < p.sms && place < 0; ++i)
-      if (atomicCAS(p.places + i, 0, 1) == 0) place = i;
+    // No more CTAs than places run at a time (were there none free, O would stay);
+    // the first to ask for is this SM's.
+    uint32_t sm;
+    asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
+    int at = (int)(sm % (uint32_t)p.sms), left = p.sms;
+    while (left > 0 && atomicCAS(p.places + at, 0, 1) != 0) {
+      at = at + 1 == p.sms ? 0 : at + 1;
+      --left;
+    }
+    if (left > 0) place = at;
     __threadfence();
   }
   if (dim < DP) {  // columns of K and Q behind the head dimension are zeros, for good
